@@ -358,6 +358,92 @@ int lx_attention_np_f32(const float* q, int ldq, const float* k, int ldk, const 
                         int products, int out_packed, int kv_packed,
                         hipStream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* The LM in four bits                                                       */
+/* ------------------------------------------------------------------------ */
+
+/* 4-bit weights with group scales.  Groups of `group` (32, 64 or 128) consecutive
+ * inputs of a row of W (N, K), the last one short where K ends inside it: with v
+ * the group's value of largest magnitude (the first of equals), s = bf16(v / -8)
+ * and q = clamp(rint(w / s) + 8, 0, 15), a code q stands for s * (q - 8), off by
+ * at most |s| / 2 (the largest magnitude: |s| / 32; one of the opposite sign as
+ * large: |s|).  All zeros: zeros.  A group that holds an infinity or a NaN
+ * stands for NaN.  Any N, K % 4 == 0.
+ * lx_q4_bytes: size of the packed weight (codes in MFMA fragment order, then the
+ * scales), about K / 2 + 2 K / group bytes a row; 0 for a bad shape.
+ * lx_q4_pack_f32 quantises W (16-byte aligned, row-major) into Wq (16-byte
+ * aligned), once, as lx_wfrag_pack_f32; lx_q4_unpack_f32 writes back what the
+ * codes stand for.  No counterpart in the reference (its weights stay fp32). */
+size_t lx_q4_bytes(int N, int K, int group);
+int lx_q4_pack_f32(const float* W, void* Wq, int N, int K, int group, hipStream_t stream);
+int lx_q4_unpack_f32(const void* Wq, float* W, int N, int K, int group, hipStream_t stream);
+
+/* Projection of few rows on such a weight:  y = epi(x @ W~^T + bias), W~ what the
+ * packed codes stand for, fp32 arithmetic (x as three bf16 parts, exact products
+ * with the codes, fp32 sums; the scale applied to each group's sum).  x: (M, K),
+ * 1 <= M <= 64, row stride ldx; y: (M, N), row stride ldy (N / 2 columns for
+ * SWIGLU_PAIRED, N even); y must not overlap x.  Epilogues: none, GELU_TANH, RESID,
+ * SWIGLU_PAIRED (others: LX_ERR_ARG); bias (N) or NULL.  K and ldx multiples of
+ * 4, x and Wq 16-byte aligned.  An infinite or NaN element of x, or one above
+ * 3.3895e38 in magnitude, makes NaN of its row.  The result does not depend on
+ * timing.  Replaces linear() (src/llm/ops.cpp:13-19) for weights given in 4 bits. */
+int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int group, const float* bias,
+                     float* y, long ldy, int M, int N, int K, const lx_epilogue* epi,
+                     hipStream_t stream);
+
+/* A key/value cache held in 4 bits (4.5 with its scales): `batch` sequences of up
+ * to max_rows rows, n_kv_heads heads of head_dim (64 or 128) channels.  Keys and
+ * values alike: the 64 channels of a group of a row share z = the largest bf16
+ * not above their minimum and s = the smallest bf16 not below (max - z) / 15; a
+ * code q = clamp(rint((x - z) / s), 0, 15) stands for z + s * q (s = 0: z).  A
+ * group that holds an infinity or a NaN, or whose |z| + 16 s passes fp32, stands
+ * for NaN.  `data`: device memory of lx_kv4_bytes() bytes (0 for a bad
+ * shape), 16-byte aligned, which needs no initialisation; rows that were never
+ * appended hold anything.  How many rows of each sequence are in use is the
+ * caller's to know (device int32[batch], so captured graphs can be replayed).
+ * No counterpart in the reference (its cache is host fp32 vectors,
+ * include/larynx/llm/llm.h:77-84). */
+typedef struct lx_kv4 {
+  void* data;
+  int batch, n_kv_heads, head_dim, max_rows;
+} lx_kv4;
+size_t lx_kv4_bytes(int batch, int n_kv_heads, int head_dim, int max_rows);
+
+/* Quantises T rows of keys (roped) and values per sequence into rows pos[b] ..
+ * pos[b] + T - 1.  k, v: (batch, T, *), row strides ldk / ldv (sequences T rows
+ * apart), head g at column g * head_dim; pos: device int32[batch].  Rows outside
+ * [0, max_rows) are not written (pos[b] <= -T leaves a sequence alone), and no
+ * other row changes.  Calls that write one cache, or write and read it, must not
+ * overlap.  Replaces the cache append of src/llm/llm.cpp:200-204. */
+int lx_kv4_append_f32(const lx_kv4* cache, const float* k, long ldk, const float* v, long ldv,
+                      int T, const int* pos, hipStream_t stream);
+/* Writes what rows pos[b] .. pos[b] + T - 1 stand for into k and v, (batch, T,
+ * n_kv_heads * head_dim) fp32; rows outside [0, max_rows) read as zero.  The
+ * 4-bit form of LLM::cache_key / cache_value (include/larynx/llm/llm.h:80-84). */
+int lx_kv4_read_f32(const lx_kv4* cache, float* k, float* v, int T, const int* pos,
+                    hipStream_t stream);
+
+/* Attention over such a cache, flash-style, fp32 arithmetic:
+ *   o[b, t, h*hd:(h+1)*hd] = softmax(scale * q_h k~_g^T) v~_g,  g = h / (n_heads / n_kv_heads)
+ * over the first lens[b] rows of sequence b (device int32[batch]; a value outside
+ * [0, max_rows] is taken as the nearer end).  causal != 0: query t stands at row
+ * lens[b] - Tq + t and sees the rows up to its own (the usual call: append Tq
+ * rows, then attend with the lengths that count them).  A query that sees no row
+ * gives zeros.  q, o: (batch, Tq, *), row strides ldq / ldo (multiples of 4,
+ * sequences Tq rows apart), 16-byte aligned, head h at column h * hd; o must not
+ * overlap q.  What unseen rows hold does not matter, NaN included; a NaN or an
+ * infinity in a query makes NaN of its row and head.
+ * max_len: the largest length expected (0: max_rows).  It only sizes the launch:
+ * the keys of one sequence are split over more workgroups when there are few, and
+ * joined by a second launch; longer sequences are right too.  ws:
+ * lx_attention_kv4_ws_floats() floats of scratch for that call, 16-byte aligned
+ * (NULL when that is 0); calls that share it must not overlap.
+ * Replaces attention() over the cache (src/llm/ops.cpp:49-65). */
+size_t lx_attention_kv4_ws_floats(const lx_kv4* cache, int Tq, int n_heads, int max_len);
+int lx_attention_kv4_f32(const float* q, long ldq, const lx_kv4* cache, const int* lens, float* o,
+                         long ldo, int Tq, int n_heads, float scale, int causal, int max_len,
+                         float* ws, size_t ws_floats, hipStream_t stream);
+
 /* Causal grouped conv1d + Mish (one CausalConvPositionEmbedding half):
  *   y[b,t,oc] = mish(bias[oc] + sum_{k<K, ic<C/G} w[oc, ic, k] *
  *                                 x[b, t-(K-1)+k, g*(C/G)+ic]) (+ resid[b,t,oc])

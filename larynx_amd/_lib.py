@@ -66,6 +66,11 @@ class LinearBx(C.Structure):
     ]
 
 
+class Kv4(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("batch", C.c_int), ("n_kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("max_rows", C.c_int)]
+
+
 _DIT_BLOCK_FIELDS = [
     "attn_norm_w", "attn_norm_b", "to_q_w", "to_q_b", "to_k_w", "to_k_b", "to_v_w", "to_v_b",
     "to_out_w", "to_out_b", "ff0_w", "ff0_b", "ff2_w", "ff2_b",
@@ -164,6 +169,21 @@ SIGNATURES = [
     ("lx_attention_np_f32", C.c_int,
      [fp, C.c_int, fp, C.c_int, fp, C.c_int, fp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
       C.c_int, C.c_int, C.c_float, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, stream_t]),
+    ("lx_q4_bytes", C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    ("lx_q4_pack_f32", C.c_int, [fp, C.c_void_p, C.c_int, C.c_int, C.c_int, stream_t]),
+    ("lx_q4_unpack_f32", C.c_int, [C.c_void_p, fp, C.c_int, C.c_int, C.c_int, stream_t]),
+    ("lx_linear_q4_f32", C.c_int,
+     [fp, C.c_long, C.c_void_p, C.c_int, fp, fp, C.c_long, C.c_int, C.c_int, C.c_int,
+      C.POINTER(Epilogue), stream_t]),
+    ("lx_kv4_bytes", C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    ("lx_kv4_append_f32", C.c_int,
+     [C.POINTER(Kv4), fp, C.c_long, fp, C.c_long, C.c_int, ip, stream_t]),
+    ("lx_kv4_read_f32", C.c_int, [C.POINTER(Kv4), fp, fp, C.c_int, ip, stream_t]),
+    ("lx_attention_kv4_ws_floats", C.c_size_t,
+     [C.POINTER(Kv4), C.c_int, C.c_int, C.c_int]),
+    ("lx_attention_kv4_f32", C.c_int,
+     [fp, C.c_long, C.POINTER(Kv4), ip, fp, C.c_long, C.c_int, C.c_int, C.c_float, C.c_int,
+      C.c_int, fp, C.c_size_t, stream_t]),
     ("lx_conv_pos_mish_f32", C.c_int,
      [fp, fp, fp, fp, fp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, stream_t]),
     ("lx_conv_pack_weight_f32", C.c_int, [fp, fp, C.c_int, C.c_int, C.c_int, stream_t]),

@@ -1,0 +1,564 @@
+// A key/value cache held in 4 bits: append, read back, attention over it.
+//
+// The 64 channels of a group (one head at head_dim 64, half of one at 128) of one cached row
+// share z = the largest bf16 not above their minimum and s = the smallest bf16 not below
+// (max - z) / 15; a code q = rint((x - z) / s) stands for x~ = z + s q, so every value lies
+// inside the range and is off by at most s / 2.  4.5 bits a value.
+//
+// Layout: per sequence, kv head and block of 32 rows one record of 2304 bytes a channel group:
+// 1 KB of key codes, 1 KB of value codes, then per row the key and the value (s, z) pairs as
+// dwords (s low, z high).  Both code planes are MFMA fragments (lx_four_bit.hpp), 16 bytes a
+// lane: for S^T = K Q^T the keys are rows and the channels k, for O^T = V^T P^T the channels are
+// rows and the keys k.  The order of the 32 keys in V's k index is the one in which a lane
+// already holds its scores (4 c .. 4 c + 3 of both 16-key tiles, c = lane / 16), so the softmax
+// weights go from one product's result to the other's operand without leaving the lane.
+#include <algorithm>
+#include <climits>
+
+#include "lx_four_bit.hpp"
+
+namespace lx {
+namespace {
+
+constexpr int kBlk = 32;       // rows of a record
+constexpr int kGrp = 64;       // channels of a group
+constexpr int kCodes = 1024;   // bytes of one group's key (or value) codes in a record
+constexpr int kRec = 2 * kCodes + 2 * kBlk * 4;  // bytes of a record, per channel group
+
+// Record of (sequence, kv head, block): ng groups of key codes, ng of value codes, ng x 32 key
+// (s, z), ng x 32 value (s, z).
+struct Kv4 {
+  char* data;
+  int batch, heads, ng, rows, blocks;
+  __host__ __device__ size_t record(int b, int h, int blk) const {
+    return (((size_t)b * heads + h) * blocks + blk) * ((size_t)ng * kRec);
+  }
+};
+
+struct AppendArgs {
+  Kv4 c;
+  const float *k, *v;
+  long ldk, ldv;
+  int T, touched;
+  const int* pos;
+};
+
+// z and s of a group with extremes lo and hi (both finite), and the quotient in 64 bits: a value
+// next to a border decides a whole step.
+struct Affine {
+  float s, z;
+};
+__device__ __forceinline__ Affine affine(float lo, float hi) {
+  unsigned zb = __float_as_uint(lo);
+  const unsigned cut = zb & 0xffff0000u;
+  zb = lo < 0.0f && cut != zb ? cut + 0x10000u : cut;
+  Affine a;
+  a.z = __uint_as_float(zb);
+  const double r = ((double)hi - (double)a.z) / 15.0;
+  float f = (float)r;
+  unsigned sb = __float_as_uint(f);
+  if ((double)f < r) ++sb;
+  a.s = __uint_as_float((sb + 0xffffu) & 0xffff0000u);
+  return a;
+}
+__device__ __forceinline__ unsigned affine_code(float x, Affine a) {
+  if (!(a.s > 0.0f)) return 0;
+  const double q = rint(((double)x - (double)a.z) / (double)a.s);
+  return (unsigned)(int)fmin(fmax(q, 0.0), 15.0);
+}
+
+// Codes and pair of one group, lane = channel.  A group that holds an infinity or a NaN, or
+// whose |z| + 16 s passes fp32 (the attention forms z - 16 s), stores NaN.
+__device__ __forceinline__ unsigned quantise(float x, unsigned* pair) {
+  const float hi = wave_max(x), lo = -wave_max(-x);
+  const bool bad = __any(!(fabsf(x) <= 3.402823466e38f));
+  const Affine a = affine(lo, hi);
+  if (bad || !(fmaf(16.0f, a.s, fabsf(a.z)) <= 3.402823466e38f)) {
+    *pair = 0x7fc07fc0u;
+    return 0;
+  }
+  *pair = __float_as_uint(a.s) >> 16 | (__float_as_uint(a.z) & 0xffff0000u);
+  return affine_code(x, a);
+}
+
+// One workgroup per (32-row record touched, kv head, sequence); wave w owns the rows whose value
+// codes share dwords, 4 w .. 4 w + 3 of both halves, lane = channel.
+__global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int i = blockIdx.x % a.touched;
+  const int bh = blockIdx.x / a.touched, b = bh / a.c.heads, h = bh % a.c.heads;
+  const long pos = a.pos[b];
+  const long blk = max(pos, 0L) / kBlk + i;
+  if (blk >= a.c.blocks) return;
+  char* rec = a.c.data + a.c.record(b, h, (int)blk);
+  const int ng = a.c.ng;
+  for (int g = 0; g < ng; ++g) {
+    unsigned vword = 0, vmask = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int row = 4 * w + (j & 3) + 16 * (j >> 2);
+      const long t = blk * kBlk + row - pos;
+      if (t < 0 || t >= a.T || blk * kBlk + row >= a.c.rows) continue;
+      const long ch = (long)(h * ng + g) * kGrp + lane;
+      const float kx = a.k[((long)b * a.T + t) * a.ldk + ch];
+      const float vx = a.v[((long)b * a.T + t) * a.ldv + ch];
+      unsigned kp, vp;
+      const unsigned kq = quantise(kx, &kp), vq = quantise(vx, &vp);
+      vword |= q4_put(vq, j);
+      vmask |= q4_put(15u, j);
+      // eight channels make a dword of key codes
+      unsigned kw = q4_put(kq, lane & 7);
+      kw |= __shfl_xor(kw, 1, 64);
+      kw |= __shfl_xor(kw, 2, 64);
+      kw |= __shfl_xor(kw, 4, 64);
+      if ((lane & 7) == 0) {
+        const int ks = lane >> 5, c = (lane >> 3) & 3;
+        reinterpret_cast<unsigned*>(rec + g * kCodes)[((c * 16 + (row & 15)) * 2 + (row >> 4)) * 2 +
+                                                      ks] = kw;
+      }
+      if (lane == 0) {
+        unsigned* pairs = reinterpret_cast<unsigned*>(rec + 2 * ng * kCodes);
+        pairs[g * kBlk + row] = kp;
+        pairs[(ng + g) * kBlk + row] = vp;
+      }
+    }
+    if (vmask) {
+      unsigned* p = reinterpret_cast<unsigned*>(rec + (ng + g) * kCodes) +
+                    (w * 16 + (lane & 15)) * 4 + (lane >> 4);
+      *p = (*p & ~vmask) | vword;
+    }
+  }
+}
+
+struct ReadArgs {
+  Kv4 c;
+  float *k, *v;
+  int T;
+  const int* pos;
+};
+
+// One thread per (row, channel); rows outside the cache read as zero.
+__global__ __launch_bounds__(256) void kv4_read_kernel(ReadArgs a) {
+  const int hd = a.c.ng * kGrp, width = a.c.heads * hd;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long)a.c.batch * a.T * width) return;
+  const int ch = (int)(i % hd), h = (int)(i / hd % a.c.heads);
+  const long bt = i / width;
+  const int b = (int)(bt / a.T);
+  const long row = (long)a.pos[b] + bt % a.T;
+  float k = 0.0f, v = 0.0f;
+  if (row >= 0 && row < a.c.rows) {
+    const char* rec = a.c.data + a.c.record(b, h, (int)(row / kBlk));
+    const int r = (int)(row % kBlk), g = ch / kGrp, x = ch % kGrp, ng = a.c.ng;
+    const unsigned* kc = reinterpret_cast<const unsigned*>(rec + g * kCodes);
+    const unsigned* vc = reinterpret_cast<const unsigned*>(rec + (ng + g) * kCodes);
+    const unsigned* pairs = reinterpret_cast<const unsigned*>(rec + 2 * ng * kCodes);
+    const unsigned kw = kc[((((x >> 3) & 3) * 16 + (r & 15)) * 2 + (r >> 4)) * 2 + (x >> 5)];
+    const unsigned vw = vc[(((r & 15) >> 2) * 16 + (x & 15)) * 4 + (x >> 4)];
+    const unsigned kp = pairs[g * kBlk + r], vp = pairs[(ng + g) * kBlk + r];
+    k = fmaf(bf16_lo(kp), (float)q4_get(kw, x & 7), bf16_hi(kp));
+    v = fmaf(bf16_lo(vp), (float)q4_get(vw, (r & 3) + 4 * (r >> 4)), bf16_hi(vp));
+  }
+  a.k[i] = k;
+  a.v[i] = v;
+}
+
+// ---- attention --------------------------------------------------------------------------
+
+constexpr int kQ = 16;  // query rows of a tile: (t, head of the group) pairs, t-major
+
+struct AttnArgs {
+  Kv4 c;
+  const float* q;
+  long ldq;
+  const int* lens;
+  float* o;
+  long ldo;
+  float* ws;
+  int Tq, rep, tiles, splits, causal;
+  float scale2;  // scale * log2(e)
+};
+
+// Partial states in the workspace, per (sequence, kv head, query tile, split): 16 rows of hd
+// unnormalised outputs, then 16 maxima (in units of log2) and 16 sums.
+__host__ __device__ constexpr long part_floats(int ng) { return (long)kQ * (ng * kGrp + 2); }
+
+// One workgroup of four waves per (sequence, kv head, tile of 16 query rows, split of the
+// keys); the waves take the split's records in turn, each with a running softmax of its own.
+// Scores are kept in units of log2 (q carries scale * log2 e), transposed: lane l holds query
+// row l % 16.
+template <int NG>
+__global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
+  constexpr int HD = NG * kGrp;
+  __shared__ float om[4][kQ][HD + 4];
+  __shared__ float ml[4][2][kQ];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int col = lane & 15, c = lane >> 4;
+  const int sp = blockIdx.x % a.splits;
+  const long rest = blockIdx.x / a.splits;
+  const int qt = (int)(rest % a.tiles);
+  const int bh = (int)(rest / a.tiles), b = bh / a.c.heads, h = bh % a.c.heads;
+  const int len = min(max(a.lens[b], 0), a.c.rows);
+  const int nrow = a.Tq * a.rep;
+  const int row = qt * kQ + col;           // the lane's query row
+  const int t = min(row, nrow - 1) / a.rep, hr = min(row, nrow - 1) % a.rep;
+  // keys the row sees: [0, limit)
+  const int limit = row >= nrow ? 0 : a.causal ? max(len - a.Tq + t + 1, 0) : len;
+  const int t_last = min(qt * kQ + kQ - 1, nrow - 1) / a.rep, t_first = qt * kQ / a.rep;
+  const int most = a.causal ? max(len - a.Tq + t_last + 1, 0) : len;   // of any row of the tile
+  const int least = a.causal ? max(len - a.Tq + t_first + 1, 0) : len;
+  const int nblk = (most + kBlk - 1) / kBlk;
+  const int per = (nblk + a.splits - 1) / a.splits;
+  const int b0 = sp * per, b1 = min(b0 + per, nblk);
+
+  sbf16x8 qf[NG][2][3];
+  float qsum[NG];
+  {
+    const float* q = a.q + ((long)b * a.Tq + t) * a.ldq + (long)(h * a.rep + hr) * HD + c * 8;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float s = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float4 u = *reinterpret_cast<const float4*>(q + g * kGrp + ks * 32 + 4 * e);
+          x[4 * e] = u.x * a.scale2;
+          x[4 * e + 1] = u.y * a.scale2;
+          x[4 * e + 2] = u.z * a.scale2;
+          x[4 * e + 3] = u.w * a.scale2;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += x[j];
+        split3(x, qf[g][ks]);
+      }
+      s += lane_xor16(s);
+      s += lane_xor32(s);
+      qsum[g] = s;
+    }
+  }
+  floatx4 o[NG][4];
+  float zsum[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    zsum[g] = 0.0f;
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct) o[g][ct] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  float m = -INFINITY, l = 0.0f;
+  for (int blk = b0 + wave; blk < b1; blk += 4) {
+    const char* rec = a.c.data + a.c.record(b, h, blk);
+    uintx4_t kc[NG], vc[NG], kp[NG][2], vp[NG][2];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      kc[g] = reinterpret_cast<const uintx4_t*>(rec + g * kCodes)[lane];
+      vc[g] = reinterpret_cast<const uintx4_t*>(rec + (NG + g) * kCodes)[lane];
+      const uintx4_t* pairs = reinterpret_cast<const uintx4_t*>(rec + 2 * NG * kCodes);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        kp[g][i] = pairs[g * 8 + i * 4 + c];
+        vp[g][i] = pairs[(NG + g) * 8 + i * 4 + c];
+      }
+    }
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          const sbf16x8 kf = q4_frag(kc[g][i * 2 + ks]);
+#pragma unroll
+          for (int p = 2; p >= 0; --p) acc = mfma_bf16(kf, qf[g][ks][p], acc);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float ss = bf16_lo(kp[g][i][e]), z = bf16_hi(kp[g][i][e]);
+          const float v = fmaf(ss, acc[e], fmaf(-16.0f, ss, z) * qsum[g]);
+          s[i * 4 + e] = g == 0 ? v : s[i * 4 + e] + v;
+        }
+      }
+    }
+    if (blk * kBlk + kBlk > least) {
+      // a key the row does not see may hold anything (NaN, rows never written): neither its
+      // score nor its value takes part
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (blk * kBlk + 16 * (j >> 2) + 4 * c + (j & 3) >= limit) {
+          s[j] = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) vp[g][j >> 2][j & 3] = 0;
+        }
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[j]);
+    mx = fmaxf(mx, lane_xor16(mx));
+    mx = fmaxf(mx, lane_xor32(mx));
+    if (__any(mx > m)) {
+      const float mn = fmaxf(m, mx);
+      const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= al;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        zsum[g] *= al;
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct) o[g][ct] *= al;
+      }
+    }
+    // a row that has seen no key yet: every weight exp2(-inf - 0) = 0
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      p[j] = __builtin_amdgcn_exp2f(s[j] - ref);
+      l += p[j];
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float ps[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float ss = bf16_lo(vp[g][j >> 2][j & 3]), z = bf16_hi(vp[g][j >> 2][j & 3]);
+        ps[j] = p[j] * ss;
+        zsum[g] = fmaf(p[j], fmaf(-16.0f, ss, z), zsum[g]);
+      }
+      sbf16x8 pf[3];
+      split3(ps, pf);
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) {
+        const sbf16x8 vf = q4_frag(vc[g][ct]);
+#pragma unroll
+        for (int i = 2; i >= 0; --i) o[g][ct] = mfma_bf16(vf, pf[i], o[g][ct]);
+      }
+    }
+  }
+  // the lane's sums over its keys -> the row's
+  l += lane_xor16(l);
+  l += lane_xor32(l);
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    zsum[g] += lane_xor16(zsum[g]);
+    zsum[g] += lane_xor32(zsum[g]);
+#pragma unroll
+    for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        om[wave][col][g * kGrp + ct * 16 + 4 * c + e] = o[g][ct][e] + zsum[g];
+  }
+  if (c == 0) {
+    ml[wave][0][col] = m;
+    ml[wave][1][col] = l;
+  }
+  __syncthreads();
+  // the four waves' states, joined in wave order
+  float* part = a.ws + (((long)bh * a.tiles + qt) * a.splits + sp) * part_floats(NG);
+  for (int i = tid; i < kQ * (HD / 4); i += 256) {
+    const int r = i / (HD / 4), ch = i % (HD / 4) * 4, rr = qt * kQ + r;
+    if (rr >= nrow) continue;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w][0][r]);
+    float L = 0.0f;
+    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float mw = ml[w][0][r];
+      const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
+      L += f * ml[w][1][r];
+      const float4 u = *reinterpret_cast<const float4*>(&om[w][r][ch]);
+      O.x += f * u.x;
+      O.y += f * u.y;
+      O.z += f * u.z;
+      O.w += f * u.w;
+    }
+    if (a.splits == 1) {
+      const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+      float* dst = a.o + ((long)b * a.Tq + rr / a.rep) * a.ldo +
+                   (long)(h * a.rep + rr % a.rep) * HD + ch;
+      *reinterpret_cast<float4*>(dst) = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+    } else {
+      *reinterpret_cast<float4*>(part + r * HD + ch) = O;
+      if (ch == 0) {
+        part[kQ * HD + r] = M;
+        part[kQ * HD + kQ + r] = L;
+      }
+    }
+  }
+}
+
+// The splits' states of a row, joined in split order: one thread per four channels of a row.
+template <int NG>
+__global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a) {
+  constexpr int HD = NG * kGrp;
+  const int nrow = a.Tq * a.rep;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const int ch = (int)(i % (HD / 4)) * 4;
+  const long rg = i / (HD / 4);  // (sequence, kv head) * nrow + row
+  if (rg >= (long)a.c.batch * a.c.heads * nrow) return;
+  const int rr = (int)(rg % nrow);
+  const long bh = rg / nrow;
+  const int b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads);
+  const float* p = a.ws + (bh * a.tiles + rr / kQ) * a.splits * part_floats(NG);
+  const int r = rr % kQ;
+  float M = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, p[s * part_floats(NG) + kQ * HD + r]);
+  float L = 0.0f;
+  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < a.splits; ++s) {
+    const float* ps = p + s * part_floats(NG);
+    const float ms = ps[kQ * HD + r];
+    if (ms == -INFINITY) continue;
+    const float f = __builtin_amdgcn_exp2f(ms - M);
+    L += f * ps[kQ * HD + kQ + r];
+    const float4 u = *reinterpret_cast<const float4*>(ps + r * HD + ch);
+    O.x += f * u.x;
+    O.y += f * u.y;
+    O.z += f * u.z;
+    O.w += f * u.w;
+  }
+  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+  float* dst = a.o + ((long)b * a.Tq + rr / a.rep) * a.ldo + (long)(h * a.rep + rr % a.rep) * HD +
+               ch;
+  *reinterpret_cast<float4*>(dst) = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+}
+
+// Splits of the keys: about two workgroups per CU, at least four records (one a wave) each.
+int kv4_splits(long wgs, int max_len) {
+  const int blocks = (max_len + kBlk - 1) / kBlk;
+  const long want = 2L * device_cus() / std::max(wgs, 1L);
+  return (int)std::max(1L, std::min<long>(want, (blocks + 3) / 4));
+}
+
+bool kv4_shape_ok(int batch, int heads, int hd, int rows) {
+  return batch > 0 && heads > 0 && (hd == 64 || hd == 128) && rows > 0 &&
+         (long)batch * heads < INT_MAX && rows <= INT_MAX - kBlk;
+}
+
+int kv4_view(const lx_kv4* c, const char* what, Kv4* out) {
+  LX_REQUIRE(c && c->data, "%s: null cache", what);
+  LX_REQUIRE(kv4_shape_ok(c->batch, c->n_kv_heads, c->head_dim, c->max_rows),
+             "%s: bad cache (%d sequences, %d heads of %d, %d rows)", what, c->batch,
+             c->n_kv_heads, c->head_dim, c->max_rows);
+  LX_REQUIRE((uintptr_t)c->data % 16 == 0, "%s: unaligned cache", what);
+  *out = Kv4{static_cast<char*>(c->data), c->batch, c->n_kv_heads, c->head_dim / kGrp, c->max_rows,
+             (c->max_rows + kBlk - 1) / kBlk};
+  return LX_OK;
+}
+
+}  // namespace
+}  // namespace lx
+
+using namespace lx;
+
+extern "C" size_t lx_kv4_bytes(int batch, int n_kv_heads, int head_dim, int max_rows) {
+  if (!kv4_shape_ok(batch, n_kv_heads, head_dim, max_rows)) return 0;
+  return (size_t)batch * n_kv_heads * ((max_rows + kBlk - 1) / kBlk) * (head_dim / kGrp) * kRec;
+}
+
+extern "C" int lx_kv4_append_f32(const lx_kv4* cache, const float* k, long ldk, const float* v,
+                                 long ldv, int T, const int* pos, hipStream_t stream) {
+  AppendArgs a{};
+  LX_TRY(kv4_view(cache, "kv4_append", &a.c));
+  LX_REQUIRE(k && v && pos, "kv4_append: null pointer");
+  const long width = (long)cache->n_kv_heads * cache->head_dim;
+  LX_REQUIRE(T > 0 && ldk >= width && ldv >= width, "kv4_append: bad shape T=%d ldk=%ld ldv=%ld",
+             T, ldk, ldv);
+  a.k = k;
+  a.v = v;
+  a.ldk = ldk;
+  a.ldv = ldv;
+  a.T = T;
+  a.pos = pos;
+  // records that T rows can touch, wherever they begin
+  a.touched = (int)std::min<long>(((long)T + kBlk - 2) / kBlk + 1, a.c.blocks);
+  const long grid = (long)a.touched * cache->batch * cache->n_kv_heads;
+  LX_REQUIRE(grid <= INT_MAX, "kv4_append: %ld workgroups", grid);
+  hipLaunchKernelGGL(kv4_append_kernel, dim3((unsigned)grid), dim3(256), 0, stream, a);
+  return check_launch("kv4_append_kernel");
+}
+
+extern "C" int lx_kv4_read_f32(const lx_kv4* cache, float* k, float* v, int T, const int* pos,
+                               hipStream_t stream) {
+  ReadArgs a{};
+  LX_TRY(kv4_view(cache, "kv4_read", &a.c));
+  LX_REQUIRE(k && v && pos, "kv4_read: null pointer");
+  LX_REQUIRE(T > 0, "kv4_read: bad shape T=%d", T);
+  a.k = k;
+  a.v = v;
+  a.T = T;
+  a.pos = pos;
+  const long n = (long)cache->batch * T * cache->n_kv_heads * cache->head_dim;
+  LX_REQUIRE((n + 255) / 256 <= INT_MAX, "kv4_read: %ld values", n);
+  hipLaunchKernelGGL(kv4_read_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
+  return check_launch("kv4_read_kernel");
+}
+
+extern "C" size_t lx_attention_kv4_ws_floats(const lx_kv4* cache, int Tq, int n_heads,
+                                             int max_len) {
+  Kv4 c;
+  if (kv4_view(cache, "attention_kv4_ws_floats", &c) != LX_OK || Tq <= 0 || n_heads <= 0 ||
+      n_heads % c.heads)
+    return 0;
+  const long tiles = ((long)Tq * (n_heads / c.heads) + kQ - 1) / kQ;
+  const long wgs = tiles * c.batch * c.heads;
+  const int len = max_len <= 0 || max_len > c.rows ? c.rows : max_len;
+  const int splits = kv4_splits(wgs, len);
+  return splits == 1 ? 0 : (size_t)wgs * splits * part_floats(c.ng);
+}
+
+extern "C" int lx_attention_kv4_f32(const float* q, long ldq, const lx_kv4* cache, const int* lens,
+                                    float* o, long ldo, int Tq, int n_heads, float scale,
+                                    int causal, int max_len, float* ws, size_t ws_floats,
+                                    hipStream_t stream) {
+  AttnArgs a{};
+  LX_TRY(kv4_view(cache, "attention_kv4", &a.c));
+  LX_REQUIRE(q && lens && o, "attention_kv4: null pointer");
+  const long width = (long)n_heads * cache->head_dim;
+  LX_REQUIRE(Tq > 0 && n_heads > 0 && n_heads % a.c.heads == 0 && ldq >= width && ldo >= width &&
+                 ldq % 4 == 0 && ldo % 4 == 0,
+             "attention_kv4: bad shape Tq=%d heads=%d/%d ldq=%ld ldo=%ld", Tq, n_heads, a.c.heads,
+             ldq, ldo);
+  LX_REQUIRE(((uintptr_t)q | (uintptr_t)o) % 16 == 0, "attention_kv4: q and o must be 16-byte "
+             "aligned");
+  LX_REQUIRE((long)Tq * n_heads / a.c.heads <= INT_MAX - kQ, "attention_kv4: Tq=%d too long", Tq);
+  a.q = q;
+  a.ldq = ldq;
+  a.lens = lens;
+  a.o = o;
+  a.ldo = ldo;
+  a.Tq = Tq;
+  a.rep = n_heads / a.c.heads;
+  a.tiles = (Tq * a.rep + kQ - 1) / kQ;
+  a.causal = causal != 0;
+  a.scale2 = scale * 1.4426950408889634f;
+  const long wgs = (long)a.tiles * a.c.batch * a.c.heads;
+  const int len = max_len <= 0 || max_len > a.c.rows ? a.c.rows : max_len;
+  a.splits = kv4_splits(wgs, len);
+  if (a.splits > 1) {
+    const size_t need = (size_t)wgs * a.splits * part_floats(a.c.ng);
+    LX_REQUIRE(ws && ws_floats >= need && (uintptr_t)ws % 16 == 0,
+               "attention_kv4: workspace of %zu floats, %zu needed", ws ? ws_floats : 0, need);
+    a.ws = ws;
+  }
+  LX_REQUIRE(wgs * a.splits <= INT_MAX, "attention_kv4: %ld workgroups", wgs * a.splits);
+  const dim3 grid((unsigned)(wgs * a.splits));
+  if (a.c.ng == 1)
+    hipLaunchKernelGGL(kv4_attn_kernel<1>, grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL(kv4_attn_kernel<2>, grid, dim3(256), 0, stream, a);
+  LX_TRY(check_launch("kv4_attn_kernel"));
+  if (a.splits > 1) {
+    const long n = (long)a.c.batch * a.c.heads * Tq * a.rep * (cache->head_dim / 4);
+    const dim3 jg((unsigned)((n + 255) / 256));
+    if (a.c.ng == 1)
+      hipLaunchKernelGGL(kv4_join_kernel<1>, jg, dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL(kv4_join_kernel<2>, jg, dim3(256), 0, stream, a);
+    return check_launch("kv4_join_kernel");
+  }
+  return LX_OK;
+}

@@ -7,12 +7,13 @@ layout; work is enqueued on torch's current stream.  Every call goes through
 liblxops.so; a failing call raises LxError (no fallback path exists).
 """
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
 from ._lib import (LX_BX_OUT_F32, LX_BX_OUT_PACKED, LX_BX_OUT_PARTIAL, LX_EPI_GATED_RESID,
                    LX_EPI_GELU_TANH, LX_EPI_NONE, LX_EPI_RESID, LX_EPI_ROPE_PARTIAL,
-                   LX_EPI_SWIGLU_PAIRED, Epilogue, LinearBx, check, lib)
+                   LX_EPI_SWIGLU_PAIRED, Epilogue, Kv4, LinearBx, check, lib)
 
 __all__ = [
     "stream", "ada_ln", "adaln_resid", "adaln_emb", "rope_partial", "gelu_tanh", "gated_residual",
@@ -21,7 +22,8 @@ __all__ = [
     "Epilogue", "split_planes", "linear_split", "wfrag_pack", "linear_bx", "bx_scratch",
     "LX_EPI_NONE", "LX_EPI_GELU_TANH", "LX_EPI_GATED_RESID", "LX_EPI_ROPE_PARTIAL",
     "LX_EPI_RESID", "LX_EPI_SWIGLU_PAIRED", "LX_BX_OUT_F32", "LX_BX_OUT_PARTIAL",
-    "LX_BX_OUT_PACKED",
+    "LX_BX_OUT_PACKED", "Q4Weight", "q4_pack", "q4_unpack", "linear_q4", "Kv4Cache", "kv4_cache",
+    "kv4_append", "kv4_read", "attention_kv4",
 ]
 
 
@@ -327,3 +329,166 @@ def conv_pos_mish_bx(x, wf, bias, resid=None, groups=16, kernel=31, products=3):
     check(lib.lx_conv_pos_mish_bx_f32(_p(x), wf.data_ptr(), _p(bias), _p(resid), _p(y), B, T, Cc,
                                       groups, kernel, products, stream()))
     return y
+
+
+# ---- the LM in four bits ----------------------------------------------------------------
+
+
+def _on_device(**tensors):
+    """The named tensors (None skipped) live on the current device, where the launch goes."""
+    for name, t in tensors.items():
+        if t is not None and (not t.is_cuda or t.get_device() != _device()):
+            raise ValueError(f"{name} must be a tensor on the current device")
+
+
+def _rows(t, name, dims, width, dtype=torch.float32):
+    """Row stride of t (..., width): rows of contiguous elements, the leading dimensions one
+    uniform run of rows."""
+    if t.dtype != dtype or t.dim() != dims or t.shape[-1] != width:
+        raise ValueError(f"{name} must be {dims}-dimensional {dtype} with rows of {width}")
+    if width > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the elements of a row must be contiguous")
+    many = dims == 3 and t.shape[0] > 1
+    ld = t.stride(-2) if t.shape[-2] > 1 else t.stride(0) if many else width
+    if many and t.stride(0) != t.shape[1] * ld:
+        raise ValueError(f"{name}: sequences must lie a whole number of rows apart")
+    return ld
+
+
+class Q4Weight(NamedTuple):
+    """A weight (N, K) in 4 bits with group scales, as q4_pack lays it out."""
+    data: torch.Tensor
+    N: int
+    K: int
+    group: int
+
+
+def q4_pack(W, group=64):
+    """W (N, K) fp32 -> Q4Weight for linear_q4: per `group` (32, 64, 128) inputs of a row the
+    bf16 scale s = bf16(v / -8), v the value of largest magnitude, and codes q = clamp(rint(w /
+    s) + 8, 0, 15) that stand for s * (q - 8)."""
+    _on_device(W=W)
+    if W.dim() != 2 or W.dtype != torch.float32 or not W.is_contiguous():
+        raise ValueError("W must be a contiguous 2-dimensional float32 tensor")
+    N, K = W.shape
+    n = lib.lx_q4_bytes(N, K, group)
+    if not n:
+        raise ValueError(f"q4_pack: unsupported shape ({N}, {K}) or group {group}")
+    w = Q4Weight(torch.empty(n, device=W.device, dtype=torch.uint8), N, K, group)
+    check(lib.lx_q4_pack_f32(W.data_ptr(), w.data.data_ptr(), N, K, group, stream()))
+    return w
+
+
+def q4_unpack(w):
+    """The fp32 (N, K) matrix that a Q4Weight stands for."""
+    _on_device(w=w.data)
+    W = torch.empty(w.N, w.K, device=w.data.device, dtype=torch.float32)
+    check(lib.lx_q4_unpack_f32(w.data.data_ptr(), W.data_ptr(), w.N, w.K, w.group, stream()))
+    return W
+
+
+def linear_q4(x, w, b=None, epilogue=None, out=None):
+    """epi(x @ W~^T + b) for 1 to 64 rows x (M, K) (row stride may exceed K) on a Q4Weight;
+    epilogue: none, GELU, residual (out= the residual stream) or SwiGLU over interleaved rows.
+    src/llm/ops.cpp:13-19."""
+    _on_device(x=x, w=w.data, b=b, out=out)
+    ldx = _rows(x, "x", 2, w.K)
+    M = x.shape[0]
+    kind = epilogue.kind if epilogue is not None else LX_EPI_NONE
+    cols = w.N // 2 if kind == LX_EPI_SWIGLU_PAIRED else w.N
+    if b is not None and (b.dtype != torch.float32 or b.numel() != w.N or not b.is_contiguous()):
+        raise ValueError(f"b must be {w.N} contiguous float32 values")
+    if out is None:
+        if kind == LX_EPI_RESID:
+            raise ValueError("residual epilogues need out= (the residual stream)")
+        out = torch.empty(M, cols, device=x.device, dtype=torch.float32)
+        ldy = cols
+    else:
+        if out.dim() != 2 or out.shape[0] != M:
+            raise ValueError(f"out must have {M} rows")
+        ldy = _rows(out, "out", 2, cols)
+    check(lib.lx_linear_q4_f32(x.data_ptr(), ldx, w.data.data_ptr(), w.group, _p(b),
+                               out.data_ptr(), ldy, M, w.N, w.K,
+                               C.byref(epilogue) if epilogue is not None else None, stream()))
+    return out
+
+
+class Kv4Cache:
+    """A key/value cache in 4 bits: `batch` sequences of up to max_rows rows, n_kv_heads heads of
+    head_dim (64 or 128) channels (kv4_cache makes one).  Which rows are in use is the
+    caller's to know."""
+
+    def __init__(self, data, batch, n_kv_heads, head_dim, max_rows):
+        self.data, self.batch, self.n_kv_heads = data, batch, n_kv_heads
+        self.head_dim, self.max_rows = head_dim, max_rows
+        self.width = n_kv_heads * head_dim
+        self._c = Kv4(data.data_ptr(), batch, n_kv_heads, head_dim, max_rows)
+        self._ref = C.byref(self._c)
+
+
+def kv4_cache(batch, n_kv_heads, max_rows, head_dim=64, device=None):
+    """An empty Kv4Cache on `device` (the current one)."""
+    n = lib.lx_kv4_bytes(batch, n_kv_heads, head_dim, max_rows)
+    if not n:
+        raise ValueError(f"kv4_cache: unsupported shape ({batch} sequences of {max_rows} rows, "
+                         f"{n_kv_heads} heads of {head_dim})")
+    data = torch.empty(n, device="cuda" if device is None else device, dtype=torch.uint8)
+    return Kv4Cache(data, batch, n_kv_heads, head_dim, max_rows)
+
+
+def _counts(t, name, batch):
+    if t.dtype != torch.int32 or t.numel() != batch or not t.is_contiguous():
+        raise ValueError(f"{name} must be {batch} contiguous int32 values")
+
+
+def kv4_append(cache, k, v, pos):
+    """Quantises rows k (roped), v (B, T, n_kv_heads * head_dim) into rows pos[b] .. pos[b] + T - 1
+    of sequence b (pos: device int32 (B); rows outside the cache are not written).
+    src/llm/llm.cpp:200-204."""
+    _on_device(cache=cache.data, k=k, v=v, pos=pos)
+    ldk, ldv = _rows(k, "k", 3, cache.width), _rows(v, "v", 3, cache.width)
+    T = k.shape[1]
+    if k.shape[0] != cache.batch or v.shape != k.shape:
+        raise ValueError(f"k and v must both be ({cache.batch}, T, {cache.width})")
+    _counts(pos, "pos", cache.batch)
+    check(lib.lx_kv4_append_f32(cache._ref, k.data_ptr(), ldk, v.data_ptr(), ldv, T,
+                                pos.data_ptr(), stream()))
+
+
+def kv4_read(cache, pos, T):
+    """(k, v), each (B, T, n_kv_heads * head_dim) fp32: what rows pos[b] .. pos[b] + T - 1 stand
+    for (rows outside the cache: zeros).  include/larynx/llm/llm.h:80-84."""
+    _on_device(cache=cache.data, pos=pos)
+    _counts(pos, "pos", cache.batch)
+    k = torch.empty(cache.batch, T, cache.width, device=cache.data.device, dtype=torch.float32)
+    v = torch.empty_like(k)
+    check(lib.lx_kv4_read_f32(cache._ref, k.data_ptr(), v.data_ptr(), T, pos.data_ptr(), stream()))
+    return k, v
+
+
+def attention_kv4(q, cache, lens, n_heads, scale=None, causal=True, out=None, max_len=0):
+    """softmax(scale q k~^T) v~ over the first lens[b] rows of each sequence of a Kv4Cache; q (B,
+    Tq, n_heads * head_dim), lens device int32 (B).  causal: query t stands at row lens[b] - Tq +
+    t.  A query that sees no row gives zeros.  max_len: the largest length expected (sizes
+    the launch only).  src/llm/ops.cpp:49-65."""
+    _on_device(q=q, cache=cache.data, lens=lens, out=out)
+    width = n_heads * cache.head_dim
+    ldq = _rows(q, "q", 3, width)
+    B, Tq = q.shape[0], q.shape[1]
+    if B != cache.batch:
+        raise ValueError(f"q must have {cache.batch} sequences")
+    _counts(lens, "lens", B)
+    if out is None:
+        out = torch.empty(B, Tq, width, device=q.device, dtype=torch.float32)
+        ldo = width
+    else:
+        if out.shape != q.shape:
+            raise ValueError("out must have q's shape")
+        ldo = _rows(out, "out", 3, width)
+    n = lib.lx_attention_kv4_ws_floats(cache._ref, Tq, n_heads, max_len)
+    ws = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
+    check(lib.lx_attention_kv4_f32(q.data_ptr(), ldq, cache._ref, lens.data_ptr(), out.data_ptr(),
+                                   ldo, Tq, n_heads,
+                                   cache.head_dim ** -0.5 if scale is None else scale,
+                                   int(causal), max_len, _p(ws), n, stream()))
+    return out
