@@ -379,23 +379,27 @@ int lx_q4_pack_f32(const float* W, void* Wq, int N, int K, int group, hipStream_
 int lx_q4_unpack_f32(const void* Wq, float* W, int N, int K, int group, hipStream_t stream);
 
 /* Projection of few rows on such a weight:  y = epi(x @ W~^T + bias), W~ what the
- * packed codes stand for, fp32 arithmetic (x as three bf16 parts, exact products
- * with the codes, fp32 sums; the scale applied to each group's sum).  x: (M, K),
+ * packed codes stand for, fp32 arithmetic (x as two fp16 parts after a power of two
+ * per row and 128 inputs, exact products with the codes, fp32 sums; the scale
+ * applied to each group's sum).  x: (M, K),
  * 1 <= M <= 64, row stride ldx; y: (M, N), row stride ldy (N / 2 columns for
  * SWIGLU_PAIRED, N even); y must not overlap x.  Epilogues: none, GELU_TANH, RESID,
  * SWIGLU_PAIRED (others: LX_ERR_ARG); bias (N) or NULL.  K and ldx multiples of
- * 4, x and Wq 16-byte aligned.  An infinite or NaN element of x, or one above
- * 3.3895e38 in magnitude, makes NaN of its row.  The result does not depend on
- * timing.  Replaces linear() (src/llm/ops.cpp:13-19) for weights given in 4 bits. */
+ * 4, x and Wq 16-byte aligned.  An infinite or NaN element of x makes NaN of its
+ * row.  The result does not depend on timing.  ws: lx_linear_q4_ws_floats() floats
+ * of scratch, 16-byte aligned (NULL when that is 0: up to 8 rows, and most calls of
+ * up to 16); calls that share it must not overlap.
+ * Replaces linear() (src/llm/ops.cpp:13-19) for weights given in 4 bits. */
+size_t lx_linear_q4_ws_floats(int M, int N, int K);
 int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int group, const float* bias,
-                     float* y, long ldy, int M, int N, int K, const lx_epilogue* epi,
-                     hipStream_t stream);
+                     float* y, long ldy, int M, int N, int K, const lx_epilogue* epi, float* ws,
+                     size_t ws_floats, hipStream_t stream);
 
 /* A key/value cache held in 4 bits (4.5 with its scales): `batch` sequences of up
  * to max_rows rows, n_kv_heads heads of head_dim (64 or 128) channels.  Keys and
  * values alike: the 64 channels of a group of a row share z = the largest bf16
  * not above their minimum and s = the smallest bf16 not below (max - z) / 15; a
- * code q = clamp(rint((x - z) / s), 0, 15) stands for z + s * q (s = 0: z).  A
+ * code q = clamp(rint((x - z) / s), 0, 15) stands for z + s * q (no range: z).  A
  * group that holds an infinity or a NaN, or whose |z| + 16 s passes fp32, stands
  * for NaN.  `data`: device memory of lx_kv4_bytes() bytes (0 for a bad
  * shape), 16-byte aligned, which needs no initialisation; rows that were never
@@ -432,7 +436,8 @@ int lx_kv4_read_f32(const lx_kv4* cache, float* k, float* v, int T, const int* p
  * gives zeros.  q, o: (batch, Tq, *), row strides ldq / ldo (multiples of 4,
  * sequences Tq rows apart), 16-byte aligned, head h at column h * hd; o must not
  * overlap q.  What unseen rows hold does not matter, NaN included; a NaN or an
- * infinity in a query makes NaN of its row and head.
+ * infinity in a query makes NaN of its row and head, and so may keys above 2^118 in
+ * magnitude (their sums are formed with the query scaled to 1 .. 2).
  * max_len: the largest length expected (0: max_rows).  It only sizes the launch:
  * the keys of one sequence are split over more workgroups when there are few, and
  * joined by a second launch; longer sequences are right too.  ws:

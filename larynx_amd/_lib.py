@@ -172,9 +172,10 @@ SIGNATURES = [
     ("lx_q4_bytes", C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     ("lx_q4_pack_f32", C.c_int, [fp, C.c_void_p, C.c_int, C.c_int, C.c_int, stream_t]),
     ("lx_q4_unpack_f32", C.c_int, [C.c_void_p, fp, C.c_int, C.c_int, C.c_int, stream_t]),
+    ("lx_linear_q4_ws_floats", C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     ("lx_linear_q4_f32", C.c_int,
      [fp, C.c_long, C.c_void_p, C.c_int, fp, fp, C.c_long, C.c_int, C.c_int, C.c_int,
-      C.POINTER(Epilogue), stream_t]),
+      C.POINTER(Epilogue), fp, C.c_size_t, stream_t]),
     ("lx_kv4_bytes", C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
     ("lx_kv4_append_f32", C.c_int,
      [C.POINTER(Kv4), fp, C.c_long, fp, C.c_long, C.c_int, ip, stream_t]),

@@ -1,63 +1,71 @@
 // Four-bit codes as MFMA operands (lx_q4.hip, lx_kv4.hip).
 //
-// A dword holds the eight codes of one lane's bf16 fragment (v_mfma_f32_16x16x32_bf16: lane l
-// holds row or column l % 16, k = (l / 16) * 8 .. + 7).  Code q becomes the bf16 number 16 + q,
-// whose four low bits of significance lie at bits 3..6 above the pattern of 16.0 (0x4180): the
-// codes of elements 2r and 2r + 1 are stored at bits 3 + 4r and 19 + 4r (mod 32), so one rotate
-// and one and-or make both halves of fragment register r, 7 instructions for eight codes.
-// (A signed bf16 number costs a subtraction that gfx950 has no packed bf16 form of.)  What the
-// codes stand for is affine in q, so the 16 goes into a constant of the group; it is at most
-// half of a code's magnitude, which costs under one bit of the fp32 sums.
+// A dword holds the eight codes of one lane's fp16 fragment (v_mfma_f32_16x16x32_f16: lane l
+// holds row or column l % 16, k = (l / 16) * 8 .. + 7), elements 2r and 2r + 1 at bits 4r and
+// 16 + 4r.  An and-or with the pattern of 1024.0 makes both halves of a fragment register 1024 + q
+// or 1024 + 16 q, a packed fp16 add or fma makes them q - 8, exactly: 9 instructions for eight
+// codes.  Signed codes keep the fp32 sums as small as the values they stand for; an offset left
+// in and taken off later (bf16 has no packed add: 7 instructions) cost a digit where values
+// average out, or twice the matrix instructions.
+//
+// The other operand is fp32 data as two fp16 parts, after a power of two of its own per row that
+// brings the largest value to 1 .. 2: x = x0 + x1 to within 2^-23 of x, or 2^-25 of the row's
+// largest where the second part runs out of fp16's range, fp32's own level.  (Larger numbers
+// would gain nothing and cost the sums' range.)
 #pragma once
 
 #include "lx_gemm_common.hpp"
 
 namespace lx {
 
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef unsigned short ushortx4_t __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ unsigned rotr32(unsigned w, int r) {
-  return __builtin_amdgcn_alignbit(w, w, r);
+__device__ __forceinline__ half8_t q4_frag(unsigned w) {
+  const half2_t off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+  const half2_t off16 = {(_Float16)-72.0f, (_Float16)-72.0f};
+  const half2_t r16 = {(_Float16)0.0625f, (_Float16)0.0625f};
+  const unsigned v = w >> 8;
+  half8_t f;
+  const half2_t h0 = __builtin_bit_cast(half2_t, (w & 0x000f000fu) | 0x64006400u) + off;
+  const half2_t h1 = __builtin_elementwise_fma(
+      __builtin_bit_cast(half2_t, (w & 0x00f000f0u) | 0x64006400u), r16, off16);
+  const half2_t h2 = __builtin_bit_cast(half2_t, (v & 0x000f000fu) | 0x64006400u) + off;
+  const half2_t h3 = __builtin_elementwise_fma(
+      __builtin_bit_cast(half2_t, (v & 0x00f000f0u) | 0x64006400u), r16, off16);
+  const uintx4_t u = {__builtin_bit_cast(unsigned, h0), __builtin_bit_cast(unsigned, h1),
+                      __builtin_bit_cast(unsigned, h2), __builtin_bit_cast(unsigned, h3)};
+  return __builtin_bit_cast(half8_t, u);
 }
 
-// The fragment of a dword: element j is 16 + code j.
-__device__ __forceinline__ sbf16x8 q4_frag(unsigned w) {
-  const uintx4_t f = {(w & 0x00780078u) | 0x41804180u, ((w >> 4) & 0x00780078u) | 0x41804180u,
-                      ((w >> 8) & 0x00780078u) | 0x41804180u,
-                      (rotr32(w, 12) & 0x00780078u) | 0x41804180u};
-  return __builtin_bit_cast(sbf16x8, f);
-}
-
-// Bit position of element j's code.
-__device__ __forceinline__ int q4_shift(int j) { return (3 + 4 * (j >> 1) + 16 * (j & 1)) & 31; }
-// Code q (< 16) at its bits in the dword (element 7's wrap around).
+// Code q (< 16) at element j's bits in the dword, and back.
 __device__ __forceinline__ unsigned q4_put(unsigned q, int j) {
-  const int s = q4_shift(j);
-  return s > 28 ? (q << s) | (q >> (32 - s)) : q << s;
+  return q << (4 * (j >> 1) + 16 * (j & 1));
 }
 __device__ __forceinline__ unsigned q4_get(unsigned w, int j) {
-  return rotr32(w, q4_shift(j)) & 15u;
+  return (w >> (4 * (j >> 1) + 16 * (j & 1))) & 15u;
 }
 
-// x as the sum of three bf16 numbers (exact for normal x: 24 significant bits); contraction
-// off, as in pack2_bf16.
-__device__ __forceinline__ void split3(const float (&x)[8], sbf16x8 (&p)[3]) {
+// x (scaled) as two fp16 parts; contraction off, as in pack2_bf16.
+__device__ __forceinline__ void split2(const float (&x)[8], half8_t& p0, half8_t& p1) {
 #pragma clang fp contract(off)
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    floatx4 v = {x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]};
+  for (int j = 0; j < 8; ++j) p0[j] = (_Float16)x[j];
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const bf16x4_t h = __builtin_convertvector(v, bf16x4_t);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) p[i][4 * e + j] = h[j];
-      if (i < 2) v = v - bf16x4_back(h);
-    }
-  }
+  for (int j = 0; j < 8; ++j) p1[j] = (_Float16)(x[j] - (float)p0[j]);
 }
 
-__device__ __forceinline__ floatx4 mfma_bf16(sbf16x8 a, sbf16x8 b, floatx4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+// The power of two that brings a row with largest magnitude `top` to 1 .. 2, and its inverse
+// (both normal numbers; an infinite top stays infinite).
+__device__ __forceinline__ float row_scale(float top, float* inverse) {
+  const unsigned e = min(max(__float_as_uint(top) >> 23 & 255u, 1u), 253u);
+  *inverse = __uint_as_float(e << 23);
+  return __uint_as_float((254u - e) << 23);
+}
+
+__device__ __forceinline__ floatx4 mfma_f16(half8_t a, half8_t b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
 // fp32 bits of the bf16 in the low or high half of a dword.

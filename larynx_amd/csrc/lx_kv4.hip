@@ -77,7 +77,12 @@ __device__ __forceinline__ unsigned quantise(float x, unsigned* pair) {
     *pair = 0x7fc07fc0u;
     return 0;
   }
-  *pair = __float_as_uint(a.s) >> 16 | (__float_as_uint(a.z) & 0xffff0000u);
+  // no range: every code is 0 whatever s is; 2^-40 of z keeps what the attention makes of the
+  // largest s from dwarfing z
+  unsigned s16 = __float_as_uint(a.s) >> 16;
+  const int ez = (int)(__float_as_uint(a.z) >> 23 & 255u);
+  if (a.s == 0.0f) s16 = (unsigned)max(ez - 40, 0) << 7;
+  *pair = s16 | (__float_as_uint(a.z) & 0xffff0000u);
   return affine_code(x, a);
 }
 
@@ -179,14 +184,55 @@ struct AttnArgs {
   float scale2;  // scale * log2(e)
 };
 
+// Channels chn .. chn + 3 of query row rr: O / L, zero where no key was seen (L = 0).
+__device__ __forceinline__ void store_row(const AttnArgs& a, int b, int h, int rr, int chn, int hd,
+                                          float4 O, float L) {
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  float* dst =
+      a.o + ((long)b * a.Tq + rr / a.rep) * a.ldo + (long)(h * a.rep + rr % a.rep) * hd + chn;
+  *reinterpret_cast<float4*>(dst) = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+}
+
 // Partial states in the workspace, per (sequence, kv head, query tile, split): 16 rows of hd
 // unnormalised outputs, then 16 maxima (in units of log2) and 16 sums.
 __host__ __device__ constexpr long part_floats(int ng) { return (long)kQ * (ng * kGrp + 2); }
 
+// log2 of what the weights carry for values whose largest scale is vtop: 6 - E, within what
+// sums of 2^20 weights leave of fp32's range.
+__device__ __forceinline__ float value_lift(float vtop) {
+  const int e = (int)(__float_as_uint(vtop) >> 23 & 255u) - 127;
+  return (float)(6 - max(e, -90));
+}
+
+// One record's operands: key and value codes, (s, z) pairs of the lane's keys 4 c + e and 16 +
+// 4 c + e.
+template <int NG>
+struct Rec {
+  uintx4_t kc[NG], vc[NG], kp[NG][2], vp[NG][2];
+  __device__ __forceinline__ void load(const char* rec, int lane, int c) {
+    const uintx4_t* pairs = reinterpret_cast<const uintx4_t*>(rec + 2 * NG * kCodes);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      kc[g] = reinterpret_cast<const uintx4_t*>(rec + g * kCodes)[lane];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) kp[g][i] = pairs[g * 8 + i * 4 + c];
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      vc[g] = reinterpret_cast<const uintx4_t*>(rec + (NG + g) * kCodes)[lane];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) vp[g][i] = pairs[(NG + g) * 8 + i * 4 + c];
+    }
+  }
+};
+
 // One workgroup of four waves per (sequence, kv head, tile of 16 query rows, split of the
 // keys); the waves take the split's records in turn, each with a running softmax of its own.
-// Scores are kept in units of log2 (q carries scale * log2 e), transposed: lane l holds query
-// row l % 16.
+// Scores are transposed: lane l holds query row l % 16.  Codes count from their middle, x~ =
+// (z + 8 s) + s (q - 8).  q carries scale * log2 e and the power of two that its two fp16 parts
+// want (S' = S / f, f a constant of the row).  The weights p s of the values want one too: every
+// p carries 2^lg, lg = 6 - E with E the largest exponent of s so far, so that p s stays below 2^7.
+// It is a running reference like the maximum, and part of the same exponent.
 template <int NG>
 __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
   constexpr int HD = NG * kGrp;
@@ -211,27 +257,39 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
   const int per = (nblk + a.splits - 1) / a.splits;
   const int b0 = sp * per, b1 = min(b0 + per, nblk);
 
-  sbf16x8 qf[NG][2][3];
-  float qsum[NG];
+  half8_t qf[NG][2][2];
+  float qsum[NG], f;
   {
     const float* q = a.q + ((long)b * a.Tq + t) * a.ldq + (long)(h * a.rep + hr) * HD + c * 8;
+    float x[NG][2][8], top = 0.0f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float4 u = *reinterpret_cast<const float4*>(q + g * kGrp + ks * 32 + 4 * e);
+          x[g][ks][4 * e] = u.x * a.scale2;
+          x[g][ks][4 * e + 1] = u.y * a.scale2;
+          x[g][ks][4 * e + 2] = u.z * a.scale2;
+          x[g][ks][4 * e + 3] = u.w * a.scale2;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[g][ks][4 * e + j]));
+        }
+    top = fmaxf(top, lane_xor16(top));
+    top = fmaxf(top, lane_xor32(top));
+    const float sc = row_scale(top, &f);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       float s = 0.0f;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        float x[8];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float4 u = *reinterpret_cast<const float4*>(q + g * kGrp + ks * 32 + 4 * e);
-          x[4 * e] = u.x * a.scale2;
-          x[4 * e + 1] = u.y * a.scale2;
-          x[4 * e + 2] = u.z * a.scale2;
-          x[4 * e + 3] = u.w * a.scale2;
+        for (int j = 0; j < 8; ++j) {
+          x[g][ks][j] *= sc;
+          s += x[g][ks][j];
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s += x[j];
-        split3(x, qf[g][ks]);
+        split2(x[g][ks], qf[g][ks][0], qf[g][ks][1]);
       }
       s += lane_xor16(s);
       s += lane_xor32(s);
@@ -246,37 +304,26 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
 #pragma unroll
     for (int ct = 0; ct < 4; ++ct) o[g][ct] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
-  float m = -INFINITY, l = 0.0f;
-  for (int blk = b0 + wave; blk < b1; blk += 4) {
-    const char* rec = a.c.data + a.c.record(b, h, blk);
-    uintx4_t kc[NG], vc[NG], kp[NG][2], vp[NG][2];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      kc[g] = reinterpret_cast<const uintx4_t*>(rec + g * kCodes)[lane];
-      vc[g] = reinterpret_cast<const uintx4_t*>(rec + (NG + g) * kCodes)[lane];
-      const uintx4_t* pairs = reinterpret_cast<const uintx4_t*>(rec + 2 * NG * kCodes);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        kp[g][i] = pairs[g * 8 + i * 4 + c];
-        vp[g][i] = pairs[(NG + g) * 8 + i * 4 + c];
-      }
-    }
+  // m: the largest S' so far; vtop: the largest s of a value so far; l, zsum and o carry 2^lg
+  float m = -INFINITY, l = 0.0f, vtop = 0.0f, lg = value_lift(0.0f);
+  const size_t rstride = (size_t)NG * kRec;
+  const char* recs = a.c.data + a.c.record(b, h, 0);
+
+  auto step = [&](Rec<NG>& r, int blk) {
     float s[8];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
+        const half8_t k0 = q4_frag(r.kc[g][i * 2]), k1 = q4_frag(r.kc[g][i * 2 + 1]);
         floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          const sbf16x8 kf = q4_frag(kc[g][i * 2 + ks]);
-#pragma unroll
-          for (int p = 2; p >= 0; --p) acc = mfma_bf16(kf, qf[g][ks][p], acc);
-        }
+        for (int p = 1; p >= 0; --p)
+          acc = mfma_f16(k1, qf[g][1][p], mfma_f16(k0, qf[g][0][p], acc));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float ss = bf16_lo(kp[g][i][e]), z = bf16_hi(kp[g][i][e]);
-          const float v = fmaf(ss, acc[e], fmaf(-16.0f, ss, z) * qsum[g]);
+          const float ss = bf16_lo(r.kp[g][i][e]), z = bf16_hi(r.kp[g][i][e]);
+          const float v = fmaf(ss, acc[e], fmaf(8.0f, ss, z) * qsum[g]);
           s[i * 4 + e] = g == 0 ? v : s[i * 4 + e] + v;
         }
       }
@@ -289,18 +336,27 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
         if (blk * kBlk + 16 * (j >> 2) + 4 * c + (j & 3) >= limit) {
           s[j] = -INFINITY;
 #pragma unroll
-          for (int g = 0; g < NG; ++g) vp[g][j >> 2][j & 3] = 0;
+          for (int g = 0; g < NG; ++g) r.vp[g][j >> 2][j & 3] = 0;
         }
     }
-    float mx = s[0];
+    float mx = s[0], vx = vtop;
 #pragma unroll
     for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[j]);
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vx = fmaxf(vx, bf16_lo(r.vp[g][j >> 2][j & 3]));
     mx = fmaxf(mx, lane_xor16(mx));
     mx = fmaxf(mx, lane_xor32(mx));
-    if (__any(mx > m)) {
-      const float mn = fmaxf(m, mx);
-      const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+    vx = fmaxf(vx, lane_xor16(vx));
+    vx = fmaxf(vx, lane_xor32(vx));
+    if (__any(mx > m || vx > vtop)) {
+      // the sums so far move to the new maximum and the new lift
+      const float mn = fmaxf(m, mx), lgn = value_lift(vx);
+      const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m - mn, f, lgn - lg));
       m = mn;
+      vtop = vx;
+      lg = lgn;
       l *= al;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -309,12 +365,13 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
         for (int ct = 0; ct < 4; ++ct) o[g][ct] *= al;
       }
     }
-    // a row that has seen no key yet: every weight exp2(-inf - 0) = 0
+    // a row that has seen no key yet: every weight exp2(-inf) = 0.  The difference comes first,
+    // so that no weight passes 2^lg however large the scores
     const float ref = m == -INFINITY ? 0.0f : m;
     float p[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      p[j] = __builtin_amdgcn_exp2f(s[j] - ref);
+      p[j] = __builtin_amdgcn_exp2f(fmaf(s[j] - ref, f, lg));
       l += p[j];
     }
 #pragma unroll
@@ -322,21 +379,33 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
       float ps[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float ss = bf16_lo(vp[g][j >> 2][j & 3]), z = bf16_hi(vp[g][j >> 2][j & 3]);
+        const float ss = bf16_lo(r.vp[g][j >> 2][j & 3]), z = bf16_hi(r.vp[g][j >> 2][j & 3]);
         ps[j] = p[j] * ss;
-        zsum[g] = fmaf(p[j], fmaf(-16.0f, ss, z), zsum[g]);
+        zsum[g] = fmaf(p[j], fmaf(8.0f, ss, z), zsum[g]);
       }
-      sbf16x8 pf[3];
-      split3(ps, pf);
+      half8_t p0, p1;
+      split2(ps, p0, p1);
 #pragma unroll
       for (int ct = 0; ct < 4; ++ct) {
-        const sbf16x8 vf = q4_frag(vc[g][ct]);
-#pragma unroll
-        for (int i = 2; i >= 0; --i) o[g][ct] = mfma_bf16(vf, pf[i], o[g][ct]);
+        const half8_t vf = q4_frag(r.vc[g][ct]);
+        o[g][ct] = mfma_f16(vf, p0, mfma_f16(vf, p1, o[g][ct]));
       }
     }
+  };
+  // the next record's loads are under way while one is worked on
+  if (b0 + wave < b1) {
+    Rec<NG> r0, r1;
+    r0.load(recs + (b0 + wave) * rstride, lane, c);
+    for (int blk = b0 + wave; blk < b1; blk += 8) {
+      r1.load(recs + min(blk + 4, b1 - 1) * rstride, lane, c);
+      step(r0, blk);
+      if (blk + 4 >= b1) break;
+      r0.load(recs + min(blk + 8, b1 - 1) * rstride, lane, c);
+      step(r1, blk + 4);
+    }
   }
-  // the lane's sums over its keys -> the row's
+  // the lane's sums over its keys -> the row's, without the lift
+  const float drop = __builtin_amdgcn_exp2f(-lg);
   l += lane_xor16(l);
   l += lane_xor32(l);
 #pragma unroll
@@ -344,21 +413,23 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
     zsum[g] += lane_xor16(zsum[g]);
     zsum[g] += lane_xor32(zsum[g]);
 #pragma unroll
-    for (int ct = 0; ct < 4; ++ct)
+    for (int ct = 0; ct < 4; ++ct) {
+      floatx4 v = o[g][ct] + floatx4{zsum[g], zsum[g], zsum[g], zsum[g]};
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        om[wave][col][g * kGrp + ct * 16 + 4 * c + e] = o[g][ct][e] + zsum[g];
+      for (int e = 0; e < 4; ++e) v[e] *= drop;
+      *reinterpret_cast<floatx4*>(&om[wave][col][g * kGrp + ct * 16 + 4 * c]) = v;
+    }
   }
   if (c == 0) {
-    ml[wave][0][col] = m;
-    ml[wave][1][col] = l;
+    ml[wave][0][col] = m * f;
+    ml[wave][1][col] = l * drop;
   }
   __syncthreads();
   // the four waves' states, joined in wave order
   float* part = a.ws + (((long)bh * a.tiles + qt) * a.splits + sp) * part_floats(NG);
   for (int i = tid; i < kQ * (HD / 4); i += 256) {
-    const int r = i / (HD / 4), ch = i % (HD / 4) * 4, rr = qt * kQ + r;
-    if (rr >= nrow) continue;
+    const int r = i / (HD / 4), chn = i % (HD / 4) * 4, rr = qt * kQ + r;
+    if (rr >= nrow) break;
     float M = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w][0][r]);
@@ -369,20 +440,17 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
       const float mw = ml[w][0][r];
       const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
       L += f * ml[w][1][r];
-      const float4 u = *reinterpret_cast<const float4*>(&om[w][r][ch]);
+      const float4 u = *reinterpret_cast<const float4*>(&om[w][r][chn]);
       O.x += f * u.x;
       O.y += f * u.y;
       O.z += f * u.z;
       O.w += f * u.w;
     }
     if (a.splits == 1) {
-      const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-      float* dst = a.o + ((long)b * a.Tq + rr / a.rep) * a.ldo +
-                   (long)(h * a.rep + rr % a.rep) * HD + ch;
-      *reinterpret_cast<float4*>(dst) = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+      store_row(a, b, h, rr, chn, HD, O, L);
     } else {
-      *reinterpret_cast<float4*>(part + r * HD + ch) = O;
-      if (ch == 0) {
+      *reinterpret_cast<float4*>(part + r * HD + chn) = O;
+      if (chn == 0) {
         part[kQ * HD + r] = M;
         part[kQ * HD + kQ + r] = L;
       }
@@ -390,46 +458,64 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
   }
 }
 
-// The splits' states of a row, joined in split order: one thread per four channels of a row.
+// The splits' states of a row joined: one workgroup a row, HD / 4 lanes of four channels, the
+// other lanes' groups taking every kG-th split; the groups' states are joined in group order, so
+// the result does not depend on timing.
 template <int NG>
 __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a) {
-  constexpr int HD = NG * kGrp;
+  constexpr int HD = NG * kGrp, L4 = HD / 4, kG = 256 / L4;
+  __shared__ float om[kG][HD + 4];
+  __shared__ float ml[2][kG];
   const int nrow = a.Tq * a.rep;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const int ch = (int)(i % (HD / 4)) * 4;
-  const long rg = i / (HD / 4);  // (sequence, kv head) * nrow + row
-  if (rg >= (long)a.c.batch * a.c.heads * nrow) return;
-  const int rr = (int)(rg % nrow);
-  const long bh = rg / nrow;
-  const int b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads);
+  const int chn = (int)(threadIdx.x % L4) * 4, gr = (int)(threadIdx.x / L4);
+  const int rr = (int)(blockIdx.x % nrow);
+  const long bh = blockIdx.x / nrow;
+  const int b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads), r = rr % kQ;
   const float* p = a.ws + (bh * a.tiles + rr / kQ) * a.splits * part_floats(NG);
-  const int r = rr % kQ;
-  float M = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, p[s * part_floats(NG) + kQ * HD + r]);
-  float L = 0.0f;
+  float M = -INFINITY, L = 0.0f;
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < a.splits; ++s) {
+#pragma unroll 2
+  for (int s = gr; s < a.splits; s += kG) {
     const float* ps = p + s * part_floats(NG);
-    const float ms = ps[kQ * HD + r];
-    if (ms == -INFINITY) continue;
-    const float f = __builtin_amdgcn_exp2f(ms - M);
-    L += f * ps[kQ * HD + kQ + r];
-    const float4 u = *reinterpret_cast<const float4*>(ps + r * HD + ch);
+    const float ms = ps[kQ * HD + r], ls = ps[kQ * HD + kQ + r];
+    const float4 u = *reinterpret_cast<const float4*>(ps + r * HD + chn);
+    const float mn = fmaxf(M, ms), ref = mn == -INFINITY ? 0.0f : mn;
+    const float fo = __builtin_amdgcn_exp2f(M - ref), fn = __builtin_amdgcn_exp2f(ms - ref);
+    M = mn;
+    L = fo * L + fn * ls;
+    O = make_float4(fo * O.x + fn * u.x, fo * O.y + fn * u.y, fo * O.z + fn * u.z,
+                    fo * O.w + fn * u.w);
+  }
+  *reinterpret_cast<float4*>(&om[gr][chn]) = O;
+  if (chn == 0) {
+    ml[0][gr] = M;
+    ml[1][gr] = L;
+  }
+  __syncthreads();
+  if (gr) return;
+  M = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < kG; ++g) M = fmaxf(M, ml[0][g]);
+  const float ref = M == -INFINITY ? 0.0f : M;
+  L = 0.0f;
+  O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int g = 0; g < kG; ++g) {
+    const float f = __builtin_amdgcn_exp2f(ml[0][g] - ref);
+    const float4 u = *reinterpret_cast<const float4*>(&om[g][chn]);
+    L += f * ml[1][g];
     O.x += f * u.x;
     O.y += f * u.y;
     O.z += f * u.z;
     O.w += f * u.w;
   }
-  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-  float* dst = a.o + ((long)b * a.Tq + rr / a.rep) * a.ldo + (long)(h * a.rep + rr % a.rep) * HD +
-               ch;
-  *reinterpret_cast<float4*>(dst) = make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
+  store_row(a, b, h, rr, chn, HD, O, L);
 }
 
-// Splits of the keys: about two workgroups per CU, at least four records (one a wave) each.
+// Splits of the keys: about four workgroups per CU, at least four records (one a wave) each.
 int kv4_splits(long wgs, int max_len) {
   const int blocks = (max_len + kBlk - 1) / kBlk;
-  const long want = 2L * device_cus() / std::max(wgs, 1L);
+  const long want = 4L * device_cus() / std::max(wgs, 1L);
   return (int)std::max(1L, std::min<long>(want, (blocks + 3) / 4));
 }
 
@@ -552,8 +638,7 @@ extern "C" int lx_attention_kv4_f32(const float* q, long ldq, const lx_kv4* cach
     hipLaunchKernelGGL(kv4_attn_kernel<2>, grid, dim3(256), 0, stream, a);
   LX_TRY(check_launch("kv4_attn_kernel"));
   if (a.splits > 1) {
-    const long n = (long)a.c.batch * a.c.heads * Tq * a.rep * (cache->head_dim / 4);
-    const dim3 jg((unsigned)((n + 255) / 256));
+    const dim3 jg((unsigned)((long)a.c.batch * a.c.heads * Tq * a.rep));
     if (a.c.ng == 1)
       hipLaunchKernelGGL(kv4_join_kernel<1>, jg, dim3(256), 0, stream, a);
     else

@@ -3,10 +3,9 @@
 //   w~[n, k] = s[n, k / G] * (q[n, k] - 8),  y = epi(x w~^T + bias),  G = 32, 64 or 128.
 //
 // What bounds it is the weight stream (half a byte a weight), so the codes go from memory to
-// the matrix cores with seven instructions for eight of them (lx_four_bit.hpp) and the scale is
-// applied once per group to the fp32 sum, not to the weights: a group's products with 16 + q
-// start from -24 times the sum of its x, and the sum times s joins the row's total.  x enters
-// as three bf16 parts, so every product is exact and the sums are fp32.
+// the matrix cores with nine instructions for eight of them (lx_four_bit.hpp) and the scale is
+// applied once per group to the fp32 sum, not to the weights.  x enters as two fp16 parts after a
+// power of two per row and block of 128 inputs, so every product is exact.
 //
 // Layout (lx_q4_pack_f32): per tile of 16 rows and block of 128 inputs 1 KB of codes, the 64
 // lanes' 16-byte fragments (dword t of lane l: row l % 16, k = 32 t + 8 (l / 16) + 0..7), then
@@ -24,7 +23,6 @@ namespace {
 constexpr int kTileN = 16;    // rows of a tile
 constexpr int kBlockK = 128;  // inputs of a block
 constexpr int kMaxRows = 64;
-constexpr int kPackedCols = 5;  // rows of x whose three parts fit one fragment's 16 columns
 
 struct Q4Args {
   const float* x;
@@ -35,6 +33,8 @@ struct Q4Args {
   float* y;
   long ldy;
   int M, N, K, kb, epi;
+  int splits;
+  float* ws;
 };
 
 __host__ __device__ inline long q4_tiles(int N) { return (N + kTileN - 1) / kTileN; }
@@ -137,140 +137,409 @@ __global__ __launch_bounds__(256) void q4_unpack_kernel(const unsigned* __restri
 
 // ---- the product ------------------------------------------------------------------------
 
-// A workgroup owns one tile of 16 weight rows against all M rows of x; its waves take the
-// blocks of K in turn and their sums meet in LDS, in wave order.  PC: at most 5 rows of x,
-// whose three parts are columns 3 m + part of one fragment (one product per 32 inputs); else
-// CT column tiles of 16 rows, three products each.
-template <int CT, bool PC, int G>
-__global__ __launch_bounds__(1024) void q4_linear_kernel(Q4Args a) {
-  constexpr int TG = G / 32, NG = 4 / TG, NP = PC ? 1 : 3;
-  extern __shared__ float red[];  // [waves][CT * 4][64]
+// bias and residual of output (m, n) [SwiGLU: of the pair n, n + 1], and the epilogue.
+struct Q4EpiIn {
+  float b0, b1, y;
+};
+__device__ __forceinline__ Q4EpiIn q4_epi_load(const Q4Args& a, int m, long n) {
+  Q4EpiIn in = {0.0f, 0.0f, 0.0f};
+  if (a.bias) {
+    in.b0 = a.bias[n];
+    if (a.epi == LX_EPI_SWIGLU_PAIRED) in.b1 = a.bias[n + 1];
+  }
+  if (a.epi == LX_EPI_RESID) in.y = a.y[m * a.ldy + n];
+  return in;
+}
+__device__ __forceinline__ void q4_epi_store(const Q4Args& a, int m, long n, float v, float v1,
+                                             const Q4EpiIn& in) {
+  v += in.b0;
+  if (a.epi == LX_EPI_SWIGLU_PAIRED) {
+    a.y[m * a.ldy + (n >> 1)] = (v / (1.0f + expf(-v))) * (v1 + in.b1);
+    return;
+  }
+  a.y[m * a.ldy + n] = a.epi == LX_EPI_GELU_TANH ? gelu_tanh(v)
+                       : a.epi == LX_EPI_RESID   ? in.y + v
+                                                 : v;
+}
+
+// At most MB rows of x.  A workgroup owns one tile of 16 weight rows; its waves take the blocks
+// of K in turn, each splitting its own 128 inputs of x into a slice of LDS, and their sums meet
+// in LDS at the end (in a fixed order).  MB <= 8: column 2 m + part of one fragment; MB = 16:
+// column m of two.
+constexpr int kFewRow = 272;  // bytes of a staged row (128 fp16, and 16 against bank conflicts)
+
+template <int MB>
+constexpr int few_bytes() {
+  constexpr int b = 2 * MB * kFewRow;
+  return b < 1024 ? 1024 : b;
+}
+
+template <int MB, int G>
+struct FewIn {
+  static constexpr int NG = kBlockK / G;
+  uintx4_t w;
+  ushortx4_t sc[NG];
+  float2 x[MB];
+  __device__ __forceinline__ void load(const Q4Args& a, long rt, int kb, int lane) {
+    const long tile = rt * a.kb + kb;
+    w = a.codes[tile * 64 + lane];
+    const ushortx4_t* sp =
+        reinterpret_cast<const ushortx4_t*>(a.scales) + (tile * 4 + (lane >> 4)) * NG;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) sc[g] = sp[g];
+    const int k = min(kb * kBlockK + 2 * lane, a.K - 2);
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+      x[m] = *reinterpret_cast<const float2*>(a.x + (long)min(m, a.M - 1) * a.ldx + k);
+  }
+};
+
+template <int MB, int G>
+__global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
+  constexpr int TG = G / 32, NG = kBlockK / G;
+  constexpr bool PK = MB <= 8;
+  constexpr int NP = PK ? 1 : 2;
+  extern __shared__ __attribute__((aligned(16))) char lds[];  // [waves][few_bytes]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
   const int c = lane >> 4, col = lane & 15;
   const long rt = blockIdx.x;
-  const float* xr[CT];
-  bool live[CT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int m = PC ? col / 3 : ct * 16 + col;
-    live[ct] = m < a.M && (!PC || col < 15);
-    xr[ct] = a.x + (long)min(m, a.M - 1) * a.ldx;
+  char* mine = lds + wave * few_bytes<MB>();
+  const int rows = a.epi == LX_EPI_SWIGLU_PAIRED ? kTileN / 2 : kTileN;
+  const int nout = rows * a.M, step = a.epi == LX_EPI_SWIGLU_PAIRED ? 2 : 1;
+  // four threads an output in the end; what its epilogue reads is requested first
+  Q4EpiIn pre = {0.0f, 0.0f, 0.0f};
+  {
+    const int i = tid >> 2, m = i / rows;
+    const long n = rt * kTileN + i % rows * step;
+    if (i < nout && n < a.N) pre = q4_epi_load(a, m, n);
   }
-  floatx4 tot[CT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) tot[ct] = floatx4{0.f, 0.f, 0.f, 0.f};
+  floatx4 tot = {0.f, 0.f, 0.f, 0.f};
+  FewIn<MB, G> in;
+  in.load(a, rt, wave, lane);
   for (int kb = wave; kb < a.kb; kb += waves) {
-    const long tile = rt * a.kb + kb;
-    const uintx4_t w = a.codes[tile * 64 + lane];
-    const ushortx4_t* sp =
-        reinterpret_cast<const ushortx4_t*>(a.scales) + (tile * 4 + c) * NG;
+    const bool past = kb * kBlockK + 2 * lane >= a.K;
+    float f = 0.0f;
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+      float2 x = in.x[m];
+      if (past) x = make_float2(0.f, 0.f);
+      float inv;
+      const float sc = row_scale(wave_max(fmaxf(fabsf(x.x), fabsf(x.y))), &inv);
+      f = (PK ? col >> 1 : col) == m ? inv : f;
+      x.x *= sc;
+      x.y *= sc;
+      const half2_t h = {(_Float16)x.x, (_Float16)x.y};
+      const half2_t l = {(_Float16)(x.x - (float)h[0]), (_Float16)(x.y - (float)h[1])};
+      half2_t* row = reinterpret_cast<half2_t*>(mine + 2 * m * kFewRow) + lane;
+      row[0] = h;
+      row[kFewRow / 4] = l;
+    }
+    const uintx4_t w = in.w;
     ushortx4_t sc[NG];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) sc[g] = sp[g];
+    for (int g = 0; g < NG; ++g) sc[g] = in.sc[g];
+    if (kb + waves < a.kb) in.load(a, rt, kb + waves, lane);
+    // the staged rows are this wave's own: in program order, no barrier
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const char* xr = mine + (PK ? min(col, 2 * MB - 1) : 2 * col) * kFewRow + c * 16;
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      sbf16x8 wf[TG];
+      floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int t = 0; t < TG; ++t) wf[t] = q4_frag(w[g * TG + t]);
+      for (int t = g * TG; t < (g + 1) * TG; ++t) {
+        const half8_t wf = q4_frag(w[t]);
+#pragma unroll
+        for (int p = NP - 1; p >= 0; --p)
+          acc = mfma_f16(wf, *reinterpret_cast<const half8_t*>(xr + p * kFewRow + t * 64), acc);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] = fmaf(bf16_lo(sc[g][i]), acc[i], sum[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tot[i] = fmaf(f, sum[i], tot[i]);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) reinterpret_cast<float*>(mine)[i * 64 + lane] = tot[i];
+  __syncthreads();
+  // row r of the tile against row m of x; thread q of four takes every fourth wave
+  const int q = tid & 3;
+  auto value = [&](int r, int m) {
+    float s = 0.0f;
+    for (int w = q; w < waves; w += 4) {
+      const float* p = reinterpret_cast<const float*>(lds + w * few_bytes<MB>()) + (r & 3) * 64 +
+                       (r >> 2) * 16;
+      s += PK ? p[2 * m + 1] + p[2 * m] : p[m];
+    }
+    s += dpp_mov<kDppXor1>(s);
+    s += dpp_mov<kDppXor2>(s);
+    return s;
+  };
+  for (int i = tid >> 2; i < nout; i += blockDim.x >> 2) {
+    const int m = i / rows, r = i % rows * step;
+    const long n = rt * kTileN + r;
+    const float v = value(r, m), v1 = step == 2 ? value(r + 1, m) : 0.0f;
+    if (q == 0 && n < a.N)
+      q4_epi_store(a, m, n, v, v1, i == tid >> 2 ? pre : q4_epi_load(a, m, n));
+  }
+}
+
+// 9 to 64 rows of x in CT column tiles of 16.  A workgroup of eight waves owns 8 RT tiles of
+// weight rows over one of a.splits ranges of the blocks of K.  x goes through LDS as fragments of
+// its two parts, a chunk of 8 / CT blocks at a time, each wave splitting the 16 rows x 128 inputs
+// of one (block, column tile); the next chunk's x is on its way meanwhile, and the weights
+// arrive one block ahead.  One split: the epilogue from the accumulators; more: partial sums into
+// ws (splits, M, N up to 16), which q4_join_kernel adds in split order.
+constexpr int kManyWaves = 8;
+
+template <int CT>
+constexpr int many_blocks() { return CT == 1 ? 8 : CT == 2 ? 4 : 2; }
+template <int CT>
+constexpr size_t many_bytes() {
+  return (size_t)many_blocks<CT>() * CT * (8 * 1024 + 64);
+}
+
+template <int CT, int RT, int G>
+__global__ __launch_bounds__(64 * kManyWaves) void q4_many_kernel(Q4Args a) {
+  constexpr int TG = G / 32, NG = kBlockK / G, CH = many_blocks<CT>();
+  // [block][step][column tile][part][lane] fragments, then [block][column tile][16] scales
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  half8_t* frag = reinterpret_cast<half8_t*>(lds);
+  float* inv = reinterpret_cast<float*>(lds + CH * CT * 8 * 1024);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int c = lane >> 4, col = lane & 15;
+  const int sp = blockIdx.x % a.splits;
+  const long rt0 = ((long)(blockIdx.x / a.splits) * kManyWaves + wave) * RT;
+  const long tiles = q4_tiles(a.N);
+  const int per = (a.kb + a.splits - 1) / a.splits;
+  const int k0 = sp * per, k1 = min(k0 + per, a.kb);
+  const int sb = wave / CT, sct = wave % CT;  // what this wave splits
+  float4 xs[4][2];
+  auto load_x = [&](int kb) {
+    const float* xr = a.x + (long)min(sct * 16 + col, a.M - 1) * a.ldx;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        xs[t][e] = *reinterpret_cast<const float4*>(
+            xr + min(kb * kBlockK + 32 * t + 8 * c + 4 * e, a.K - 4));
+  };
+  auto store_x = [&](int kb) {
+    float v[4][8], top = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const bool past = kb * kBlockK + 32 * t + 8 * c + 4 * e >= a.K;
+        v[t][4 * e] = past ? 0.0f : xs[t][e].x;
+        v[t][4 * e + 1] = past ? 0.0f : xs[t][e].y;
+        v[t][4 * e + 2] = past ? 0.0f : xs[t][e].z;
+        v[t][4 * e + 3] = past ? 0.0f : xs[t][e].w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(v[t][4 * e + j]));
+      }
+    top = fmaxf(top, lane_xor16(top));
+    top = fmaxf(top, lane_xor32(top));
+    float f;
+    const float sc = row_scale(top, &f);
+    if (c == 0) inv[(sb * CT + sct) * 16 + col] = f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[t][j] *= sc;
+      half8_t p0, p1;
+      split2(v[t], p0, p1);
+      half8_t* dst = frag + (((sb * 4 + t) * CT + sct) * 2) * 64 + lane;
+      dst[0] = p0;
+      dst[64] = p1;
+    }
+  };
+  uintx4_t w[RT], wn[RT];
+  ushortx4_t sc[RT][NG], scn[RT][NG];
+  auto load_w = [&](int kb) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const long tile = min(rt0 + r, tiles - 1) * a.kb + kb;
+      wn[r] = a.codes[tile * 64 + lane];
+      const ushortx4_t* p = reinterpret_cast<const ushortx4_t*>(a.scales) + (tile * 4 + c) * NG;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) scn[r][g] = p[g];
+    }
+  };
+  floatx4 tot[RT][CT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) tot[r][ct] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const bool stages = sb < CH;
+  if (k0 < k1) load_w(k0);
+  if (stages && k0 + sb < k1) load_x(k0 + sb);
+  for (int kc = k0; kc < k1; kc += CH) {
+    if (kc > k0) __syncthreads();  // the last chunk has been read
+    if (stages && kc + sb < k1) store_x(kc + sb);
+    __syncthreads();
+    if (stages && kc + CH + sb < k1) load_x(kc + CH + sb);
+    const int nb = min(CH, k1 - kc);
+    for (int i = 0; i < nb; ++i) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        w[r] = wn[r];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) sc[r][g] = scn[r][g];
+      }
+      if (kc + i + 1 < k1) load_w(kc + i + 1);
+      const half8_t* fb = frag + i * 4 * CT * 128 + lane;
+      floatx4 sum[RT][CT];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        floatx4 acc[RT][CT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) acc[r][ct] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = g * TG; t < (g + 1) * TG; ++t) {
+          half8_t wf[RT];
+#pragma unroll
+          for (int r = 0; r < RT; ++r) wf[r] = q4_frag(w[r][t]);
+#pragma unroll
+          for (int p = 1; p >= 0; --p)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+              const half8_t xf = fb[((t * CT + ct) * 2 + p) * 64];
+#pragma unroll
+              for (int r = 0; r < RT; ++r) acc[r][ct] = mfma_f16(wf[r], xf, acc[r][ct]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              sum[r][ct][e] = g == 0 ? bf16_lo(sc[r][g][e]) * acc[r][ct][e]
+                                     : fmaf(bf16_lo(sc[r][g][e]), acc[r][ct][e], sum[r][ct][e]);
+      }
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        sbf16x8 xf[TG][NP];
-        float sum = 0.0f;
+        const float f = inv[(i * CT + ct) * 16 + col];
 #pragma unroll
-        for (int t = 0; t < TG; ++t) {
-          const int k = kb * kBlockK + (g * TG + t) * 32 + c * 8;
-          float v[8];
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float4 u = live[ct] && k + 4 * e < a.K
-                                 ? *reinterpret_cast<const float4*>(xr[ct] + k + 4 * e)
-                                 : make_float4(0.f, 0.f, 0.f, 0.f);
-            v[4 * e] = u.x;
-            v[4 * e + 1] = u.y;
-            v[4 * e + 2] = u.z;
-            v[4 * e + 3] = u.w;
-          }
-          sbf16x8 p[3];
-          split3(v, p);
-          if constexpr (PC) {
-            const int part = col % 3;
-            xf[t][0] = part == 0 ? p[0] : part == 1 ? p[1] : p[2];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum += (float)xf[t][0][j];
-          } else {
-#pragma unroll
-            for (int i = 0; i < 3; ++i) xf[t][i] = p[i];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum += v[j];
-          }
-        }
-        sum += lane_xor16(sum);
-        sum += lane_xor32(sum);
-        const float c0 = -24.0f * sum;
-        floatx4 acc = {c0, c0, c0, c0};
-#pragma unroll
-        for (int t = 0; t < TG; ++t)
-#pragma unroll
-          for (int i = NP - 1; i >= 0; --i) acc = mfma_bf16(wf[t], xf[t][i], acc);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tot[ct][i] += bf16_lo(sc[g][i]) * acc[i];
+          for (int e = 0; e < 4; ++e) tot[r][ct][e] = fmaf(f, sum[r][ct][e], tot[r][ct][e]);
       }
     }
   }
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct)
+  for (int r = 0; r < RT; ++r) {
+    const long n = (rt0 + r) * kTileN + 4 * c;
+    if (rt0 + r >= tiles) break;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) red[((wave * CT + ct) * 4 + i) * 64 + lane] = tot[ct][i];
-  __syncthreads();
-  // value of row r of the tile against row m of x
-  auto value = [&](int r, int m) {
-    float s = 0.0f;
-    for (int w = 0; w < waves; ++w) {
-      const float* p = red + (w * CT * 4 + (r & 3)) * 64 + (r >> 2) * 16;
-      if constexpr (PC) {
-        s += (p[3 * m + 2] + p[3 * m + 1]) + p[3 * m];
+    for (int ct = 0; ct < CT; ++ct) {
+      const int m = ct * 16 + col;
+      if (m >= a.M) continue;
+      if (a.splits > 1) {
+        *reinterpret_cast<floatx4*>(a.ws + ((long)sp * a.M + m) * (tiles * kTileN) + n) =
+            tot[r][ct];
+        continue;
+      }
+      if (a.epi == LX_EPI_SWIGLU_PAIRED) {
+#pragma unroll
+        for (int e = 0; e < 4; e += 2)
+          if (n + e < a.N)
+            q4_epi_store(a, m, n + e, tot[r][ct][e], tot[r][ct][e + 1], q4_epi_load(a, m, n + e));
       } else {
-        s += p[(m >> 4) * 256 + (m & 15)];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < a.N)
+            q4_epi_store(a, m, n + e, tot[r][ct][e], 0.0f, q4_epi_load(a, m, n + e));
       }
-    }
-    return s;
-  };
-  const int rows = a.epi == LX_EPI_SWIGLU_PAIRED ? kTileN / 2 : kTileN;
-  for (int i = tid; i < rows * a.M; i += blockDim.x) {
-    const int m = i / rows, r = i % rows;
-    if (a.epi == LX_EPI_SWIGLU_PAIRED) {
-      const long n = rt * kTileN + 2 * r;
-      if (n >= a.N) continue;
-      float g = value(2 * r, m), u = value(2 * r + 1, m);
-      if (a.bias) {
-        g += a.bias[n];
-        u += a.bias[n + 1];
-      }
-      a.y[m * a.ldy + (n >> 1)] = (g / (1.0f + expf(-g))) * u;
-    } else {
-      const long n = rt * kTileN + r;
-      if (n >= a.N) continue;
-      float v = value(r, m);
-      if (a.bias) v += a.bias[n];
-      float* y = a.y + m * a.ldy + n;
-      *y = a.epi == LX_EPI_GELU_TANH ? gelu_tanh(v) : a.epi == LX_EPI_RESID ? *y + v : v;
     }
   }
 }
 
-template <int CT, bool PC>
-int launch_linear(const Q4Args& a, int G, hipStream_t s) {
-  const int waves = std::min(PC || CT == 1 ? 16 : 8, a.kb);
-  const dim3 grid((unsigned)q4_tiles(a.N)), block(64 * waves);
-  const size_t lds = (size_t)waves * CT * 1024;
-  if (G == 32)
-    hipLaunchKernelGGL((q4_linear_kernel<CT, PC, 32>), grid, block, lds, s, a);
-  else if (G == 64)
-    hipLaunchKernelGGL((q4_linear_kernel<CT, PC, 64>), grid, block, lds, s, a);
-  else
-    hipLaunchKernelGGL((q4_linear_kernel<CT, PC, 128>), grid, block, lds, s, a);
-  return check_launch("q4_linear_kernel");
+// The splits' sums added in split order, and the epilogue: one thread per four rows of W.
+__global__ __launch_bounds__(256) void q4_join_kernel(Q4Args a) {
+  const long np4 = q4_tiles(a.N) * (kTileN / 4);
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= np4 * a.M) return;
+  const int m = (int)(i / np4);
+  const long n = i % np4 * 4;
+  const float* p = a.ws + ((long)m * np4) * 4 + n;
+  floatx4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int k = 0; k < a.splits; ++k)
+    s += *reinterpret_cast<const floatx4*>(p + (long)k * a.M * np4 * 4);
+  if (a.epi == LX_EPI_SWIGLU_PAIRED) {
+#pragma unroll
+    for (int e = 0; e < 4; e += 2)
+      if (n + e < a.N) q4_epi_store(a, m, n + e, s[e], s[e + 1], q4_epi_load(a, m, n + e));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < a.N) q4_epi_store(a, m, n + e, s[e], 0.0f, q4_epi_load(a, m, n + e));
+  }
 }
+
+#define LX_Q4_GROUPS(KERNEL, ...)                                        \
+  if (G == 32)                                                           \
+    hipLaunchKernelGGL((KERNEL<__VA_ARGS__, 32>), grid, block, lds, s, a);  \
+  else if (G == 64)                                                      \
+    hipLaunchKernelGGL((KERNEL<__VA_ARGS__, 64>), grid, block, lds, s, a);  \
+  else                                                                   \
+    hipLaunchKernelGGL((KERNEL<__VA_ARGS__, 128>), grid, block, lds, s, a);
+
+template <int MB>
+int launch_few(const Q4Args& a, int G, hipStream_t s) {
+  const int waves = std::min(std::min(16, a.kb), 64 * 1024 / few_bytes<MB>());
+  const dim3 grid((unsigned)q4_tiles(a.N)), block(64 * waves);
+  const size_t lds = (size_t)waves * few_bytes<MB>();
+  LX_Q4_GROUPS(q4_few_kernel, MB)
+  return check_launch("q4_few_kernel");
+}
+
+template <int CT, int RT, int G>
+int raise_many() {
+  static LdsLimit once;
+  return raise_lds_limit(reinterpret_cast<const void*>(q4_many_kernel<CT, RT, G>),
+                         many_bytes<CT>(), once, "q4_many_kernel");
+}
+
+// What q4_many_kernel runs with: tiles a wave and splits of K.
+struct ManyPlan {
+  int rt, splits;
+};
+ManyPlan many_plan(int M, int N, int K) {
+  const int cus = device_cus(), kb = (int)q4_blocks(K);
+  const long tiles = q4_tiles(N);
+  ManyPlan p;
+  // two tiles a wave share each fragment of x they read from LDS
+  p.rt = tiles > 8 * kManyWaves ? 2 : 1;
+  const long wgs = (tiles + kManyWaves * p.rt - 1) / (kManyWaves * p.rt);
+  p.splits = (int)std::max(1L, std::min<long>(kb, cus / wgs));
+  const int per = (kb + p.splits - 1) / p.splits;
+  p.splits = (kb + per - 1) / per;
+  return p;
+}
+
+template <int CT, int RT>
+int launch_many(const Q4Args& a, int G, hipStream_t s) {
+  LX_TRY(G == 32 ? (raise_many<CT, RT, 32>())
+                 : G == 64 ? (raise_many<CT, RT, 64>()) : (raise_many<CT, RT, 128>()));
+  const long wgs = (q4_tiles(a.N) + kManyWaves * RT - 1) / (kManyWaves * RT);
+  const dim3 grid((unsigned)(wgs * a.splits)), block(64 * kManyWaves);
+  const size_t lds = many_bytes<CT>();
+  LX_Q4_GROUPS(q4_many_kernel, CT, RT)
+  return check_launch("q4_many_kernel");
+}
+#undef LX_Q4_GROUPS
+
+// Rows of x that run on q4_few_kernel.
+bool q4_takes_few(int M, int N) { return M <= 8 || (M <= 16 && q4_tiles(N) <= 1024); }
 
 bool q4_shape_ok(int N, int K, int group) {
   return N > 0 && K > 0 && K % 4 == 0 && (group == 32 || group == 64 || group == 128) &&
@@ -323,9 +592,16 @@ extern "C" int lx_q4_unpack_f32(const void* Wq, float* W, int N, int K, int grou
   return check_launch("q4_unpack_kernel");
 }
 
+extern "C" size_t lx_linear_q4_ws_floats(int M, int N, int K) {
+  if (M < 1 || M > kMaxRows || !q4_shape_ok(N, K, 64) || q4_takes_few(M, N)) return 0;
+  const ManyPlan p = many_plan(M, N, K);
+  return p.splits == 1 ? 0 : (size_t)p.splits * M * q4_tiles(N) * kTileN;
+}
+
 extern "C" int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int group,
                                 const float* bias, float* y, long ldy, int M, int N, int K,
-                                const lx_epilogue* epi, hipStream_t stream) {
+                                const lx_epilogue* epi, float* ws, size_t ws_floats,
+                                hipStream_t stream) {
   LX_REQUIRE(x && Wq && y, "linear_q4: null pointer");
   LX_REQUIRE(q4_shape_ok(N, K, group), "linear_q4: bad shape N=%d K=%d group=%d", N, K, group);
   LX_REQUIRE(M >= 1 && M <= kMaxRows, "linear_q4: %d rows outside [1, %d]", M, kMaxRows);
@@ -353,11 +629,34 @@ extern "C" int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int gr
   a.K = K;
   a.kb = (int)q4_blocks(K);
   a.epi = kind;
-  if (M <= kPackedCols) return launch_linear<1, true>(a, group, stream);
-  switch ((M + 15) / 16) {
-    case 1: return launch_linear<1, false>(a, group, stream);
-    case 2: return launch_linear<2, false>(a, group, stream);
-    case 3: return launch_linear<3, false>(a, group, stream);
-    default: return launch_linear<4, false>(a, group, stream);
+  a.splits = 1;
+  if (q4_takes_few(M, N)) {
+    if (M == 1) return launch_few<1>(a, group, stream);
+    if (M == 2) return launch_few<2>(a, group, stream);
+    if (M <= 4) return launch_few<4>(a, group, stream);
+    if (M <= 8) return launch_few<8>(a, group, stream);
+    return launch_few<16>(a, group, stream);
   }
+  const ManyPlan p = many_plan(M, N, K);
+  a.splits = p.splits;
+  if (p.splits > 1) {
+    const size_t need = (size_t)p.splits * M * q4_tiles(N) * kTileN;
+    LX_REQUIRE(ws && ws_floats >= need && (uintptr_t)ws % 16 == 0,
+               "linear_q4: workspace of %zu floats, %zu needed", ws ? ws_floats : 0, need);
+    a.ws = ws;
+  }
+  switch ((M + 15) / 16 * 2 + p.rt) {
+    case 3: LX_TRY((launch_many<1, 1>(a, group, stream))); break;
+    case 4: LX_TRY((launch_many<1, 2>(a, group, stream))); break;
+    case 5: LX_TRY((launch_many<2, 1>(a, group, stream))); break;
+    case 6: LX_TRY((launch_many<2, 2>(a, group, stream))); break;
+    case 7: LX_TRY((launch_many<3, 1>(a, group, stream))); break;
+    case 8: LX_TRY((launch_many<3, 2>(a, group, stream))); break;
+    case 9: LX_TRY((launch_many<4, 1>(a, group, stream))); break;
+    default: LX_TRY((launch_many<4, 2>(a, group, stream))); break;
+  }
+  if (p.splits == 1) return LX_OK;
+  const long n = q4_tiles(N) * (kTileN / 4) * M;
+  hipLaunchKernelGGL(q4_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
+  return check_launch("q4_join_kernel");
 }

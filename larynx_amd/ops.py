@@ -407,9 +407,12 @@ def linear_q4(x, w, b=None, epilogue=None, out=None):
         if out.dim() != 2 or out.shape[0] != M:
             raise ValueError(f"out must have {M} rows")
         ldy = _rows(out, "out", 2, cols)
+    n = 0 if M <= 8 else lib.lx_linear_q4_ws_floats(M, w.N, w.K)
+    ws = torch.empty(n, device=x.device, dtype=torch.float32) if n else None
     check(lib.lx_linear_q4_f32(x.data_ptr(), ldx, w.data.data_ptr(), w.group, _p(b),
                                out.data_ptr(), ldy, M, w.N, w.K,
-                               C.byref(epilogue) if epilogue is not None else None, stream()))
+                               C.byref(epilogue) if epilogue is not None else None, _p(ws), n,
+                               stream()))
     return out
 
 

@@ -38,9 +38,10 @@ def test_pack_refusals():
         assert lib.lx_q4_unpack_f32(*args, None) == LX_ERR_ARG, args
 
 
-def _linear(x=P, ldx=64, w=P, group=64, bias=None, y=P, ldy=32, M=1, N=32, K=64, kind=None):
+def _linear(x=P, ldx=64, w=P, group=64, bias=None, y=P, ldy=32, M=1, N=32, K=64, kind=None,
+            ws=None, n=0):
     epi = None if kind is None else C.byref(Epilogue(kind=kind))
-    return lib.lx_linear_q4_f32(x, ldx, w, group, bias, y, ldy, M, N, K, epi, None)
+    return lib.lx_linear_q4_f32(x, ldx, w, group, bias, y, ldy, M, N, K, epi, ws, n, None)
 
 
 @pytest.mark.parametrize("kw", [
@@ -53,6 +54,17 @@ def _linear(x=P, ldx=64, w=P, group=64, bias=None, y=P, ldy=32, M=1, N=32, K=64,
 def test_linear_refusals(kw):
     assert _linear(**kw) == LX_ERR_ARG
     assert b"linear_q4" in lib.lx_last_error()
+
+
+def test_linear_workspace():
+    assert lib.lx_linear_q4_ws_floats(1, 896, 4864) == lib.lx_linear_q4_ws_floats(8, 896, 896) == 0
+    for bad in [(0, 896, 896), (65, 896, 896), (17, 0, 896), (17, 896, 6)]:
+        assert lib.lx_linear_q4_ws_floats(*bad) == 0
+    need = lib.lx_linear_q4_ws_floats(64, 1000, 8192)
+    assert need and need % (64 * 1008) == 0
+    for ws, n in [(None, need), (P, need - 1), (P + 4, need)]:
+        assert _linear(M=64, N=1000, K=8192, ldx=8192, ldy=1000, ws=ws, n=n) == LX_ERR_ARG
+        assert b"workspace" in lib.lx_last_error()
 
 
 def _cache(data=P, batch=2, heads=2, hd=64, rows=100):
