@@ -22,18 +22,26 @@ typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef unsigned short ushortx4_t __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ half8_t q4_frag(unsigned w) {
+// The pattern of 1024.0 in both halves, in a vector register: as a constant known to the compiler
+// it becomes a literal, and a literal each for mask and pattern makes two instructions of one.
+__device__ __forceinline__ unsigned q4_pattern() {
+  unsigned m;
+  asm("v_mov_b32 %0, 0x64006400" : "=v"(m));
+  return m;
+}
+
+__device__ __forceinline__ half8_t q4_frag(unsigned w, unsigned pattern) {
   const half2_t off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
   const half2_t off16 = {(_Float16)-72.0f, (_Float16)-72.0f};
   const half2_t r16 = {(_Float16)0.0625f, (_Float16)0.0625f};
   const unsigned v = w >> 8;
   half8_t f;
-  const half2_t h0 = __builtin_bit_cast(half2_t, (w & 0x000f000fu) | 0x64006400u) + off;
+  const half2_t h0 = __builtin_bit_cast(half2_t, (w & 0x000f000fu) | pattern) + off;
   const half2_t h1 = __builtin_elementwise_fma(
-      __builtin_bit_cast(half2_t, (w & 0x00f000f0u) | 0x64006400u), r16, off16);
-  const half2_t h2 = __builtin_bit_cast(half2_t, (v & 0x000f000fu) | 0x64006400u) + off;
+      __builtin_bit_cast(half2_t, (w & 0x00f000f0u) | pattern), r16, off16);
+  const half2_t h2 = __builtin_bit_cast(half2_t, (v & 0x000f000fu) | pattern) + off;
   const half2_t h3 = __builtin_elementwise_fma(
-      __builtin_bit_cast(half2_t, (v & 0x00f000f0u) | 0x64006400u), r16, off16);
+      __builtin_bit_cast(half2_t, (v & 0x00f000f0u) | pattern), r16, off16);
   const uintx4_t u = {__builtin_bit_cast(unsigned, h0), __builtin_bit_cast(unsigned, h1),
                       __builtin_bit_cast(unsigned, h2), __builtin_bit_cast(unsigned, h3)};
   return __builtin_bit_cast(half8_t, u);

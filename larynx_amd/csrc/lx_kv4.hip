@@ -170,7 +170,9 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(ReadArgs a) {
 
 // ---- attention --------------------------------------------------------------------------
 
-constexpr int kQ = 16;  // query rows of a tile: (t, head of the group) pairs, t-major
+constexpr int kMaxWaves = 8;    // of an attention workgroup
+constexpr int kMaxSplits = 64;  // of a sequence's keys
+constexpr int kQ = 16;  // columns of a tile: query rows, (t, head of the group) pairs, t-major
 
 struct AttnArgs {
   Kv4 c;
@@ -180,9 +182,33 @@ struct AttnArgs {
   float* o;
   long ldo;
   float* ws;
-  int Tq, rep, tiles, splits, causal;
+  int Tq, rep, tiles, trows, kp, splits, chunk, causal;
   float scale2;  // scale * log2(e)
 };
+
+// The keys of a tile of query rows, in steps of kp records: split sp takes steps [sp * per, sp *
+// per + per) of n_step.  A split is a.chunk steps long, so that the workgroups of sequences of
+// all lengths have the same work, and longer only where a sequence passes the length the
+// launch was sized for.
+struct Span {
+  int most, least;  // the longest and the shortest run of keys a row of the tile sees
+  int n_blk, n_step, per;
+};
+__device__ __forceinline__ Span attn_span(const AttnArgs& a, int len, int qt, int nrow) {
+  Span s;
+  s.most = s.least = len;
+  if (a.causal && a.Tq > 1) {
+    const int t_first = qt * a.trows / a.rep;
+    const int t_last = min(qt * a.trows + a.trows - 1, nrow - 1) / a.rep;
+    s.most = max(len - a.Tq + t_last + 1, 0);
+    s.least = max(len - a.Tq + t_first + 1, 0);
+  }
+  s.n_blk = (s.most + kBlk - 1) / kBlk;
+  s.n_step = (s.n_blk + a.kp - 1) / a.kp;
+  s.per = a.chunk;
+  if (s.n_step > a.chunk * a.splits) s.per = (s.n_step + a.splits - 1) / a.splits;
+  return s;
+}
 
 // Channels chn .. chn + 3 of query row rr: O / L, zero where no key was seen (L = 0).
 __device__ __forceinline__ void store_row(const AttnArgs& a, int b, int h, int rr, int chn, int hd,
@@ -204,63 +230,90 @@ __device__ __forceinline__ float value_lift(float vtop) {
   return (float)(6 - max(e, -90));
 }
 
-// One record's operands: key and value codes, (s, z) pairs of the lane's keys 4 c + e and 16 +
-// 4 c + e.
-template <int NG>
-struct Rec {
-  uintx4_t kc[NG], vc[NG], kp[NG][2], vp[NG][2];
-  __device__ __forceinline__ void load(const char* rec, int lane, int c) {
-    const uintx4_t* pairs = reinterpret_cast<const uintx4_t*>(rec + 2 * NG * kCodes);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      kc[g] = reinterpret_cast<const uintx4_t*>(rec + g * kCodes)[lane];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) kp[g][i] = pairs[g * 8 + i * 4 + c];
-    }
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      vc[g] = reinterpret_cast<const uintx4_t*>(rec + (NG + g) * kCodes)[lane];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) vp[g][i] = pairs[(NG + g) * 8 + i * 4 + c];
-    }
+// One workgroup of up to kMaxWaves waves per (sequence, kv head, tile of query rows, split of the
+// keys).  A tile has 16 / KP query rows, the columns of the matrix instructions; with KP > 1 (few
+// query rows: single tokens) the rows stand KP times side by side and a step takes KP records, the
+// i-th set of columns the softmax of the i-th record, so that no lane works on a row that is not
+// there.  The waves take the steps in turn, each column with a running softmax of its own.
+// Scores are transposed: lane l holds column l % 16.  Codes count from their middle, x~ = (z + 8
+// s) + s (q - 8).  q carries scale * log2 e and the power of two that its two fp16 parts want (S'
+// = S / f, f a constant of the row).  The weights p s of the values want one too: every p carries
+// 2^lg, lg = 6 - E with E the largest exponent of s so far, so that p s stays below 2^7.  It is a
+// running reference like the maximum, and part of the same exponent.
+// A spilled register costs more than a wave gains: the registers follow from NG and KP.
+template <int NG, int KP>
+__global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
+    amdgpu_waves_per_eu(NG == 2 ? 2 : KP == 4 ? 3 : 4))) void kv4_attn_kernel(AttnArgs a) {
+  constexpr int HD = NG * kGrp, R = kQ / KP;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  float (*om)[kQ][HD + 4] = reinterpret_cast<float (*)[kQ][HD + 4]>(lds);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+  float (*ml)[2][kQ] =
+      reinterpret_cast<float (*)[2][kQ]>(lds + (size_t)waves * kQ * (HD + 4) * sizeof(float));
+  const int col = lane & 15, c = lane >> 4, set = col / R;
+  const unsigned pattern = q4_pattern();
+  const int h = blockIdx.y, b = blockIdx.z;
+  int sp = blockIdx.x, qt = 0;
+  if (KP == 1 && a.tiles > 1) {
+    qt = sp / a.splits;
+    sp -= qt * a.splits;
   }
-};
-
-// One workgroup of four waves per (sequence, kv head, tile of 16 query rows, split of the
-// keys); the waves take the split's records in turn, each with a running softmax of its own.
-// Scores are transposed: lane l holds query row l % 16.  Codes count from their middle, x~ =
-// (z + 8 s) + s (q - 8).  q carries scale * log2 e and the power of two that its two fp16 parts
-// want (S' = S / f, f a constant of the row).  The weights p s of the values want one too: every
-// p carries 2^lg, lg = 6 - E with E the largest exponent of s so far, so that p s stays below 2^7.
-// It is a running reference like the maximum, and part of the same exponent.
-template <int NG>
-__global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
-  constexpr int HD = NG * kGrp;
-  __shared__ float om[4][kQ][HD + 4];
-  __shared__ float ml[4][2][kQ];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int col = lane & 15, c = lane >> 4;
-  const int sp = blockIdx.x % a.splits;
-  const long rest = blockIdx.x / a.splits;
-  const int qt = (int)(rest % a.tiles);
-  const int bh = (int)(rest / a.tiles), b = bh / a.c.heads, h = bh % a.c.heads;
-  const int len = min(max(a.lens[b], 0), a.c.rows);
   const int nrow = a.Tq * a.rep;
-  const int row = qt * kQ + col;           // the lane's query row
-  const int t = min(row, nrow - 1) / a.rep, hr = min(row, nrow - 1) % a.rep;
-  // keys the row sees: [0, limit)
-  const int limit = row >= nrow ? 0 : a.causal ? max(len - a.Tq + t + 1, 0) : len;
-  const int t_last = min(qt * kQ + kQ - 1, nrow - 1) / a.rep, t_first = qt * kQ / a.rep;
-  const int most = a.causal ? max(len - a.Tq + t_last + 1, 0) : len;   // of any row of the tile
-  const int least = a.causal ? max(len - a.Tq + t_first + 1, 0) : len;
-  const int nblk = (most + kBlk - 1) / kBlk;
-  const int per = (nblk + a.splits - 1) / a.splits;
-  const int b0 = sp * per, b1 = min(b0 + per, nblk);
-
-  half8_t qf[NG][2][2];
-  float qsum[NG], f;
+  const int row = qt * R + col % R;        // the lane's query row
+  int t = 0, hr = min(row, nrow - 1);
+  if (a.Tq > 1) {
+    t = hr / a.rep;
+    hr -= t * a.rep;
+  }
+  // the query first: it is on its way while the length and the records arrive
+  float4 qx[NG][2][2];
   {
     const float* q = a.q + ((long)b * a.Tq + t) * a.ldq + (long)(h * a.rep + hr) * HD + c * 8;
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          qx[g][ks][e] = *reinterpret_cast<const float4*>(q + g * kGrp + ks * 32 + 4 * e);
+  }
+  const int len = min(max(a.lens[b], 0), a.c.rows);
+  const Span n = attn_span(a, len, qt, nrow);
+  const int s0 = sp * n.per, s1 = min(s0 + n.per, n.n_step);
+  if (sp > 0 && s0 >= s1) return;
+  // keys the row sees: [0, limit)
+  const int limit = row >= nrow ? 0 : a.causal ? max(len - a.Tq + t + 1, 0) : len;
+
+  const size_t rstride = (size_t)NG * kRec;
+  const char* recs = a.c.data + a.c.record(b, h, 0);
+  // a step's operands: the codes of KP records, and the (s, z) pairs of the lane's own one, keys 4
+  // c + e and 16 + 4 c + e.  Past the last record the last one stands in, masked by its index.
+  uintx4_t kc[KP][NG], vc[KP][NG], kp[NG][2], vp[NG][2];
+  auto load = [&](int st, int plane, uintx4_t (&codes)[KP][NG], uintx4_t (&pairs)[NG][2]) {
+    const char* own = recs + min(st * KP + set, n.n_blk - 1) * rstride;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+#pragma unroll
+      for (int r = 0; r < KP; ++r)
+        codes[r][g] = reinterpret_cast<const uintx4_t*>(
+            recs + min(st * KP + r, n.n_blk - 1) * rstride + (plane * NG + g) * kCodes)[lane];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        pairs[g][i] = reinterpret_cast<const uintx4_t*>(
+            own + 2 * NG * kCodes)[(plane * NG + g) * 8 + i * 4 + c];
+    }
+  };
+  if (s0 + wave < s1) {
+    load(s0 + wave, 0, kc, kp);
+    load(s0 + wave, 1, vc, vp);
+  }
+
+  // every wave splits the whole tile's query the same way; two groups of it would hold 32 registers,
+  // so with two they stay in LDS (wave 0's)
+  half8_t qf[NG][2][2];
+  half8_t* ql = reinterpret_cast<half8_t*>(ml + waves) + lane;
+  float qsum[NG], f;
+  {
     float x[NG][2][8], top = 0.0f;
 #pragma unroll
     for (int g = 0; g < NG; ++g)
@@ -268,7 +321,7 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
       for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float4 u = *reinterpret_cast<const float4*>(q + g * kGrp + ks * 32 + 4 * e);
+          const float4 u = qx[g][ks][e];
           x[g][ks][4 * e] = u.x * a.scale2;
           x[g][ks][4 * e + 1] = u.y * a.scale2;
           x[g][ks][4 * e + 2] = u.z * a.scale2;
@@ -290,11 +343,16 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
           s += x[g][ks][j];
         }
         split2(x[g][ks], qf[g][ks][0], qf[g][ks][1]);
+        if (NG == 2 && wave == 0) {
+          ql[(g * 4 + ks * 2) * 64] = qf[g][ks][0];
+          ql[(g * 4 + ks * 2 + 1) * 64] = qf[g][ks][1];
+        }
       }
       s += lane_xor16(s);
       s += lane_xor32(s);
       qsum[g] = s;
     }
+    if (NG == 2) __syncthreads();
   }
   floatx4 o[NG][4];
   float zsum[NG];
@@ -306,37 +364,49 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
   }
   // m: the largest S' so far; vtop: the largest s of a value so far; l, zsum and o carry 2^lg
   float m = -INFINITY, l = 0.0f, vtop = 0.0f, lg = value_lift(0.0f);
-  const size_t rstride = (size_t)NG * kRec;
-  const char* recs = a.c.data + a.c.record(b, h, 0);
 
-  auto step = [&](Rec<NG>& r, int blk) {
+  for (int st = s0 + wave; st < s1; st += waves) {
     float s[8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int g = 0; g < NG; ++g) {
+      if constexpr (NG == 2) {
+        asm volatile("" ::: "memory");  // read here, not ahead of the loop
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const half8_t k0 = q4_frag(r.kc[g][i * 2]), k1 = q4_frag(r.kc[g][i * 2 + 1]);
-        floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 4; ++i) qf[g][i >> 1][i & 1] = ql[(g * 4 + i) * 64];
+      }
 #pragma unroll
-        for (int p = 1; p >= 0; --p)
-          acc = mfma_f16(k1, qf[g][1][p], mfma_f16(k0, qf[g][0][p], acc));
+      for (int i = 0; i < 2; ++i) {
+        floatx4 dot = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < KP; ++r) {
+          const half8_t k0 = q4_frag(kc[r][g][i * 2], pattern);
+          const half8_t k1 = q4_frag(kc[r][g][i * 2 + 1], pattern);
+          floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int p = 1; p >= 0; --p)
+            acc = mfma_f16(k1, qf[g][1][p], mfma_f16(k0, qf[g][0][p], acc));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dot[e] = r == 0 || set == r ? acc[e] : dot[e];
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float ss = bf16_lo(r.kp[g][i][e]), z = bf16_hi(r.kp[g][i][e]);
-          const float v = fmaf(ss, acc[e], fmaf(8.0f, ss, z) * qsum[g]);
+          const float ss = bf16_lo(kp[g][i][e]), z = bf16_hi(kp[g][i][e]);
+          const float v = fmaf(ss, dot[e], fmaf(8.0f, ss, z) * qsum[g]);
           s[i * 4 + e] = g == 0 ? v : s[i * 4 + e] + v;
         }
       }
     }
-    if (blk * kBlk + kBlk > least) {
+    const bool more = st + waves < s1;
+    if (more) load(st + waves, 0, kc, kp);
+    if ((st + 1) * (KP * kBlk) > n.least) {
       // a key the row does not see may hold anything (NaN, rows never written): neither its
       // score nor its value takes part
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (blk * kBlk + 16 * (j >> 2) + 4 * c + (j & 3) >= limit) {
+        if ((st * KP + set) * kBlk + 16 * (j >> 2) + 4 * c + (j & 3) >= limit) {
           s[j] = -INFINITY;
 #pragma unroll
-          for (int g = 0; g < NG; ++g) r.vp[g][j >> 2][j & 3] = 0;
+          for (int g = 0; g < NG; ++g) vp[g][j >> 2][j & 3] = 0;
         }
     }
     float mx = s[0], vx = vtop;
@@ -345,7 +415,7 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) vx = fmaxf(vx, bf16_lo(r.vp[g][j >> 2][j & 3]));
+      for (int j = 0; j < 8; ++j) vx = fmaxf(vx, bf16_lo(vp[g][j >> 2][j & 3]));
     mx = fmaxf(mx, lane_xor16(mx));
     mx = fmaxf(mx, lane_xor32(mx));
     vx = fmaxf(vx, lane_xor16(vx));
@@ -379,32 +449,27 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
       float ps[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float ss = bf16_lo(r.vp[g][j >> 2][j & 3]), z = bf16_hi(r.vp[g][j >> 2][j & 3]);
+        const float ss = bf16_lo(vp[g][j >> 2][j & 3]), z = bf16_hi(vp[g][j >> 2][j & 3]);
         ps[j] = p[j] * ss;
         zsum[g] = fmaf(p[j], fmaf(8.0f, ss, z), zsum[g]);
       }
       half8_t p0, p1;
       split2(ps, p0, p1);
 #pragma unroll
-      for (int ct = 0; ct < 4; ++ct) {
-        const half8_t vf = q4_frag(r.vc[g][ct]);
-        o[g][ct] = mfma_f16(vf, p0, mfma_f16(vf, p1, o[g][ct]));
+      for (int r = 0; r < KP; ++r) {
+        // the weights of this record's columns alone: the others' belong to other values
+        const half8_t none = {};
+        const half8_t r0 = KP == 1 || set == r ? p0 : none, r1 = KP == 1 || set == r ? p1 : none;
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct) {
+          const half8_t vf = q4_frag(vc[r][g][ct], pattern);
+          o[g][ct] = mfma_f16(vf, r0, mfma_f16(vf, r1, o[g][ct]));
+        }
       }
     }
-  };
-  // the next record's loads are under way while one is worked on
-  if (b0 + wave < b1) {
-    Rec<NG> r0, r1;
-    r0.load(recs + (b0 + wave) * rstride, lane, c);
-    for (int blk = b0 + wave; blk < b1; blk += 8) {
-      r1.load(recs + min(blk + 4, b1 - 1) * rstride, lane, c);
-      step(r0, blk);
-      if (blk + 4 >= b1) break;
-      r0.load(recs + min(blk + 8, b1 - 1) * rstride, lane, c);
-      step(r1, blk + 4);
-    }
+    if (more) load(st + waves, 1, vc, vp);
   }
-  // the lane's sums over its keys -> the row's, without the lift
+  // the lane's sums over its keys -> the column's, without the lift
   const float drop = __builtin_amdgcn_exp2f(-lg);
   l += lane_xor16(l);
   l += lane_xor32(l);
@@ -425,27 +490,39 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(AttnArgs a) {
     ml[wave][1][col] = l * drop;
   }
   __syncthreads();
-  // the four waves' states, joined in wave order
-  float* part = a.ws + (((long)bh * a.tiles + qt) * a.splits + sp) * part_floats(NG);
-  for (int i = tid; i < kQ * (HD / 4); i += 256) {
-    const int r = i / (HD / 4), chn = i % (HD / 4) * 4, rr = qt * kQ + r;
+  // the states of the waves and column sets joined, four threads an output taking every fourth,
+  // in a fixed order
+  float* part =
+      a.ws + ((((long)b * a.c.heads + h) * a.tiles + qt) * a.splits + sp) * part_floats(NG);
+  const int qd = tid & 3;
+  for (int i = tid >> 2; i < R * (HD / 4); i += blockDim.x >> 2) {
+    const int r = i / (HD / 4), chn = i % (HD / 4) * 4, rr = qt * R + r;
     if (rr >= nrow) break;
     float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w][0][r]);
+    for (int e = qd; e < waves * KP; e += 4) M = fmaxf(M, ml[e / KP][0][e % KP * R + r]);
+    M = fmaxf(M, dpp_mov<kDppXor1>(M));
+    M = fmaxf(M, dpp_mov<kDppXor2>(M));
+    const float ref = M == -INFINITY ? 0.0f : M;
     float L = 0.0f;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float mw = ml[w][0][r];
-      const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
-      L += f * ml[w][1][r];
-      const float4 u = *reinterpret_cast<const float4*>(&om[w][r][chn]);
-      O.x += f * u.x;
-      O.y += f * u.y;
-      O.z += f * u.z;
-      O.w += f * u.w;
+#pragma unroll 2
+    for (int e = qd; e < waves * KP; e += 4) {
+      const int w = e / KP, k = e % KP * R + r;
+      const float fw = __builtin_amdgcn_exp2f(ml[w][0][k] - ref);
+      const float4 u = *reinterpret_cast<const float4*>(&om[w][k][chn]);
+      L += fw * ml[w][1][k];
+      O.x += fw * u.x;
+      O.y += fw * u.y;
+      O.z += fw * u.z;
+      O.w += fw * u.w;
     }
+    auto quad = [](float x) {
+      x += dpp_mov<kDppXor1>(x);
+      return x + dpp_mov<kDppXor2>(x);
+    };
+    L = quad(L);
+    O = make_float4(quad(O.x), quad(O.y), quad(O.z), quad(O.w));
+    if (qd) continue;
     if (a.splits == 1) {
       store_row(a, b, h, rr, chn, HD, O, L);
     } else {
@@ -466,25 +543,44 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a) {
   constexpr int HD = NG * kGrp, L4 = HD / 4, kG = 256 / L4;
   __shared__ float om[kG][HD + 4];
   __shared__ float ml[2][kG];
-  const int nrow = a.Tq * a.rep;
   const int chn = (int)(threadIdx.x % L4) * 4, gr = (int)(threadIdx.x / L4);
-  const int rr = (int)(blockIdx.x % nrow);
-  const long bh = blockIdx.x / nrow;
-  const int b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads), r = rr % kQ;
-  const float* p = a.ws + (bh * a.tiles + rr / kQ) * a.splits * part_floats(NG);
+  const int rr = blockIdx.x, h = blockIdx.y, b = blockIdx.z, nrow = a.Tq * a.rep;
+  const int qt = rr / a.trows, r = rr - qt * a.trows;
+  const Span n = attn_span(a, min(max(a.lens[b], 0), a.c.rows), qt, nrow);
+  const int count = max((n.n_step + n.per - 1) / n.per, 1);
+  const float* p =
+      a.ws + (((long)b * a.c.heads + h) * a.tiles + qt) * a.splits * part_floats(NG);
   float M = -INFINITY, L = 0.0f;
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-  for (int s = gr; s < a.splits; s += kG) {
-    const float* ps = p + s * part_floats(NG);
-    const float ms = ps[kQ * HD + r], ls = ps[kQ * HD + kQ + r];
-    const float4 u = *reinterpret_cast<const float4*>(ps + r * HD + chn);
-    const float mn = fmaxf(M, ms), ref = mn == -INFINITY ? 0.0f : mn;
-    const float fo = __builtin_amdgcn_exp2f(M - ref), fn = __builtin_amdgcn_exp2f(ms - ref);
-    M = mn;
-    L = fo * L + fn * ls;
-    O = make_float4(fo * O.x + fn * u.x, fo * O.y + fn * u.y, fo * O.z + fn * u.z,
-                    fo * O.w + fn * u.w);
+  // every state of a group requested before the first is used
+  constexpr int U = kMaxSplits / kG;
+  float ms[U], ls[U];
+  float4 u[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const float* ps = p + min(gr + i * kG, count - 1) * part_floats(NG);
+    ms[i] = ps[kQ * HD + r];
+    ls[i] = ps[kQ * HD + kQ + r];
+    u[i] = *reinterpret_cast<const float4*>(ps + r * HD + chn);
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    if (gr + i * kG >= count) {  // no such state
+      ms[i] = -INFINITY;
+      ls[i] = 0.0f;
+      u[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    M = fmaxf(M, ms[i]);
+  }
+  const float base = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const float f = __builtin_amdgcn_exp2f(ms[i] - base);
+    L += f * ls[i];
+    O.x += f * u[i].x;
+    O.y += f * u[i].y;
+    O.z += f * u[i].z;
+    O.w += f * u[i].w;
   }
   *reinterpret_cast<float4*>(&om[gr][chn]) = O;
   if (chn == 0) {
@@ -512,16 +608,57 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a) {
   store_row(a, b, h, rr, chn, HD, O, L);
 }
 
-// Splits of the keys: about four workgroups per CU, at least four records (one a wave) each.
-int kv4_splits(long wgs, int max_len) {
-  const int blocks = (max_len + kBlk - 1) / kBlk;
-  const long want = 4L * device_cus() / std::max(wgs, 1L);
-  return (int)std::max(1L, std::min<long>(want, (blocks + 3) / 4));
+// How a call runs: records side by side, tiles of query rows, waves a workgroup, splits of the
+// keys and steps of one.
+struct AttnPlan {
+  int kp, tiles, waves, splits, chunk;
+};
+
+AttnPlan attn_plan(const Kv4& c, int nrow, int max_len) {
+  AttnPlan p;
+  p.kp = nrow <= 4 ? 4 : nrow <= 8 ? 2 : 1;
+  p.tiles = (nrow + kQ / p.kp - 1) / (kQ / p.kp);
+  const int cus = device_cus(), len = max_len <= 0 || max_len > c.rows ? c.rows : max_len;
+  const long wgs = (long)p.tiles * c.batch * c.heads;
+  const int steps = (len + kBlk * p.kp - 1) / (kBlk * p.kp);
+  // Splits take four waves, one per SIMD; the time in steps of a wave is workgroups a CU x steps
+  // a wave, and about five for the join's launch.
+  constexpr int kWaves = 4;
+  constexpr long kJoin = 5;
+  long best = LONG_MAX;
+  p.splits = 1;
+  for (int s = 1; s <= std::min(steps, kMaxSplits); ++s) {
+    const long t = (wgs * s + cus - 1) / cus * ((steps + kWaves * s - 1) / (kWaves * s)) +
+                   (s > 1 ? kJoin : 0);
+    if (t < best) {
+      best = t;
+      p.splits = s;
+    }
+  }
+  p.chunk = (steps + p.splits - 1) / p.splits;
+  p.splits = (steps + p.chunk - 1) / p.chunk;
+  p.waves = p.splits > 1 ? kWaves : kMaxWaves;
+  while (p.waves > 1 && p.waves / 2 >= p.chunk) p.waves /= 2;
+  return p;
+}
+
+template <int NG, int KP>
+int launch_attn(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
+  // states, and the query's fragments with two groups
+  constexpr size_t kState = kQ * (NG * kGrp + 6) * sizeof(float), kQuery = NG == 2 ? 8192 : 0;
+  const size_t lds = p.waves * kState + kQuery;
+  static LdsLimit once;
+  LX_TRY(raise_lds_limit(reinterpret_cast<const void*>(kv4_attn_kernel<NG, KP>),
+                         kMaxWaves * kState + kQuery, once, "kv4_attn_kernel"));
+  hipLaunchKernelGGL((kv4_attn_kernel<NG, KP>),
+                     dim3((unsigned)(p.tiles * p.splits), a.c.heads, a.c.batch),
+                     dim3(64 * p.waves), lds, s, a);
+  return check_launch("kv4_attn_kernel");
 }
 
 bool kv4_shape_ok(int batch, int heads, int hd, int rows) {
-  return batch > 0 && heads > 0 && (hd == 64 || hd == 128) && rows > 0 &&
-         (long)batch * heads < INT_MAX && rows <= INT_MAX - kBlk;
+  return batch > 0 && batch <= 65535 && heads > 0 && heads <= 65535 && (hd == 64 || hd == 128) &&
+         rows > 0 && rows <= INT_MAX - kBlk;
 }
 
 int kv4_view(const lx_kv4* c, const char* what, Kv4* out) {
@@ -587,13 +724,11 @@ extern "C" size_t lx_attention_kv4_ws_floats(const lx_kv4* cache, int Tq, int n_
                                              int max_len) {
   Kv4 c;
   if (kv4_view(cache, "attention_kv4_ws_floats", &c) != LX_OK || Tq <= 0 || n_heads <= 0 ||
-      n_heads % c.heads)
+      n_heads % c.heads || (long)Tq * (n_heads / c.heads) > INT_MAX - kQ)
     return 0;
-  const long tiles = ((long)Tq * (n_heads / c.heads) + kQ - 1) / kQ;
-  const long wgs = tiles * c.batch * c.heads;
-  const int len = max_len <= 0 || max_len > c.rows ? c.rows : max_len;
-  const int splits = kv4_splits(wgs, len);
-  return splits == 1 ? 0 : (size_t)wgs * splits * part_floats(c.ng);
+  const AttnPlan p = attn_plan(c, Tq * (n_heads / c.heads), max_len);
+  return p.splits == 1 ? 0
+                       : (size_t)p.tiles * c.batch * c.heads * p.splits * part_floats(c.ng);
 }
 
 extern "C" int lx_attention_kv4_f32(const float* q, long ldq, const lx_kv4* cache, const int* lens,
@@ -610,7 +745,8 @@ extern "C" int lx_attention_kv4_f32(const float* q, long ldq, const lx_kv4* cach
              ldq, ldo);
   LX_REQUIRE(((uintptr_t)q | (uintptr_t)o) % 16 == 0, "attention_kv4: q and o must be 16-byte "
              "aligned");
-  LX_REQUIRE((long)Tq * n_heads / a.c.heads <= INT_MAX - kQ, "attention_kv4: Tq=%d too long", Tq);
+  LX_REQUIRE((long)Tq * (n_heads / a.c.heads) <= INT_MAX - kQ, "attention_kv4: Tq=%d too long",
+             Tq);
   a.q = q;
   a.ldq = ldq;
   a.lens = lens;
@@ -618,32 +754,35 @@ extern "C" int lx_attention_kv4_f32(const float* q, long ldq, const lx_kv4* cach
   a.ldo = ldo;
   a.Tq = Tq;
   a.rep = n_heads / a.c.heads;
-  a.tiles = (Tq * a.rep + kQ - 1) / kQ;
   a.causal = causal != 0;
   a.scale2 = scale * 1.4426950408889634f;
-  const long wgs = (long)a.tiles * a.c.batch * a.c.heads;
-  const int len = max_len <= 0 || max_len > a.c.rows ? a.c.rows : max_len;
-  a.splits = kv4_splits(wgs, len);
-  if (a.splits > 1) {
-    const size_t need = (size_t)wgs * a.splits * part_floats(a.c.ng);
+  const AttnPlan p = attn_plan(a.c, Tq * a.rep, max_len);
+  a.tiles = p.tiles;
+  a.trows = kQ / p.kp;
+  a.kp = p.kp;
+  a.splits = p.splits;
+  a.chunk = p.chunk;
+  const long wgs = (long)p.tiles * a.c.batch * a.c.heads;
+  LX_REQUIRE((long)p.tiles * p.splits <= INT_MAX, "attention_kv4: Tq=%d too long", Tq);
+  if (p.splits > 1) {
+    const size_t need = (size_t)wgs * p.splits * part_floats(a.c.ng);
     LX_REQUIRE(ws && ws_floats >= need && (uintptr_t)ws % 16 == 0,
                "attention_kv4: workspace of %zu floats, %zu needed", ws ? ws_floats : 0, need);
     a.ws = ws;
   }
-  LX_REQUIRE(wgs * a.splits <= INT_MAX, "attention_kv4: %ld workgroups", wgs * a.splits);
-  const dim3 grid((unsigned)(wgs * a.splits));
   if (a.c.ng == 1)
-    hipLaunchKernelGGL(kv4_attn_kernel<1>, grid, dim3(256), 0, stream, a);
+    LX_TRY(p.kp == 4   ? (launch_attn<1, 4>(a, p, stream))
+           : p.kp == 2 ? (launch_attn<1, 2>(a, p, stream))
+                       : (launch_attn<1, 1>(a, p, stream)));
   else
-    hipLaunchKernelGGL(kv4_attn_kernel<2>, grid, dim3(256), 0, stream, a);
-  LX_TRY(check_launch("kv4_attn_kernel"));
-  if (a.splits > 1) {
-    const dim3 jg((unsigned)((long)a.c.batch * a.c.heads * Tq * a.rep));
-    if (a.c.ng == 1)
-      hipLaunchKernelGGL(kv4_join_kernel<1>, jg, dim3(256), 0, stream, a);
-    else
-      hipLaunchKernelGGL(kv4_join_kernel<2>, jg, dim3(256), 0, stream, a);
-    return check_launch("kv4_join_kernel");
-  }
-  return LX_OK;
+    LX_TRY(p.kp == 4   ? (launch_attn<2, 4>(a, p, stream))
+           : p.kp == 2 ? (launch_attn<2, 2>(a, p, stream))
+                       : (launch_attn<2, 1>(a, p, stream)));
+  if (p.splits == 1) return LX_OK;
+  const dim3 rows((unsigned)(Tq * a.rep), a.c.heads, a.c.batch);
+  if (a.c.ng == 1)
+    hipLaunchKernelGGL(kv4_join_kernel<1>, rows, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL(kv4_join_kernel<2>, rows, dim3(256), 0, stream, a);
+  return check_launch("kv4_join_kernel");
 }

@@ -202,6 +202,7 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];  // [waves][few_bytes]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
   const int c = lane >> 4, col = lane & 15;
+  const unsigned pattern = q4_pattern();
   const long rt = blockIdx.x;
   char* mine = lds + wave * few_bytes<MB>();
   const int rows = a.epi == LX_EPI_SWIGLU_PAIRED ? kTileN / 2 : kTileN;
@@ -250,7 +251,7 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
       floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int t = g * TG; t < (g + 1) * TG; ++t) {
-        const half8_t wf = q4_frag(w[t]);
+        const half8_t wf = q4_frag(w[t], pattern);
 #pragma unroll
         for (int p = NP - 1; p >= 0; --p)
           acc = mfma_f16(wf, *reinterpret_cast<const half8_t*>(xr + p * kFewRow + t * 64), acc);
@@ -312,6 +313,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void q4_many_kernel(Q4Args a) {
   float* inv = reinterpret_cast<float*>(lds + CH * CT * 8 * 1024);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int c = lane >> 4, col = lane & 15;
+  const unsigned pattern = q4_pattern();
   const int sp = blockIdx.x % a.splits;
   const long rt0 = ((long)(blockIdx.x / a.splits) * kManyWaves + wave) * RT;
   const long tiles = q4_tiles(a.N);
@@ -405,7 +407,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void q4_many_kernel(Q4Args a) {
         for (int t = g * TG; t < (g + 1) * TG; ++t) {
           half8_t wf[RT];
 #pragma unroll
-          for (int r = 0; r < RT; ++r) wf[r] = q4_frag(w[r][t]);
+          for (int r = 0; r < RT; ++r) wf[r] = q4_frag(w[r][t], pattern);
 #pragma unroll
           for (int p = 1; p >= 0; --p)
 #pragma unroll

@@ -7,7 +7,6 @@ layout; work is enqueued on torch's current stream.  Every call goes through
 liblxops.so; a failing call raises LxError (no fallback path exists).
 """
 import ctypes as C
-from typing import NamedTuple
 
 import torch
 
@@ -33,6 +32,8 @@ __all__ = [
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                       lambda device: torch.cuda.current_stream().cuda_stream)
 _device = torch.cuda.current_device
+# the same without torch's initialisation check, for operands that are on a device already
+_current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def stream():
@@ -333,57 +334,66 @@ def conv_pos_mish_bx(x, wf, bias, resid=None, groups=16, kernel=31, products=3):
 
 # ---- the LM in four bits ----------------------------------------------------------------
 
-
-def _on_device(**tensors):
-    """The named tensors (None skipped) live on the current device, where the launch goes."""
-    for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.get_device() != _device()):
-            raise ValueError(f"{name} must be a tensor on the current device")
+_F32, _I32 = torch.float32, torch.int32
 
 
-def _rows(t, name, dims, width, dtype=torch.float32):
-    """Row stride of t (..., width): rows of contiguous elements, the leading dimensions one
-    uniform run of rows."""
-    if t.dtype != dtype or t.dim() != dims or t.shape[-1] != width:
-        raise ValueError(f"{name} must be {dims}-dimensional {dtype} with rows of {width}")
-    if width > 1 and t.stride(-1) != 1:
+def _rows(t, name, shape):
+    """Row stride of the fp32 tensor t of `shape`: rows of contiguous elements, the leading
+    dimensions one uniform run of rows."""
+    if t.dtype is not _F32 or t.shape != shape:
+        raise ValueError(f"{name} must be float32 of shape {tuple(shape)}")
+    if t.is_contiguous():
+        return shape[-1]
+    st = t.stride()
+    if st[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{name}: the elements of a row must be contiguous")
-    many = dims == 3 and t.shape[0] > 1
-    ld = t.stride(-2) if t.shape[-2] > 1 else t.stride(0) if many else width
-    if many and t.stride(0) != t.shape[1] * ld:
+    many = len(shape) == 3 and shape[0] > 1
+    ld = st[-2] if shape[-2] > 1 else st[0] if many else shape[-1]
+    if many and st[0] != shape[1] * ld:
         raise ValueError(f"{name}: sequences must lie a whole number of rows apart")
     return ld
 
 
-class Q4Weight(NamedTuple):
-    """A weight (N, K) in 4 bits with group scales, as q4_pack lays it out."""
-    data: torch.Tensor
-    N: int
-    K: int
-    group: int
+def _elsewhere(name):
+    raise ValueError(f"{name} must be a tensor on the current device")
+
+
+class Q4Weight:
+    """A weight (N, K) in 4 bits with a scale per `group` inputs of a row, as q4_pack lays it
+    out in `data`."""
+    __slots__ = ("data", "N", "K", "group", "_ptr", "_dev")
+
+    def __init__(self, data, N, K, group):
+        self.data, self.N, self.K, self.group = data, N, K, group
+        self._ptr, self._dev = data.data_ptr(), data.get_device()
+        n = lib.lx_q4_bytes(N, K, group)
+        if not n or data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() != n:
+            raise ValueError(f"not the packed form of a ({N}, {K}) weight in groups of {group}")
 
 
 def q4_pack(W, group=64):
     """W (N, K) fp32 -> Q4Weight for linear_q4: per `group` (32, 64, 128) inputs of a row the
     bf16 scale s = bf16(v / -8), v the value of largest magnitude, and codes q = clamp(rint(w /
     s) + 8, 0, 15) that stand for s * (q - 8)."""
-    _on_device(W=W)
-    if W.dim() != 2 or W.dtype != torch.float32 or not W.is_contiguous():
+    if W.dim() != 2 or W.dtype is not _F32 or not W.is_contiguous():
         raise ValueError("W must be a contiguous 2-dimensional float32 tensor")
     N, K = W.shape
     n = lib.lx_q4_bytes(N, K, group)
     if not n:
         raise ValueError(f"q4_pack: unsupported shape ({N}, {K}) or group {group}")
+    if not W.is_cuda or W.get_device() != _current():
+        _elsewhere("W")
     w = Q4Weight(torch.empty(n, device=W.device, dtype=torch.uint8), N, K, group)
-    check(lib.lx_q4_pack_f32(W.data_ptr(), w.data.data_ptr(), N, K, group, stream()))
+    check(lib.lx_q4_pack_f32(W.data_ptr(), w._ptr, N, K, group, stream()))
     return w
 
 
 def q4_unpack(w):
     """The fp32 (N, K) matrix that a Q4Weight stands for."""
-    _on_device(w=w.data)
-    W = torch.empty(w.N, w.K, device=w.data.device, dtype=torch.float32)
-    check(lib.lx_q4_unpack_f32(w.data.data_ptr(), W.data_ptr(), w.N, w.K, w.group, stream()))
+    if w._dev < 0 or w._dev != _current():
+        _elsewhere("w")
+    W = torch.empty(w.N, w.K, device=w.data.device, dtype=_F32)
+    check(lib.lx_q4_unpack_f32(w._ptr, W.data_ptr(), w.N, w.K, w.group, stream()))
     return W
 
 
@@ -391,42 +401,62 @@ def linear_q4(x, w, b=None, epilogue=None, out=None):
     """epi(x @ W~^T + b) for 1 to 64 rows x (M, K) (row stride may exceed K) on a Q4Weight;
     epilogue: none, GELU, residual (out= the residual stream) or SwiGLU over interleaved rows.
     src/llm/ops.cpp:13-19."""
-    _on_device(x=x, w=w.data, b=b, out=out)
-    ldx = _rows(x, "x", 2, w.K)
+    N, K = w.N, w.K
     M = x.shape[0]
-    kind = epilogue.kind if epilogue is not None else LX_EPI_NONE
-    cols = w.N // 2 if kind == LX_EPI_SWIGLU_PAIRED else w.N
-    if b is not None and (b.dtype != torch.float32 or b.numel() != w.N or not b.is_contiguous()):
-        raise ValueError(f"b must be {w.N} contiguous float32 values")
+    ldx = _rows(x, "x", (M, K))
+    dev = x.get_device()
+    if dev < 0 or dev != w._dev or dev != _current():
+        _elsewhere("x, as w,")
+    kind = LX_EPI_NONE if epilogue is None else epilogue.kind
+    cols = N // 2 if kind == LX_EPI_SWIGLU_PAIRED else N
+    bias = None
+    if b is not None:
+        if b.dtype is not _F32 or b.numel() != N or not b.is_contiguous():
+            raise ValueError(f"b must be {N} contiguous float32 values")
+        if b.get_device() != dev:
+            _elsewhere("b")
+        bias = b.data_ptr()
     if out is None:
         if kind == LX_EPI_RESID:
             raise ValueError("residual epilogues need out= (the residual stream)")
-        out = torch.empty(M, cols, device=x.device, dtype=torch.float32)
+        out = x.new_empty((M, cols))
         ldy = cols
     else:
-        if out.dim() != 2 or out.shape[0] != M:
-            raise ValueError(f"out must have {M} rows")
-        ldy = _rows(out, "out", 2, cols)
-    n = 0 if M <= 8 else lib.lx_linear_q4_ws_floats(M, w.N, w.K)
-    ws = torch.empty(n, device=x.device, dtype=torch.float32) if n else None
-    check(lib.lx_linear_q4_f32(x.data_ptr(), ldx, w.data.data_ptr(), w.group, _p(b),
-                               out.data_ptr(), ldy, M, w.N, w.K,
-                               C.byref(epilogue) if epilogue is not None else None, _p(ws), n,
-                               stream()))
+        ldy = _rows(out, "out", (M, cols))
+        if out.get_device() != dev:
+            _elsewhere("out")
+    n, ws = 0, None
+    if M > 8:
+        n = lib.lx_linear_q4_ws_floats(M, N, K)
+        ws = x.new_empty(n) if n else None
+    check(lib.lx_linear_q4_f32(x.data_ptr(), ldx, w._ptr, w.group, bias, out.data_ptr(), ldy, M,
+                               N, K, None if epilogue is None else C.byref(epilogue),
+                               None if ws is None else ws.data_ptr(), n, _raw_stream(dev)))
     return out
 
 
 class Kv4Cache:
     """A key/value cache in 4 bits: `batch` sequences of up to max_rows rows, n_kv_heads heads of
-    head_dim (64 or 128) channels (kv4_cache makes one).  Which rows are in use is the
-    caller's to know."""
+    head_dim (64 or 128) channels, in `data` (kv4_cache makes one).  Which rows are in use is
+    the caller's to know."""
 
     def __init__(self, data, batch, n_kv_heads, head_dim, max_rows):
+        n = lib.lx_kv4_bytes(batch, n_kv_heads, head_dim, max_rows)
+        if not n or data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() != n:
+            raise ValueError("data is not the cache's uint8 bytes")
         self.data, self.batch, self.n_kv_heads = data, batch, n_kv_heads
         self.head_dim, self.max_rows = head_dim, max_rows
         self.width = n_kv_heads * head_dim
+        self._dev = data.get_device()
         self._c = Kv4(data.data_ptr(), batch, n_kv_heads, head_dim, max_rows)
         self._ref = C.byref(self._c)
+
+    def _check(self, counts, name):
+        if counts.dtype is not _I32 or counts.numel() != self.batch or \
+                not counts.is_contiguous():
+            raise ValueError(f"{name} must be {self.batch} contiguous int32 values")
+        if self._dev < 0 or counts.get_device() != self._dev or self._dev != _current():
+            _elsewhere(f"{name}, as the cache,")
 
 
 def kv4_cache(batch, n_kv_heads, max_rows, head_dim=64, device=None):
@@ -439,33 +469,30 @@ def kv4_cache(batch, n_kv_heads, max_rows, head_dim=64, device=None):
     return Kv4Cache(data, batch, n_kv_heads, head_dim, max_rows)
 
 
-def _counts(t, name, batch):
-    if t.dtype != torch.int32 or t.numel() != batch or not t.is_contiguous():
-        raise ValueError(f"{name} must be {batch} contiguous int32 values")
-
-
 def kv4_append(cache, k, v, pos):
     """Quantises rows k (roped), v (B, T, n_kv_heads * head_dim) into rows pos[b] .. pos[b] + T - 1
     of sequence b (pos: device int32 (B); rows outside the cache are not written).
     src/llm/llm.cpp:200-204."""
-    _on_device(cache=cache.data, k=k, v=v, pos=pos)
-    ldk, ldv = _rows(k, "k", 3, cache.width), _rows(v, "v", 3, cache.width)
+    cache._check(pos, "pos")
     T = k.shape[1]
-    if k.shape[0] != cache.batch or v.shape != k.shape:
-        raise ValueError(f"k and v must both be ({cache.batch}, T, {cache.width})")
-    _counts(pos, "pos", cache.batch)
+    shape = (cache.batch, T, cache.width)
+    ldk, ldv = _rows(k, "k", shape), _rows(v, "v", shape)
+    dev = cache._dev
+    if k.get_device() != dev or v.get_device() != dev:
+        _elsewhere("k, as v,")
     check(lib.lx_kv4_append_f32(cache._ref, k.data_ptr(), ldk, v.data_ptr(), ldv, T,
-                                pos.data_ptr(), stream()))
+                                pos.data_ptr(), _raw_stream(dev)))
 
 
 def kv4_read(cache, pos, T):
     """(k, v), each (B, T, n_kv_heads * head_dim) fp32: what rows pos[b] .. pos[b] + T - 1 stand
     for (rows outside the cache: zeros).  include/larynx/llm/llm.h:80-84."""
-    _on_device(cache=cache.data, pos=pos)
-    _counts(pos, "pos", cache.batch)
-    k = torch.empty(cache.batch, T, cache.width, device=cache.data.device, dtype=torch.float32)
-    v = torch.empty_like(k)
-    check(lib.lx_kv4_read_f32(cache._ref, k.data_ptr(), v.data_ptr(), T, pos.data_ptr(), stream()))
+    cache._check(pos, "pos")
+    both = torch.empty((2, cache.batch, T, cache.width), device=cache.data.device, dtype=_F32)
+    k, v = both.unbind(0)
+    p = both.data_ptr()
+    check(lib.lx_kv4_read_f32(cache._ref, p, p + 2 * both.numel(), T, pos.data_ptr(),
+                              _raw_stream(cache._dev)))
     return k, v
 
 
@@ -474,24 +501,28 @@ def attention_kv4(q, cache, lens, n_heads, scale=None, causal=True, out=None, ma
     Tq, n_heads * head_dim), lens device int32 (B).  causal: query t stands at row lens[b] - Tq +
     t.  A query that sees no row gives zeros.  max_len: the largest length expected (sizes
     the launch only).  src/llm/ops.cpp:49-65."""
-    _on_device(q=q, cache=cache.data, lens=lens, out=out)
+    cache._check(lens, "lens")
+    Tq = q.shape[1]
     width = n_heads * cache.head_dim
-    ldq = _rows(q, "q", 3, width)
-    B, Tq = q.shape[0], q.shape[1]
-    if B != cache.batch:
-        raise ValueError(f"q must have {cache.batch} sequences")
-    _counts(lens, "lens", B)
-    if out is None:
-        out = torch.empty(B, Tq, width, device=q.device, dtype=torch.float32)
-        ldo = width
-    else:
-        if out.shape != q.shape:
-            raise ValueError("out must have q's shape")
-        ldo = _rows(out, "out", 3, width)
+    shape = (cache.batch, Tq, width)
+    ldq = _rows(q, "q", shape)
+    dev = cache._dev
+    if q.get_device() != dev:
+        _elsewhere("q")
     n = lib.lx_attention_kv4_ws_floats(cache._ref, Tq, n_heads, max_len)
-    ws = torch.empty(n, device=q.device, dtype=torch.float32) if n else None
-    check(lib.lx_attention_kv4_f32(q.data_ptr(), ldq, cache._ref, lens.data_ptr(), out.data_ptr(),
-                                   ldo, Tq, n_heads,
-                                   cache.head_dim ** -0.5 if scale is None else scale,
-                                   int(causal), max_len, _p(ws), n, stream()))
+    if out is None:
+        # the splits' states behind the output (rows of 64: aligned)
+        m = cache.batch * Tq * width
+        buf = q.new_empty(m + n)
+        out, ldo, o = buf[:m].view(shape) if n else buf.view(shape), width, buf.data_ptr()
+        ws = o + 4 * m if n else None
+    else:
+        ldo, o = _rows(out, "out", shape), out.data_ptr()
+        if out.get_device() != dev:
+            _elsewhere("out")
+        buf = q.new_empty(n) if n else None
+        ws = buf.data_ptr() if n else None
+    check(lib.lx_attention_kv4_f32(q.data_ptr(), ldq, cache._ref, lens.data_ptr(), o, ldo, Tq,
+                                   n_heads, cache.head_dim ** -0.5 if scale is None else scale,
+                                   int(causal), max_len, ws, n, _raw_stream(dev)))
     return out

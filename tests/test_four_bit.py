@@ -24,7 +24,7 @@ def test_sizes():
     assert lib.lx_kv4_bytes(3, 1, 128, 33) == 3 * 2 * 2 * 2304
     assert lib.lx_kv4_bytes(64, 32, 128, 1 << 22) == 64 * 32 * (1 << 17) * 4608  # past 32 bits
     for bad in [(0, 1, 64, 1), (1, 0, 64, 1), (1, 1, 32, 1), (1, 1, 96, 1), (1, 1, 64, 0),
-                (1, 1, 64, -5), (1, 1, 64, 2 ** 31 - 1), (2 ** 30, 4, 64, 1)]:
+                (1, 1, 64, -5), (1, 1, 64, 2 ** 31 - 1), (65536, 4, 64, 1), (4, 65536, 64, 1)]:
         assert lib.lx_kv4_bytes(*bad) == 0, bad
 
 
@@ -113,7 +113,7 @@ def test_python_refuses_host_tensors():
     x = torch.zeros(1, 64)
     with pytest.raises(ValueError):
         ops.q4_pack(x)
-    w = ops.Q4Weight(torch.zeros(2112, dtype=torch.uint8), 16, 64, 64)
+    w = ops.Q4Weight(torch.zeros(1024 + 64, dtype=torch.uint8), 16, 64, 64)
     with pytest.raises(ValueError):
         ops.linear_q4(x, w)
     with pytest.raises(ValueError):
@@ -130,35 +130,38 @@ def test_python_refuses_host_tensors():
         ops.attention_kv4(torch.zeros(1, 1, 128), cache, n, 2)
 
 
-@pytest.mark.parametrize("shape,width,strides,ok", [
-    ((3, 64), 64, None, 64), ((3, 64), 64, (80, 1), 80), ((1, 64), 64, (7, 1), 64),
-    ((3, 64), 60, None, None), ((3, 64), 64, (1, 3), None),
-    ((2, 3, 64), 64, None, 64), ((2, 3, 64), 64, (240, 80, 1), 80),
-    ((2, 3, 64), 64, (250, 80, 1), None), ((2, 1, 64), 64, (96, 5, 1), 96),
-    ((1, 3, 64), 64, (7, 64, 1), 64), ((1, 1, 64), 64, (7, 7, 1), 64)])
-def test_row_strides(shape, width, strides, ok):
-    n = 1000
-    t = torch.zeros(n)
-    t = t[:3 * 2 * 64].new_zeros(shape) if strides is None else t.as_strided(shape, strides)
+@pytest.mark.parametrize("shape,want,strides,ok", [
+    ((3, 64), (3, 64), None, 64), ((3, 64), (3, 64), (80, 1), 80), ((1, 64), (1, 64), (7, 1), 64),
+    ((3, 64), (3, 60), None, None), ((3, 64), (2, 64), None, None), ((3, 64), (3, 64), (1, 3), None),
+    ((2, 3, 64), (2, 3, 64), None, 64), ((2, 3, 64), (2, 3, 64), (240, 80, 1), 80),
+    ((2, 3, 64), (2, 3, 64), (250, 80, 1), None), ((2, 1, 64), (2, 1, 64), (96, 5, 1), 96),
+    ((1, 3, 64), (1, 3, 64), (7, 64, 1), 64), ((1, 1, 64), (1, 1, 64), (7, 7, 1), 64),
+    ((2, 3, 64), (6, 64), None, None)])
+def test_row_strides(shape, want, strides, ok):
+    t = torch.zeros(shape) if strides is None else torch.zeros(1000).as_strided(shape, strides)
     if ok is None:
         with pytest.raises(ValueError):
-            ops._rows(t, "t", len(shape), width)
+            ops._rows(t, "t", want)
     else:
-        assert ops._rows(t, "t", len(shape), width) == ok
+        assert ops._rows(t, "t", want) == ok
 
 
-def test_row_types():
+def test_types_and_containers():
     with pytest.raises(ValueError):
-        ops._rows(torch.zeros(2, 64, dtype=torch.float16), "t", 2, 64)
+        ops._rows(torch.zeros(2, 64, dtype=torch.float16), "t", (2, 64))
+    cache = ops.Kv4Cache(torch.zeros(2 * 4608, dtype=torch.uint8), 2, 2, 64, 16)
+    for bad in (torch.zeros(2, dtype=torch.int64), torch.zeros(3, dtype=torch.int32),
+                torch.zeros(4, dtype=torch.int32)[::2], torch.zeros(2, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            cache._check(bad, "n")
     with pytest.raises(ValueError):
-        ops._counts(torch.zeros(2, dtype=torch.int64), "n", 2)
+        ops.Kv4Cache(torch.zeros(4608, dtype=torch.uint8), 2, 2, 64, 16)
     with pytest.raises(ValueError):
-        ops._counts(torch.zeros(3, dtype=torch.int32), "n", 2)
+        ops.Kv4Cache(torch.zeros(4608 // 4), 1, 2, 64, 16)
     with pytest.raises(ValueError):
-        ops._counts(torch.zeros(4, dtype=torch.int32)[::2], "n", 2)
-    ops._counts(torch.zeros(2, dtype=torch.int32), "n", 2)
-
-
+        ops.Q4Weight(torch.zeros(2111, dtype=torch.uint8), 16, 64, 64)
+    with pytest.raises(ValueError):
+        ops.Q4Weight(torch.zeros(0, dtype=torch.uint8), 16, 62, 64)
 
 
 def test_struct_layout_matches_header():

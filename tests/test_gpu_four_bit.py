@@ -405,6 +405,26 @@ def test_attention_does_not_see_later_rows(gpu):
     assert torch.isnan(got[:, 3:]).all()
 
 
+@pytest.mark.parametrize("rows,Tq", [(40, 1), (4000, 1), (700, 30)])
+def test_attention_nan_stays_in_its_query(gpu, rows, Tq):
+    """A query with a NaN or an infinity makes NaN of its row and head, split keys or not, and of
+    nothing else."""
+    from larynx_amd import ops
+    announce(f"kv4 attention NaN query rows={rows} Tq={Tq}")
+    rng = _gen(rows)
+    q, k, v, cache = _attn_case(gpu, rng, 2, Tq, 14, 2, 64, rows, [rows, rows])
+    n = torch.tensor([rows, rows], dtype=torch.int32, device=gpu)
+    clean = ops.attention_kv4(_dev(q, gpu), cache, n, 14)
+    for bad in (np.nan, np.inf):
+        q2 = q.copy()
+        q2[1, Tq // 2, 5 * 64 + 3] = bad
+        got = ops.attention_kv4(_dev(q2, gpu), cache, n, 14)
+        hit = torch.zeros_like(clean, dtype=torch.bool)
+        hit[1, Tq // 2, 5 * 64:6 * 64] = True
+        assert torch.isnan(got[hit]).all()
+        assert torch.equal(got[~hit], clean[~hit])
+
+
 def test_attention_lengths_outside_the_cache(gpu):
     from larynx_amd import ops
     announce("kv4 attention lengths clamped")
