@@ -163,23 +163,20 @@ __device__ __forceinline__ void q4_epi_store(const Q4Args& a, int m, long n, flo
 }
 
 // At most MB rows of x.  A workgroup owns one tile of 16 weight rows; its waves take the blocks
-// of K in turn, each splitting its own 128 inputs of x into a slice of LDS, and their sums meet
-// in LDS at the end (in a fixed order).  MB <= 8: column 2 m + part of one fragment; MB = 16:
-// column m of two.
+// of K in turn, each splitting its own 128 inputs of x into a slice of LDS (16 lanes a row, four
+// rows at a time), and their sums meet in LDS at the end (in a fixed order).  MB <= 8: column 2 m
+// + part of one fragment; MB = 16: column m of two.
 constexpr int kFewRow = 272;  // bytes of a staged row (128 fp16, and 16 against bank conflicts)
 
 template <int MB>
-constexpr int few_bytes() {
-  constexpr int b = 2 * MB * kFewRow;
-  return b < 1024 ? 1024 : b;
-}
+constexpr int few_bytes() { return 2 * MB * kFewRow + 64; }  // rows, then 16 inverse scales
 
 template <int MB, int G>
 struct FewIn {
   static constexpr int NG = kBlockK / G;
   uintx4_t w;
   ushortx4_t sc[NG];
-  float2 x[MB];
+  float4 x[MB / 4][2];
   __device__ __forceinline__ void load(const Q4Args& a, long rt, int kb, int lane) {
     const long tile = rt * a.kb + kb;
     w = a.codes[tile * 64 + lane];
@@ -187,10 +184,14 @@ struct FewIn {
         reinterpret_cast<const ushortx4_t*>(a.scales) + (tile * 4 + (lane >> 4)) * NG;
 #pragma unroll
     for (int g = 0; g < NG; ++g) sc[g] = sp[g];
-    const int k = min(kb * kBlockK + 2 * lane, a.K - 2);
+    const int k = kb * kBlockK + 8 * (lane & 15);
 #pragma unroll
-    for (int m = 0; m < MB; ++m)
-      x[m] = *reinterpret_cast<const float2*>(a.x + (long)min(m, a.M - 1) * a.ldx + k);
+    for (int p = 0; p < MB / 4; ++p) {
+      const float* xr = a.x + (long)min(4 * p + (lane >> 4), a.M - 1) * a.ldx;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        x[p][e] = *reinterpret_cast<const float4*>(xr + min(k + 4 * e, a.K - 4));
+    }
   }
 };
 
@@ -205,35 +206,49 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
   const unsigned pattern = q4_pattern();
   const long rt = blockIdx.x;
   char* mine = lds + wave * few_bytes<MB>();
-  const int rows = a.epi == LX_EPI_SWIGLU_PAIRED ? kTileN / 2 : kTileN;
-  const int nout = rows * a.M, step = a.epi == LX_EPI_SWIGLU_PAIRED ? 2 : 1;
+  float* finv = reinterpret_cast<float*>(mine + 2 * MB * kFewRow);
+  const int step = a.epi == LX_EPI_SWIGLU_PAIRED ? 2 : 1;
+  const int rshift = step == 2 ? 3 : 4, nout = a.M << rshift;  // 8 or 16 outputs a row of x
   // four threads an output in the end; what its epilogue reads is requested first
+  FewIn<MB, G> in;
+  in.load(a, rt, wave, lane);
   Q4EpiIn pre = {0.0f, 0.0f, 0.0f};
   {
-    const int i = tid >> 2, m = i / rows;
-    const long n = rt * kTileN + i % rows * step;
+    const int i = tid >> 2, m = i >> rshift;
+    const long n = rt * kTileN + (i & ((1 << rshift) - 1)) * step;
     if (i < nout && n < a.N) pre = q4_epi_load(a, m, n);
   }
   floatx4 tot = {0.f, 0.f, 0.f, 0.f};
-  FewIn<MB, G> in;
-  in.load(a, rt, wave, lane);
   for (int kb = wave; kb < a.kb; kb += waves) {
-    const bool past = kb * kBlockK + 2 * lane >= a.K;
-    float f = 0.0f;
+    const int past = a.K - kb * kBlockK - 8 * col;  // inputs of the lane's eight that exist
 #pragma unroll
-    for (int m = 0; m < MB; ++m) {
-      float2 x = in.x[m];
-      if (past) x = make_float2(0.f, 0.f);
+    for (int p = 0; p < MB / 4; ++p) {
+      float v[8], top = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float4 x = in.x[p][e];
+        const bool none = past <= 4 * e;
+        v[4 * e] = none ? 0.0f : x.x;
+        v[4 * e + 1] = none ? 0.0f : x.y;
+        v[4 * e + 2] = none ? 0.0f : x.z;
+        v[4 * e + 3] = none ? 0.0f : x.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
+      top = fmaxf(top, dpp_mov<kDppXor1>(top));
+      top = fmaxf(top, dpp_mov<kDppXor2>(top));
+      top = fmaxf(top, dpp_mov<kDppHalfMirror>(top));
+      top = fmaxf(top, dpp_mov<kDppMirror>(top));
       float inv;
-      const float sc = row_scale(wave_max(fmaxf(fabsf(x.x), fabsf(x.y))), &inv);
-      f = (PK ? col >> 1 : col) == m ? inv : f;
-      x.x *= sc;
-      x.y *= sc;
-      const half2_t h = {(_Float16)x.x, (_Float16)x.y};
-      const half2_t l = {(_Float16)(x.x - (float)h[0]), (_Float16)(x.y - (float)h[1])};
-      half2_t* row = reinterpret_cast<half2_t*>(mine + 2 * m * kFewRow) + lane;
-      row[0] = h;
-      row[kFewRow / 4] = l;
+      const float sc = row_scale(top, &inv);
+      if (col == 0) finv[4 * p + c] = inv;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= sc;
+      half8_t p0, p1;
+      split2(v, p0, p1);
+      char* row = mine + 2 * (4 * p + c) * kFewRow + col * 16;
+      *reinterpret_cast<half8_t*>(row) = p0;
+      *reinterpret_cast<half8_t*>(row + kFewRow) = p1;
     }
     const uintx4_t w = in.w;
     ushortx4_t sc[NG];
@@ -245,6 +260,7 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     const char* xr = mine + (PK ? min(col, 2 * MB - 1) : 2 * col) * kFewRow + c * 16;
+    const float f = finv[PK ? min(col >> 1, MB - 1) : col];
     floatx4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
@@ -271,6 +287,7 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
   const int q = tid & 3;
   auto value = [&](int r, int m) {
     float s = 0.0f;
+#pragma unroll 2
     for (int w = q; w < waves; w += 4) {
       const float* p = reinterpret_cast<const float*>(lds + w * few_bytes<MB>()) + (r & 3) * 64 +
                        (r >> 2) * 16;
@@ -281,7 +298,7 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
     return s;
   };
   for (int i = tid >> 2; i < nout; i += blockDim.x >> 2) {
-    const int m = i / rows, r = i % rows * step;
+    const int m = i >> rshift, r = (i & ((1 << rshift) - 1)) * step;
     const long n = rt * kTileN + r;
     const float v = value(r, m), v1 = step == 2 ? value(r + 1, m) : 0.0f;
     if (q == 0 && n < a.N)
@@ -633,8 +650,6 @@ extern "C" int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int gr
   a.epi = kind;
   a.splits = 1;
   if (q4_takes_few(M, N)) {
-    if (M == 1) return launch_few<1>(a, group, stream);
-    if (M == 2) return launch_few<2>(a, group, stream);
     if (M <= 4) return launch_few<4>(a, group, stream);
     if (M <= 8) return launch_few<8>(a, group, stream);
     return launch_few<16>(a, group, stream);
