@@ -33,6 +33,7 @@ struct Q4Args {
   float* y;
   long ldy;
   int M, N, K, kb, epi;
+  int vec;  // y, its rows and bias 16-byte aligned
   int splits;
   float* ws;
 };
@@ -160,6 +161,31 @@ __device__ __forceinline__ void q4_epi_store(const Q4Args& a, int m, long n, flo
   a.y[m * a.ldy + n] = a.epi == LX_EPI_GELU_TANH ? gelu_tanh(v)
                        : a.epi == LX_EPI_RESID   ? in.y + v
                                                  : v;
+}
+
+// Outputs n .. n + 3 (n a multiple of 4) of row m.
+__device__ __forceinline__ void q4_epi_quad(const Q4Args& a, int m, long n, floatx4 v) {
+  if (a.vec && n + 3 < a.N) {
+    if (a.bias) v += *reinterpret_cast<const floatx4*>(a.bias + n);
+    if (a.epi == LX_EPI_SWIGLU_PAIRED) {
+      const float2 o = make_float2((v[0] / (1.0f + expf(-v[0]))) * v[1],
+                                   (v[2] / (1.0f + expf(-v[2]))) * v[3]);
+      *reinterpret_cast<float2*>(a.y + m * a.ldy + (n >> 1)) = o;
+      return;
+    }
+    floatx4* y = reinterpret_cast<floatx4*>(a.y + m * a.ldy + n);
+    if (a.epi == LX_EPI_GELU_TANH)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = gelu_tanh(v[e]);
+    if (a.epi == LX_EPI_RESID) v = *y + v;
+    *y = v;
+    return;
+  }
+  const int step = a.epi == LX_EPI_SWIGLU_PAIRED ? 2 : 1;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e % step == 0 && n + e < a.N)
+      q4_epi_store(a, m, n + e, v[e], v[e | 1], q4_epi_load(a, m, n + e));
 }
 
 // At most MB rows of x.  A workgroup owns one tile of 16 weight rows; its waves take the blocks
@@ -306,54 +332,60 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
   }
 }
 
-// 9 to 64 rows of x in CT column tiles of 16.  A workgroup of eight waves owns 8 RT tiles of
-// weight rows over one of a.splits ranges of the blocks of K.  x goes through LDS as fragments of
-// its two parts, a chunk of 8 / CT blocks at a time, each wave splitting the 16 rows x 128 inputs
-// of one (block, column tile); the next chunk's x is on its way meanwhile, and the weights
-// arrive one block ahead.  One split: the epilogue from the accumulators; more: partial sums into
-// ws (splits, M, N up to 16), which q4_join_kernel adds in split order.
+// Up to 64 rows of x in CT column tiles of 16.  A workgroup of eight waves takes groups of 8 RT
+// tiles of weight rows, RT a wave, over one of a.splits ranges of the blocks of K.  x goes through
+// LDS as fragments of its two parts, a chunk of 8 / CT blocks at a time, each wave splitting the 16
+// rows x 128 inputs of one (block, column tile).  Where the range is one chunk, x is split once
+// and the workgroup walks over the groups; else the next chunk is split into a second buffer
+// while one is worked on, a barrier a chunk.  The weights come D blocks ahead, over the ends of
+// groups too.  One split: the epilogue from the accumulators; more: partial sums into ws (splits, M, N up
+// to 16), which q4_join_kernel adds in split order.
 constexpr int kManyWaves = 8;
 
 template <int CT>
 constexpr int many_blocks() { return CT == 1 ? 8 : CT == 2 ? 4 : 2; }
+// Tiles a wave: two share each fragment of x that they read, while the registers hold them.
+constexpr int many_rt(int ct, int g) { return ct <= 2 || g == 32 ? 1 : 2; }
+// bytes of `blocks` blocks of x
 template <int CT>
-constexpr size_t many_bytes() {
-  return (size_t)many_blocks<CT>() * CT * (8 * 1024 + 64);
-}
+constexpr size_t many_bytes(int blocks) { return (size_t)blocks * CT * (8 * 1024 + 64); }
 
-template <int CT, int RT, int G>
-__global__ __launch_bounds__(64 * kManyWaves) void q4_many_kernel(Q4Args a) {
-  constexpr int TG = G / 32, NG = kBlockK / G, CH = many_blocks<CT>();
-  // [block][step][column tile][part][lane] fragments, then [block][column tile][16] scales
+template <int CT, int G>
+__global__ __launch_bounds__(64 * kManyWaves) __attribute__((
+    amdgpu_waves_per_eu(CT == 1 ? 4 : 2))) void q4_many_kernel(Q4Args a) {
+  constexpr int TG = G / 32, NG = kBlockK / G, CH = many_blocks<CT>(), RT = many_rt(CT, G);
+  constexpr int D = 2;
+  // per buffer [block][step][column tile][part][lane] fragments, then [block][column tile][16]
+  // inverse scales
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  half8_t* frag = reinterpret_cast<half8_t*>(lds);
-  float* inv = reinterpret_cast<float*>(lds + CH * CT * 8 * 1024);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int c = lane >> 4, col = lane & 15;
   const unsigned pattern = q4_pattern();
-  const int sp = blockIdx.x % a.splits;
-  const long rt0 = ((long)(blockIdx.x / a.splits) * kManyWaves + wave) * RT;
+  const int sp = blockIdx.y, per = (a.kb + a.splits - 1) / a.splits;
+  const int k0 = sp * per, nb = min(per, a.kb - k0);  // > 0
   const long tiles = q4_tiles(a.N);
-  const int per = (a.kb + a.splits - 1) / a.splits;
-  const int k0 = sp * per, k1 = min(k0 + per, a.kb);
-  const int sb = wave / CT, sct = wave % CT;  // what this wave splits
+  const int groups = (int)((tiles + kManyWaves * RT - 1) / (kManyWaves * RT));
+  const int items = ((groups - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) * nb;
+  const int bufb = min(nb, CH) * CT;  // fragments of a buffer, in 8 KB
+  const int sb = wave / CT, sct = wave % CT;  // what this wave splits of a chunk
   float4 xs[4][2];
-  auto load_x = [&](int kb) {
+  auto load_x = [&](int kb) {  // kb: within the range
     const float* xr = a.x + (long)min(sct * 16 + col, a.M - 1) * a.ldx;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         xs[t][e] = *reinterpret_cast<const float4*>(
-            xr + min(kb * kBlockK + 32 * t + 8 * c + 4 * e, a.K - 4));
+            xr + min((k0 + kb) * kBlockK + 32 * t + 8 * c + 4 * e, a.K - 4));
   };
-  auto store_x = [&](int kb) {
+  auto buffer = [&](int chunk) { return lds + (size_t)(chunk & 1) * bufb * (8 * 1024 + 64); };
+  auto store_x = [&](int kb, char* buf) {
     float v[4][8], top = 0.0f;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const bool past = kb * kBlockK + 32 * t + 8 * c + 4 * e >= a.K;
+        const bool past = (k0 + kb) * kBlockK + 32 * t + 8 * c + 4 * e >= a.K;
         v[t][4 * e] = past ? 0.0f : xs[t][e].x;
         v[t][4 * e + 1] = past ? 0.0f : xs[t][e].y;
         v[t][4 * e + 2] = past ? 0.0f : xs[t][e].z;
@@ -365,54 +397,66 @@ __global__ __launch_bounds__(64 * kManyWaves) void q4_many_kernel(Q4Args a) {
     top = fmaxf(top, lane_xor32(top));
     float f;
     const float sc = row_scale(top, &f);
-    if (c == 0) inv[(sb * CT + sct) * 16 + col] = f;
+    if (c == 0)
+      reinterpret_cast<float*>(buf + bufb * 8 * 1024)[(sb * CT + sct) * 16 + col] = f;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[t][j] *= sc;
       half8_t p0, p1;
       split2(v[t], p0, p1);
-      half8_t* dst = frag + (((sb * 4 + t) * CT + sct) * 2) * 64 + lane;
+      half8_t* dst = reinterpret_cast<half8_t*>(buf) + (((sb * 4 + t) * CT + sct) * 2) * 64 + lane;
       dst[0] = p0;
       dst[64] = p1;
     }
   };
-  uintx4_t w[RT], wn[RT];
-  ushortx4_t sc[RT][NG], scn[RT][NG];
-  auto load_w = [&](int kb) {
+  uintx4_t w[D][RT];
+  ushortx4_t sc[D][RT][NG];
+  // item i of this workgroup: block i % nb of its (i / nb)-th group; kept as running counters
+  int lg = blockIdx.x, lk = 0, left = items;
+  auto load_w = [&](int d) {
+    if (left <= 0) return;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const long tile = min(rt0 + r, tiles - 1) * a.kb + kb;
-      wn[r] = a.codes[tile * 64 + lane];
+      const long tile = min(((long)lg * kManyWaves + wave) * RT + r, tiles - 1) * a.kb + k0 + lk;
+      w[d][r] = a.codes[tile * 64 + lane];
       const ushortx4_t* p = reinterpret_cast<const ushortx4_t*>(a.scales) + (tile * 4 + c) * NG;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) scn[r][g] = p[g];
+      for (int g = 0; g < NG; ++g) sc[d][r][g] = p[g];
+    }
+    --left;
+    if (++lk == nb) {
+      lk = 0;
+      lg += gridDim.x;
     }
   };
-  floatx4 tot[RT][CT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) tot[r][ct] = floatx4{0.f, 0.f, 0.f, 0.f};
   const bool stages = sb < CH;
-  if (k0 < k1) load_w(k0);
-  if (stages && k0 + sb < k1) load_x(k0 + sb);
-  for (int kc = k0; kc < k1; kc += CH) {
-    if (kc > k0) __syncthreads();  // the last chunk has been read
-    if (stages && kc + sb < k1) store_x(kc + sb);
-    __syncthreads();
-    if (stages && kc + CH + sb < k1) load_x(kc + CH + sb);
-    const int nb = min(CH, k1 - kc);
-    for (int i = 0; i < nb; ++i) {
+  if (stages && sb < nb) load_x(sb);
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        w[r] = wn[r];
+  for (int d = 0; d < D; ++d) load_w(d);
+  if (stages && sb < nb) store_x(sb, buffer(0));
+  __syncthreads();
+  if (stages && CH + sb < nb) load_x(CH + sb);
+
+  floatx4 tot[RT][CT];
+  int kb = 0, chunk = 0, in_chunk = 0, group = blockIdx.x;
+  for (int i = 0; i < items; i += D) {
 #pragma unroll
-        for (int g = 0; g < NG; ++g) sc[r][g] = scn[r][g];
-      }
-      if (kc + i + 1 < k1) load_w(kc + i + 1);
-      const half8_t* fb = frag + i * 4 * CT * 128 + lane;
-      floatx4 sum[RT][CT];
+    for (int d = 0; d < D; ++d) {
+      if (i + d >= items) break;
+      if (kb == 0)
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) tot[r][ct] = floatx4{0.f, 0.f, 0.f, 0.f};
+      const char* buf = buffer(chunk);
+      const half8_t* fb =
+          reinterpret_cast<const half8_t*>(buf) + in_chunk * 4 * CT * 128 + lane;
+      float f[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+        f[ct] = reinterpret_cast<const float*>(buf + bufb * 8 * 1024)[(in_chunk * CT + ct) * 16 +
+                                                                      col];
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         floatx4 acc[RT][CT];
@@ -424,7 +468,7 @@ __global__ __launch_bounds__(64 * kManyWaves) void q4_many_kernel(Q4Args a) {
         for (int t = g * TG; t < (g + 1) * TG; ++t) {
           half8_t wf[RT];
 #pragma unroll
-          for (int r = 0; r < RT; ++r) wf[r] = q4_frag(w[r][t], pattern);
+          for (int r = 0; r < RT; ++r) wf[r] = q4_frag(w[d][r][t], pattern);
 #pragma unroll
           for (int p = 1; p >= 0; --p)
 #pragma unroll
@@ -437,46 +481,45 @@ __global__ __launch_bounds__(64 * kManyWaves) void q4_many_kernel(Q4Args a) {
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
+          for (int e = 0; e < 4; ++e) {
+            const float s = bf16_lo(sc[d][r][g][e]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              sum[r][ct][e] = g == 0 ? bf16_lo(sc[r][g][e]) * acc[r][ct][e]
-                                     : fmaf(bf16_lo(sc[r][g][e]), acc[r][ct][e], sum[r][ct][e]);
+            for (int ct = 0; ct < CT; ++ct)
+              tot[r][ct][e] = fmaf(s * f[ct], acc[r][ct][e], tot[r][ct][e]);
+          }
       }
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const float f = inv[(i * CT + ct) * 16 + col];
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) tot[r][ct][e] = fmaf(f, sum[r][ct][e], tot[r][ct][e]);
-      }
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const long n = (rt0 + r) * kTileN + 4 * c;
-    if (rt0 + r >= tiles) break;
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const int m = ct * 16 + col;
-      if (m >= a.M) continue;
-      if (a.splits > 1) {
-        *reinterpret_cast<floatx4*>(a.ws + ((long)sp * a.M + m) * (tiles * kTileN) + n) =
-            tot[r][ct];
+      load_w(d);
+      if (++kb < nb) {
+        if (++in_chunk == CH) {
+          // the next chunk into the other buffer, which all have read since the last barrier
+          ++chunk;
+          in_chunk = 0;
+          if (stages && chunk * CH + sb < nb) store_x(chunk * CH + sb, buffer(chunk));
+          __syncthreads();
+          if (stages && (chunk + 1) * CH + sb < nb) load_x((chunk + 1) * CH + sb);
+        }
         continue;
       }
-      if (a.epi == LX_EPI_SWIGLU_PAIRED) {
+      // the group is done (with more than one, x is a single chunk)
 #pragma unroll
-        for (int e = 0; e < 4; e += 2)
-          if (n + e < a.N)
-            q4_epi_store(a, m, n + e, tot[r][ct][e], tot[r][ct][e + 1], q4_epi_load(a, m, n + e));
-      } else {
+      for (int r = 0; r < RT; ++r) {
+        const long tile = ((long)group * kManyWaves + wave) * RT + r, n = tile * kTileN + 4 * c;
+        if (tile >= tiles) break;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < a.N)
-            q4_epi_store(a, m, n + e, tot[r][ct][e], 0.0f, q4_epi_load(a, m, n + e));
+        for (int ct = 0; ct < CT; ++ct) {
+          const int m = ct * 16 + col;
+          if (m >= a.M) continue;
+          if (a.splits > 1) {
+            *reinterpret_cast<floatx4*>(a.ws + ((long)sp * a.M + m) * (tiles * kTileN) + n) =
+                tot[r][ct];
+            continue;
+          }
+          q4_epi_quad(a, m, n, tot[r][ct]);
+        }
       }
+      kb = 0;
+      in_chunk = 0;
+      group += gridDim.x;
     }
   }
 }
@@ -493,15 +536,7 @@ __global__ __launch_bounds__(256) void q4_join_kernel(Q4Args a) {
 #pragma unroll 4
   for (int k = 0; k < a.splits; ++k)
     s += *reinterpret_cast<const floatx4*>(p + (long)k * a.M * np4 * 4);
-  if (a.epi == LX_EPI_SWIGLU_PAIRED) {
-#pragma unroll
-    for (int e = 0; e < 4; e += 2)
-      if (n + e < a.N) q4_epi_store(a, m, n + e, s[e], s[e + 1], q4_epi_load(a, m, n + e));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < a.N) q4_epi_store(a, m, n + e, s[e], 0.0f, q4_epi_load(a, m, n + e));
-  }
+  q4_epi_quad(a, m, n, s);
 }
 
 #define LX_Q4_GROUPS(KERNEL, ...)                                        \
@@ -521,44 +556,49 @@ int launch_few(const Q4Args& a, int G, hipStream_t s) {
   return check_launch("q4_few_kernel");
 }
 
-template <int CT, int RT, int G>
+// Splits of K of q4_many_kernel: about one workgroup a CU.
+int many_splits(int M, int N, int K) {
+  const int kb = (int)q4_blocks(K), rows = kManyWaves * (M > 32 ? 2 : 1);
+  if (M <= 8) return 1;
+  const long groups = (q4_tiles(N) + rows - 1) / rows;
+  const int s = (int)std::max(1L, std::min<long>(kb, device_cus() / groups));
+  const int per = (kb + s - 1) / s;
+  return (kb + per - 1) / per;
+}
+
+template <int CT, int G>
 int raise_many() {
   static LdsLimit once;
-  return raise_lds_limit(reinterpret_cast<const void*>(q4_many_kernel<CT, RT, G>),
-                         many_bytes<CT>(), once, "q4_many_kernel");
+  return raise_lds_limit(reinterpret_cast<const void*>(q4_many_kernel<CT, G>),
+                         many_bytes<CT>(2 * many_blocks<CT>()), once, "q4_many_kernel");
 }
 
-// What q4_many_kernel runs with: tiles a wave and splits of K.
-struct ManyPlan {
-  int rt, splits;
-};
-ManyPlan many_plan(int M, int N, int K) {
-  const int cus = device_cus(), kb = (int)q4_blocks(K);
-  const long tiles = q4_tiles(N);
-  ManyPlan p;
-  // two tiles a wave share each fragment of x they read from LDS
-  p.rt = tiles > 8 * kManyWaves ? 2 : 1;
-  const long wgs = (tiles + kManyWaves * p.rt - 1) / (kManyWaves * p.rt);
-  p.splits = (int)std::max(1L, std::min<long>(kb, cus / wgs));
-  const int per = (kb + p.splits - 1) / p.splits;
-  p.splits = (kb + per - 1) / per;
-  return p;
-}
-
-template <int CT, int RT>
+template <int CT>
 int launch_many(const Q4Args& a, int G, hipStream_t s) {
-  LX_TRY(G == 32 ? (raise_many<CT, RT, 32>())
-                 : G == 64 ? (raise_many<CT, RT, 64>()) : (raise_many<CT, RT, 128>()));
-  const long wgs = (q4_tiles(a.N) + kManyWaves * RT - 1) / (kManyWaves * RT);
-  const dim3 grid((unsigned)(wgs * a.splits)), block(64 * kManyWaves);
-  const size_t lds = many_bytes<CT>();
-  LX_Q4_GROUPS(q4_many_kernel, CT, RT)
+  LX_TRY(G == 32 ? (raise_many<CT, 32>())
+                 : G == 64 ? (raise_many<CT, 64>()) : (raise_many<CT, 128>()));
+  const int per = (a.kb + a.splits - 1) / a.splits, chunk = many_blocks<CT>();
+  const int rows = kManyWaves * many_rt(CT, G);
+  const long groups = (q4_tiles(a.N) + rows - 1) / rows;
+  // one chunk of x: two workgroups a CU walk over the groups
+  const long wgs = per <= chunk ? std::min(groups, 2L * device_cus()) : groups;
+  const dim3 grid((unsigned)wgs, a.splits), block(64 * kManyWaves);
+  const size_t lds = many_bytes<CT>(per <= chunk ? per : 2 * chunk);
+  LX_Q4_GROUPS(q4_many_kernel, CT)
   return check_launch("q4_many_kernel");
 }
 #undef LX_Q4_GROUPS
 
-// Rows of x that run on q4_few_kernel.
-bool q4_takes_few(int M, int N) { return M <= 8 || (M <= 16 && q4_tiles(N) <= 1024); }
+// Calls that run on q4_few_kernel, which has no fixed cost but splits x again for every tile; in
+// units of tile x block.  Times of both, us, at K = 896 (few / many): M = 1, N = 40000 9.6 / 10.6,
+// N = 151936 28 / 18.8; M = 8, N = 9728 5.6 / 7.4, N = 40000 14.3 / 11.3 (and below 2048 tiles the
+// other needs a second launch); M = 16, N = 1152 4.6 / 6.3, N = 9728 8.8 / 7.9; N = 896, K = 4864
+// (few tiles, each a long run of blocks) 11.8 / 8.5.
+bool q4_takes_few(int M, int N, int K) {
+  const long tiles = q4_tiles(N), kb = q4_blocks(K), work = tiles * kb;
+  if (M <= 8) return tiles < 2048 || work <= (M <= 4 ? 35000 : 9000);
+  return M <= 16 && work <= 4096 && kb <= 16;
+}
 
 bool q4_shape_ok(int N, int K, int group) {
   return N > 0 && K > 0 && K % 4 == 0 && (group == 32 || group == 64 || group == 128) &&
@@ -612,9 +652,9 @@ extern "C" int lx_q4_unpack_f32(const void* Wq, float* W, int N, int K, int grou
 }
 
 extern "C" size_t lx_linear_q4_ws_floats(int M, int N, int K) {
-  if (M < 1 || M > kMaxRows || !q4_shape_ok(N, K, 64) || q4_takes_few(M, N)) return 0;
-  const ManyPlan p = many_plan(M, N, K);
-  return p.splits == 1 ? 0 : (size_t)p.splits * M * q4_tiles(N) * kTileN;
+  if (M < 1 || M > kMaxRows || !q4_shape_ok(N, K, 64) || q4_takes_few(M, N, K)) return 0;
+  const int splits = many_splits(M, N, K);
+  return splits == 1 ? 0 : (size_t)splits * M * q4_tiles(N) * kTileN;
 }
 
 extern "C" int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int group,
@@ -643,36 +683,32 @@ extern "C" int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int gr
   a.bias = bias;
   a.y = y;
   a.ldy = ldy;
+  a.vec = ldy % 4 == 0 && ((uintptr_t)y | (uintptr_t)bias) % 16 == 0;
   a.M = M;
   a.N = N;
   a.K = K;
   a.kb = (int)q4_blocks(K);
   a.epi = kind;
   a.splits = 1;
-  if (q4_takes_few(M, N)) {
+  if (q4_takes_few(M, N, K)) {
     if (M <= 4) return launch_few<4>(a, group, stream);
     if (M <= 8) return launch_few<8>(a, group, stream);
     return launch_few<16>(a, group, stream);
   }
-  const ManyPlan p = many_plan(M, N, K);
-  a.splits = p.splits;
-  if (p.splits > 1) {
-    const size_t need = (size_t)p.splits * M * q4_tiles(N) * kTileN;
+  a.splits = many_splits(M, N, K);
+  if (a.splits > 1) {
+    const size_t need = (size_t)a.splits * M * q4_tiles(N) * kTileN;
     LX_REQUIRE(ws && ws_floats >= need && (uintptr_t)ws % 16 == 0,
                "linear_q4: workspace of %zu floats, %zu needed", ws ? ws_floats : 0, need);
     a.ws = ws;
   }
-  switch ((M + 15) / 16 * 2 + p.rt) {
-    case 3: LX_TRY((launch_many<1, 1>(a, group, stream))); break;
-    case 4: LX_TRY((launch_many<1, 2>(a, group, stream))); break;
-    case 5: LX_TRY((launch_many<2, 1>(a, group, stream))); break;
-    case 6: LX_TRY((launch_many<2, 2>(a, group, stream))); break;
-    case 7: LX_TRY((launch_many<3, 1>(a, group, stream))); break;
-    case 8: LX_TRY((launch_many<3, 2>(a, group, stream))); break;
-    case 9: LX_TRY((launch_many<4, 1>(a, group, stream))); break;
-    default: LX_TRY((launch_many<4, 2>(a, group, stream))); break;
+  switch ((M + 15) / 16) {
+    case 1: LX_TRY(launch_many<1>(a, group, stream)); break;
+    case 2: LX_TRY(launch_many<2>(a, group, stream)); break;
+    case 3: LX_TRY(launch_many<3>(a, group, stream)); break;
+    default: LX_TRY(launch_many<4>(a, group, stream)); break;
   }
-  if (p.splits == 1) return LX_OK;
+  if (a.splits == 1) return LX_OK;
   const long n = q4_tiles(N) * (kTileN / 4) * M;
   hipLaunchKernelGGL(q4_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
   return check_launch("q4_join_kernel");

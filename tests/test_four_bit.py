@@ -62,6 +62,7 @@ def test_linear_workspace():
         assert lib.lx_linear_q4_ws_floats(*bad) == 0
     need = lib.lx_linear_q4_ws_floats(64, 1000, 8192)
     assert need and need % (64 * 1008) == 0
+    assert lib.lx_linear_q4_ws_floats(1, 151936, 896) == 0
     for ws, n in [(None, need), (P, need - 1), (P + 4, need)]:
         assert _linear(M=64, N=1000, K=8192, ldx=8192, ldy=1000, ws=ws, n=n) == LX_ERR_ARG
         assert b"workspace" in lib.lx_last_error()

@@ -156,6 +156,29 @@ def test_linear_bit_exact_on_whole_numbers(gpu, M, N, K, G):
     assert (got[M:] == -77).all() and (got[:, N:] == -77).all()
 
 
+@pytest.mark.parametrize("M,N,K,G", [
+    (1, 90004, 896, 64), (4, 151936, 896, 32), (7, 33000, 700, 128),   # one chunk of x, walked over
+    (16, 9999, 896, 64), (12, 300, 4100, 32), (16, 2500, 8192, 128),   # 8 blocks a chunk, splits
+    (31, 70, 8192, 64), (17, 40001, 260, 64), (32, 5000, 2000, 128),
+    (40, 33, 1028, 32), (48, 4097, 1500, 64), (64, 3000, 3000, 32), (64, 20000, 512, 64),
+    (64, 130, 8192, 128)])
+def test_linear_bit_exact_on_larger_shapes(gpu, M, N, K, G):
+    """As above, on the shapes of the kernel that shares x: whole numbers, against torch in 64 bits
+    on the device; columns past N and rows past M untouched."""
+    from larynx_amd import ops
+    announce(f"q4 linear exact, larger M={M} N={N} K={K} G={G}")
+    g = torch.Generator(device=gpu).manual_seed(M + N + K)
+    W = torch.randint(-8, 8, (N, K), device=gpu, generator=g).float()
+    W[:, ::G] = -8
+    x = torch.randint(-3, 4, (M, K), device=gpu, generator=g).float()
+    b = torch.randint(-9, 10, (N,), device=gpu, generator=g).float()
+    out = torch.full((M + 1, N + 5), -77.0, device=gpu)
+    ops.linear_q4(x, ops.q4_pack(W, G), b, out=out[:M, :N])
+    want = (x.double() @ W.t().contiguous().double() + b).float()
+    assert torch.equal(out[:M, :N], want)
+    assert (out[M:] == -77).all() and (out[:, N:] == -77).all()
+
+
 def _linear_tolerance(x, sc, G):
     """Per output: the group sums run through 4 G / 8 accumulations (three parts and the sum of
     x) of partial sums below (24 + 31) sum |x| times the scale, then over the groups."""
