@@ -696,6 +696,17 @@ int lx_qwen2_decode(lx_qwen2* m, int token, float* logits, float* final_norm,
  * graph every step (src/llm/llm.cpp:232-275). */
 int lx_qwen2_set_decode_graph(lx_qwen2* m, int enable);
 
+/* Decode's weights: bits = 32 (the default; group unused) or 4, the q|k|v, gate/up
+ * and down projections and the head on copies in 4 bits with a scale per `group`
+ * (32, 64 or 128) inputs (lx_q4_pack_f32, lx_linear_q4_f32): 7.9 MB of them and
+ * o_proj's 3.2 MB of fp32 a layer of Qwen2-0.5B instead of 59.6 MB.  o_proj, whose
+ * launch also forms the attention, the embeddings, norms and the K/V cache keep
+ * fp32, and so does the whole prefill.  The call waits for the device, packs from
+ * the model's fp32 weights, which stay, and drops captured decode graphs; the
+ * first one with 4 allocates the copies (held until destroy; LX_ERR_ALLOC changes
+ * nothing).  Not to be called during a capture.  No counterpart in the reference. */
+int lx_qwen2_set_decode_bits(lx_qwen2* m, int bits, int group);
+
 /* Prefill projections' split-operand products, 3 (the default) or 6, as
  * lx_dit_set_products (decode's GEMVs are fp32 either way).  No counterpart
  * in the reference (src/llm/llm.cpp:141-173 runs fp32 ggml_mul_mat). */

@@ -234,6 +234,12 @@ struct DecGemvArgs {
   const float* inv_freq = nullptr;  // device: 32 rotary inverse frequencies
 };
 int dec_gemv(int epi, const DecGemvArgs& a, hipStream_t stream);
+// The same on a 4-bit weight (lx_q4.hip; a.W unused): Wq from q4_pack, for DEC_QKV_ROPE with neox
+// (rows of a head in rotary pairs), K <= 2048 where x is normalised.
+int dec_gemv_q4(int epi, const DecGemvArgs& a, const void* Wq, int group, hipStream_t stream);
+// lx_q4_bytes, and lx_q4_pack_f32 with the row order of dec_gemv_q4.
+size_t q4_bytes(int N, int K, int group);
+int q4_pack(const float* W, void* Wq, int N, int K, int group, int neox, hipStream_t stream);
 // True when the decode kernels cover this geometry (K = hidden <= 2048,
 // K = intermediate <= 6144).
 bool dec_supported(int hidden, int intermediate);

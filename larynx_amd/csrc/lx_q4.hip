@@ -43,16 +43,18 @@ __host__ __device__ inline long q4_blocks(int K) { return (K + kBlockK - 1) / kB
 
 // ---- quantise and lay out ---------------------------------------------------------------
 
-// One wave per (row tile, block): lane l holds row l % 16, inputs 32 t + 8 (l / 16) + j.
+// One wave per (row tile, block): lane l holds row l % 16, inputs 32 t + 8 (l / 16) + j.  neox:
+// rows 2 i and 2 i + 1 of a head of 64 are its rows i and i + 32, a rotary pair, side by side.
 template <int G>
 __global__ __launch_bounds__(64) void q4_pack_kernel(const float* __restrict__ W,
                                                      uintx4_t* __restrict__ codes,
                                                      unsigned short* __restrict__ scales, int N,
-                                                     int K, int kb) {
+                                                     int K, int kb, int neox) {
   constexpr int TG = G / 32;  // 32-wide steps of a group
   const int lane = threadIdx.x, c = lane >> 4, r = lane & 15;
   const long tile = blockIdx.x;  // row tile * kb + block
   const long n = tile / kb * kTileN + r;
+  const long src = neox ? (n & ~63L) + ((n & 63) >> 1) + (n & 1) * 32 : n;
   const int k0 = (int)(tile % kb) * kBlockK;
   float w[4][8];
 #pragma unroll
@@ -60,7 +62,7 @@ __global__ __launch_bounds__(64) void q4_pack_kernel(const float* __restrict__ W
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int k = k0 + 32 * t + 8 * c + 4 * e;
-      const float4 v = n < N && k < K ? *reinterpret_cast<const float4*>(W + n * K + k)
+      const float4 v = n < N && k < K ? *reinterpret_cast<const float4*>(W + src * K + k)
                                       : make_float4(0.f, 0.f, 0.f, 0.f);
       w[t][4 * e] = v.x;
       w[t][4 * e + 1] = v.y;
@@ -197,6 +199,9 @@ constexpr int kFewRow = 272;  // bytes of a staged row (128 fp16, and 16 against
 template <int MB>
 constexpr int few_bytes() { return 2 * MB * kFewRow + 64; }  // rows, then 16 inverse scales
 
+// The decode kernel's staged row of two parts, later its 2 x 16 sums.
+constexpr int dec_bytes() { return 2 * kFewRow; }
+
 template <int MB, int G>
 struct FewIn {
   static constexpr int NG = kBlockK / G;
@@ -329,6 +334,162 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
     const float v = value(r, m), v1 = step == 2 ? value(r + 1, m) : 0.0f;
     if (q == 0 && n < a.N)
       q4_epi_store(a, m, n, v, v1, i == tid >> 2 ? pre : q4_epi_load(a, m, n));
+  }
+}
+
+// One row of x, as the LM's decode runs it: q4_few_kernel's product between the input's RMSNorm
+// (every wave sums the row's squares itself) and the epilogues of dec_gemv, whose arguments it
+// takes.  DEC_QKV_ROPE reads rows laid out in rotary pairs (q4_pack_kernel's neox).
+template <int G, int EPI>
+__global__ __launch_bounds__(1024) void q4_dec_kernel(Q4Args a, DecGemvArgs d) {
+  constexpr int TG = G / 32, NG = kBlockK / G;
+  constexpr bool NORM = EPI != DEC_RESID, PAIR = EPI == DEC_QKV_ROPE || EPI == DEC_SWIGLU;
+  extern __shared__ __attribute__((aligned(16))) char lds[];  // [waves][few_bytes<1>]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+  const int c = lane >> 4, col = lane & 15;
+  const unsigned pattern = q4_pattern();
+  const long rt = blockIdx.x;
+  char* mine = lds + wave * dec_bytes();
+  uintx4_t w;
+  ushortx4_t sc[NG];
+  float4 x[2], nw[2];
+  auto load = [&](int kb) {
+    const long tile = rt * a.kb + kb;
+    w = a.codes[tile * 64 + lane];
+    const ushortx4_t* sp = reinterpret_cast<const ushortx4_t*>(a.scales) + (tile * 4 + c) * NG;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) sc[g] = sp[g];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int k = min(kb * kBlockK + 8 * col + 4 * e, a.K - 4);
+      x[e] = *reinterpret_cast<const float4*>(a.x + k);
+      if (NORM) nw[e] = *reinterpret_cast<const float4*>(d.norm_w + k);
+    }
+  };
+  load(wave);
+  float4 row[8];
+  if (NORM) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      row[j] = *reinterpret_cast<const float4*>(a.x + 4 * min(lane + 64 * j, a.K / 4 - 1));
+  }
+  // what the outputs' epilogue reads, under the weights' latency: four threads an output
+  const int o = tid >> 2, r = PAIR ? 2 * o : o;  // the tile's row
+  const long n = rt * kTileN + r;
+  const bool out = r < kTileN && n < a.N;
+  float b0 = 0.0f, b1 = 0.0f, sn = 0.0f, cs = 1.0f;
+  int pos = 0;
+  const int head = (int)(n >> 6), hc = (int)(n & 63) >> 1;
+  if (out) {
+    if (EPI == DEC_QKV_ROPE) {
+      pos = *d.pos;
+      b0 = d.bias[head * 64 + hc];
+      b1 = d.bias[head * 64 + hc + 32];
+      if (head < d.rope_heads) sincosf((float)pos * d.inv_freq[hc], &sn, &cs);
+    }
+    if (EPI == DEC_RESID) b0 = d.y[n];
+  }
+  float rs = 1.0f;
+  if (NORM) {
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (lane + 64 * j < a.K / 4)
+        s += (row[j].x * row[j].x + row[j].y * row[j].y) +
+             (row[j].z * row[j].z + row[j].w * row[j].w);
+    rs = 1.0f / sqrtf(wave_sum(s) / (float)a.K + d.eps);
+  }
+  floatx4 tot = {0.f, 0.f, 0.f, 0.f};
+  for (int kb = wave; kb < a.kb; kb += waves) {
+    const int k = kb * kBlockK + 8 * col;
+    float v[8], top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const bool none = k + 4 * e >= a.K;
+      float4 u = x[e];
+      if (NORM)
+        u = make_float4((u.x * rs) * nw[e].x, (u.y * rs) * nw[e].y, (u.z * rs) * nw[e].z,
+                        (u.w * rs) * nw[e].w);
+      if (EPI == DEC_HEAD && d.y2 && rt == 0 && c == 0 && !none)
+        *reinterpret_cast<float4*>(d.y2 + k + 4 * e) = u;
+      v[4 * e] = none ? 0.0f : u.x;
+      v[4 * e + 1] = none ? 0.0f : u.y;
+      v[4 * e + 2] = none ? 0.0f : u.z;
+      v[4 * e + 3] = none ? 0.0f : u.w;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
+    top = fmaxf(top, dpp_mov<kDppXor1>(top));
+    top = fmaxf(top, dpp_mov<kDppXor2>(top));
+    top = fmaxf(top, dpp_mov<kDppHalfMirror>(top));
+    top = fmaxf(top, dpp_mov<kDppMirror>(top));
+    float f;
+    const float xs = row_scale(top, &f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= xs;
+    half8_t p0, p1;
+    split2(v, p0, p1);
+    if (c == 0) {
+      *reinterpret_cast<half8_t*>(mine + col * 16) = p0;
+      *reinterpret_cast<half8_t*>(mine + kFewRow + col * 16) = p1;
+    }
+    const uintx4_t wc = w;
+    ushortx4_t scc[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) scc[g] = sc[g];
+    if (kb + waves < a.kb) load(kb + waves);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const char* xr = mine + min(col, 1) * kFewRow + c * 16;
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = g * TG; t < (g + 1) * TG; ++t)
+        acc = mfma_f16(q4_frag(wc[t], pattern), *reinterpret_cast<const half8_t*>(xr + t * 64),
+                       acc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] = fmaf(bf16_lo(scc[g][i]), acc[i], sum[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tot[i] = fmaf(f, sum[i], tot[i]);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  // columns 0 and 1 (the two parts) of the 16 rows
+  if (col < 2) *reinterpret_cast<floatx4*>(mine + (col * 4 + c) * 16) = tot;
+  __syncthreads();
+  if (r >= kTileN) return;
+  const int q = tid & 3;
+  auto value = [&](int row) {
+    float s = 0.0f;
+#pragma unroll 4
+    for (int i = q; i < waves; i += 4) {
+      const float* p = reinterpret_cast<const float*>(lds + i * dec_bytes()) + row;
+      s += p[16] + p[0];
+    }
+    s += dpp_mov<kDppXor1>(s);
+    return s + dpp_mov<kDppXor2>(s);
+  };
+  float v0 = value(r), v1 = PAIR ? value(r + 1) : 0.0f;
+  if (q || !out) return;
+  if (EPI == DEC_QKV_ROPE) {
+    v0 += b0;
+    v1 += b1;
+    const float x0 = v0 * cs - v1 * sn, x1 = v1 * cs + v0 * sn;
+    const int cl = head * 64 + hc;
+    float* dst = cl < d.q_cols ? d.y + cl
+                 : cl < d.q_cols + d.kv_cols
+                     ? d.k_cache + (long)pos * d.kv_cols + (cl - d.q_cols)
+                     : d.v_cache + (long)pos * d.kv_cols + (cl - d.q_cols - d.kv_cols);
+    dst[0] = x0;
+    dst[32] = x1;
+  } else if (EPI == DEC_SWIGLU) {
+    d.y[n >> 1] = (v0 / (1.0f + expf(-v0))) * v1;
+  } else {
+    d.y[n] = EPI == DEC_RESID ? b0 + v0 : v0;
   }
 }
 
@@ -618,10 +779,14 @@ extern "C" size_t lx_q4_bytes(int N, int K, int group) {
          (size_t)q4_tiles(N) * q4_blocks(K) * (kBlockK / group) * kTileN * sizeof(unsigned short);
 }
 
-extern "C" int lx_q4_pack_f32(const float* W, void* Wq, int N, int K, int group,
-                              hipStream_t stream) {
+namespace lx {
+
+size_t q4_bytes(int N, int K, int group) { return lx_q4_bytes(N, K, group); }
+
+int q4_pack(const float* W, void* Wq, int N, int K, int group, int neox, hipStream_t stream) {
   LX_REQUIRE(W && Wq, "q4_pack: null pointer");
-  LX_REQUIRE(q4_shape_ok(N, K, group), "q4_pack: bad shape N=%d K=%d group=%d", N, K, group);
+  LX_REQUIRE(q4_shape_ok(N, K, group) && (!neox || N % 64 == 0),
+             "q4_pack: bad shape N=%d K=%d group=%d", N, K, group);
   LX_REQUIRE(((uintptr_t)W | (uintptr_t)Wq) % 16 == 0, "q4_pack: unaligned");
   const int kb = (int)q4_blocks(K);
   const dim3 grid((unsigned)(q4_tiles(N) * kb));
@@ -629,12 +794,65 @@ extern "C" int lx_q4_pack_f32(const float* W, void* Wq, int N, int K, int group,
   auto* scales =
       reinterpret_cast<unsigned short*>(static_cast<char*>(Wq) + q4_code_bytes(N, K));
   if (group == 32)
-    hipLaunchKernelGGL(q4_pack_kernel<32>, grid, dim3(64), 0, stream, W, codes, scales, N, K, kb);
+    hipLaunchKernelGGL(q4_pack_kernel<32>, grid, dim3(64), 0, stream, W, codes, scales, N, K, kb,
+                       neox);
   else if (group == 64)
-    hipLaunchKernelGGL(q4_pack_kernel<64>, grid, dim3(64), 0, stream, W, codes, scales, N, K, kb);
+    hipLaunchKernelGGL(q4_pack_kernel<64>, grid, dim3(64), 0, stream, W, codes, scales, N, K, kb,
+                       neox);
   else
-    hipLaunchKernelGGL(q4_pack_kernel<128>, grid, dim3(64), 0, stream, W, codes, scales, N, K, kb);
+    hipLaunchKernelGGL(q4_pack_kernel<128>, grid, dim3(64), 0, stream, W, codes, scales, N, K, kb,
+                       neox);
   return check_launch("q4_pack_kernel");
+}
+
+namespace {
+template <int EPI>
+int launch_dec(const Q4Args& a, const DecGemvArgs& d, int G, hipStream_t s) {
+  const int waves = std::min(16, a.kb);
+  const dim3 grid((unsigned)q4_tiles(a.N)), block(64 * waves);
+  const size_t lds = (size_t)waves * dec_bytes();
+  if (G == 32)
+    hipLaunchKernelGGL((q4_dec_kernel<32, EPI>), grid, block, lds, s, a, d);
+  else if (G == 64)
+    hipLaunchKernelGGL((q4_dec_kernel<64, EPI>), grid, block, lds, s, a, d);
+  else
+    hipLaunchKernelGGL((q4_dec_kernel<128, EPI>), grid, block, lds, s, a, d);
+  return check_launch("q4_dec_kernel");
+}
+}  // namespace
+
+int dec_gemv_q4(int epi, const DecGemvArgs& d, const void* Wq, int group, hipStream_t s) {
+  LX_REQUIRE(Wq && d.x && d.y && d.N <= INT_MAX && q4_shape_ok((int)d.N, d.K, group),
+             "dec_gemv_q4: bad args");
+  LX_REQUIRE(epi == DEC_RESID || (d.norm_w && d.K <= 2048), "dec_gemv_q4: norm args");
+  Q4Args a{};
+  a.x = d.x;
+  a.codes = static_cast<const uintx4_t*>(Wq);
+  a.scales = reinterpret_cast<const unsigned short*>(static_cast<const char*>(Wq) +
+                                                     q4_code_bytes((int)d.N, d.K));
+  a.N = (int)d.N;
+  a.K = d.K;
+  a.kb = (int)q4_blocks(d.K);
+  switch (epi) {
+    case DEC_QKV_ROPE:
+      LX_REQUIRE(d.N % 64 == 0 && d.bias && d.pos && d.k_cache && d.v_cache && d.inv_freq,
+                 "dec_gemv_q4: qkv args");
+      return launch_dec<DEC_QKV_ROPE>(a, d, group, s);
+    case DEC_SWIGLU:
+      LX_REQUIRE(d.N % 2 == 0, "dec_gemv_q4: swiglu needs an even N");
+      return launch_dec<DEC_SWIGLU>(a, d, group, s);
+    case DEC_RESID: return launch_dec<DEC_RESID>(a, d, group, s);
+    case DEC_HEAD: return launch_dec<DEC_HEAD>(a, d, group, s);
+  }
+  set_error("dec_gemv_q4: unsupported epilogue %d", epi);
+  return LX_ERR_ARG;
+}
+
+}  // namespace lx
+
+extern "C" int lx_q4_pack_f32(const float* W, void* Wq, int N, int K, int group,
+                              hipStream_t stream) {
+  return q4_pack(W, Wq, N, K, group, 0, stream);
 }
 
 extern "C" int lx_q4_unpack_f32(const void* Wq, float* W, int N, int K, int group,

@@ -32,6 +32,9 @@ struct Layer {
   // the prefill projections' weights in MFMA fragment order (wfrag_pack), for
   // the split-operand GEMM; decode streams the fp32 copies above
   void *qkv_wf = nullptr, *o_wf = nullptr, *gu_wf = nullptr, *down_wf = nullptr;
+  // decode's weights in 4 bits (lx_qwen2_set_decode_bits; o_proj keeps fp32, its launch forms the
+  // attention too)
+  void *qkv_q4 = nullptr, *gu_q4 = nullptr, *down_q4 = nullptr;
 };
 
 // Six products run on the fragment-operand GEMMs up to this many rows (64 rows 1.05x
@@ -95,6 +98,8 @@ struct lx_qwen2 {
   float* rope_tab = nullptr;  // device copy of the rotary inverse frequencies
   float* rope_cs = nullptr;   // their cosines and sines at every position (rope_table)
   bool use_graph = true;      // replay the layer stack as one HIP graph
+  int q4_group = 0;           // decode on 4-bit weights in groups of this many inputs (0: fp32)
+  void* head_q4 = nullptr;    // llm_decoder in 4 bits
   hipStream_t cap_stream = nullptr;
   // [0]: the cache fits one attention split; [1 + c]: split class c
   hipGraphExec_t graph[1 + kDecAttnClasses] = {};
@@ -336,6 +341,11 @@ int prefill_layer(lx_qwen2* m, Layer& L, int rows, const float* next_norm, hipSt
   return prefill_mlp(m, L, rows, next_norm, s, LX_ACT_F32, LX_ACT_F32);
 }
 
+// A decode projection on its fp32 or its 4-bit weight.
+int dec_proj(const lx_qwen2* m, int epi, const DecGemvArgs& a, const void* q4, hipStream_t s) {
+  return m->q4_group ? dec_gemv_q4(epi, a, q4, m->q4_group, s) : dec_gemv(epi, a, s);
+}
+
 // One decode layer (src/llm/llm.cpp:254-289): RMSNorm + QKV + rotary + cache
 // append; attention; o_proj + residual; RMSNorm + gate/up + SwiGLU;
 // down_proj + residual.  While the cache fits one split (cls 0) the attention is
@@ -361,7 +371,7 @@ int decode_layer(lx_qwen2* m, Layer& L, int cls, hipStream_t s) {
   q.k_cache = L.k_cache;
   q.v_cache = L.v_cache;
   q.inv_freq = m->rope_tab;
-  LX_TRY(dec_gemv(DEC_QKV_ROPE, q, s));
+  LX_TRY(dec_proj(m, DEC_QKV_ROPE, q, L.qkv_q4, s));
   DecAttnArgs at;
   at.q = m->hn;
   at.k_cache = L.k_cache;
@@ -397,14 +407,14 @@ int decode_layer(lx_qwen2* m, Layer& L, int cls, hipStream_t s) {
   gu.y = m->act;
   gu.N = 2L * m->I;
   gu.K = H;
-  LX_TRY(dec_gemv(DEC_SWIGLU, gu, s));
+  LX_TRY(dec_proj(m, DEC_SWIGLU, gu, L.gu_q4, s));
   DecGemvArgs d;
   d.x = m->act;
   d.W = L.down_w;
   d.y = m->x;
   d.N = H;
   d.K = m->I;
-  return dec_gemv(DEC_RESID, d, s);
+  return dec_proj(m, DEC_RESID, d, L.down_q4, s);
 }
 
 int decode_stack(lx_qwen2* m, int cls, hipStream_t s) {
@@ -744,7 +754,7 @@ extern "C" int lx_qwen2_decode(lx_qwen2* m, int token, float* logits, float* fin
   h.y2 = final_norm;
   h.N = m->speech_vocab;
   h.K = H;
-  LX_TRY(dec_gemv(DEC_HEAD, h, s));
+  LX_TRY(dec_proj(m, DEC_HEAD, h, m->head_q4, s));
   m->cache_len += 1;
   return LX_OK;
 }
@@ -766,6 +776,56 @@ extern "C" int lx_qwen2_set_products(lx_qwen2* m, int products) {
   LX_REQUIRE(products == 3 || products == 6, "qwen2_set_products: %d products (3 or 6)",
              products);
   m->products = products;
+  return LX_OK;
+}
+
+extern "C" int lx_qwen2_set_decode_bits(lx_qwen2* m, int bits, int group) {
+  LX_REQUIRE(m, "qwen2_set_decode_bits: null model");
+  LX_REQUIRE(bits == 32 || (bits == 4 && (group == 32 || group == 64 || group == 128)),
+             "qwen2_set_decode_bits: %d bits in groups of %d (32, or 4 in groups of 32, 64 or 128)",
+             bits, group);
+  const int want = bits == 4 ? group : 0;
+  if (want == m->q4_group) return LX_OK;
+  // decode steps under way read the weights and the graphs that go
+  if (hipDeviceSynchronize() != hipSuccess) {
+    set_error("qwen2_set_decode_bits: synchronisation failed");
+    return LX_ERR_LAUNCH;
+  }
+  auto drop_graphs = [&] {  // captured with the other weights
+    for (hipGraphExec_t& g : m->graph) {
+      if (g) (void)hipGraphExecDestroy(g);
+      g = nullptr;
+    }
+  };
+  const int H = m->H, I = m->I;
+  if (!want) drop_graphs();
+  if (want) {
+    // allocated once, for the smallest groups
+    auto A = [&](void** p, int N, int K) {
+      if (!*p) *p = m->arena.alloc<char>(q4_bytes(N, K, 32));
+      return *p != nullptr;
+    };
+    bool ok = A(&m->head_q4, m->speech_vocab, H);
+    for (auto& L : m->layers)
+      ok = ok && A(&L.qkv_q4, m->QKV, H) && A(&L.gu_q4, 2 * I, H) && A(&L.down_q4, H, I);
+    if (!ok) {
+      set_error("qwen2_set_decode_bits: device allocation failed");
+      return LX_ERR_ALLOC;
+    }
+    drop_graphs();
+    m->q4_group = 0;  // until every weight is packed
+    LX_TRY(q4_pack(m->llm_decoder, m->head_q4, m->speech_vocab, H, want, 0, nullptr));
+    for (auto& L : m->layers) {
+      LX_TRY(q4_pack(L.qkv_w, L.qkv_q4, m->QKV, H, want, 1, nullptr));
+      LX_TRY(q4_pack(L.gu_w, L.gu_q4, 2 * I, H, want, 0, nullptr));
+      LX_TRY(q4_pack(L.down_w, L.down_q4, H, I, want, 0, nullptr));
+    }
+    if (hipStreamSynchronize(nullptr) != hipSuccess) {
+      set_error("qwen2_set_decode_bits: packing failed");
+      return LX_ERR_LAUNCH;
+    }
+  }
+  m->q4_group = want;
   return LX_OK;
 }
 

@@ -197,6 +197,11 @@ class Qwen2LM:
         eagerly (False)."""
         check(lib.lx_qwen2_set_decode_graph(self._h, 1 if enable else 0))
 
+    def set_decode_bits(self, bits, group=64):
+        """Decode's weights: 32 (fp32, the default) or 4, q|k|v, gate/up, down and the head on 4-bit
+        copies with a scale per `group` (32, 64, 128) inputs.  The prefill keeps fp32."""
+        check(lib.lx_qwen2_set_decode_bits(self._h, int(bits), int(group)))
+
     def set_products(self, products):
         """Split-operand products of the prefill projections: 3 (the default) or 6."""
         check(lib.lx_qwen2_set_products(self._h, int(products)))

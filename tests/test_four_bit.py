@@ -171,3 +171,7 @@ def test_struct_layout_matches_header():
     got = _c_layout("lx_kv4", fields)
     assert got[0] == C.sizeof(Kv4)
     assert got[1:] == [getattr(Kv4, f).offset for f in fields]
+
+
+def test_decode_bits_refuse_a_null_model():
+    assert lib.lx_qwen2_set_decode_bits(None, 4, 64) == LX_ERR_ARG
