@@ -199,9 +199,6 @@ constexpr int kFewRow = 272;  // bytes of a staged row (128 fp16, and 16 against
 template <int MB>
 constexpr int few_bytes() { return 2 * MB * kFewRow + 64; }  // rows, then 16 inverse scales
 
-// The decode kernel's staged row of two parts, later its 2 x 16 sums.
-constexpr int dec_bytes() { return 2 * kFewRow; }
-
 template <int MB, int G>
 struct FewIn {
   static constexpr int NG = kBlockK / G;
@@ -337,159 +334,133 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
   }
 }
 
-// One row of x, as the LM's decode runs it: q4_few_kernel's product between the input's RMSNorm
-// (every wave sums the row's squares itself) and the epilogues of dec_gemv, whose arguments it
-// takes.  DEC_QKV_ROPE reads rows laid out in rotary pairs (q4_pack_kernel's neox).
-template <int G, int EPI>
-__global__ __launch_bounds__(1024) void q4_dec_kernel(Q4Args a, DecGemvArgs d) {
-  constexpr int TG = G / 32, NG = kBlockK / G;
-  constexpr bool NORM = EPI != DEC_RESID, PAIR = EPI == DEC_QKV_ROPE || EPI == DEC_SWIGLU;
-  extern __shared__ __attribute__((aligned(16))) char lds[];  // [waves][few_bytes<1>]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
-  const int c = lane >> 4, col = lane & 15;
+// One normalised row of x, as the LM's decode runs it (arguments and epilogues of dec_gemv).  One
+// wave is one tile of 16 rows over the whole of K <= 128 NB: it requests all its weights, forms
+// RMSNorm and the two parts of the row itself (2 NB values a lane; one power of two for the row)
+// and hands them to its lanes as fragments through LDS of its own, so nothing waits for another
+// wave and the sums are complete in place.  (As q4_few_kernel runs it, seven waves a tile at K =
+// 896, the row is formed 4256 times for gate/up, 3 us of instructions: 6.9 us in the decode
+// chain.)  DEC_QKV_ROPE reads rows laid out in rotary pairs (q4_pack_kernel's neox).
+constexpr int row_bytes(int nb) { return 2 * (nb * 256 + 16); }
+
+template <int G, int EPI, int NB>
+__global__ __launch_bounds__(64) void q4_row_kernel(Q4Args a, DecGemvArgs d) {
+  constexpr int TG = G / 32, NG = kBlockK / G, ROW = NB * 256 + 16, H = NB < 8 ? NB : 8;
+  __shared__ __attribute__((aligned(16))) char lds[row_bytes(NB)];
+  const int lane = threadIdx.x, c = lane >> 4, col = lane & 15;
   const unsigned pattern = q4_pattern();
   const long rt = blockIdx.x;
-  char* mine = lds + wave * dec_bytes();
-  uintx4_t w;
-  ushortx4_t sc[NG];
-  float4 x[2], nw[2];
-  auto load = [&](int kb) {
-    const long tile = rt * a.kb + kb;
-    w = a.codes[tile * 64 + lane];
-    const ushortx4_t* sp = reinterpret_cast<const ushortx4_t*>(a.scales) + (tile * 4 + c) * NG;
+  const int kb = a.kb;
+  float2 x[NB], g[NB];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) sc[g] = sp[g];
+  for (int j = 0; j < NB; ++j) {
+    const int k = min(j * kBlockK + 2 * lane, a.K - 2);
+    x[j] = *reinterpret_cast<const float2*>(a.x + k);
+    g[j] = *reinterpret_cast<const float2*>(d.norm_w + k);
+  }
+  uintx4_t w[H];
+  ushortx4_t sc[H][NG];
+  auto load = [&](int first) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int k = min(kb * kBlockK + 8 * col + 4 * e, a.K - 4);
-      x[e] = *reinterpret_cast<const float4*>(a.x + k);
-      if (NORM) nw[e] = *reinterpret_cast<const float4*>(d.norm_w + k);
+    for (int j = 0; j < H; ++j) {
+      const long tile = rt * kb + min(first + j, kb - 1);
+      w[j] = a.codes[tile * 64 + lane];
+      const ushortx4_t* sp = reinterpret_cast<const ushortx4_t*>(a.scales) + (tile * 4 + c) * NG;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) sc[j][i] = sp[i];
     }
   };
-  load(wave);
-  float4 row[8];
-  if (NORM) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      row[j] = *reinterpret_cast<const float4*>(a.x + 4 * min(lane + 64 * j, a.K / 4 - 1));
-  }
-  // what the outputs' epilogue reads, under the weights' latency: four threads an output
-  const int o = tid >> 2, r = PAIR ? 2 * o : o;  // the tile's row
-  const long n = rt * kTileN + r;
-  const bool out = r < kTileN && n < a.N;
-  float b0 = 0.0f, b1 = 0.0f, sn = 0.0f, cs = 1.0f;
-  int pos = 0;
+  load(0);
+  // what the epilogue of the lane's rows n .. n + 3 reads, under the weights' latency
+  const long n = rt * kTileN + 4 * c;
   const int head = (int)(n >> 6), hc = (int)(n & 63) >> 1;
-  if (out) {
-    if (EPI == DEC_QKV_ROPE) {
-      pos = *d.pos;
-      b0 = d.bias[head * 64 + hc];
-      b1 = d.bias[head * 64 + hc + 32];
-      if (head < d.rope_heads) sincosf((float)pos * d.inv_freq[hc], &sn, &cs);
-    }
-    if (EPI == DEC_RESID) b0 = d.y[n];
-  }
-  float rs = 1.0f;
-  if (NORM) {
-    float s = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (lane + 64 * j < a.K / 4)
-        s += (row[j].x * row[j].x + row[j].y * row[j].y) +
-             (row[j].z * row[j].z + row[j].w * row[j].w);
-    rs = 1.0f / sqrtf(wave_sum(s) / (float)a.K + d.eps);
-  }
-  floatx4 tot = {0.f, 0.f, 0.f, 0.f};
-  for (int kb = wave; kb < a.kb; kb += waves) {
-    const int k = kb * kBlockK + 8 * col;
-    float v[8], top = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const bool none = k + 4 * e >= a.K;
-      float4 u = x[e];
-      if (NORM)
-        u = make_float4((u.x * rs) * nw[e].x, (u.y * rs) * nw[e].y, (u.z * rs) * nw[e].z,
-                        (u.w * rs) * nw[e].w);
-      if (EPI == DEC_HEAD && d.y2 && rt == 0 && c == 0 && !none)
-        *reinterpret_cast<float4*>(d.y2 + k + 4 * e) = u;
-      v[4 * e] = none ? 0.0f : u.x;
-      v[4 * e + 1] = none ? 0.0f : u.y;
-      v[4 * e + 2] = none ? 0.0f : u.z;
-      v[4 * e + 3] = none ? 0.0f : u.w;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
-    top = fmaxf(top, dpp_mov<kDppXor1>(top));
-    top = fmaxf(top, dpp_mov<kDppXor2>(top));
-    top = fmaxf(top, dpp_mov<kDppHalfMirror>(top));
-    top = fmaxf(top, dpp_mov<kDppMirror>(top));
-    float f;
-    const float xs = row_scale(top, &f);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= xs;
-    half8_t p0, p1;
-    split2(v, p0, p1);
-    if (c == 0) {
-      *reinterpret_cast<half8_t*>(mine + col * 16) = p0;
-      *reinterpret_cast<half8_t*>(mine + kFewRow + col * 16) = p1;
-    }
-    const uintx4_t wc = w;
-    ushortx4_t scc[NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) scc[g] = sc[g];
-    if (kb + waves < a.kb) load(kb + waves);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const char* xr = mine + min(col, 1) * kFewRow + c * 16;
-    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      floatx4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int t = g * TG; t < (g + 1) * TG; ++t)
-        acc = mfma_f16(q4_frag(wc[t], pattern), *reinterpret_cast<const half8_t*>(xr + t * 64),
-                       acc);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] = fmaf(bf16_lo(scc[g][i]), acc[i], sum[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) tot[i] = fmaf(f, sum[i], tot[i]);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  }
-  // columns 0 and 1 (the two parts) of the 16 rows
-  if (col < 2) *reinterpret_cast<floatx4*>(mine + (col * 4 + c) * 16) = tot;
-  __syncthreads();
-  if (r >= kTileN) return;
-  const int q = tid & 3;
-  auto value = [&](int row) {
-    float s = 0.0f;
-#pragma unroll 4
-    for (int i = q; i < waves; i += 4) {
-      const float* p = reinterpret_cast<const float*>(lds + i * dec_bytes()) + row;
-      s += p[16] + p[0];
-    }
-    s += dpp_mov<kDppXor1>(s);
-    return s + dpp_mov<kDppXor2>(s);
-  };
-  float v0 = value(r), v1 = PAIR ? value(r + 1) : 0.0f;
-  if (q || !out) return;
+  int pos = 0;
+  float b[4] = {0.f, 0.f, 0.f, 0.f}, sn[2] = {0.f, 0.f}, cs[2] = {1.f, 1.f};
   if (EPI == DEC_QKV_ROPE) {
-    v0 += b0;
-    v1 += b1;
-    const float x0 = v0 * cs - v1 * sn, x1 = v1 * cs + v0 * sn;
+    pos = *d.pos;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = d.bias[head * 64 + hc + (i >> 1) + 32 * (i & 1)];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float f = d.inv_freq[hc + i];
+      if (head < d.rope_heads) sincosf((float)pos * f, &sn[i], &cs[i]);
+    }
+  }
+  float ss = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    if (j * kBlockK + 2 * lane >= a.K) x[j] = make_float2(0.f, 0.f);
+    ss += x[j].x * x[j].x + x[j].y * x[j].y;
+  }
+  const float rs = 1.0f / sqrtf(wave_sum(ss) / (float)a.K + d.eps);
+  float top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    x[j] = make_float2((x[j].x * rs) * g[j].x, (x[j].y * rs) * g[j].y);
+    const int k = j * kBlockK + 2 * lane;
+    if (EPI == DEC_HEAD && rt == 0 && d.y2 && k < a.K)
+      *reinterpret_cast<float2*>(d.y2 + k) = x[j];
+    top = fmaxf(top, fmaxf(fabsf(x[j].x), fabsf(x[j].y)));
+  }
+  float f;
+  const float xs = row_scale(wave_max(top), &f);
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const float v0 = x[j].x * xs, v1 = x[j].y * xs;
+    const half2_t p0 = {(_Float16)v0, (_Float16)v1};
+    const half2_t p1 = {(_Float16)(v0 - (float)p0[0]), (_Float16)(v1 - (float)p0[1])};
+    *reinterpret_cast<half2_t*>(lds + j * 256 + lane * 4) = p0;
+    *reinterpret_cast<half2_t*>(lds + ROW + j * 256 + lane * 4) = p1;
+  }
+  __syncthreads();  // of one wave
+  const char* xr = lds + (col & 1) * ROW + c * 16;  // column 0: first parts, 1: second parts
+  floatx4 tot = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int first = 0; first < NB; first += H) {
+    if (first > 0) load(first);
+#pragma unroll
+    for (int j = 0; j < H; ++j) {
+      if (first + j >= kb) break;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = i * TG; t < (i + 1) * TG; ++t)
+          acc = mfma_f16(q4_frag(w[j][t], pattern),
+                         *reinterpret_cast<const half8_t*>(xr + (first + j) * 256 + t * 64), acc);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tot[e] = fmaf(bf16_lo(sc[j][i][e]), acc[e], tot[e]);
+      }
+    }
+  }
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    tot[e] *= f;
+    v[e] = tot[e] + dpp_mov<kDppXor1>(tot[e]);
+  }
+  if (col) return;
+  if (EPI == DEC_QKV_ROPE) {
     const int cl = head * 64 + hc;
     float* dst = cl < d.q_cols ? d.y + cl
                  : cl < d.q_cols + d.kv_cols
                      ? d.k_cache + (long)pos * d.kv_cols + (cl - d.q_cols)
                      : d.v_cache + (long)pos * d.kv_cols + (cl - d.q_cols - d.kv_cols);
-    dst[0] = x0;
-    dst[32] = x1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float x0 = v[2 * i] + b[2 * i], x1 = v[2 * i + 1] + b[2 * i + 1];
+      dst[i] = x0 * cs[i] - x1 * sn[i];
+      dst[32 + i] = x1 * cs[i] + x0 * sn[i];
+    }
   } else if (EPI == DEC_SWIGLU) {
-    d.y[n >> 1] = (v0 / (1.0f + expf(-v0))) * v1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (n + 2 * i < a.N)
+        d.y[(n >> 1) + i] = (v[2 * i] / (1.0f + expf(-v[2 * i]))) * v[2 * i + 1];
   } else {
-    d.y[n] = EPI == DEC_RESID ? b0 + v0 : v0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < a.N) d.y[n + e] = v[e];
   }
 }
 
@@ -806,43 +777,52 @@ int q4_pack(const float* W, void* Wq, int N, int K, int group, int neox, hipStre
 }
 
 namespace {
-template <int EPI>
-int launch_dec(const Q4Args& a, const DecGemvArgs& d, int G, hipStream_t s) {
-  const int waves = std::min(16, a.kb);
-  const dim3 grid((unsigned)q4_tiles(a.N)), block(64 * waves);
-  const size_t lds = (size_t)waves * dec_bytes();
+template <int EPI, int NB>
+int launch_row(const Q4Args& a, const DecGemvArgs& d, int G, hipStream_t s) {
+  const dim3 grid((unsigned)q4_tiles(a.N)), block(64);
   if (G == 32)
-    hipLaunchKernelGGL((q4_dec_kernel<32, EPI>), grid, block, lds, s, a, d);
+    hipLaunchKernelGGL((q4_row_kernel<32, EPI, NB>), grid, block, 0, s, a, d);
   else if (G == 64)
-    hipLaunchKernelGGL((q4_dec_kernel<64, EPI>), grid, block, lds, s, a, d);
+    hipLaunchKernelGGL((q4_row_kernel<64, EPI, NB>), grid, block, 0, s, a, d);
   else
-    hipLaunchKernelGGL((q4_dec_kernel<128, EPI>), grid, block, lds, s, a, d);
-  return check_launch("q4_dec_kernel");
+    hipLaunchKernelGGL((q4_row_kernel<128, EPI, NB>), grid, block, 0, s, a, d);
+  return check_launch("q4_row_kernel");
 }
 }  // namespace
 
 int dec_gemv_q4(int epi, const DecGemvArgs& d, const void* Wq, int group, hipStream_t s) {
   LX_REQUIRE(Wq && d.x && d.y && d.N <= INT_MAX && q4_shape_ok((int)d.N, d.K, group),
              "dec_gemv_q4: bad args");
-  LX_REQUIRE(epi == DEC_RESID || (d.norm_w && d.K <= 2048), "dec_gemv_q4: norm args");
+  const int N = (int)d.N;
+  if (epi == DEC_RESID) {
+    lx_epilogue resid{};
+    resid.kind = LX_EPI_RESID;
+    return lx_linear_q4_f32(d.x, d.K, Wq, group, nullptr, d.y, N, 1, N, d.K, &resid, nullptr, 0,
+                            s);
+  }
+  LX_REQUIRE(d.norm_w && d.K <= 2048, "dec_gemv_q4: norm args");
   Q4Args a{};
   a.x = d.x;
   a.codes = static_cast<const uintx4_t*>(Wq);
   a.scales = reinterpret_cast<const unsigned short*>(static_cast<const char*>(Wq) +
-                                                     q4_code_bytes((int)d.N, d.K));
-  a.N = (int)d.N;
+                                                     q4_code_bytes(N, d.K));
+  a.N = N;
   a.K = d.K;
   a.kb = (int)q4_blocks(d.K);
+  const bool wide = a.kb > 8;
   switch (epi) {
     case DEC_QKV_ROPE:
-      LX_REQUIRE(d.N % 64 == 0 && d.bias && d.pos && d.k_cache && d.v_cache && d.inv_freq,
+      LX_REQUIRE(N % 64 == 0 && d.bias && d.pos && d.k_cache && d.v_cache && d.inv_freq,
                  "dec_gemv_q4: qkv args");
-      return launch_dec<DEC_QKV_ROPE>(a, d, group, s);
+      return wide ? launch_row<DEC_QKV_ROPE, 16>(a, d, group, s)
+                  : launch_row<DEC_QKV_ROPE, 8>(a, d, group, s);
     case DEC_SWIGLU:
-      LX_REQUIRE(d.N % 2 == 0, "dec_gemv_q4: swiglu needs an even N");
-      return launch_dec<DEC_SWIGLU>(a, d, group, s);
-    case DEC_RESID: return launch_dec<DEC_RESID>(a, d, group, s);
-    case DEC_HEAD: return launch_dec<DEC_HEAD>(a, d, group, s);
+      LX_REQUIRE(N % 2 == 0, "dec_gemv_q4: swiglu needs an even N");
+      return wide ? launch_row<DEC_SWIGLU, 16>(a, d, group, s)
+                  : launch_row<DEC_SWIGLU, 8>(a, d, group, s);
+    case DEC_HEAD:
+      return wide ? launch_row<DEC_HEAD, 16>(a, d, group, s)
+                  : launch_row<DEC_HEAD, 8>(a, d, group, s);
   }
   set_error("dec_gemv_q4: unsupported epilogue %d", epi);
   return LX_ERR_ARG;

@@ -95,9 +95,11 @@ def test_switching_back_gives_the_fp32_bits(gpu, lm4):
 
 
 @pytest.mark.parametrize("kw", [dict(hidden=320, intermediate=1100, n_heads=5, n_kv_heads=1),
-                                dict(hidden=1024, intermediate=132, n_heads=16, n_kv_heads=8)])
+                                dict(hidden=1024, intermediate=132, n_heads=16, n_kv_heads=8),
+                                dict(hidden=1536, intermediate=2048, n_heads=24, n_kv_heads=4)])
 def test_other_geometries(gpu, kw):
-    """Widths that are no multiple of a group or a block, one and eight kv heads."""
+    """Widths that are no multiple of a group or a block, one to eight kv heads, and one past the
+    eight blocks that a wave requests at once."""
     announce(f"4-bit decode {kw}")
     cfg, params, lm = _model(gpu, 92, **kw)
     lm.set_decode_bits(4, 64)
