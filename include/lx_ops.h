@@ -396,8 +396,8 @@ int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int group, const 
                      size_t ws_floats, hipStream_t stream);
 
 /* A key/value cache held in 4 bits (4.5 with its scales): `batch` sequences of up
- * to max_rows rows, n_kv_heads heads (both at most 65535) of head_dim (64 or 128)
- * channels.  Keys and
+ * to max_rows rows, n_kv_heads heads (at most 65535 and 32767) of head_dim (64 or
+ * 128) channels.  Keys and
  * values alike: the 64 channels of a group of a row share z = the largest bf16
  * not above their minimum and s = the smallest bf16 not below (max - z) / 15; a
  * code q = clamp(rint((x - z) / s), 0, 15) stands for z + s * q (no range: z).  A

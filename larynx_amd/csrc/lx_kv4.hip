@@ -39,12 +39,13 @@ struct AppendArgs {
   Kv4 c;
   const float *k, *v;
   long ldk, ldv;
-  int T, touched;
+  int T;
   const int* pos;
 };
 
-// z and s of a group with extremes lo and hi (both finite), and the quotient in 64 bits: a value
-// next to a border decides a whole step.
+// z and s of a group with extremes lo and hi (finite).  Both quotients here decide by a border, so
+// they are the 64-bit ones; where the fp32 quotient (off by less than 2^-21 of itself) is clear of
+// every border, which is all but one in some thousands, it decides the same.
 struct Affine {
   float s, z;
 };
@@ -54,21 +55,28 @@ __device__ __forceinline__ Affine affine(float lo, float hi) {
   zb = lo < 0.0f && cut != zb ? cut + 0x10000u : cut;
   Affine a;
   a.z = __uint_as_float(zb);
-  const double r = ((double)hi - (double)a.z) / 15.0;
-  float f = (float)r;
-  unsigned sb = __float_as_uint(f);
-  if ((double)f < r) ++sb;
+  unsigned sb = __float_as_uint((hi - a.z) * (1.0f / 15.0f));
+  const unsigned low = sb & 0xffffu;
+  if (low < 64u || low > 0xffffu - 64u || sb < 0x01000000u) {  // a bf16 number near, or tiny
+    const double r = ((double)hi - (double)a.z) / 15.0;
+    const float f = (float)r;
+    sb = __float_as_uint(f) + ((double)f < r ? 1u : 0u);
+  }
   a.s = __uint_as_float((sb + 0xffffu) & 0xffff0000u);
   return a;
 }
 __device__ __forceinline__ unsigned affine_code(float x, Affine a) {
   if (!(a.s > 0.0f)) return 0;
-  const double q = rint(((double)x - (double)a.z) / (double)a.s);
-  return (unsigned)(int)fmin(fmax(q, 0.0), 15.0);
+  const float u = (x - a.z) * (1.0f / a.s);
+  float q = rintf(u);
+  // (a subnormal s has no inverse: u is then infinite or NaN)
+  if (__any(!(fabsf(fabsf(u - q) - 0.5f) > 1e-4f && u < 64.0f)))
+    q = (float)rint(((double)x - (double)a.z) / (double)a.s);
+  return (unsigned)(int)fminf(fmaxf(q, 0.0f), 15.0f);
 }
 
-// Codes and pair of one group, lane = channel.  A group that holds an infinity or a NaN, or
-// whose |z| + 16 s passes fp32 (the attention forms z - 16 s), stores NaN.
+// Code and pair of one group, lane = channel.  A group that holds an infinity or a NaN, or whose
+// |z| + 16 s passes fp32, stores NaN.
 __device__ __forceinline__ unsigned quantise(float x, unsigned* pair) {
   const float hi = wave_max(x), lo = -wave_max(-x);
   const bool bad = __any(!(fabsf(x) <= 3.402823466e38f));
@@ -86,53 +94,62 @@ __device__ __forceinline__ unsigned quantise(float x, unsigned* pair) {
   return affine_code(x, a);
 }
 
-// One workgroup per (32-row record touched, kv head, sequence); wave w owns the rows whose value
-// codes share dwords, 4 w .. 4 w + 3 of both halves, lane = channel.
-__global__ __launch_bounds__(256) void kv4_append_kernel(AppendArgs a) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int i = blockIdx.x % a.touched;
-  const int bh = blockIdx.x / a.touched, b = bh / a.c.heads, h = bh % a.c.heads;
+// One workgroup of eight waves per (32-row record touched, channel group of a kv head, sequence):
+// four for the keys, four for the values, lane = channel.  Wave w of a plane owns the rows whose
+// value codes share dwords, 4 w .. 4 w + 3 of both halves; all eight are requested at once.
+__global__ __launch_bounds__(512) void kv4_append_kernel(AppendArgs a) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6 & 3, plane = threadIdx.x >> 8;
+  const int ng = a.c.ng, hg = blockIdx.y, b = blockIdx.z;  // hg: head * ng + group
+  const int h = ng == 1 ? hg : hg >> 1, g = ng == 1 ? 0 : hg & 1;
   const long pos = a.pos[b];
-  const long blk = max(pos, 0L) / kBlk + i;
+  const long blk = max(pos, 0L) / kBlk + blockIdx.x;
   if (blk >= a.c.blocks) return;
   char* rec = a.c.data + a.c.record(b, h, (int)blk);
-  const int ng = a.c.ng;
-  for (int g = 0; g < ng; ++g) {
-    unsigned vword = 0, vmask = 0;
+  const long t0 = blk * kBlk - pos;  // the record's first row in k and v
+  auto row_of = [&](int j) { return 4 * w + (j & 3) + 16 * (j >> 2); };
+  const float* src = plane ? a.v : a.k;
+  const long ld = plane ? a.ldv : a.ldk;
+  float x[8];
+  bool live[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int row = 4 * w + (j & 3) + 16 * (j >> 2);
-      const long t = blk * kBlk + row - pos;
-      if (t < 0 || t >= a.T || blk * kBlk + row >= a.c.rows) continue;
-      const long ch = (long)(h * ng + g) * kGrp + lane;
-      const float kx = a.k[((long)b * a.T + t) * a.ldk + ch];
-      const float vx = a.v[((long)b * a.T + t) * a.ldv + ch];
-      unsigned kp, vp;
-      const unsigned kq = quantise(kx, &kp), vq = quantise(vx, &vp);
-      vword |= q4_put(vq, j);
-      vmask |= q4_put(15u, j);
-      // eight channels make a dword of key codes
-      unsigned kw = q4_put(kq, lane & 7);
-      kw |= __shfl_xor(kw, 1, 64);
-      kw |= __shfl_xor(kw, 2, 64);
-      kw |= __shfl_xor(kw, 4, 64);
-      if ((lane & 7) == 0) {
-        const int ks = lane >> 5, c = (lane >> 3) & 3;
-        reinterpret_cast<unsigned*>(rec + g * kCodes)[((c * 16 + (row & 15)) * 2 + (row >> 4)) * 2 +
-                                                      ks] = kw;
-      }
-      if (lane == 0) {
-        unsigned* pairs = reinterpret_cast<unsigned*>(rec + 2 * ng * kCodes);
-        pairs[g * kBlk + row] = kp;
-        pairs[(ng + g) * kBlk + row] = vp;
-      }
-    }
-    if (vmask) {
-      unsigned* p = reinterpret_cast<unsigned*>(rec + (ng + g) * kCodes) +
-                    (w * 16 + (lane & 15)) * 4 + (lane >> 4);
-      *p = (*p & ~vmask) | vword;
+  for (int j = 0; j < 8; ++j) {
+    const long t = t0 + row_of(j);
+    live[j] = t >= 0 && t < a.T && blk * kBlk + row_of(j) < a.c.rows;
+    x[j] = src[((long)b * a.T + min(max(t, 0L), (long)a.T - 1)) * ld + (long)hg * kGrp + lane];
+  }
+  unsigned kept = 0, mask = 0, pairs = 0;  // keys: the lane's dword of row lane % 8
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (!live[j]) continue;  // uniform
+    unsigned pair;
+    const unsigned q = quantise(x[j], &pair);
+    if ((lane & 7) == j) pairs = pair;
+    if (plane) {
+      kept |= q4_put(q, j);
+      mask |= q4_put(15u, j);
+    } else {
+      // eight channels make a dword
+      int kw = (int)q4_put(q, lane & 7);
+      kw |= __builtin_amdgcn_mov_dpp(kw, kDppXor1, 0xF, 0xF, false);
+      kw |= __builtin_amdgcn_mov_dpp(kw, kDppXor2, 0xF, 0xF, false);
+      kw |= __builtin_amdgcn_mov_dpp(kw, kDppHalfMirror, 0xF, 0xF, false);
+      if ((lane & 7) == j) kept = (unsigned)kw;
     }
   }
+  const int j = lane & 7, r = row_of(j), o = lane >> 3;
+  const long tj = t0 + r;
+  const bool mine = tj >= 0 && tj < a.T && blk * kBlk + r < a.c.rows;
+  unsigned* codes = reinterpret_cast<unsigned*>(rec + (plane * ng + g) * kCodes);
+  if (plane) {
+    if (mask) {
+      unsigned* p = codes + (w * 16 + (lane & 15)) * 4 + (lane >> 4);
+      *p = mask == ~0u ? kept : (*p & ~mask) | kept;
+    }
+  } else if (mine) {
+    codes[(((o & 3) * 16 + (r & 15)) * 2 + (r >> 4)) * 2 + (o >> 2)] = kept;
+  }
+  if (lane < 8 && mine)
+    reinterpret_cast<unsigned*>(rec + 2 * ng * kCodes)[(plane * ng + g) * kBlk + r] = pairs;
 }
 
 struct ReadArgs {
@@ -622,14 +639,17 @@ AttnPlan attn_plan(const Kv4& c, int nrow, int max_len) {
   const long wgs = (long)p.tiles * c.batch * c.heads;
   const int steps = (len + kBlk * p.kp - 1) / (kBlk * p.kp);
   // Splits take four waves, one per SIMD; the time in steps of a wave is workgroups a CU x steps
-  // a wave, and about five for the join's launch.
-  constexpr int kWaves = 4;
-  constexpr long kJoin = 5;
-  long best = LONG_MAX;
+  // a wave, and about five for the join's launch (1 sequence of 2001 rows, 2 kv heads: one
+  // split 11.1 us, eight 7.6 with the join; 48 of up to 4000: two 18.1, eight 15.2; 156 tiles of a
+  // prompt chunk over 1708 rows: one 13.9, two 20.2).
+  constexpr int kWaves = 4, kJoin = 5;
+  const int base = (int)std::min<long>(wgs, 1 << 20);
+  int best = INT_MAX;
   p.splits = 1;
-  for (int s = 1; s <= std::min(steps, kMaxSplits); ++s) {
-    const long t = (wgs * s + cus - 1) / cus * ((steps + kWaves * s - 1) / (kWaves * s)) +
-                   (s > 1 ? kJoin : 0);
+  for (const int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 40, 48, 64}) {
+    if (s > steps) break;
+    const int t = (base * s + cus - 1) / cus * ((steps + kWaves * s - 1) / (kWaves * s)) +
+                  (s > 1 ? kJoin : 0);
     if (t < best) {
       best = t;
       p.splits = s;
@@ -657,7 +677,7 @@ int launch_attn(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
 }
 
 bool kv4_shape_ok(int batch, int heads, int hd, int rows) {
-  return batch > 0 && batch <= 65535 && heads > 0 && heads <= 65535 && (hd == 64 || hd == 128) &&
+  return batch > 0 && batch <= 65535 && heads > 0 && heads <= 32767 && (hd == 64 || hd == 128) &&
          rows > 0 && rows <= INT_MAX - kBlk;
 }
 
@@ -697,10 +717,10 @@ extern "C" int lx_kv4_append_f32(const lx_kv4* cache, const float* k, long ldk, 
   a.T = T;
   a.pos = pos;
   // records that T rows can touch, wherever they begin
-  a.touched = (int)std::min<long>(((long)T + kBlk - 2) / kBlk + 1, a.c.blocks);
-  const long grid = (long)a.touched * cache->batch * cache->n_kv_heads;
-  LX_REQUIRE(grid <= INT_MAX, "kv4_append: %ld workgroups", grid);
-  hipLaunchKernelGGL(kv4_append_kernel, dim3((unsigned)grid), dim3(256), 0, stream, a);
+  const long touched = std::min<long>(((long)T + kBlk - 2) / kBlk + 1, a.c.blocks);
+  hipLaunchKernelGGL(kv4_append_kernel,
+                     dim3((unsigned)touched, a.c.heads * a.c.ng, cache->batch), dim3(512), 0,
+                     stream, a);
   return check_launch("kv4_append_kernel");
 }
 

@@ -509,20 +509,17 @@ def attention_kv4(q, cache, lens, n_heads, scale=None, causal=True, out=None, ma
     dev = cache._dev
     if q.get_device() != dev:
         _elsewhere("q")
-    n = lib.lx_attention_kv4_ws_floats(cache._ref, Tq, n_heads, max_len)
     if out is None:
-        # the splits' states behind the output (rows of 64: aligned)
-        m = cache.batch * Tq * width
-        buf = q.new_empty(m + n)
-        out, ldo, o = buf[:m].view(shape) if n else buf.view(shape), width, buf.data_ptr()
-        ws = o + 4 * m if n else None
+        out, ldo = q.new_empty(shape), width
     else:
-        ldo, o = _rows(out, "out", shape), out.data_ptr()
+        ldo = _rows(out, "out", shape)
         if out.get_device() != dev:
             _elsewhere("out")
-        buf = q.new_empty(n) if n else None
-        ws = buf.data_ptr() if n else None
-    check(lib.lx_attention_kv4_f32(q.data_ptr(), ldq, cache._ref, lens.data_ptr(), o, ldo, Tq,
-                                   n_heads, cache.head_dim ** -0.5 if scale is None else scale,
-                                   int(causal), max_len, ws, n, _raw_stream(dev)))
+    n = lib.lx_attention_kv4_ws_floats(cache._ref, Tq, n_heads, max_len)
+    ws = q.new_empty(n) if n else None
+    check(lib.lx_attention_kv4_f32(q.data_ptr(), ldq, cache._ref, lens.data_ptr(), out.data_ptr(),
+                                   ldo, Tq, n_heads,
+                                   cache.head_dim ** -0.5 if scale is None else scale,
+                                   int(causal), max_len, ws.data_ptr() if n else None, n,
+                                   _raw_stream(dev)))
     return out

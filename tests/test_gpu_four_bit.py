@@ -291,6 +291,31 @@ def test_append_equals_the_definition_and_leaves_other_rows(gpu, hd, kv, T, pos)
         assert np.array_equal(got.astype(np.float64), ref.astype(np.float32))
 
 
+def test_append_codes_next_to_borders(gpu):
+    """Values on the borders between codes and one step of fp32 to either side, under scales of
+    many sizes, subnormal ones too: where a quotient taken in 32 bits could fall either way."""
+    from larynx_amd import ops
+    announce("kv4 append borders")
+    rng = _gen(21)
+    rows = 2000
+    s = (2.0 ** rng.integers(-20, 20, (rows, 1)) * (1 + rng.integers(0, 128, (rows, 1)) / 128))
+    s[-200:] = 2.0 ** -133 * rng.integers(1, 200, (200, 1))
+    z = np.float32(s * rng.integers(-128, 128, (rows, 1)) * 2.0 ** rng.integers(-3, 3, (rows, 1)))
+    z = np.float32(_bf16_steps(z.astype(np.float64), np.floor))
+    q = rng.integers(0, 15, (rows, 64)) + rng.choice([0.0, 0.5, 0.5], (rows, 64))
+    x = np.float32(z + s * q)
+    x = np.where(rng.random(x.shape) < 0.3, np.nextafter(x, np.float32(np.inf)), x)
+    x = np.where(rng.random(x.shape) < 0.3, np.nextafter(x, np.float32(-np.inf)), x)
+    x[:, 0], x[:, 1] = z[:, 0], np.float32(z + 15 * s)[:, 0]
+    x = x.astype(np.float32)[None]
+    cache = ops.kv4_cache(1, 1, rows)
+    zero = torch.zeros(1, dtype=torch.int32, device=gpu)
+    ops.kv4_append(cache, _dev(x, gpu), _dev(-x, gpu), zero)
+    for got, src in zip(ops.kv4_read(cache, zero, rows), (x, -x)):
+        ref = ref_cache(src.reshape(1, rows, 1, 64))[0].reshape(1, rows, 64)
+        assert np.array_equal(got.cpu().numpy(), ref.astype(np.float32))
+
+
 def test_append_outside_the_cache_writes_nothing(gpu):
     from larynx_amd import ops
     announce("kv4 append outside")
