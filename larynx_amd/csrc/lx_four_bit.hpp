@@ -55,13 +55,12 @@ __device__ __forceinline__ unsigned q4_get(unsigned w, int j) {
   return (w >> (4 * (j >> 1) + 16 * (j & 1))) & 15u;
 }
 
-// x (scaled) as two fp16 parts; contraction off, as in pack2_bf16.
-__device__ __forceinline__ void split2(const float (&x)[8], half8_t& p0, half8_t& p1) {
-#pragma clang fp contract(off)
+// x s as two fp16 parts, s a power of two (the fused remainder is exact, as x s is).
+__device__ __forceinline__ void split2(const float (&x)[8], float s, half8_t& p0, half8_t& p1) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) p0[j] = (_Float16)x[j];
+  for (int j = 0; j < 8; ++j) p0[j] = (_Float16)(x[j] * s);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) p1[j] = (_Float16)(x[j] - (float)p0[j]);
+  for (int j = 0; j < 8; ++j) p1[j] = (_Float16)fmaf(x[j], s, -(float)p0[j]);
 }
 
 // The power of two that brings a row with largest magnitude `top` to 1 .. 2, and its inverse

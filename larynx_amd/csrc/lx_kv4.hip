@@ -355,11 +355,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[g][ks][j] *= sc;
-          s += x[g][ks][j];
-        }
-        split2(x[g][ks], qf[g][ks][0], qf[g][ks][1]);
+        for (int j = 0; j < 8; ++j) s = fmaf(x[g][ks][j], sc, s);
+        split2(x[g][ks], sc, qf[g][ks][0], qf[g][ks][1]);
         if (NG == 2 && wave == 0) {
           ql[(g * 4 + ks * 2) * 64] = qf[g][ks][0];
           ql[(g * 4 + ks * 2 + 1) * 64] = qf[g][ks][1];
@@ -463,15 +460,14 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
     }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      float ps[8];
+      half8_t p0, p1;  // of p s: the remainder of the first part is taken from the exact product
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float ss = bf16_lo(vp[g][j >> 2][j & 3]), z = bf16_hi(vp[g][j >> 2][j & 3]);
-        ps[j] = p[j] * ss;
+        p0[j] = (_Float16)(p[j] * ss);
+        p1[j] = (_Float16)fmaf(p[j], ss, -(float)p0[j]);
         zsum[g] = fmaf(p[j], fmaf(8.0f, ss, z), zsum[g]);
       }
-      half8_t p0, p1;
-      split2(ps, p0, p1);
 #pragma unroll
       for (int r = 0; r < KP; ++r) {
         // the weights of this record's columns alone: the others' belong to other values

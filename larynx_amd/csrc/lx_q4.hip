@@ -270,10 +270,8 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
       float inv;
       const float sc = row_scale(top, &inv);
       if (col == 0) finv[4 * p + c] = inv;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= sc;
       half8_t p0, p1;
-      split2(v, p0, p1);
+      split2(v, sc, p0, p1);
       char* row = mine + 2 * (4 * p + c) * kFewRow + col * 16;
       *reinterpret_cast<half8_t*>(row) = p0;
       *reinterpret_cast<half8_t*>(row + kFewRow) = p1;
@@ -464,194 +462,134 @@ __global__ __launch_bounds__(64) void q4_row_kernel(Q4Args a, DecGemvArgs d) {
   }
 }
 
-// Up to 64 rows of x in CT column tiles of 16.  A workgroup of eight waves takes groups of 8 RT
-// tiles of weight rows, RT a wave, over one of a.splits ranges of the blocks of K.  x goes through
-// LDS as fragments of its two parts, a chunk of 8 / CT blocks at a time, each wave splitting the 16
-// rows x 128 inputs of one (block, column tile).  Where the range is one chunk, x is split once
-// and the workgroup walks over the groups; else the next chunk is split into a second buffer
-// while one is worked on, a barrier a chunk.  The weights come D blocks ahead, over the ends of
-// groups too.  One split: the epilogue from the accumulators; more: partial sums into ws (splits, M, N up
-// to 16), which q4_join_kernel adds in split order.
+// Up to 64 rows of x in CT column tiles of 16.  The waves of a workgroup own one block of K each, of
+// the at most eight of a split: a wave splits its 16 CT rows x 128 inputs of x once, keeps the
+// fragments in registers (32 CT of them) and streams the weights of its block past them, RT tiles
+// of 16 rows at a time, one group of tiles ahead.  The waves' sums meet in one of two LDS buffers
+// (a barrier a group), added in wave order; each thread adds and finishes one quad of outputs.
+// More than one split: partial sums into ws (splits, M, N up to 16), which q4_join_kernel adds in
+// split order.  (With x in LDS and whole K ranges a wave, every fragment of x is read again for
+// every two tiles: 64 rows 8192 x 8192 33 us, 9728 x 896 17.)
 constexpr int kManyWaves = 8;
-
-template <int CT>
-constexpr int many_blocks() { return CT == 1 ? 8 : CT == 2 ? 4 : 2; }
-// Tiles a wave: two share each fragment of x that they read, while the registers hold them.
-constexpr int many_rt(int ct, int g) { return ct <= 2 || g == 32 ? 1 : 2; }
-// bytes of `blocks` blocks of x
-template <int CT>
-constexpr size_t many_bytes(int blocks) { return (size_t)blocks * CT * (8 * 1024 + 64); }
+constexpr int many_rt(int ct) { return ct == 1 ? 4 : 2; }
+constexpr size_t many_bytes(int ct) { return (size_t)2 * kManyWaves * many_rt(ct) * ct * 1024; }
 
 template <int CT, int G>
 __global__ __launch_bounds__(64 * kManyWaves) __attribute__((
     amdgpu_waves_per_eu(CT == 1 ? 4 : 2))) void q4_many_kernel(Q4Args a) {
-  constexpr int TG = G / 32, NG = kBlockK / G, CH = many_blocks<CT>(), RT = many_rt(CT, G);
-  constexpr int D = 2;
-  // per buffer [block][step][column tile][part][lane] fragments, then [block][column tile][16]
-  // inverse scales
-  extern __shared__ __attribute__((aligned(16))) char lds[];
+  constexpr int TG = G / 32, NG = kBlockK / G, RT = many_rt(CT);
+  extern __shared__ __attribute__((aligned(16))) char lds[];  // [2][wave][RT][CT][lane] quads
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int c = lane >> 4, col = lane & 15;
   const unsigned pattern = q4_pattern();
   const int sp = blockIdx.y, per = (a.kb + a.splits - 1) / a.splits;
-  const int k0 = sp * per, nb = min(per, a.kb - k0);  // > 0
+  const int nb = min(per, a.kb - sp * per);  // blocks of this split, 1 .. 8: the waves that multiply
+  const int kb = sp * per + min(wave, nb - 1);
   const long tiles = q4_tiles(a.N);
-  const int groups = (int)((tiles + kManyWaves * RT - 1) / (kManyWaves * RT));
-  const int items = ((groups - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) * nb;
-  const int bufb = min(nb, CH) * CT;  // fragments of a buffer, in 8 KB
-  const int sb = wave / CT, sct = wave % CT;  // what this wave splits of a chunk
-  float4 xs[4][2];
-  auto load_x = [&](int kb) {  // kb: within the range
-    const float* xr = a.x + (long)min(sct * 16 + col, a.M - 1) * a.ldx;
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        xs[t][e] = *reinterpret_cast<const float4*>(
-            xr + min((k0 + kb) * kBlockK + 32 * t + 8 * c + 4 * e, a.K - 4));
-  };
-  auto buffer = [&](int chunk) { return lds + (size_t)(chunk & 1) * bufb * (8 * 1024 + 64); };
-  auto store_x = [&](int kb, char* buf) {
-    float v[4][8], top = 0.0f;
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const bool past = (k0 + kb) * kBlockK + 32 * t + 8 * c + 4 * e >= a.K;
-        v[t][4 * e] = past ? 0.0f : xs[t][e].x;
-        v[t][4 * e + 1] = past ? 0.0f : xs[t][e].y;
-        v[t][4 * e + 2] = past ? 0.0f : xs[t][e].z;
-        v[t][4 * e + 3] = past ? 0.0f : xs[t][e].w;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(v[t][4 * e + j]));
-      }
-    top = fmaxf(top, lane_xor16(top));
-    top = fmaxf(top, lane_xor32(top));
-    float f;
-    const float sc = row_scale(top, &f);
-    if (c == 0)
-      reinterpret_cast<float*>(buf + bufb * 8 * 1024)[(sb * CT + sct) * 16 + col] = f;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[t][j] *= sc;
-      half8_t p0, p1;
-      split2(v[t], p0, p1);
-      half8_t* dst = reinterpret_cast<half8_t*>(buf) + (((sb * 4 + t) * CT + sct) * 2) * 64 + lane;
-      dst[0] = p0;
-      dst[64] = p1;
-    }
-  };
-  uintx4_t w[D][RT];
-  ushortx4_t sc[D][RT][NG];
-  // item i of this workgroup: block i % nb of its (i / nb)-th group; kept as running counters
-  int lg = blockIdx.x, lk = 0, left = items;
-  auto load_w = [&](int d) {
-    if (left <= 0) return;
+  const int groups = (int)((tiles + RT - 1) / RT);
+  uintx4_t w[RT];
+  ushortx4_t sc[RT][NG];
+  auto load_w = [&](int group) {
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const long tile = min(((long)lg * kManyWaves + wave) * RT + r, tiles - 1) * a.kb + k0 + lk;
-      w[d][r] = a.codes[tile * 64 + lane];
+      const long tile = min((long)group * RT + r, tiles - 1) * a.kb + kb;
+      w[r] = a.codes[tile * 64 + lane];
       const ushortx4_t* p = reinterpret_cast<const ushortx4_t*>(a.scales) + (tile * 4 + c) * NG;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) sc[d][r][g] = p[g];
-    }
-    --left;
-    if (++lk == nb) {
-      lk = 0;
-      lg += gridDim.x;
+      for (int g = 0; g < NG; ++g) sc[r][g] = p[g];
     }
   };
-  const bool stages = sb < CH;
-  if (stages && sb < nb) load_x(sb);
+  load_w(blockIdx.x);
+  half8_t xf[CT][4][2];
+  float f[CT];
+  {
+    float4 u[CT][4][2];  // all requested before the first is used
 #pragma unroll
-  for (int d = 0; d < D; ++d) load_w(d);
-  if (stages && sb < nb) store_x(sb, buffer(0));
-  __syncthreads();
-  if (stages && CH + sb < nb) load_x(CH + sb);
-
-  floatx4 tot[RT][CT];
-  int kb = 0, chunk = 0, in_chunk = 0, group = blockIdx.x;
-  for (int i = 0; i < items; i += D) {
+    for (int ct = 0; ct < CT; ++ct) {
+      const float* xr = a.x + (long)min(ct * 16 + col, a.M - 1) * a.ldx;
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-      if (i + d >= items) break;
-      if (kb == 0)
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+        for (int e = 0; e < 2; ++e)
+          u[ct][t][e] = *reinterpret_cast<const float4*>(
+              xr + min(kb * kBlockK + 32 * t + 8 * c + 4 * e, a.K - 4));
+    }
+    const bool ragged = (kb + 1) * kBlockK > a.K;
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) tot[r][ct] = floatx4{0.f, 0.f, 0.f, 0.f};
-      const char* buf = buffer(chunk);
-      const half8_t* fb =
-          reinterpret_cast<const half8_t*>(buf) + in_chunk * 4 * CT * 128 + lane;
-      float f[CT];
+    for (int ct = 0; ct < CT; ++ct) {
+      float v[4][8], top = 0.0f;
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-        f[ct] = reinterpret_cast<const float*>(buf + bufb * 8 * 1024)[(in_chunk * CT + ct) * 16 +
-                                                                      col];
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        floatx4 acc[RT][CT];
+        for (int e = 0; e < 2; ++e) {
+          float4 x = u[ct][t][e];
+          if (ragged && kb * kBlockK + 32 * t + 8 * c + 4 * e >= a.K)
+            x = make_float4(0.f, 0.f, 0.f, 0.f);
+          v[t][4 * e] = x.x;
+          v[t][4 * e + 1] = x.y;
+          v[t][4 * e + 2] = x.z;
+          v[t][4 * e + 3] = x.w;
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) acc[r][ct] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int t = g * TG; t < (g + 1) * TG; ++t) {
-          half8_t wf[RT];
-#pragma unroll
-          for (int r = 0; r < RT; ++r) wf[r] = q4_frag(w[d][r][t], pattern);
-#pragma unroll
-          for (int p = 1; p >= 0; --p)
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-              const half8_t xf = fb[((t * CT + ct) * 2 + p) * 64];
-#pragma unroll
-              for (int r = 0; r < RT; ++r) acc[r][ct] = mfma_f16(wf[r], xf, acc[r][ct]);
-            }
+          for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(v[t][4 * e + j]));
         }
+      top = fmaxf(top, lane_xor16(top));
+      top = fmaxf(top, lane_xor32(top));
+      const float xs = row_scale(top, &f[ct]);
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float s = bf16_lo(sc[d][r][g][e]);
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct)
-              tot[r][ct][e] = fmaf(s * f[ct], acc[r][ct][e], tot[r][ct][e]);
-          }
-      }
-      load_w(d);
-      if (++kb < nb) {
-        if (++in_chunk == CH) {
-          // the next chunk into the other buffer, which all have read since the last barrier
-          ++chunk;
-          in_chunk = 0;
-          if (stages && chunk * CH + sb < nb) store_x(chunk * CH + sb, buffer(chunk));
-          __syncthreads();
-          if (stages && (chunk + 1) * CH + sb < nb) load_x((chunk + 1) * CH + sb);
-        }
-        continue;
-      }
-      // the group is done (with more than one, x is a single chunk)
+      for (int t = 0; t < 4; ++t) split2(v[t], xs, xf[ct][t][0], xf[ct][t][1]);
+    }
+  }
+  int buf = 0;
+  for (int group = blockIdx.x; group < groups; group += gridDim.x, buf ^= 1) {
+    char* red = lds + (size_t)buf * kManyWaves * RT * CT * 1024;
+    if (wave < nb) {
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        const long tile = ((long)group * kManyWaves + wave) * RT + r, n = tile * kTileN + 4 * c;
-        if (tile >= tiles) break;
+        floatx4 tot[CT];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          floatx4 acc[CT];
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) acc[ct] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int t = g * TG; t < (g + 1) * TG; ++t) {
+            const half8_t wf = q4_frag(w[r][t], pattern);
+#pragma unroll
+            for (int p = 1; p >= 0; --p)
+#pragma unroll
+              for (int ct = 0; ct < CT; ++ct) acc[ct] = mfma_f16(wf, xf[ct][t][p], acc[ct]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float s = bf16_lo(sc[r][g][e]);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+              tot[ct][e] = g == 0 ? s * acc[ct][e] : fmaf(s, acc[ct][e], tot[ct][e]);
+          }
+        }
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-          const int m = ct * 16 + col;
-          if (m >= a.M) continue;
-          if (a.splits > 1) {
-            *reinterpret_cast<floatx4*>(a.ws + ((long)sp * a.M + m) * (tiles * kTileN) + n) =
-                tot[r][ct];
-            continue;
-          }
-          q4_epi_quad(a, m, n, tot[r][ct]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) tot[ct][e] *= f[ct];
+          reinterpret_cast<floatx4*>(red)[((wave * RT + r) * CT + ct) * 64 + lane] = tot[ct];
         }
       }
-      kb = 0;
-      in_chunk = 0;
-      group += gridDim.x;
+      if (group + (int)gridDim.x < groups) load_w(group + gridDim.x);
+    }
+    __syncthreads();
+    for (int u = tid; u < RT * CT * 64; u += 64 * kManyWaves) {
+      const int ct = (u >> 6) % CT, r = (u >> 6) / CT;
+      const int m = ct * 16 + col;
+      const long tile = (long)group * RT + r, n = tile * kTileN + 4 * c;
+      if (m >= a.M || tile >= tiles) continue;
+      floatx4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kManyWaves; ++i)
+        if (i < nb) s += reinterpret_cast<const floatx4*>(red)[i * RT * CT * 64 + u];
+      if (a.splits > 1)
+        *reinterpret_cast<floatx4*>(a.ws + ((long)sp * a.M + m) * (tiles * kTileN) + n) = s;
+      else
+        q4_epi_quad(a, m, n, s);
     }
   }
 }
@@ -688,34 +626,26 @@ int launch_few(const Q4Args& a, int G, hipStream_t s) {
   return check_launch("q4_few_kernel");
 }
 
-// Splits of K of q4_many_kernel: about one workgroup a CU.
-int many_splits(int M, int N, int K) {
-  const int kb = (int)q4_blocks(K), rows = kManyWaves * (M > 32 ? 2 : 1);
-  if (M <= 8) return 1;
-  const long groups = (q4_tiles(N) + rows - 1) / rows;
-  const int s = (int)std::max(1L, std::min<long>(kb, device_cus() / groups));
-  const int per = (kb + s - 1) / s;
-  return (kb + per - 1) / per;
-}
+// Splits of K of q4_many_kernel: at most a block a wave.
+int many_splits(int K) { return (int)((q4_blocks(K) + kManyWaves - 1) / kManyWaves); }
 
 template <int CT, int G>
 int raise_many() {
   static LdsLimit once;
-  return raise_lds_limit(reinterpret_cast<const void*>(q4_many_kernel<CT, G>),
-                         many_bytes<CT>(2 * many_blocks<CT>()), once, "q4_many_kernel");
+  return raise_lds_limit(reinterpret_cast<const void*>(q4_many_kernel<CT, G>), many_bytes(CT),
+                         once, "q4_many_kernel");
 }
 
 template <int CT>
 int launch_many(const Q4Args& a, int G, hipStream_t s) {
   LX_TRY(G == 32 ? (raise_many<CT, 32>())
                  : G == 64 ? (raise_many<CT, 64>()) : (raise_many<CT, 128>()));
-  const int per = (a.kb + a.splits - 1) / a.splits, chunk = many_blocks<CT>();
-  const int rows = kManyWaves * many_rt(CT, G);
-  const long groups = (q4_tiles(a.N) + rows - 1) / rows;
-  // one chunk of x: two workgroups a CU walk over the groups
-  const long wgs = per <= chunk ? std::min(groups, 2L * device_cus()) : groups;
-  const dim3 grid((unsigned)wgs, a.splits), block(64 * kManyWaves);
-  const size_t lds = many_bytes<CT>(per <= chunk ? per : 2 * chunk);
+  const long groups = (q4_tiles(a.N) + many_rt(CT) - 1) / many_rt(CT);
+  // as many workgroups as the CUs hold at once walk over the groups
+  const long slots = (CT == 1 ? 2L : 1L) * device_cus();
+  const dim3 grid((unsigned)std::min(groups, std::max(1L, slots / a.splits)), a.splits),
+      block(64 * kManyWaves);
+  const size_t lds = many_bytes(CT);
   LX_Q4_GROUPS(q4_many_kernel, CT)
   return check_launch("q4_many_kernel");
 }
@@ -728,7 +658,7 @@ int launch_many(const Q4Args& a, int G, hipStream_t s) {
 // (few tiles, each a long run of blocks) 11.8 / 8.5.
 bool q4_takes_few(int M, int N, int K) {
   const long tiles = q4_tiles(N), kb = q4_blocks(K), work = tiles * kb;
-  if (M <= 8) return tiles < 2048 || work <= (M <= 4 ? 35000 : 9000);
+  if (M <= 8) return kb > kManyWaves || work <= (M <= 4 ? 35000 : 9000);
   return M <= 16 && work <= 4096 && kb <= 16;
 }
 
@@ -851,7 +781,7 @@ extern "C" int lx_q4_unpack_f32(const void* Wq, float* W, int N, int K, int grou
 
 extern "C" size_t lx_linear_q4_ws_floats(int M, int N, int K) {
   if (M < 1 || M > kMaxRows || !q4_shape_ok(N, K, 64) || q4_takes_few(M, N, K)) return 0;
-  const int splits = many_splits(M, N, K);
+  const int splits = many_splits(K);
   return splits == 1 ? 0 : (size_t)splits * M * q4_tiles(N) * kTileN;
 }
 
@@ -893,7 +823,7 @@ extern "C" int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int gr
     if (M <= 8) return launch_few<8>(a, group, stream);
     return launch_few<16>(a, group, stream);
   }
-  a.splits = many_splits(M, N, K);
+  a.splits = many_splits(K);
   if (a.splits > 1) {
     const size_t need = (size_t)a.splits * M * q4_tiles(N) * kTileN;
     LX_REQUIRE(ws && ws_floats >= need && (uintptr_t)ws % 16 == 0,
