@@ -387,8 +387,8 @@ int lx_q4_unpack_f32(const void* Wq, float* W, int N, int K, int group, hipStrea
  * SWIGLU_PAIRED (others: LX_ERR_ARG); bias (N) or NULL.  K and ldx multiples of
  * 4, x and Wq 16-byte aligned.  An infinite or NaN element of x makes NaN of its
  * row.  The result does not depend on timing.  ws: lx_linear_q4_ws_floats() floats
- * of scratch, 16-byte aligned (NULL when that is 0: up to 8 rows, and most calls of
- * up to 16); calls that share it must not overlap.
+ * of scratch, 16-byte aligned (NULL when that is 0: up to 4 rows, and K up to 1024);
+ * calls that share it must not overlap.
  * Replaces linear() (src/llm/ops.cpp:13-19) for weights given in 4 bits. */
 size_t lx_linear_q4_ws_floats(int M, int N, int K);
 int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int group, const float* bias,

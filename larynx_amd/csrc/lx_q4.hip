@@ -192,8 +192,8 @@ __device__ __forceinline__ void q4_epi_quad(const Q4Args& a, int m, long n, floa
 
 // At most MB rows of x.  A workgroup owns one tile of 16 weight rows; its waves take the blocks
 // of K in turn, each splitting its own 128 inputs of x into a slice of LDS (16 lanes a row, four
-// rows at a time), and their sums meet in LDS at the end (in a fixed order).  MB <= 8: column 2 m
-// + part of one fragment; MB = 16: column m of two.
+// rows at a time), and their sums meet in LDS at the end (in a fixed order).  Column 2 m + part of
+// the fragments is a part of row m.
 constexpr int kFewRow = 272;  // bytes of a staged row (128 fp16, and 16 against bank conflicts)
 
 template <int MB>
@@ -226,8 +226,6 @@ struct FewIn {
 template <int MB, int G>
 __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
   constexpr int TG = G / 32, NG = kBlockK / G;
-  constexpr bool PK = MB <= 8;
-  constexpr int NP = PK ? 1 : 2;
   extern __shared__ __attribute__((aligned(16))) char lds[];  // [waves][few_bytes]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
   const int c = lane >> 4, col = lane & 15;
@@ -285,18 +283,15 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const char* xr = mine + (PK ? min(col, 2 * MB - 1) : 2 * col) * kFewRow + c * 16;
-    const float f = finv[PK ? min(col >> 1, MB - 1) : col];
+    const char* xr = mine + min(col, 2 * MB - 1) * kFewRow + c * 16;
+    const float f = finv[min(col >> 1, MB - 1)];
     floatx4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int t = g * TG; t < (g + 1) * TG; ++t) {
-        const half8_t wf = q4_frag(w[t], pattern);
-#pragma unroll
-        for (int p = NP - 1; p >= 0; --p)
-          acc = mfma_f16(wf, *reinterpret_cast<const half8_t*>(xr + p * kFewRow + t * 64), acc);
+        acc = mfma_f16(q4_frag(w[t], pattern), *reinterpret_cast<const half8_t*>(xr + t * 64), acc);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[i] = fmaf(bf16_lo(sc[g][i]), acc[i], sum[i]);
@@ -317,7 +312,7 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
     for (int w = q; w < waves; w += 4) {
       const float* p = reinterpret_cast<const float*>(lds + w * few_bytes<MB>()) + (r & 3) * 64 +
                        (r >> 2) * 16;
-      s += PK ? p[2 * m + 1] + p[2 * m] : p[m];
+      s += p[2 * m + 1] + p[2 * m];
     }
     s += dpp_mov<kDppXor1>(s);
     s += dpp_mov<kDppXor2>(s);
@@ -471,13 +466,17 @@ __global__ __launch_bounds__(64) void q4_row_kernel(Q4Args a, DecGemvArgs d) {
 // split order.  (With x in LDS and whole K ranges a wave, every fragment of x is read again for
 // every two tiles: 64 rows 8192 x 8192 33 us, 9728 x 896 17.)
 constexpr int kManyWaves = 8;
-constexpr int many_rt(int ct) { return ct == 1 ? 4 : 2; }
-constexpr size_t many_bytes(int ct) { return (size_t)2 * kManyWaves * many_rt(ct) * ct * 1024; }
+constexpr int kManyTiles = 2;  // RT
+constexpr size_t many_bytes(int ct) {
+  const size_t sums = (size_t)2 * kManyWaves * kManyTiles * ct * 1024;
+  const size_t split = (size_t)kManyWaves * few_bytes<16>();
+  return sums > split ? sums : split;
+}
 
 template <int CT, int G>
 __global__ __launch_bounds__(64 * kManyWaves) __attribute__((
     amdgpu_waves_per_eu(CT == 1 ? 4 : 2))) void q4_many_kernel(Q4Args a) {
-  constexpr int TG = G / 32, NG = kBlockK / G, RT = many_rt(CT);
+  constexpr int TG = G / 32, NG = kBlockK / G, RT = kManyTiles;
   extern __shared__ __attribute__((aligned(16))) char lds[];  // [2][wave][RT][CT][lane] quads
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int c = lane >> 4, col = lane & 15;
@@ -487,62 +486,100 @@ __global__ __launch_bounds__(64 * kManyWaves) __attribute__((
   const int kb = sp * per + min(wave, nb - 1);
   const long tiles = q4_tiles(a.N);
   const int groups = (int)((tiles + RT - 1) / RT);
-  uintx4_t w[RT];
-  ushortx4_t sc[RT][NG];
-  auto load_w = [&](int group) {
+  uintx4_t w[RT], wn[RT];
+  ushortx4_t sc[RT][NG], scn[RT][NG];
+  auto load_w = [&](int group) {  // past the last group: the last
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const long tile = min((long)group * RT + r, tiles - 1) * a.kb + kb;
-      w[r] = a.codes[tile * 64 + lane];
+      wn[r] = a.codes[tile * 64 + lane];
       const ushortx4_t* p = reinterpret_cast<const ushortx4_t*>(a.scales) + (tile * 4 + c) * NG;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) sc[r][g] = p[g];
+      for (int g = 0; g < NG; ++g) scn[r][g] = p[g];
     }
   };
   load_w(blockIdx.x);
   half8_t xf[CT][4][2];
   float f[CT];
   {
+    // 16 lanes a row, so that an instruction reads whole lines (a lane a row reads 64 of them:
+    // 17000 accesses, 7 us, for 64 rows), then through this wave's slice of LDS
+    char* mine = lds + wave * few_bytes<16>();
+    float* finv = reinterpret_cast<float*>(mine + 32 * kFewRow);
     float4 u[CT][4][2];  // all requested before the first is used
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const float* xr = a.x + (long)min(ct * 16 + col, a.M - 1) * a.ldx;
+    for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int p = 0; p < 4; ++p) {
+        const float* xr = a.x + (long)min(ct * 16 + 4 * p + c, a.M - 1) * a.ldx;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          u[ct][t][e] = *reinterpret_cast<const float4*>(
-              xr + min(kb * kBlockK + 32 * t + 8 * c + 4 * e, a.K - 4));
-    }
-    const bool ragged = (kb + 1) * kBlockK > a.K;
+          u[ct][p][e] = *reinterpret_cast<const float4*>(
+              xr + min(kb * kBlockK + 64 * e + 4 * col, a.K - 4));
+      }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      float v[4][8], top = 0.0f;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        float v[8], top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const bool none = kb * kBlockK + 64 * e + 4 * col >= a.K;
+          const float4 x = u[ct][p][e];
+          v[4 * e] = none ? 0.0f : x.x;
+          v[4 * e + 1] = none ? 0.0f : x.y;
+          v[4 * e + 2] = none ? 0.0f : x.z;
+          v[4 * e + 3] = none ? 0.0f : x.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
+        top = fmaxf(top, dpp_mov<kDppXor1>(top));
+        top = fmaxf(top, dpp_mov<kDppXor2>(top));
+        top = fmaxf(top, dpp_mov<kDppHalfMirror>(top));
+        top = fmaxf(top, dpp_mov<kDppMirror>(top));
+        float inv;
+        const float xs = row_scale(top, &inv);
+        if (col == 0) finv[4 * p + c] = inv;
+        half8_t p0, p1;
+        split2(v, xs, p0, p1);
+        const uintx4_t b0 = __builtin_bit_cast(uintx4_t, p0), b1 = __builtin_bit_cast(uintx4_t, p1);
+        char* row = mine + 2 * (4 * p + c) * kFewRow + col * 8;
+        *reinterpret_cast<uintx2_t*>(row) = uintx2_t{b0[0], b0[1]};
+        *reinterpret_cast<uintx2_t*>(row + 128) = uintx2_t{b0[2], b0[3]};
+        *reinterpret_cast<uintx2_t*>(row + kFewRow) = uintx2_t{b1[0], b1[1]};
+        *reinterpret_cast<uintx2_t*>(row + kFewRow + 128) = uintx2_t{b1[2], b1[3]};
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      f[ct] = finv[col];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float4 x = u[ct][t][e];
-          if (ragged && kb * kBlockK + 32 * t + 8 * c + 4 * e >= a.K)
-            x = make_float4(0.f, 0.f, 0.f, 0.f);
-          v[t][4 * e] = x.x;
-          v[t][4 * e + 1] = x.y;
-          v[t][4 * e + 2] = x.z;
-          v[t][4 * e + 3] = x.w;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(v[t][4 * e + j]));
-        }
-      top = fmaxf(top, lane_xor16(top));
-      top = fmaxf(top, lane_xor32(top));
-      const float xs = row_scale(top, &f[ct]);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) split2(v[t], xs, xf[ct][t][0], xf[ct][t][1]);
+        for (int p = 0; p < 2; ++p)
+          xf[ct][t][p] = *reinterpret_cast<const half8_t*>(mine + (2 * col + p) * kFewRow + t * 64 +
+                                                           c * 16);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
     }
+    __syncthreads();  // the slices become the buffers of sums
   }
+  if (wave >= nb)  // no block: zeros for good
+#pragma unroll
+    for (int i = 0; i < 2 * RT * CT; ++i)
+      reinterpret_cast<floatx4*>(lds)[((i & 1) * kManyWaves + wave) * RT * CT * 64 +
+                                      (i >> 1) * 64 + lane] = floatx4{0.f, 0.f, 0.f, 0.f};
   int buf = 0;
   for (int group = blockIdx.x; group < groups; group += gridDim.x, buf ^= 1) {
     char* red = lds + (size_t)buf * kManyWaves * RT * CT * 1024;
     if (wave < nb) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        w[r] = wn[r];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) sc[r][g] = scn[r][g];
+      }
+      if (group + (int)gridDim.x < groups) load_w(group + gridDim.x);
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         floatx4 tot[CT];
@@ -574,7 +611,6 @@ __global__ __launch_bounds__(64 * kManyWaves) __attribute__((
           reinterpret_cast<floatx4*>(red)[((wave * RT + r) * CT + ct) * 64 + lane] = tot[ct];
         }
       }
-      if (group + (int)gridDim.x < groups) load_w(group + gridDim.x);
     }
     __syncthreads();
     for (int u = tid; u < RT * CT * 64; u += 64 * kManyWaves) {
@@ -582,10 +618,10 @@ __global__ __launch_bounds__(64 * kManyWaves) __attribute__((
       const int m = ct * 16 + col;
       const long tile = (long)group * RT + r, n = tile * kTileN + 4 * c;
       if (m >= a.M || tile >= tiles) continue;
-      floatx4 s = {0.f, 0.f, 0.f, 0.f};
+      floatx4 s = reinterpret_cast<const floatx4*>(red)[u];
 #pragma unroll
-      for (int i = 0; i < kManyWaves; ++i)
-        if (i < nb) s += reinterpret_cast<const floatx4*>(red)[i * RT * CT * 64 + u];
+      for (int i = 1; i < kManyWaves; ++i)
+        s += reinterpret_cast<const floatx4*>(red)[i * RT * CT * 64 + u];
       if (a.splits > 1)
         *reinterpret_cast<floatx4*>(a.ws + ((long)sp * a.M + m) * (tiles * kTileN) + n) = s;
       else
@@ -640,7 +676,7 @@ template <int CT>
 int launch_many(const Q4Args& a, int G, hipStream_t s) {
   LX_TRY(G == 32 ? (raise_many<CT, 32>())
                  : G == 64 ? (raise_many<CT, 64>()) : (raise_many<CT, 128>()));
-  const long groups = (q4_tiles(a.N) + many_rt(CT) - 1) / many_rt(CT);
+  const long groups = (q4_tiles(a.N) + kManyTiles - 1) / kManyTiles;
   // as many workgroups as the CUs hold at once walk over the groups
   const long slots = (CT == 1 ? 2L : 1L) * device_cus();
   const dim3 grid((unsigned)std::min(groups, std::max(1L, slots / a.splits)), a.splits),
@@ -651,15 +687,15 @@ int launch_many(const Q4Args& a, int G, hipStream_t s) {
 }
 #undef LX_Q4_GROUPS
 
-// Calls that run on q4_few_kernel, which has no fixed cost but splits x again for every tile; in
-// units of tile x block.  Times of both, us, at K = 896 (few / many): M = 1, N = 40000 9.6 / 10.6,
-// N = 151936 28 / 18.8; M = 8, N = 9728 5.6 / 7.4, N = 40000 14.3 / 11.3 (and below 2048 tiles the
-// other needs a second launch); M = 16, N = 1152 4.6 / 6.3, N = 9728 8.8 / 7.9; N = 896, K = 4864
-// (few tiles, each a long run of blocks) 11.8 / 8.5.
+// Calls that run on q4_few_kernel, which has little fixed cost but splits x again for every tile;
+// in units of tile x block, and more where the other kernel needs a second launch (K > 1024; never
+// for up to 4 rows).  Times of both, us, K = 896 (few / many): M = 1, N = 20000 5.7 / 7.0, N = 40000
+// 9.8 / 8.7, N = 151936 28.5 / 18.7; M = 8, N = 9728 5.5 / 6.2, N = 20000 8.2 / 7.0; M = 16, N =
+// 1152 4.6 / 4.4, N = 9728 8.6 / 6.2; N = 896, K = 4864 11.7 / 7.0.
 bool q4_takes_few(int M, int N, int K) {
-  const long tiles = q4_tiles(N), kb = q4_blocks(K), work = tiles * kb;
-  if (M <= 8) return kb > kManyWaves || work <= (M <= 4 ? 35000 : 9000);
-  return M <= 16 && work <= 4096 && kb <= 16;
+  const long kb = q4_blocks(K), work = q4_tiles(N) * kb;
+  if (M <= 4) return kb > kManyWaves || work <= 12000;
+  return M <= 8 && work <= (kb > kManyWaves ? 12000 : 6000);
 }
 
 bool q4_shape_ok(int N, int K, int group) {
@@ -820,8 +856,7 @@ extern "C" int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int gr
   a.splits = 1;
   if (q4_takes_few(M, N, K)) {
     if (M <= 4) return launch_few<4>(a, group, stream);
-    if (M <= 8) return launch_few<8>(a, group, stream);
-    return launch_few<16>(a, group, stream);
+    return launch_few<8>(a, group, stream);
   }
   a.splits = many_splits(K);
   if (a.splits > 1) {

@@ -426,7 +426,7 @@ def linear_q4(x, w, b=None, epilogue=None, out=None):
         if out.get_device() != dev:
             _elsewhere("out")
     n, ws = 0, None
-    if M > 8:
+    if M > 4:
         n = lib.lx_linear_q4_ws_floats(M, N, K)
         ws = x.new_empty(n) if n else None
     check(lib.lx_linear_q4_f32(x.data_ptr(), ldx, w._ptr, w.group, bias, out.data_ptr(), ldy, M,

@@ -57,7 +57,9 @@ def test_linear_refusals(kw):
 
 
 def test_linear_workspace():
-    assert lib.lx_linear_q4_ws_floats(1, 896, 4864) == lib.lx_linear_q4_ws_floats(8, 896, 896) == 0
+    # up to 4 rows, and K up to 1024, take none
+    for M, N, K in [(1, 896, 4864), (4, 151936, 8192), (8, 896, 896), (64, 9728, 1024)]:
+        assert lib.lx_linear_q4_ws_floats(M, N, K) == 0
     for bad in [(0, 896, 896), (65, 896, 896), (17, 0, 896), (17, 896, 6)]:
         assert lib.lx_linear_q4_ws_floats(*bad) == 0
     need = lib.lx_linear_q4_ws_floats(64, 1000, 8192)
