@@ -460,14 +460,18 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
     }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      half8_t p0, p1;  // of p s: the remainder of the first part is taken from the exact product
+      float ps[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float ss = bf16_lo(vp[g][j >> 2][j & 3]), z = bf16_hi(vp[g][j >> 2][j & 3]);
-        p0[j] = (_Float16)(p[j] * ss);
-        p1[j] = (_Float16)fmaf(p[j], ss, -(float)p0[j]);
+        ps[j] = p[j] * ss;
+        // the product as rounded to fp32 goes into both parts: folded into the conversion of one
+        // of its uses, the two would be parts of different numbers next to a tie (2^-11 off)
+        asm("" : "+v"(ps[j]));
         zsum[g] = fmaf(p[j], fmaf(8.0f, ss, z), zsum[g]);
       }
+      half8_t p0, p1;
+      split2(ps, 1.0f, p0, p1);
 #pragma unroll
       for (int r = 0; r < KP; ++r) {
         // the weights of this record's columns alone: the others' belong to other values

@@ -486,6 +486,37 @@ def test_attention_lengths_outside_the_cache(gpu):
     assert torch.equal(a, b) and not a[1].any()
 
 
+@pytest.mark.parametrize("hd,heads,kv,Tq", [(64, 64, 8, 200), (128, 32, 8, 100), (64, 14, 2, 1),
+                                            (64, 16, 16, 3), (128, 32, 8, 1)])
+def test_attention_every_weight(gpu, hd, heads, kv, Tq):
+    """Six keys with scores within 2 of each other, so that each weight of each row counts in the
+    output: scores are off by 2^-24 of sums below 8 sqrt(3 hd) roundings at most, a weight's two
+    parts by 2^-22, the rest by some ten roundings.  (A weight that lost its second part would be
+    off by up to 2^-11.)"""
+    from larynx_amd import ops
+    announce(f"kv4 attention every weight hd={hd} heads={heads}/{kv} Tq={Tq}")
+    rng = _gen(hd + heads)
+    B, rows = (8, 6) if Tq > 1 else (64, 6)
+    k = (rng.standard_normal((B, rows, kv, hd)) * 0.2).astype(np.float32)
+    v = rng.standard_normal((B, rows, kv, hd)).astype(np.float32)
+    q = rng.standard_normal((B, Tq, heads * hd)).astype(np.float32)
+    cache = ops.kv4_cache(B, kv, rows, hd)
+    zero = torch.zeros(B, dtype=torch.int32, device=gpu)
+    ops.kv4_append(cache, _dev(k.reshape(B, rows, -1), gpu), _dev(v.reshape(B, rows, -1), gpu),
+                   zero)
+    got = ops.attention_kv4(_dev(q, gpu), cache, zero + rows, heads, causal=False).cpu().numpy()
+    kt, vt = ref_cache(k)[0], ref_cache(v)[0]
+    rep = heads // kv
+    s = np.einsum("btgrc,bkgc->btgrk", q.astype(np.float64).reshape(B, Tq, kv, rep, hd),
+                  kt) * hd ** -0.5
+    p = np.exp(s - s.max(-1, keepdims=True))
+    want = np.einsum("btgrk,bkgc->btgrc", p / p.sum(-1, keepdims=True), vt).reshape(got.shape)
+    assert np.abs(s).max() < 2.5
+    vmax = np.abs(vt).max()
+    tol = vmax * (U * (2 * 8 * math.sqrt(3 * hd) / math.sqrt(hd) + 16) + 2.0 ** -22)
+    assert np.abs(got - want).max() < tol, (np.abs(got - want).max(), tol)
+
+
 def test_attention_large_scores(gpu):
     """Scores in the hundreds, rising along the keys: the running maximum moves in every record."""
     from larynx_amd import ops
