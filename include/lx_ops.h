@@ -368,7 +368,9 @@ int lx_attention_np_f32(const float* q, int ldq, const float* k, int ldk, const 
  * and q = clamp(rint(w / s) + 8, 0, 15), a code q stands for s * (q - 8), off by
  * at most |s| / 2 (the largest magnitude: |s| / 32; one of the opposite sign as
  * large: |s|).  All zeros: zeros.  A group that holds an infinity or a NaN
- * stands for NaN.  Any N, K % 4 == 0.
+ * stands for NaN.  Any N, K % 4 == 0.  The products below keep fp32's accuracy for
+ * weights of 2^-100 to 2^112 in magnitude (the sums of a group are formed with x
+ * scaled to 1 .. 2 and then multiplied by s).
  * lx_q4_bytes: size of the packed weight (codes in MFMA fragment order, then the
  * scales), about K / 2 + 2 K / group bytes a row; 0 for a bad shape.
  * lx_q4_pack_f32 quantises W (16-byte aligned, row-major) into Wq (16-byte

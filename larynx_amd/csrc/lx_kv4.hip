@@ -24,6 +24,7 @@ constexpr int kBlk = 32;       // rows of a record
 constexpr int kGrp = 64;       // channels of a group
 constexpr int kCodes = 1024;   // bytes of one group's key (or value) codes in a record
 constexpr int kRec = 2 * kCodes + 2 * kBlk * 4;  // bytes of a record, per channel group
+constexpr long kMaxThreads = 0xffffff00L;        // of a launch along x
 
 // Record of (sequence, kv head, block): ng groups of key codes, ng of value codes, ng x 32 key
 // (s, z), ng x 32 value (s, z).
@@ -159,15 +160,14 @@ struct ReadArgs {
   const int* pos;
 };
 
-// One thread per (row, channel); rows outside the cache read as zero.
+// One thread per (row, channel) of a sequence; rows outside the cache read as zero.
 __global__ __launch_bounds__(256) void kv4_read_kernel(ReadArgs a) {
-  const int hd = a.c.ng * kGrp, width = a.c.heads * hd;
+  const int hd = a.c.ng * kGrp, width = a.c.heads * hd, b = blockIdx.y;
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (long)a.c.batch * a.T * width) return;
-  const int ch = (int)(i % hd), h = (int)(i / hd % a.c.heads);
-  const long bt = i / width;
-  const int b = (int)(bt / a.T);
-  const long row = (long)a.pos[b] + bt % a.T;
+  if (i >= (long)a.T * width) return;
+  const long t = i / width;
+  const int wc = (int)(i - t * width), h = wc / hd, ch = wc - h * hd;
+  const long row = (long)a.pos[b] + t;
   float k = 0.0f, v = 0.0f;
   if (row >= 0 && row < a.c.rows) {
     const char* rec = a.c.data + a.c.record(b, h, (int)(row / kBlk));
@@ -181,8 +181,9 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(ReadArgs a) {
     k = fmaf(bf16_lo(kp), (float)q4_get(kw, x & 7), bf16_hi(kp));
     v = fmaf(bf16_lo(vp), (float)q4_get(vw, (r & 3) + 4 * (r >> 4)), bf16_hi(vp));
   }
-  a.k[i] = k;
-  a.v[i] = v;
+  const long to = (long)b * a.T * width + i;
+  a.k[to] = k;
+  a.v[to] = v;
 }
 
 // ---- attention --------------------------------------------------------------------------
@@ -718,6 +719,7 @@ extern "C" int lx_kv4_append_f32(const lx_kv4* cache, const float* k, long ldk, 
   a.pos = pos;
   // records that T rows can touch, wherever they begin
   const long touched = std::min<long>(((long)T + kBlk - 2) / kBlk + 1, a.c.blocks);
+  LX_REQUIRE(touched * 512 <= kMaxThreads, "kv4_append: T=%d too long", T);
   hipLaunchKernelGGL(kv4_append_kernel,
                      dim3((unsigned)touched, a.c.heads * a.c.ng, cache->batch), dim3(512), 0,
                      stream, a);
@@ -734,9 +736,10 @@ extern "C" int lx_kv4_read_f32(const lx_kv4* cache, float* k, float* v, int T, c
   a.v = v;
   a.T = T;
   a.pos = pos;
-  const long n = (long)cache->batch * T * cache->n_kv_heads * cache->head_dim;
-  LX_REQUIRE((n + 255) / 256 <= INT_MAX, "kv4_read: %ld values", n);
-  hipLaunchKernelGGL(kv4_read_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, a);
+  const long n = (long)T * cache->n_kv_heads * cache->head_dim;
+  LX_REQUIRE(n <= kMaxThreads, "kv4_read: %ld values a sequence", n);
+  hipLaunchKernelGGL(kv4_read_kernel, dim3((unsigned)((n + 255) / 256), a.c.batch), dim3(256), 0,
+                     stream, a);
   return check_launch("kv4_read_kernel");
 }
 
@@ -783,7 +786,9 @@ extern "C" int lx_attention_kv4_f32(const float* q, long ldq, const lx_kv4* cach
   a.splits = p.splits;
   a.chunk = p.chunk;
   const long wgs = (long)p.tiles * a.c.batch * a.c.heads;
-  LX_REQUIRE((long)p.tiles * p.splits <= INT_MAX, "attention_kv4: Tq=%d too long", Tq);
+  LX_REQUIRE((long)p.tiles * p.splits * 64 * p.waves <= kMaxThreads &&
+                 (long)Tq * a.rep * 256 <= kMaxThreads,
+             "attention_kv4: Tq=%d too long", Tq);
   if (p.splits > 1) {
     const size_t need = (size_t)wgs * p.splits * part_floats(a.c.ng);
     LX_REQUIRE(ws && ws_floats >= need && (uintptr_t)ws % 16 == 0,

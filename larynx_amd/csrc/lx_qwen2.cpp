@@ -805,9 +805,15 @@ extern "C" int lx_qwen2_set_decode_bits(lx_qwen2* m, int bits, int group) {
       if (!*p) *p = m->arena.alloc<char>(q4_bytes(N, K, 32));
       return *p != nullptr;
     };
-    bool ok = A(&m->head_q4, m->speech_vocab, H);
-    for (auto& L : m->layers)
-      ok = ok && A(&L.qkv_q4, m->QKV, H) && A(&L.gu_q4, 2 * I, H) && A(&L.down_q4, H, I);
+    bool ok = true;
+    try {
+      m->arena.ptrs.reserve(m->arena.ptrs.size() + 1 + 3 * m->layers.size());
+      ok = A(&m->head_q4, m->speech_vocab, H);
+      for (auto& L : m->layers)
+        ok = ok && A(&L.qkv_q4, m->QKV, H) && A(&L.gu_q4, 2 * I, H) && A(&L.down_q4, H, I);
+    } catch (const std::bad_alloc&) {
+      ok = false;
+    }
     if (!ok) {
       set_error("qwen2_set_decode_bits: device allocation failed");
       return LX_ERR_ALLOC;

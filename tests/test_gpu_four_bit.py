@@ -180,6 +180,27 @@ def test_linear_bit_exact_on_larger_shapes(gpu, M, N, K, G):
     assert (out[M:] == -77).all() and (out[:, N:] == -77).all()
 
 
+@pytest.mark.parametrize("M", [2, 20])
+def test_linear_far_offsets(gpu, M):
+    """A weight of 4.3 GB of codes (34 GB in fp32), the last rows other than zero: offsets past 32
+    bits in packing and in the product."""
+    from larynx_amd import ops
+    announce(f"q4 far offsets M={M}")
+    N, K, n = (1 << 20) + 24, 8192, 40
+    g = torch.Generator(device=gpu).manual_seed(M)
+    W = torch.zeros(N, K, device=gpu)
+    W[-n:] = torch.randint(-8, 8, (n, K), device=gpu, generator=g).float()
+    W[-n:, ::64] = -8
+    w = ops.q4_pack(W, 64)
+    assert w.data.numel() > 1 << 32
+    x = torch.randint(-3, 4, (M, K), device=gpu, generator=g).float()
+    got = ops.linear_q4(x, w)
+    want = (x.double() @ W[-n:].t().contiguous().double()).float()
+    del W
+    assert torch.equal(got[:, -n:], want)
+    assert not got[:, :-n].any()
+
+
 def _linear_tolerance(x, sc, G):
     """Per output: the group sums run through 4 G / 8 accumulations (three parts and the sum of
     x) of partial sums below (24 + 31) sum |x| times the scale, then over the groups."""
