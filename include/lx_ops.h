@@ -368,9 +368,10 @@ int lx_attention_np_f32(const float* q, int ldq, const float* k, int ldk, const 
  * and q = clamp(rint(w / s) + 8, 0, 15), a code q stands for s * (q - 8), off by
  * at most |s| / 2 (the largest magnitude: |s| / 32; one of the opposite sign as
  * large: |s|).  All zeros: zeros.  A group that holds an infinity or a NaN
- * stands for NaN.  Any N, K % 4 == 0.  The products below keep fp32's accuracy for
- * weights of 2^-100 to 2^112 in magnitude (the sums of a group are formed with x
- * scaled to 1 .. 2 and then multiplied by s).
+ * stands for NaN.  K % 4 == 0, any N, at most 2^24 - 1 tiles of 16 rows x 128 inputs.
+ * The products below keep fp32's accuracy for weights of 2^-100 to 2^112 in
+ * magnitude (the sums of a group are formed with x scaled to 1 .. 2 and then
+ * multiplied by s).
  * lx_q4_bytes: size of the packed weight (codes in MFMA fragment order, then the
  * scales), about K / 2 + 2 K / group bytes a row; 0 for a bad shape.
  * lx_q4_pack_f32 quantises W (16-byte aligned, row-major) into Wq (16-byte
@@ -383,12 +384,11 @@ int lx_q4_unpack_f32(const void* Wq, float* W, int N, int K, int group, hipStrea
 /* Projection of few rows on such a weight:  y = epi(x @ W~^T + bias), W~ what the
  * packed codes stand for, fp32 arithmetic (x as two fp16 parts after a power of two
  * per row and 128 inputs, exact products with the codes, fp32 sums; the scale
- * applied to each group's sum).  x: (M, K),
- * 1 <= M <= 64, row stride ldx; y: (M, N), row stride ldy (N / 2 columns for
+ * applied to each group's sum).  x: (M, K), 1 <= M <= 64, row stride ldx; y: (M, N), row stride ldy (N / 2 columns for
  * SWIGLU_PAIRED, N even); y must not overlap x.  Epilogues: none, GELU_TANH, RESID,
- * SWIGLU_PAIRED (others: LX_ERR_ARG); bias (N) or NULL.  K and ldx multiples of
- * 4, x and Wq 16-byte aligned.  An infinite or NaN element of x makes NaN of its
- * row.  The result does not depend on timing.  ws: lx_linear_q4_ws_floats() floats
+ * SWIGLU_PAIRED (others: LX_ERR_ARG); bias (N) or NULL.  K (at most 2^26 - 1024 with
+ * more than 4 rows) and ldx multiples of 4, x and Wq 16-byte aligned.  An infinite or
+ * NaN element of x makes NaN of its row.  The result does not depend on timing.  ws: lx_linear_q4_ws_floats() floats
  * of scratch, 16-byte aligned (NULL when that is 0: up to 4 rows, and K up to 1024);
  * calls that share it must not overlap.
  * Replaces linear() (src/llm/ops.cpp:13-19) for weights given in 4 bits. */
@@ -398,7 +398,7 @@ int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int group, const 
                      size_t ws_floats, hipStream_t stream);
 
 /* A key/value cache held in 4 bits (4.5 with its scales): `batch` sequences of up
- * to max_rows rows, n_kv_heads heads (at most 65535 and 32767) of head_dim (64 or
+ * to max_rows (at most 2^31 - 129) rows, n_kv_heads heads (at most 65535 and 32767) of head_dim (64 or
  * 128) channels.  Keys and
  * values alike: the 64 channels of a group of a row share z = the largest bf16
  * not above their minimum and s = the smallest bf16 not below (max - z) / 15; a
@@ -700,13 +700,14 @@ int lx_qwen2_set_decode_graph(lx_qwen2* m, int enable);
 
 /* Decode's weights: bits = 32 (the default; group unused) or 4, the q|k|v, gate/up
  * and down projections and the head on copies in 4 bits with a scale per `group`
- * (32, 64 or 128) inputs (lx_q4_pack_f32, lx_linear_q4_f32): 7.9 MB of them and
+ * (32, 64 or 128) inputs (lx_q4_pack_f32, lx_linear_q4_f32): 7.5 MB of them in groups of 64 and
  * o_proj's 3.2 MB of fp32 a layer of Qwen2-0.5B instead of 59.6 MB.  o_proj, whose
  * launch also forms the attention, the embeddings, norms and the K/V cache keep
  * fp32, and so does the whole prefill.  The call waits for the device, packs from
  * the model's fp32 weights, which stay, and drops captured decode graphs; the
  * first one with 4 allocates the copies (held until destroy; LX_ERR_ALLOC changes
- * nothing).  Not to be called during a capture.  No counterpart in the reference. */
+ * nothing).  The model's device must be current (else LX_ERR_ARG).  Not to be called
+ * during a capture.  No counterpart in the reference. */
 int lx_qwen2_set_decode_bits(lx_qwen2* m, int bits, int group);
 
 /* Prefill projections' split-operand products, 3 (the default) or 6, as

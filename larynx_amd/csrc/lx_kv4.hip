@@ -644,13 +644,12 @@ AttnPlan attn_plan(const Kv4& c, int nrow, int max_len) {
   // split 11.1 us, eight 7.6 with the join; 48 of up to 4000: two 18.1, eight 15.2; 156 tiles of a
   // prompt chunk over 1708 rows: one 13.9, two 20.2).
   constexpr int kWaves = 4, kJoin = 5;
-  const int base = (int)std::min<long>(wgs, 1 << 20);
-  int best = INT_MAX;
+  long best = LONG_MAX;
   p.splits = 1;
   for (const int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 40, 48, 64}) {
     if (s > steps) break;
-    const int t = (base * s + cus - 1) / cus * ((steps + kWaves * s - 1) / (kWaves * s)) +
-                  (s > 1 ? kJoin : 0);
+    const long t = (wgs * s + cus - 1) / cus * ((steps + kWaves * s - 1) / (kWaves * s)) +
+                   (s > 1 ? kJoin : 0);
     if (t < best) {
       best = t;
       p.splits = s;
@@ -679,7 +678,7 @@ int launch_attn(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
 
 bool kv4_shape_ok(int batch, int heads, int hd, int rows) {
   return batch > 0 && batch <= 65535 && heads > 0 && heads <= 32767 && (hd == 64 || hd == 128) &&
-         rows > 0 && rows <= INT_MAX - kBlk;
+         rows > 0 && rows <= INT_MAX - 4 * kBlk;  // a step of four records past the last row
 }
 
 int kv4_view(const lx_kv4* c, const char* what, Kv4* out) {

@@ -23,6 +23,7 @@ namespace {
 constexpr int kTileN = 16;    // rows of a tile
 constexpr int kBlockK = 128;  // inputs of a block
 constexpr int kMaxRows = 64;
+constexpr long kMaxTiles = (1L << 24) - 1;  // of a weight: every launch below 2^32 threads
 
 struct Q4Args {
   const float* x;
@@ -700,7 +701,7 @@ bool q4_takes_few(int M, int N, int K) {
 
 bool q4_shape_ok(int N, int K, int group) {
   return N > 0 && K > 0 && K % 4 == 0 && (group == 32 || group == 64 || group == 128) &&
-         q4_tiles(N) * q4_blocks(K) <= INT_MAX;
+         q4_tiles(N) * q4_blocks(K) <= kMaxTiles;
 }
 
 size_t q4_code_bytes(int N, int K) { return (size_t)q4_tiles(N) * q4_blocks(K) * 1024; }
@@ -860,6 +861,7 @@ extern "C" int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int gr
   }
   a.splits = many_splits(K);
   if (a.splits > 1) {
+    LX_REQUIRE(a.splits <= 65535, "linear_q4: K=%d of %d rows too long", K, M);
     const size_t need = (size_t)a.splits * M * q4_tiles(N) * kTileN;
     LX_REQUIRE(ws && ws_floats >= need && (uintptr_t)ws % 16 == 0,
                "linear_q4: workspace of %zu floats, %zu needed", ws ? ws_floats : 0, need);

@@ -97,6 +97,7 @@ struct lx_qwen2 {
   int max_splits = 0;
   float* rope_tab = nullptr;  // device copy of the rotary inverse frequencies
   float* rope_cs = nullptr;   // their cosines and sines at every position (rope_table)
+  int device = -1;            // current when the model was made
   bool use_graph = true;      // replay the layer stack as one HIP graph
   int q4_group = 0;           // decode on 4-bit weights in groups of this many inputs (0: fp32)
   void* head_q4 = nullptr;    // llm_decoder in 4 bits
@@ -566,7 +567,7 @@ extern "C" int lx_qwen2_create(const lx_qwen2_weights* w, int max_ctx, lx_qwen2*
     return LX_ERR_ALLOC;
   }
   hipStream_t s = nullptr;
-  if (hipStreamCreate(&s) != hipSuccess) {
+  if (hipGetDevice(&m->device) != hipSuccess || hipStreamCreate(&s) != hipSuccess) {
     delete m;
     set_error("qwen2_create: stream creation failed");
     return LX_ERR_LAUNCH;
@@ -784,6 +785,9 @@ extern "C" int lx_qwen2_set_decode_bits(lx_qwen2* m, int bits, int group) {
   LX_REQUIRE(bits == 32 || (bits == 4 && (group == 32 || group == 64 || group == 128)),
              "qwen2_set_decode_bits: %d bits in groups of %d (32, or 4 in groups of 32, 64 or 128)",
              bits, group);
+  int dev = -1;
+  LX_REQUIRE(hipGetDevice(&dev) == hipSuccess && dev == m->device,
+             "qwen2_set_decode_bits: device %d is current, the model is on %d", dev, m->device);
   const int want = bits == 4 ? group : 0;
   if (want == m->q4_group) return LX_OK;
   // decode steps under way read the weights and the graphs that go

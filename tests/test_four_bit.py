@@ -17,14 +17,14 @@ def test_sizes():
     assert lib.lx_q4_bytes(17, 132, 32) == 2 * 2 * (1024 + 4 * 32)
     assert lib.lx_q4_bytes(1, 4, 128) == 1024 + 32
     for bad in [(0, 4, 64), (1, 0, 64), (1, 6, 64), (1, 4, 16), (1, 4, 0), (-1, 4, 64),
-                (2 ** 31 - 1, 2 ** 31 - 4, 64)]:
+                (2 ** 31 - 1, 2 ** 31 - 4, 64), (2 ** 28, 128, 64), (16, 2 ** 31 - 4, 64)]:
         assert lib.lx_q4_bytes(*bad) == 0, bad
     # records of 32 rows: 2304 bytes per 64 channels
     assert lib.lx_kv4_bytes(1, 2, 64, 4096) == 2 * 128 * 2304
     assert lib.lx_kv4_bytes(3, 1, 128, 33) == 3 * 2 * 2 * 2304
     assert lib.lx_kv4_bytes(64, 32, 128, 1 << 22) == 64 * 32 * (1 << 17) * 4608  # past 32 bits
     for bad in [(0, 1, 64, 1), (1, 0, 64, 1), (1, 1, 32, 1), (1, 1, 96, 1), (1, 1, 64, 0),
-                (1, 1, 64, -5), (1, 1, 64, 2 ** 31 - 1), (65536, 4, 64, 1), (4, 32768, 64, 1)]:
+                (1, 1, 64, -5), (1, 1, 64, 2 ** 31 - 1), (1, 1, 64, 2 ** 31 - 128), (65536, 4, 64, 1), (4, 32768, 64, 1)]:
         assert lib.lx_kv4_bytes(*bad) == 0, bad
 
 
@@ -65,6 +65,8 @@ def test_linear_workspace():
     need = lib.lx_linear_q4_ws_floats(64, 1000, 8192)
     assert need and need % (64 * 1008) == 0
     assert lib.lx_linear_q4_ws_floats(1, 151936, 896) == 0
+    K = 2 ** 26  # more splits than a launch has rows of workgroups
+    assert _linear(M=5, N=16, K=K, ldx=K, ldy=16, ws=P, n=2 ** 40) == LX_ERR_ARG
     for ws, n in [(None, need), (P, need - 1), (P + 4, need)]:
         assert _linear(M=64, N=1000, K=8192, ldx=8192, ldy=1000, ws=ws, n=n) == LX_ERR_ARG
         assert b"workspace" in lib.lx_last_error()
