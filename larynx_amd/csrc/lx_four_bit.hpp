@@ -55,12 +55,53 @@ __device__ __forceinline__ unsigned q4_get(unsigned w, int j) {
   return (w >> (4 * (j >> 1) + 16 * (j & 1))) & 15u;
 }
 
-// x s as two fp16 parts, s a power of two (the fused remainder is exact, as x s is).
+// x s as two fp16 parts.  The first is pinned: converted anew for the remainder, it costs half
+// as many instructions again, and where x is a product folded into one of the two conversions
+// the parts belong to different numbers next to a tie (2^-11 off).
+__device__ __forceinline__ void split_pair(float x0, float x1, float s, half2_t& p0, half2_t& p1) {
+  p0 = half2_t{(_Float16)(x0 * s), (_Float16)(x1 * s)};
+  unsigned u = __builtin_bit_cast(unsigned, p0);
+  asm("" : "+v"(u));
+  p0 = __builtin_bit_cast(half2_t, u);
+  p1 = half2_t{(_Float16)fmaf(x0, s, -(float)p0[0]), (_Float16)fmaf(x1, s, -(float)p0[1])};
+}
 __device__ __forceinline__ void split2(const float (&x)[8], float s, half8_t& p0, half8_t& p1) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) p0[j] = (_Float16)(x[j] * s);
+  for (int j = 0; j < 8; j += 2) {
+    half2_t h, l;
+    split_pair(x[j], x[j + 1], s, h, l);
+    p0[j] = h[0];
+    p0[j + 1] = h[1];
+    p1[j] = l[0];
+    p1[j + 1] = l[1];
+  }
+}
+
+// The largest magnitudes of the rows that 16 lanes hold eight values each of, n rows a lane, for
+// row_scale.  Among lanes as integers, which order as magnitudes do and need no check for a NaN; a
+// step of all the rows at once, as a lane's value can cross over two instructions after it is made.
+template <int N>
+__device__ __forceinline__ void tops16(const float4 (&x)[N][2], float (&top)[N]) {
+  unsigned u[N];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) p1[j] = (_Float16)fmaf(x[j], s, -(float)p0[j]);
+  for (int i = 0; i < N; ++i) {
+    const float4 a = x[i][0], b = x[i][1];
+    float t = fmaxf(fabsf(a.x), fabsf(a.y));
+    t = fmaxf(fmaxf(t, fabsf(a.z)), fabsf(a.w));
+    t = fmaxf(fmaxf(t, fabsf(b.x)), fabsf(b.y));
+    t = fmaxf(fmaxf(t, fabsf(b.z)), fabsf(b.w));
+    u[i] = __float_as_uint(t);
+  }
+#define LX_TOPS_STEP(CTRL)      \
+  _Pragma("unroll") for (int i = 0; i < N; ++i) u[i] = \
+      max(u[i], (unsigned)__builtin_amdgcn_update_dpp(0, (int)u[i], CTRL, 0xF, 0xF, true))
+  LX_TOPS_STEP(kDppXor1);
+  LX_TOPS_STEP(kDppXor2);
+  LX_TOPS_STEP(kDppHalfMirror);
+  LX_TOPS_STEP(kDppMirror);
+#undef LX_TOPS_STEP
+#pragma unroll
+  for (int i = 0; i < N; ++i) top[i] = __uint_as_float(u[i]);
 }
 
 // The power of two that brings a row with largest magnitude `top` to 1 .. 2, and its inverse

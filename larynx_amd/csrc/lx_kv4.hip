@@ -326,8 +326,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
     load(s0 + wave, 1, vc, vp);
   }
 
-  // every wave splits the whole tile's query the same way; two groups of it would hold 32 registers,
-  // so with two they stay in LDS (wave 0's)
+  // every wave splits the whole tile's query the same way; two groups of it would hold 32
+  // registers, so with two they stay in LDS (wave 0's)
   half8_t qf[NG][2][2];
   half8_t* ql = reinterpret_cast<half8_t*>(ml + waves) + lane;
   float qsum[NG], f;
@@ -466,9 +466,6 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
       for (int j = 0; j < 8; ++j) {
         const float ss = bf16_lo(vp[g][j >> 2][j & 3]), z = bf16_hi(vp[g][j >> 2][j & 3]);
         ps[j] = p[j] * ss;
-        // the product as rounded to fp32 goes into both parts: folded into the conversion of one
-        // of its uses, the two would be parts of different numbers next to a tie (2^-11 off)
-        asm("" : "+v"(ps[j]));
         zsum[g] = fmaf(p[j], fmaf(8.0f, ss, z), zsum[g]);
       }
       half8_t p0, p1;

@@ -228,7 +228,8 @@ template <int MB, int G>
 __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
   constexpr int TG = G / 32, NG = kBlockK / G;
   extern __shared__ __attribute__((aligned(16))) char lds[];  // [waves][few_bytes]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane >> 4, col = lane & 15;
   const unsigned pattern = q4_pattern();
   const long rt = blockIdx.x;
@@ -247,27 +248,22 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
   }
   floatx4 tot = {0.f, 0.f, 0.f, 0.f};
   for (int kb = wave; kb < a.kb; kb += waves) {
-    const int past = a.K - kb * kBlockK - 8 * col;  // inputs of the lane's eight that exist
+    if (kb * kBlockK + kBlockK > a.K) {
+      asm volatile("");  // a branch, not a select per value of every block
+#pragma unroll
+      for (int p = 0; p < MB / 4; ++p)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (kb * kBlockK + 8 * col + 4 * e >= a.K) in.x[p][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float top[MB / 4];
+    tops16(in.x, top);
 #pragma unroll
     for (int p = 0; p < MB / 4; ++p) {
-      float v[8], top = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float4 x = in.x[p][e];
-        const bool none = past <= 4 * e;
-        v[4 * e] = none ? 0.0f : x.x;
-        v[4 * e + 1] = none ? 0.0f : x.y;
-        v[4 * e + 2] = none ? 0.0f : x.z;
-        v[4 * e + 3] = none ? 0.0f : x.w;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
-      top = fmaxf(top, dpp_mov<kDppXor1>(top));
-      top = fmaxf(top, dpp_mov<kDppXor2>(top));
-      top = fmaxf(top, dpp_mov<kDppHalfMirror>(top));
-      top = fmaxf(top, dpp_mov<kDppMirror>(top));
+      const float4 x0 = in.x[p][0], x1 = in.x[p][1];
+      const float v[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
       float inv;
-      const float sc = row_scale(top, &inv);
+      const float sc = row_scale(top[p], &inv);
       if (col == 0) finv[4 * p + c] = inv;
       half8_t p0, p1;
       split2(v, sc, p0, p1);
@@ -400,9 +396,8 @@ __global__ __launch_bounds__(64) void q4_row_kernel(Q4Args a, DecGemvArgs d) {
   const float xs = row_scale(wave_max(top), &f);
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
-    const float v0 = x[j].x * xs, v1 = x[j].y * xs;
-    const half2_t p0 = {(_Float16)v0, (_Float16)v1};
-    const half2_t p1 = {(_Float16)(v0 - (float)p0[0]), (_Float16)(v1 - (float)p0[1])};
+    half2_t p0, p1;
+    split_pair(x[j].x, x[j].y, xs, p0, p1);
     *reinterpret_cast<half2_t*>(lds + j * 256 + lane * 4) = p0;
     *reinterpret_cast<half2_t*>(lds + ROW + j * 256 + lane * 4) = p1;
   }
@@ -458,8 +453,8 @@ __global__ __launch_bounds__(64) void q4_row_kernel(Q4Args a, DecGemvArgs d) {
   }
 }
 
-// Up to 64 rows of x in CT column tiles of 16.  The waves of a workgroup own one block of K each, of
-// the at most eight of a split: a wave splits its 16 CT rows x 128 inputs of x once, keeps the
+// Up to 64 rows of x in CT column tiles of 16.  The waves of a workgroup own one block of K each,
+// of the at most eight of a split: a wave splits its 16 CT rows x 128 inputs of x once, keeps the
 // fragments in registers (32 CT of them) and streams the weights of its block past them, RT tiles
 // of 16 rows at a time, one group of tiles ahead.  The waves' sums meet in one of two LDS buffers
 // (a barrier a group), added in wave order; each thread adds and finishes one quad of outputs.
@@ -479,11 +474,11 @@ __global__ __launch_bounds__(64 * kManyWaves) __attribute__((
     amdgpu_waves_per_eu(CT == 1 ? 4 : 2))) void q4_many_kernel(Q4Args a) {
   constexpr int TG = G / 32, NG = kBlockK / G, RT = kManyTiles;
   extern __shared__ __attribute__((aligned(16))) char lds[];  // [2][wave][RT][CT][lane] quads
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane >> 4, col = lane & 15;
   const unsigned pattern = q4_pattern();
   const int sp = blockIdx.y, per = (a.kb + a.splits - 1) / a.splits;
-  const int nb = min(per, a.kb - sp * per);  // blocks of this split, 1 .. 8: the waves that multiply
+  const int nb = min(per, a.kb - sp * per);  // blocks of this split, 1 .. 8: waves that multiply
   const int kb = sp * per + min(wave, nb - 1);
   const long tiles = q4_tiles(a.N);
   const int groups = (int)((tiles + RT - 1) / RT);
@@ -508,39 +503,35 @@ __global__ __launch_bounds__(64 * kManyWaves) __attribute__((
     char* mine = lds + wave * few_bytes<16>();
     float* finv = reinterpret_cast<float*>(mine + 32 * kFewRow);
     float4 u[CT][4][2];  // all requested before the first is used
+    const long x4 = 4 * a.ldx;
+    const int k0 = kb * kBlockK + 4 * col;
+    const float* last = a.x + (a.M - 1) * a.ldx;
+    const float* xr = a.x + c * a.ldx;
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
+    for (int i = 0; i < 4 * CT; ++i, xr += x4) {
+      const float* r = 4 * i + c < a.M ? xr : last;
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const float* xr = a.x + (long)min(ct * 16 + 4 * p + c, a.M - 1) * a.ldx;
+      for (int e = 0; e < 2; ++e)
+        u[i >> 2][i & 3][e] = *reinterpret_cast<const float4*>(r + min(k0 + 64 * e, a.K - 4));
+    }
+    if (kb * kBlockK + kBlockK > a.K) {
+      asm volatile("");  // a branch, not a select per value of every block
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          u[ct][p][e] = *reinterpret_cast<const float4*>(
-              xr + min(kb * kBlockK + 64 * e + 4 * col, a.K - 4));
-      }
+      for (int i = 0; i < 8 * CT; ++i)
+        if (k0 + 64 * (i & 1) >= a.K)
+          u[i >> 3][i >> 1 & 3][i & 1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
+      float top[4], inverse = 0.0f;
+      tops16(u[ct], top);
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        float v[8], top = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const bool none = kb * kBlockK + 64 * e + 4 * col >= a.K;
-          const float4 x = u[ct][p][e];
-          v[4 * e] = none ? 0.0f : x.x;
-          v[4 * e + 1] = none ? 0.0f : x.y;
-          v[4 * e + 2] = none ? 0.0f : x.z;
-          v[4 * e + 3] = none ? 0.0f : x.w;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
-        top = fmaxf(top, dpp_mov<kDppXor1>(top));
-        top = fmaxf(top, dpp_mov<kDppXor2>(top));
-        top = fmaxf(top, dpp_mov<kDppHalfMirror>(top));
-        top = fmaxf(top, dpp_mov<kDppMirror>(top));
+        const float4 x0 = u[ct][p][0], x1 = u[ct][p][1];
+        const float v[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
         float inv;
-        const float xs = row_scale(top, &inv);
-        if (col == 0) finv[4 * p + c] = inv;
+        const float xs = row_scale(top[p], &inv);
+        if (col == p) inverse = inv;
         half8_t p0, p1;
         split2(v, xs, p0, p1);
         const uintx4_t b0 = __builtin_bit_cast(uintx4_t, p0), b1 = __builtin_bit_cast(uintx4_t, p1);
@@ -550,6 +541,7 @@ __global__ __launch_bounds__(64 * kManyWaves) __attribute__((
         *reinterpret_cast<uintx2_t*>(row + kFewRow) = uintx2_t{b1[0], b1[1]};
         *reinterpret_cast<uintx2_t*>(row + kFewRow + 128) = uintx2_t{b1[2], b1[3]};
       }
+      if (col < 4) finv[4 * col + c] = inverse;
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -690,13 +682,13 @@ int launch_many(const Q4Args& a, int G, hipStream_t s) {
 
 // Calls that run on q4_few_kernel, which has little fixed cost but splits x again for every tile;
 // in units of tile x block, and more where the other kernel needs a second launch (K > 1024; never
-// for up to 4 rows).  Times of both, us, K = 896 (few / many): M = 1, N = 20000 5.7 / 7.0, N = 40000
-// 9.8 / 8.7, N = 151936 28.5 / 18.7; M = 8, N = 9728 5.5 / 6.2, N = 20000 8.2 / 7.0; M = 16, N =
-// 1152 4.6 / 4.4, N = 9728 8.6 / 6.2; N = 896, K = 4864 11.7 / 7.0.
+// for up to 4 rows).  Times of both in a graph, us (few / many): K = 896, M = 4, N = 27000 6.9 /
+// 7.5, N = 40000 9.1 / 8.1; M = 8, N = 9728 4.9 / 5.6, N = 20000 7.1 / 6.4; M = 8, N = 896, K =
+// 4864 5.5 / 6.5, 8192 x 4096 9.7 / 10.6, 8192 x 8192 15.7 / 14.0.
 bool q4_takes_few(int M, int N, int K) {
   const long kb = q4_blocks(K), work = q4_tiles(N) * kb;
-  if (M <= 4) return kb > kManyWaves || work <= 12000;
-  return M <= 8 && work <= (kb > kManyWaves ? 12000 : 6000);
+  if (M <= 4) return kb > kManyWaves || work <= 14000;
+  return M <= 8 && work <= (kb > kManyWaves ? 20000 : 6000);
 }
 
 bool q4_shape_ok(int N, int K, int group) {

@@ -159,6 +159,7 @@ def test_linear_bit_exact_on_whole_numbers(gpu, M, N, K, G):
 @pytest.mark.parametrize("M,N,K,G", [
     (1, 90004, 896, 64), (4, 151936, 896, 32), (7, 33000, 700, 128),   # few rows, many tiles
     (3, 70000, 1100, 64), (8, 9000, 2500, 64), (6, 3000, 2500, 32),    # and past 1024 inputs
+    (5, 40000, 1100, 64),
     (16, 9999, 896, 64), (12, 300, 4100, 32), (16, 2500, 8192, 128), (9, 17, 1028, 128),
     (31, 70, 8192, 64), (17, 40001, 260, 64), (32, 5000, 2000, 128),
     (40, 33, 1028, 32), (48, 4097, 1500, 64), (64, 3000, 3000, 32), (64, 20000, 512, 64),
