@@ -35,7 +35,6 @@ __device__ __forceinline__ half8_t q4_frag(unsigned w, unsigned pattern) {
   const half2_t off16 = {(_Float16)-72.0f, (_Float16)-72.0f};
   const half2_t r16 = {(_Float16)0.0625f, (_Float16)0.0625f};
   const unsigned v = w >> 8;
-  half8_t f;
   const half2_t h0 = __builtin_bit_cast(half2_t, (w & 0x000f000fu) | pattern) + off;
   const half2_t h1 = __builtin_elementwise_fma(
       __builtin_bit_cast(half2_t, (w & 0x00f000f0u) | pattern), r16, off16);

@@ -324,49 +324,51 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
   }
 }
 
-// One normalised row of x, as the LM's decode runs it (arguments and epilogues of dec_gemv).  One
-// wave is one tile of 16 rows over the whole of K <= 128 NB: it requests all its weights, forms
-// RMSNorm and the two parts of the row itself (2 NB values a lane; one power of two for the row)
-// and hands them to its lanes as fragments through LDS of its own, so nothing waits for another
-// wave and the sums are complete in place.  (As q4_few_kernel runs it, seven waves a tile at K =
-// 896, the row is formed 4256 times for gate/up, 3 us of instructions: 6.9 us in the decode
-// chain.)  DEC_QKV_ROPE reads rows laid out in rotary pairs (q4_pack_kernel's neox).
-constexpr int row_bytes(int nb) { return 2 * (nb * 256 + 16); }
+// One normalised row of x, as the LM's decode runs it (arguments and epilogues of dec_gemv).  W
+// waves are one tile of 16 rows, each over its own NB blocks of K: a wave requests all its weights,
+// forms its part of the normalised row and the two fp16 parts of that (2 NB values a lane, one
+// power of two) and hands them to its lanes as fragments through LDS of its own.  The waves meet
+// twice, for the sum of squares and for the sums of the tile.  DEC_QKV_ROPE reads rows laid out in
+// rotary pairs (q4_pack_kernel's neox).  The length of a wave's own instructions bounds it: a token
+// of the 24-layer LM (hidden 896, cache 1, groups of 64) 488 us with one wave a tile, 474 with two,
+// 452 with four, 458 with eight.
+constexpr int kRowWaves = 4;  // W
 
 template <int G, int EPI, int NB>
-__global__ __launch_bounds__(64) void q4_row_kernel(Q4Args a, DecGemvArgs d) {
-  constexpr int TG = G / 32, NG = kBlockK / G, ROW = NB * 256 + 16, H = NB < 8 ? NB : 8;
-  __shared__ __attribute__((aligned(16))) char lds[row_bytes(NB)];
-  const int lane = threadIdx.x, c = lane >> 4, col = lane & 15;
+__global__ __launch_bounds__(64 * kRowWaves) void q4_row_kernel(Q4Args a, DecGemvArgs d) {
+  constexpr int TG = G / 32, NG = kBlockK / G, ROW = NB * 256 + 16, W = kRowWaves;
+  __shared__ __attribute__((aligned(16))) char rows[W][2 * ROW];
+  __shared__ float squares[W];
+  __shared__ floatx4 sums[W][4];
+  const int lane = threadIdx.x & 63, c = lane >> 4, col = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), first = wave * NB;
+  char* mine = rows[wave];
   const unsigned pattern = q4_pattern();
   const long rt = blockIdx.x;
   const int kb = a.kb;
   float2 x[NB], g[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
-    const int k = min(j * kBlockK + 2 * lane, a.K - 2);
+    const int k = min((first + j) * kBlockK + 2 * lane, a.K - 2);
     x[j] = *reinterpret_cast<const float2*>(a.x + k);
     g[j] = *reinterpret_cast<const float2*>(d.norm_w + k);
   }
-  uintx4_t w[H];
-  ushortx4_t sc[H][NG];
-  auto load = [&](int first) {
+  uintx4_t w[NB];
+  ushortx4_t sc[NB][NG];
 #pragma unroll
-    for (int j = 0; j < H; ++j) {
-      const long tile = rt * kb + min(first + j, kb - 1);
-      w[j] = a.codes[tile * 64 + lane];
-      const ushortx4_t* sp = reinterpret_cast<const ushortx4_t*>(a.scales) + (tile * 4 + c) * NG;
+  for (int j = 0; j < NB; ++j) {
+    const long tile = rt * kb + min(first + j, kb - 1);
+    w[j] = a.codes[tile * 64 + lane];
+    const ushortx4_t* sp = reinterpret_cast<const ushortx4_t*>(a.scales) + (tile * 4 + c) * NG;
 #pragma unroll
-      for (int i = 0; i < NG; ++i) sc[j][i] = sp[i];
-    }
-  };
-  load(0);
+    for (int i = 0; i < NG; ++i) sc[j][i] = sp[i];
+  }
   // what the epilogue of the lane's rows n .. n + 3 reads, under the weights' latency
   const long n = rt * kTileN + 4 * c;
   const int head = (int)(n >> 6), hc = (int)(n & 63) >> 1;
   int pos = 0;
   float b[4] = {0.f, 0.f, 0.f, 0.f}, sn[2] = {0.f, 0.f}, cs[2] = {1.f, 1.f};
-  if (EPI == DEC_QKV_ROPE) {
+  if (EPI == DEC_QKV_ROPE && wave == 0) {
     pos = *d.pos;
 #pragma unroll
     for (int i = 0; i < 4; ++i) b[i] = d.bias[head * 64 + hc + (i >> 1) + 32 * (i & 1)];
@@ -379,15 +381,21 @@ __global__ __launch_bounds__(64) void q4_row_kernel(Q4Args a, DecGemvArgs d) {
   float ss = 0.0f;
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
-    if (j * kBlockK + 2 * lane >= a.K) x[j] = make_float2(0.f, 0.f);
+    if ((first + j) * kBlockK + 2 * lane >= a.K) x[j] = make_float2(0.f, 0.f);
     ss += x[j].x * x[j].x + x[j].y * x[j].y;
   }
-  const float rs = 1.0f / sqrtf(wave_sum(ss) / (float)a.K + d.eps);
+  ss = wave_sum(ss);
+  if (lane == 0) squares[wave] = ss;
+  __syncthreads();
+  ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) ss += squares[i];
+  const float rs = 1.0f / sqrtf(ss / (float)a.K + d.eps);
   float top = 0.0f;
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     x[j] = make_float2((x[j].x * rs) * g[j].x, (x[j].y * rs) * g[j].y);
-    const int k = j * kBlockK + 2 * lane;
+    const int k = (first + j) * kBlockK + 2 * lane;
     if (EPI == DEC_HEAD && rt == 0 && d.y2 && k < a.K)
       *reinterpret_cast<float2*>(d.y2 + k) = x[j];
     top = fmaxf(top, fmaxf(fabsf(x[j].x), fabsf(x[j].y)));
@@ -398,37 +406,41 @@ __global__ __launch_bounds__(64) void q4_row_kernel(Q4Args a, DecGemvArgs d) {
   for (int j = 0; j < NB; ++j) {
     half2_t p0, p1;
     split_pair(x[j].x, x[j].y, xs, p0, p1);
-    *reinterpret_cast<half2_t*>(lds + j * 256 + lane * 4) = p0;
-    *reinterpret_cast<half2_t*>(lds + ROW + j * 256 + lane * 4) = p1;
+    *reinterpret_cast<half2_t*>(mine + j * 256 + lane * 4) = p0;
+    *reinterpret_cast<half2_t*>(mine + ROW + j * 256 + lane * 4) = p1;
   }
-  __syncthreads();  // of one wave
-  const char* xr = lds + (col & 1) * ROW + c * 16;  // column 0: first parts, 1: second parts
+  // the staged row is this wave's own: in program order, no barrier
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  const char* xr = mine + (col & 1) * ROW + c * 16;  // column 0: first parts, 1: second parts
   floatx4 tot = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int first = 0; first < NB; first += H) {
-    if (first > 0) load(first);
+  for (int j = 0; j < NB; ++j) {
+    if (first + j >= kb) break;
 #pragma unroll
-    for (int j = 0; j < H; ++j) {
-      if (first + j >= kb) break;
+    for (int i = 0; i < NG; ++i) {
+      floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+      for (int t = i * TG; t < (i + 1) * TG; ++t)
+        acc = mfma_f16(q4_frag(w[j][t], pattern),
+                       *reinterpret_cast<const half8_t*>(xr + j * 256 + t * 64), acc);
 #pragma unroll
-        for (int t = i * TG; t < (i + 1) * TG; ++t)
-          acc = mfma_f16(q4_frag(w[j][t], pattern),
-                         *reinterpret_cast<const half8_t*>(xr + (first + j) * 256 + t * 64), acc);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) tot[e] = fmaf(bf16_lo(sc[j][i][e]), acc[e], tot[e]);
-      }
+      for (int e = 0; e < 4; ++e) tot[e] = fmaf(bf16_lo(sc[j][i][e]), acc[e], tot[e]);
     }
   }
-  float v[4];
+  floatx4 v;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     tot[e] *= f;
     v[e] = tot[e] + dpp_mov<kDppXor1>(tot[e]);
   }
-  if (col) return;
+  if (col == 0) sums[wave][c] = v;
+  __syncthreads();
+  if (wave || col) return;
+  v = sums[0][c];
+#pragma unroll
+  for (int i = 1; i < W; ++i) v += sums[i][c];
   if (EPI == DEC_QKV_ROPE) {
     const int cl = head * 64 + hc;
     float* dst = cl < d.q_cols ? d.y + cl
@@ -738,7 +750,7 @@ int q4_pack(const float* W, void* Wq, int N, int K, int group, int neox, hipStre
 namespace {
 template <int EPI, int NB>
 int launch_row(const Q4Args& a, const DecGemvArgs& d, int G, hipStream_t s) {
-  const dim3 grid((unsigned)q4_tiles(a.N)), block(64);
+  const dim3 grid((unsigned)q4_tiles(a.N)), block(64 * kRowWaves);
   if (G == 32)
     hipLaunchKernelGGL((q4_row_kernel<32, EPI, NB>), grid, block, 0, s, a, d);
   else if (G == 64)
@@ -773,15 +785,15 @@ int dec_gemv_q4(int epi, const DecGemvArgs& d, const void* Wq, int group, hipStr
     case DEC_QKV_ROPE:
       LX_REQUIRE(N % 64 == 0 && d.bias && d.pos && d.k_cache && d.v_cache && d.inv_freq,
                  "dec_gemv_q4: qkv args");
-      return wide ? launch_row<DEC_QKV_ROPE, 16>(a, d, group, s)
-                  : launch_row<DEC_QKV_ROPE, 8>(a, d, group, s);
+      return wide ? launch_row<DEC_QKV_ROPE, 16 / kRowWaves>(a, d, group, s)
+                  : launch_row<DEC_QKV_ROPE, 8 / kRowWaves>(a, d, group, s);
     case DEC_SWIGLU:
       LX_REQUIRE(N % 2 == 0, "dec_gemv_q4: swiglu needs an even N");
-      return wide ? launch_row<DEC_SWIGLU, 16>(a, d, group, s)
-                  : launch_row<DEC_SWIGLU, 8>(a, d, group, s);
+      return wide ? launch_row<DEC_SWIGLU, 16 / kRowWaves>(a, d, group, s)
+                  : launch_row<DEC_SWIGLU, 8 / kRowWaves>(a, d, group, s);
     case DEC_HEAD:
-      return wide ? launch_row<DEC_HEAD, 16>(a, d, group, s)
-                  : launch_row<DEC_HEAD, 8>(a, d, group, s);
+      return wide ? launch_row<DEC_HEAD, 16 / kRowWaves>(a, d, group, s)
+                  : launch_row<DEC_HEAD, 8 / kRowWaves>(a, d, group, s);
   }
   set_error("dec_gemv_q4: unsupported epilogue %d", epi);
   return LX_ERR_ARG;
