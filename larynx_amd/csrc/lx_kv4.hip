@@ -636,17 +636,22 @@ AttnPlan attn_plan(const Kv4& c, int nrow, int max_len) {
   const int cus = device_cus(), len = max_len <= 0 || max_len > c.rows ? c.rows : max_len;
   const long wgs = (long)p.tiles * c.batch * c.heads;
   const int steps = (len + kBlk * p.kp - 1) / (kBlk * p.kp);
-  // Splits take four waves, one per SIMD; the time in steps of a wave is workgroups a CU x steps
-  // a wave, and about five for the join's launch (1 sequence of 2001 rows, 2 kv heads: one
-  // split 11.1 us, eight 7.6 with the join; 48 of up to 4000: two 18.1, eight 15.2; 156 tiles of a
-  // prompt chunk over 1708 rows: one 13.9, two 20.2).
-  constexpr int kWaves = 4, kJoin = 5;
+  // Splits take four waves, one per SIMD, a call without splits up to eight.  The time in
+  // sixteenths of a wave's step: workgroups a CU x (steps a wave, and half of one for its start),
+  // an eighth less where two waves cover each other's waits, and five steps for the join's
+  // launch.  (1 sequence of 2001 rows, 2 kv heads: one split 11.2 us, eight 7.9 with the join; 48 of
+  // up to 4000: two 17.9, eight 15.0; 2 of 65536, 8 kv heads of 128 channels: 16 37.1, 32 33.9; 64
+  // query rows over 16384: four 33.8, eight 29.9; a prompt chunk of 156 tiles over 1708 rows: one
+  // 14.1, two 21.0.)
+  constexpr int kWaves = 4, kJoin = 80;
   long best = LONG_MAX;
   p.splits = 1;
   for (const int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 40, 48, 64}) {
     if (s > steps) break;
-    const long t = (wgs * s + cus - 1) / cus * ((steps + kWaves * s - 1) / (kWaves * s)) +
-                   (s > 1 ? kJoin : 0);
+    const long each = (wgs * s + cus - 1) / cus;
+    const int waves = s > 1 ? kWaves : kMaxWaves, n = (steps + waves * s - 1) / (waves * s);
+    const long half = s > 1 ? 2L * n + 1 : 4L * n + 1;
+    const long t = each * half * (each > 1 || s == 1 ? 7 : 8) + (s > 1 ? kJoin : 0);
     if (t < best) {
       best = t;
       p.splits = s;
