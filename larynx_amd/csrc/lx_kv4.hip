@@ -97,7 +97,10 @@ __device__ __forceinline__ unsigned quantise(float x, unsigned* pair) {
 
 // One workgroup of eight waves per (32-row record touched, channel group of a kv head, sequence):
 // four for the keys, four for the values, lane = channel.  Wave w of a plane owns the rows whose
-// value codes share dwords, 4 w .. 4 w + 3 of both halves; all eight are requested at once.
+// value codes share dwords, 4 w .. 4 w + 3 of both halves; all eight are requested at once.  A wave
+// is some 145 instructions a group (two wave-wide extremes, two quotients, the code) after one
+// memory round trip, and these bound it: 1531 rows of 2 heads 7.3 us, 1.8 MB; one row 3.3, a launch
+// and its chain.
 __global__ __launch_bounds__(512) void kv4_append_kernel(AppendArgs a) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6 & 3, plane = threadIdx.x >> 8;
   const int ng = a.c.ng, hg = blockIdx.y, b = blockIdx.z;  // hg: head * ng + group
@@ -160,7 +163,8 @@ struct ReadArgs {
   const int* pos;
 };
 
-// One thread per (row, channel) of a sequence; rows outside the cache read as zero.
+// One thread per (row, channel) of a sequence; rows outside the cache read as zero.  1531 rows of 2
+// heads 3.0 us, bound by launch and latency.
 __global__ __launch_bounds__(256) void kv4_read_kernel(ReadArgs a) {
   const int hd = a.c.ng * kGrp, width = a.c.heads * hd, b = blockIdx.y;
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
@@ -258,6 +262,11 @@ __device__ __forceinline__ float value_lift(float vtop) {
 // = S / f, f a constant of the row).  The weights p s of the values want one too: every p carries
 // 2^lg, lg = 6 - E with E the largest exponent of s so far, so that p s stays below 2^7.  It is a
 // running reference like the maximum, and part of the same exponent.
+// Half a byte a value and one read of it: the vector instructions beside the products bound long
+// contexts, 640 a step of four 128-channel records (codes to fragments 288, the softmax and the
+// weights' two parts most of the rest; the matrix pipe is 0.11 to 0.15 busy): 2 sequences of 65536
+// rows, 8 kv heads, 113 MB in 30 us, 3.8 TB/s, and 4 for the join.  Short ones are latency: 1
+// sequence of 2001 rows 4.5 us and 3.3 for the join.
 // A spilled register costs more than a wave gains: the registers follow from NG and KP.
 template <int NG, int KP>
 __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
@@ -552,7 +561,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
 
 // The splits' states of a row joined: one workgroup a row, HD / 4 lanes of four channels, the
 // other lanes' groups taking every kG-th split; the groups' states are joined in group order, so
-// the result does not depend on timing.
+// the result does not depend on timing.  A launch and two dependent round trips (the length, then
+// all states at once): 3.3 us for 14 rows, 4 for 672.
 template <int NG>
 __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a) {
   constexpr int HD = NG * kGrp, L4 = HD / 4, kG = 256 / L4;
@@ -639,10 +649,10 @@ AttnPlan attn_plan(const Kv4& c, int nrow, int max_len) {
   // Splits take four waves, one per SIMD, a call without splits up to eight.  The time in
   // sixteenths of a wave's step: workgroups a CU x (steps a wave, and half of one for its start),
   // an eighth less where two waves cover each other's waits, and five steps for the join's
-  // launch.  (1 sequence of 2001 rows, 2 kv heads: one split 11.2 us, eight 7.9 with the join; 48 of
-  // up to 4000: two 17.9, eight 15.0; 2 of 65536, 8 kv heads of 128 channels: 16 37.1, 32 33.9; 64
-  // query rows over 16384: four 33.8, eight 29.9; a prompt chunk of 156 tiles over 1708 rows: one
-  // 14.1, two 21.0.)
+  // launch.  (1 sequence of 2001 rows, 2 kv heads: one split 11.2 us, eight 7.9 with the join; 48
+  // of up to 4000: two 17.9, eight 15.0; 2 of 65536, 8 kv heads of 128 channels: 16 37.1, 32 33.9;
+  // 64 query rows over 16384: four 33.8, eight 29.9; a prompt chunk of 156 tiles over 1708 rows:
+  // one 14.1, two 21.0.)
   constexpr int kWaves = 4, kJoin = 80;
   long best = LONG_MAX;
   p.splits = 1;

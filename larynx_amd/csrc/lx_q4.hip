@@ -2,10 +2,12 @@
 //
 //   w~[n, k] = s[n, k / G] * (q[n, k] - 8),  y = epi(x w~^T + bias),  G = 32, 64 or 128.
 //
-// What bounds it is the weight stream (half a byte a weight), so the codes go from memory to
-// the matrix cores with nine instructions for eight of them (lx_four_bit.hpp) and the scale is
+// What bounds large weights is their stream (half a byte a weight), so the codes go from memory
+// to the matrix cores with nine instructions for eight of them (lx_four_bit.hpp) and the scale is
 // applied once per group to the fp32 sum, not to the weights.  x enters as two fp16 parts after a
-// power of two per row and block of 128 inputs, so every product is exact.
+// power of two per row and block of 128 inputs, so every product is exact.  Three kernels: one
+// that stages up to 8 rows per wave, one that keeps up to 64 in registers, one for the single
+// normalised row of the LM's decode.
 //
 // Layout (lx_q4_pack_f32): per tile of 16 rows and block of 128 inputs 1 KB of codes, the 64
 // lanes' 16-byte fragments (dword t of lane l: row l % 16, k = 32 t + 8 (l / 16) + 0..7), then
@@ -194,7 +196,11 @@ __device__ __forceinline__ void q4_epi_quad(const Q4Args& a, int m, long n, floa
 // At most MB rows of x.  A workgroup owns one tile of 16 weight rows; its waves take the blocks
 // of K in turn, each splitting its own 128 inputs of x into a slice of LDS (16 lanes a row, four
 // rows at a time), and their sums meet in LDS at the end (in a fixed order).  Column 2 m + part of
-// the fragments is a part of row m.
+// the fragments is a part of row m.  Everything a wave reads is requested before it computes, and
+// the next block before this one; what remains is a launch, one memory round trip, the split
+// (some 60 instructions a block) and the meeting: in a graph 1 row x 1152 x 896 2.6 us, x 9728 3.5
+// (1.3 TB/s), 4 rows x 896 x 4864 4.4, 8 rows x 9728 x 896 4.9, where a copy asks 0.1 to 1.0.
+// (With a lane per row of x each load touched 64 lines: 3 rows x 6761 5.4 us, now 3.3.)
 constexpr int kFewRow = 272;  // bytes of a staged row (128 fp16, and 16 against bank conflicts)
 
 template <int MB>
@@ -471,8 +477,13 @@ __global__ __launch_bounds__(64 * kRowWaves) void q4_row_kernel(Q4Args a, DecGem
 // of 16 rows at a time, one group of tiles ahead.  The waves' sums meet in one of two LDS buffers
 // (a barrier a group), added in wave order; each thread adds and finishes one quad of outputs.
 // More than one split: partial sums into ws (splits, M, N up to 16), which q4_join_kernel adds in
-// split order.  (With x in LDS and whole K ranges a wave, every fragment of x is read again for
-// every two tiles: 64 rows 8192 x 8192 33 us, 9728 x 896 17.)
+// split order.  16 rows x 151936 x 896 stream at 4.4 TB/s (18.7 us in a graph).  Every 16 rows more
+// cost 8192 x 8192 about 5.5 us (16: 14.2, 32: 18.9, 48: 25.1, 64: 31.8, the join's 5 among them):
+// their splitting, 100 instructions a lane, then matrix instructions at the clock the power limit
+// leaves, and 4 MB of partial sums written and read.  (With x in LDS and whole K ranges a wave,
+// every fragment of x is read again for every two tiles: 64 rows 8192 x 8192 33 us, 9728 x 896 17
+// for 11.4 now.  Sums of a group added under the next one's products, with one register buffer
+// of weights for two: 33 us.)
 constexpr int kManyWaves = 8;
 constexpr int kManyTiles = 2;  // RT
 constexpr size_t many_bytes(int ct) {
@@ -635,7 +646,8 @@ __global__ __launch_bounds__(64 * kManyWaves) __attribute__((
   }
 }
 
-// The splits' sums added in split order, and the epilogue: one thread per four rows of W.
+// The splits' sums added in split order, and the epilogue: one thread per four rows of W (64 rows
+// 8192 x 8192: 17 MB of sums in 4.6 us, 3.6 TB/s).
 __global__ __launch_bounds__(256) void q4_join_kernel(Q4Args a) {
   const long np4 = q4_tiles(a.N) * (kTileN / 4);
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
