@@ -264,9 +264,9 @@ __device__ __forceinline__ float value_lift(float vtop) {
 // running reference like the maximum, and part of the same exponent.
 // Half a byte a value and one read of it: the vector instructions beside the products bound long
 // contexts, 640 a step of four 128-channel records (codes to fragments 288, the softmax and the
-// weights' two parts most of the rest; the matrix pipe is 0.11 to 0.15 busy): 2 sequences of 65536
-// rows, 8 kv heads, 113 MB in 30 us, 3.8 TB/s, and 4 for the join.  Short ones are latency: 1
-// sequence of 2001 rows 4.5 us and 3.3 for the join.
+// weights' two parts most of the rest; the matrix pipe is 0.13 busy): 2 sequences of 65536 rows, 8
+// kv heads, 114 MB in 33 us, 3.5 TB/s, and 4 to 5 for the join.  Short ones are latency: 1 sequence
+// of 2001 rows 5.4 us and 3.3 for the join.
 // A spilled register costs more than a wave gains: the registers follow from NG and KP.
 template <int NG, int KP>
 __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
