@@ -245,6 +245,23 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, int b, int h, int r
 // unnormalised outputs, then 16 maxima (in units of log2) and 16 sums.
 __host__ __device__ constexpr long part_floats(int ng) { return (long)kQ * (ng * kGrp + 2); }
 
+// Among the four lanes of a column, l, l ^ 16, l ^ 32 and l ^ 48 (a swap leaves each lane with
+// its own and the other's value, in either order).
+template <class F>
+__device__ __forceinline__ float over_column(float v, F f) {
+  const unsigned a = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  const unsigned b = __float_as_uint(f(__uint_as_float(r[0]), __uint_as_float(r[1])));
+  const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return f(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+__device__ __forceinline__ float column_max(float v) {
+  return over_column(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float column_sum(float v) {
+  return over_column(v, [](float a, float b) { return a + b; });
+}
+
 // log2 of what the weights carry for values whose largest scale is vtop: 6 - E, within what
 // sums of 2^20 weights leave of fp32's range.
 __device__ __forceinline__ float value_lift(float vtop) {
@@ -274,7 +291,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
   constexpr int HD = NG * kGrp, R = kQ / KP;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   float (*om)[kQ][HD + 4] = reinterpret_cast<float (*)[kQ][HD + 4]>(lds);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   float (*ml)[2][kQ] =
       reinterpret_cast<float (*)[2][kQ]>(lds + (size_t)waves * kQ * (HD + 4) * sizeof(float));
   const int col = lane & 15, c = lane >> 4, set = col / R;
@@ -356,9 +374,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
 #pragma unroll
           for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[g][ks][4 * e + j]));
         }
-    top = fmaxf(top, lane_xor16(top));
-    top = fmaxf(top, lane_xor32(top));
-    const float sc = row_scale(top, &f);
+    const float sc = row_scale(column_max(top), &f);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       float s = 0.0f;
@@ -372,9 +388,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
           ql[(g * 4 + ks * 2 + 1) * 64] = qf[g][ks][1];
         }
       }
-      s += lane_xor16(s);
-      s += lane_xor32(s);
-      qsum[g] = s;
+      qsum[g] = column_sum(s);
     }
     if (NG == 2) __syncthreads();
   }
@@ -440,13 +454,11 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
     for (int g = 0; g < NG; ++g)
 #pragma unroll
       for (int j = 0; j < 8; ++j) vx = fmaxf(vx, bf16_lo(vp[g][j >> 2][j & 3]));
-    mx = fmaxf(mx, lane_xor16(mx));
-    mx = fmaxf(mx, lane_xor32(mx));
-    vx = fmaxf(vx, lane_xor16(vx));
-    vx = fmaxf(vx, lane_xor32(vx));
     if (__any(mx > m || vx > vtop)) {
-      // the sums so far move to the new maximum and the new lift
-      const float mn = fmaxf(m, mx), lgn = value_lift(vx);
+      // the sums so far move to the new maximum and the new lift of their column
+      const float mn = fmaxf(m, column_max(mx));
+      vx = column_max(vx);
+      const float lgn = value_lift(vx);
       const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m - mn, f, lgn - lg));
       m = mn;
       vtop = vx;
@@ -495,12 +507,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
   }
   // the lane's sums over its keys -> the column's, without the lift
   const float drop = __builtin_amdgcn_exp2f(-lg);
-  l += lane_xor16(l);
-  l += lane_xor32(l);
+  l = column_sum(l);
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    zsum[g] += lane_xor16(zsum[g]);
-    zsum[g] += lane_xor32(zsum[g]);
+    zsum[g] = column_sum(zsum[g]);
 #pragma unroll
     for (int ct = 0; ct < 4; ++ct) {
       floatx4 v = o[g][ct] + floatx4{zsum[g], zsum[g], zsum[g], zsum[g]};
