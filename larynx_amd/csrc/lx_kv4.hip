@@ -571,8 +571,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
 
 // The splits' states of a row joined: one workgroup a row, HD / 4 lanes of four channels, the
 // other lanes' groups taking every kG-th split; the groups' states are joined in group order, so
-// the result does not depend on timing.  A launch and two dependent round trips (the length, then
-// all states at once): 3.3 us for 14 rows, 4 for 672.
+// the result does not depend on timing.  A launch and one round trip: 3.3 us for 14 rows, 4 for
+// 672.
 template <int NG>
 __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a) {
   constexpr int HD = NG * kGrp, L4 = HD / 4, kG = 256 / L4;
@@ -581,23 +581,24 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a) {
   const int chn = (int)(threadIdx.x % L4) * 4, gr = (int)(threadIdx.x / L4);
   const int rr = blockIdx.x, h = blockIdx.y, b = blockIdx.z, nrow = a.Tq * a.rep;
   const int qt = rr / a.trows, r = rr - qt * a.trows;
-  const Span n = attn_span(a, min(max(a.lens[b], 0), a.c.rows), qt, nrow);
-  const int count = max((n.n_step + n.per - 1) / n.per, 1);
   const float* p =
       a.ws + (((long)b * a.c.heads + h) * a.tiles + qt) * a.splits * part_floats(NG);
   float M = -INFINITY, L = 0.0f;
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-  // every state of a group requested before the first is used
+  // every state of a group requested before the first is used, and before the length says how
+  // many there are
   constexpr int U = kMaxSplits / kG;
   float ms[U], ls[U];
   float4 u[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
-    const float* ps = p + min(gr + i * kG, count - 1) * part_floats(NG);
+    const float* ps = p + min(gr + i * kG, a.splits - 1) * part_floats(NG);
     ms[i] = ps[kQ * HD + r];
     ls[i] = ps[kQ * HD + kQ + r];
     u[i] = *reinterpret_cast<const float4*>(ps + r * HD + chn);
   }
+  const Span n = attn_span(a, min(max(a.lens[b], 0), a.c.rows), qt, nrow);
+  const int count = max((n.n_step + n.per - 1) / n.per, 1);
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     if (gr + i * kG >= count) {  // no such state
