@@ -204,11 +204,12 @@ struct AttnArgs {
   float* o;
   long ldo;
   float* ws;
-  int Tq, rep, tiles, trows, kp, splits, chunk, causal;
+  int Tq, rep, tiles, splits, chunk, causal;
+  int kshift;  // log2 of the records side by side; a tile has 16 >> kshift query rows
   float scale2;  // scale * log2(e)
 };
 
-// The keys of a tile of query rows, in steps of kp records: split sp takes steps [sp * per, sp *
+// The keys of a tile of query rows, in steps of 1 << kshift records: split sp takes steps [sp * per, sp *
 // per + per) of n_step.  A split is a.chunk steps long, so that the workgroups of sequences of
 // all lengths have the same work, and longer only where a sequence passes the length the
 // launch was sized for.
@@ -220,13 +221,13 @@ __device__ __forceinline__ Span attn_span(const AttnArgs& a, int len, int qt, in
   Span s;
   s.most = s.least = len;
   if (a.causal && a.Tq > 1) {
-    const int t_first = qt * a.trows / a.rep;
-    const int t_last = min(qt * a.trows + a.trows - 1, nrow - 1) / a.rep;
+    const int rows = kQ >> a.kshift, first = qt * rows;
+    const int t_first = first / a.rep, t_last = min(first + rows - 1, nrow - 1) / a.rep;
     s.most = max(len - a.Tq + t_last + 1, 0);
     s.least = max(len - a.Tq + t_first + 1, 0);
   }
   s.n_blk = (s.most + kBlk - 1) / kBlk;
-  s.n_step = (s.n_blk + a.kp - 1) / a.kp;
+  s.n_step = (s.n_blk + (1 << a.kshift) - 1) >> a.kshift;
   s.per = a.chunk;
   if (s.n_step > a.chunk * a.splits) s.per = (s.n_step + a.splits - 1) / a.splits;
   return s;
@@ -580,7 +581,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a) {
   __shared__ float ml[2][kG];
   const int chn = (int)(threadIdx.x % L4) * 4, gr = (int)(threadIdx.x / L4);
   const int rr = blockIdx.x, h = blockIdx.y, b = blockIdx.z, nrow = a.Tq * a.rep;
-  const int qt = rr / a.trows, r = rr - qt * a.trows;
+  const int qt = rr >> (4 - a.kshift), r = rr - (qt << (4 - a.kshift));
   const float* p =
       a.ws + (((long)b * a.c.heads + h) * a.tiles + qt) * a.splits * part_floats(NG);
   float M = -INFINITY, L = 0.0f;
@@ -803,8 +804,7 @@ extern "C" int lx_attention_kv4_f32(const float* q, long ldq, const lx_kv4* cach
   a.scale2 = scale * 1.4426950408889634f;
   const AttnPlan p = attn_plan(a.c, Tq * a.rep, max_len);
   a.tiles = p.tiles;
-  a.trows = kQ / p.kp;
-  a.kp = p.kp;
+  a.kshift = p.kp == 4 ? 2 : p.kp == 2 ? 1 : 0;
   a.splits = p.splits;
   a.chunk = p.chunk;
   const long wgs = (long)p.tiles * a.c.batch * a.c.heads;
