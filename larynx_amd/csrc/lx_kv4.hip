@@ -281,10 +281,11 @@ __device__ __forceinline__ float value_lift(float vtop) {
 // 2^lg, lg = 6 - E with E the largest exponent of s so far, so that p s stays below 2^7.  It is a
 // running reference like the maximum, and part of the same exponent.
 // Half a byte a value and one read of it: the vector instructions beside the products bound long
-// contexts, 640 a step of four 128-channel records (codes to fragments 288, the softmax and the
-// weights' two parts most of the rest; the matrix pipe is 0.13 busy): 2 sequences of 65536 rows, 8
-// kv heads, 114 MB in 33 us, 3.5 TB/s, and 4 to 5 for the join.  Short ones are latency: 1 sequence
-// of 2001 rows 5.4 us and 3.3 for the join.
+// contexts, some 900 a step of four 128-channel records (codes to fragments 576, the softmax and
+// the weights' two parts most of the rest; the matrix pipe is 0.13 busy): 2 sequences of 65536
+// rows, 8 kv heads, 114 MB in 33 us, 3.5 TB/s, and 4 to 5 for the join; 64 sequences of up to 4096
+// run at some 5.  Short ones are latency: 1 sequence of 2001 rows 5.4 us and 3.1 for the join, 7.5
+// for both in a graph.
 // A spilled register costs more than a wave gains: the registers follow from NG and KP.
 template <int NG, int KP>
 __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
@@ -572,8 +573,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
 
 // The splits' states of a row joined: one workgroup a row, HD / 4 lanes of four channels, the
 // other lanes' groups taking every kG-th split; the groups' states are joined in group order, so
-// the result does not depend on timing.  A launch and one round trip: 3.3 us for 14 rows, 4 for
-// 672.
+// the result does not depend on timing.  A launch and one round trip: 3.1 us for 14 rows, 3.9
+// for 672.
 template <int NG>
 __global__ __launch_bounds__(256) void kv4_join_kernel(AttnArgs a) {
   constexpr int HD = NG * kGrp, L4 = HD / 4, kG = 256 / L4;
