@@ -209,10 +209,10 @@ struct AttnArgs {
   float scale2;  // scale * log2(e)
 };
 
-// The keys of a tile of query rows, in steps of 1 << kshift records: split sp takes steps [sp * per, sp *
-// per + per) of n_step.  A split is a.chunk steps long, so that the workgroups of sequences of
-// all lengths have the same work, and longer only where a sequence passes the length the
-// launch was sized for.
+// The keys of a tile of query rows, in steps of 1 << kshift records: split sp takes steps [sp *
+// per, sp * per + per) of n_step.  A split is a.chunk steps long, so that the workgroups of
+// sequences of all lengths have the same work, and longer only where a sequence passes the
+// length the launch was sized for.
 struct Span {
   int most, least;  // the longest and the shortest run of keys a row of the tile sees
   int n_blk, n_step, per;

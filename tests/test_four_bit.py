@@ -24,7 +24,8 @@ def test_sizes():
     assert lib.lx_kv4_bytes(3, 1, 128, 33) == 3 * 2 * 2 * 2304
     assert lib.lx_kv4_bytes(64, 32, 128, 1 << 22) == 64 * 32 * (1 << 17) * 4608  # past 32 bits
     for bad in [(0, 1, 64, 1), (1, 0, 64, 1), (1, 1, 32, 1), (1, 1, 96, 1), (1, 1, 64, 0),
-                (1, 1, 64, -5), (1, 1, 64, 2 ** 31 - 1), (1, 1, 64, 2 ** 31 - 128), (65536, 4, 64, 1), (4, 32768, 64, 1)]:
+                (1, 1, 64, -5), (1, 1, 64, 2 ** 31 - 1), (1, 1, 64, 2 ** 31 - 128),
+                (65536, 4, 64, 1), (4, 32768, 64, 1)]:
         assert lib.lx_kv4_bytes(*bad) == 0, bad
 
 
