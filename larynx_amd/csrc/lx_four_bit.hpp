@@ -6,7 +6,8 @@
 // or 1024 + 16 q, a packed fp16 add or fma makes them q - 8, exactly: 9 instructions for eight
 // codes.  Signed codes keep the fp32 sums as small as the values they stand for; an offset left
 // in and taken off later (bf16 has no packed add: 7 instructions) cost a digit where values
-// average out, or twice the matrix instructions.
+// average out, or twice the matrix instructions.  (The bits alone are subnormal numbers, five
+// instructions, but the sums of their products lose ten bits.)
 //
 // The other operand is fp32 data as two fp16 parts, after a power of two of its own per row that
 // brings the largest value to 1 .. 2: x = x0 + x1 to within 2^-23 of x, or 2^-25 of the row's

@@ -539,6 +539,36 @@ def test_attention_every_weight(gpu, hd, heads, kv, Tq):
     assert np.abs(got - want).max() < tol, (np.abs(got - want).max(), tol)
 
 
+@pytest.mark.parametrize("hd,heads,kv,Tq,rows", [(64, 14, 2, 1, 37), (64, 16, 16, 1, 600),
+                                                 (128, 32, 8, 3, 200), (64, 14, 2, 50, 300),
+                                                 (128, 8, 1, 1, 3000)])
+def test_attention_does_not_drift(gpu, hd, heads, kv, Tq, rows):
+    """Weights of all sizes, down to e^-20.  The bound of test_attention_every_weight, for scores up
+    to S, is eight times what roundings that go either way come to: their root mean square is an
+    eighth of it, and their mean over N outputs sqrt(N) times less.  Sums that drop bits on one
+    side are off by little, but everywhere and alike."""
+    from larynx_amd import ops
+    announce(f"kv4 attention drift hd={hd} heads={heads}/{kv} Tq={Tq} rows={rows}")
+    rng = _gen(hd + heads + rows)
+    B = 2 if Tq > 1 else 6
+    k = rng.standard_normal((B, rows, kv, hd)).astype(np.float32)
+    v = rng.standard_normal((B, rows, kv, hd)).astype(np.float32)
+    q = (2 * rng.standard_normal((B, Tq, heads * hd))).astype(np.float32)
+    cache = ops.kv4_cache(B, kv, rows, hd)
+    zero = torch.zeros(B, dtype=torch.int32, device=gpu)
+    ops.kv4_append(cache, _dev(k.reshape(B, rows, -1), gpu), _dev(v.reshape(B, rows, -1), gpu),
+                   zero)
+    got = ops.attention_kv4(_dev(q, gpu), cache, zero + rows, heads, causal=False).cpu().numpy()
+    kt, vt = ref_cache(k)[0], ref_cache(v)[0]
+    want = ref_attention(q, kt, vt, [rows] * B, heads, hd ** -0.5, False)
+    S = np.abs(np.einsum("btgrc,bkgc->btgrk", q.astype(np.float64).reshape(
+        B, Tq, kv, heads // kv, hd), kt)).max() * hd ** -0.5
+    one = np.abs(vt).max() * (U * (28 * S + 16) + 2.0 ** -22)
+    err = got - want
+    assert math.sqrt((err ** 2).mean()) < one / 8, (math.sqrt((err ** 2).mean()), one)
+    assert abs(err.mean()) < one / math.sqrt(err.size), (err.mean(), one, err.size)
+
+
 def test_attention_large_scores(gpu):
     """Scores in the hundreds, rising along the keys: the running maximum moves in every record."""
     from larynx_amd import ops
