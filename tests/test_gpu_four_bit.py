@@ -181,6 +181,25 @@ def test_linear_bit_exact_on_larger_shapes(gpu, M, N, K, G):
     assert (out[M:] == -77).all() and (out[:, N:] == -77).all()
 
 
+@pytest.mark.parametrize("G", [32, 64, 128])
+@pytest.mark.parametrize("M", [1, 4, 7, 8, 16, 33, 64])
+@pytest.mark.parametrize("N,K", [(200, 132), (1152, 896), (97, 4864), (60000, 900)])
+def test_linear_every_bit_of_x(gpu, M, N, K, G):
+    """Whole numbers of 20 bits and both signs, a single weight a row: each output is one product,
+    exact in fp32, and x's two fp16 parts hold it exactly (11 bits each, and 2^-24 of the largest of
+    a block is below 1)."""
+    from larynx_amd import ops
+    announce(f"q4 linear bits of x M={M} N={N} K={K} G={G}")
+    g = torch.Generator(device=gpu).manual_seed(M * N + K + G)
+    at = torch.randint(0, K, (N,), device=gpu, generator=g)
+    val = -8.0 * 2.0 ** torch.randint(-3, 4, (N,), device=gpu, generator=g)
+    W = torch.zeros(N, K, device=gpu)
+    W[torch.arange(N, device=gpu), at] = val
+    x = torch.randint(-2 ** 20 + 1, 2 ** 20, (M, K), device=gpu, generator=g).float()
+    got = ops.linear_q4(x, ops.q4_pack(W, G))
+    assert torch.equal(got, x[:, at] * val)
+
+
 @pytest.mark.parametrize("M", [2, 20])
 def test_linear_far_offsets(gpu, M):
     """A weight of 4.3 GB of codes (34 GB in fp32), the last rows other than zero: offsets past 32
