@@ -385,8 +385,8 @@ int lx_q4_unpack_f32(const void* Wq, float* W, int N, int K, int group, hipStrea
  * packed codes stand for, fp32 arithmetic (x as two fp16 parts after a power of two
  * per row and 128 inputs, exact products with the codes, fp32 sums; the scale
  * applied to each group's sum).  x: (M, K), 1 <= M <= 64, row stride ldx; y: (M, N), row stride ldy (N / 2 columns for
- * SWIGLU_PAIRED, N even); y must not overlap x.  Epilogues: none, GELU_TANH, RESID,
- * SWIGLU_PAIRED (others: LX_ERR_ARG); bias (N) or NULL.  K (at most 2^26 - 1024 with
+ * SWIGLU_PAIRED, N even); y must not overlap x (LX_ERR_ARG).  Epilogues: none,
+ * GELU_TANH, RESID, SWIGLU_PAIRED (others: LX_ERR_ARG); bias (N) or NULL.  K (at most 2^26 - 1024 with
  * more than 4 rows) and ldx multiples of 4, x and Wq 16-byte aligned.  An infinite or
  * NaN element of x makes NaN of its row.  The result does not depend on timing.  ws: lx_linear_q4_ws_floats() floats
  * of scratch, 16-byte aligned (NULL when that is 0: up to 4 rows, and K up to 1024);
@@ -438,7 +438,7 @@ int lx_kv4_read_f32(const lx_kv4* cache, float* k, float* v, int T, const int* p
  * rows, then attend with the lengths that count them).  A query that sees no row
  * gives zeros.  q, o: (batch, Tq, *), row strides ldq / ldo (multiples of 4,
  * sequences Tq rows apart), 16-byte aligned, head h at column h * hd; o must not
- * overlap q.  What unseen rows hold does not matter, NaN included; a NaN or an
+ * overlap q (LX_ERR_ARG).  What unseen rows hold does not matter, NaN included; a NaN or an
  * infinity in a query makes NaN of its row and head, and so may keys above 2^118 in
  * magnitude (their sums are formed with the query scaled to 1 .. 2).
  * max_len: the largest length expected (0: max_rows).  It only sizes the launch:

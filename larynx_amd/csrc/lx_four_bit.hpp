@@ -116,6 +116,17 @@ __device__ __forceinline__ floatx4 mfma_f16(half8_t a, half8_t b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// Whether `rows` rows of ca floats every lda from a and of cb every ldb from b share memory; rows of
+// unequal strides that interleave count as sharing.
+inline bool rows_overlap(const float* a, long lda, long ca, const float* b, long ldb, long cb,
+                         long rows) {
+  const intptr_t pa = (intptr_t)a / 4, pb = (intptr_t)b / 4;
+  if (pa + (rows - 1) * lda + ca <= pb || pb + (rows - 1) * ldb + cb <= pa) return false;
+  if (lda != ldb) return true;
+  const long d = ((pb - pa) % lda + lda) % lda;  // the column of a's rows where b's begin
+  return d < ca || d + cb > lda;
+}
+
 // fp32 bits of the bf16 in the low or high half of a dword.
 __device__ __forceinline__ float bf16_lo(unsigned u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_hi(unsigned u) { return __uint_as_float(u & 0xffff0000u); }

@@ -794,6 +794,8 @@ extern "C" int lx_attention_kv4_f32(const float* q, long ldq, const lx_kv4* cach
              "aligned");
   LX_REQUIRE((long)Tq * (n_heads / a.c.heads) <= INT_MAX - kQ, "attention_kv4: Tq=%d too long",
              Tq);
+  LX_REQUIRE(!rows_overlap(q, ldq, width, o, ldo, width, (long)a.c.batch * Tq),
+             "attention_kv4: o overlaps q");
   a.q = q;
   a.ldq = ldq;
   a.lens = lens;

@@ -855,6 +855,8 @@ extern "C" int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int gr
   LX_REQUIRE(((uintptr_t)x | (uintptr_t)Wq) % 16 == 0 &&
                  ((uintptr_t)y | (uintptr_t)bias) % 4 == 0,
              "linear_q4: x and Wq must be 16-byte aligned");
+  LX_REQUIRE(!rows_overlap(x, ldx, K, y, ldy, kind == LX_EPI_SWIGLU_PAIRED ? N / 2 : N, M),
+             "linear_q4: y overlaps x");
   Q4Args a{};
   a.x = x;
   a.ldx = ldx;

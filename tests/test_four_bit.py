@@ -9,6 +9,7 @@ from larynx_amd._lib import (LX_EPI_GATED_RESID, LX_EPI_ROPE_PARTIAL,
                              LX_EPI_SWIGLU_PAIRED, LX_ERR_ARG, Epilogue, Kv4, lib)
 
 P = 4096  # stands for a device address: nothing below may reach the device
+O = 1 << 40  # another, for outputs
 
 
 def test_sizes():
@@ -39,7 +40,7 @@ def test_pack_refusals():
         assert lib.lx_q4_unpack_f32(*args, None) == LX_ERR_ARG, args
 
 
-def _linear(x=P, ldx=64, w=P, group=64, bias=None, y=P, ldy=32, M=1, N=32, K=64, kind=None,
+def _linear(x=P, ldx=64, w=P, group=64, bias=None, y=O, ldy=32, M=1, N=32, K=64, kind=None,
             ws=None, n=0):
     epi = None if kind is None else C.byref(Epilogue(kind=kind))
     return lib.lx_linear_q4_f32(x, ldx, w, group, bias, y, ldy, M, N, K, epi, ws, n, None)
@@ -48,7 +49,7 @@ def _linear(x=P, ldx=64, w=P, group=64, bias=None, y=P, ldy=32, M=1, N=32, K=64,
 @pytest.mark.parametrize("kw", [
     dict(x=None), dict(w=None), dict(y=None), dict(M=0), dict(M=65), dict(M=-1), dict(N=0),
     dict(K=62, ldx=64), dict(ldx=60), dict(ldx=66), dict(ldy=31), dict(group=16), dict(x=P + 4),
-    dict(w=P + 8), dict(y=P + 2), dict(bias=P + 1), dict(kind=LX_EPI_GATED_RESID),
+    dict(w=P + 8), dict(y=O + 2), dict(bias=P + 1), dict(kind=LX_EPI_GATED_RESID),
     dict(kind=LX_EPI_ROPE_PARTIAL), dict(kind=9), dict(kind=-1),
     dict(kind=LX_EPI_SWIGLU_PAIRED, N=31), dict(kind=LX_EPI_SWIGLU_PAIRED, ldy=15),
 ])
@@ -83,7 +84,7 @@ def test_bad_caches(cache):
     c = _cache(**cache)
     assert lib.lx_kv4_append_f32(c, P, 128, P, 128, 1, P, None) == LX_ERR_ARG
     assert lib.lx_kv4_read_f32(c, P, P, 1, P, None) == LX_ERR_ARG
-    assert lib.lx_attention_kv4_f32(P, 256, c, P, P, 256, 1, 4, 0.125, 1, 0, None, 0,
+    assert lib.lx_attention_kv4_f32(P, 256, c, P, O, 256, 1, 4, 0.125, 1, 0, None, 0,
                                     None) == LX_ERR_ARG
     assert lib.lx_attention_kv4_ws_floats(c, 1, 4, 0) == 0
     assert lib.lx_attention_kv4_ws_floats(None, 1, 4, 0) == 0
@@ -97,10 +98,10 @@ def test_cache_call_refusals():
         assert lib.lx_kv4_append_f32(c, *args, None) == LX_ERR_ARG, args
     for args in [(None, P, 1, P), (P, None, 1, P), (P, P, 0, P), (P, P, 1, None)]:
         assert lib.lx_kv4_read_f32(c, *args, None) == LX_ERR_ARG, args
-    ok = dict(q=P, ldq=256, cache=c, lens=P, o=P, ldo=256, Tq=1, heads=4)
+    ok = dict(q=P, ldq=256, cache=c, lens=P, o=O, ldo=256, Tq=1, heads=4)
     for kw in [dict(q=None), dict(lens=None), dict(o=None), dict(ldq=252), dict(ldq=258),
                dict(ldo=252), dict(ldo=257), dict(Tq=0), dict(heads=3), dict(heads=0),
-               dict(q=P + 4), dict(o=P + 8), dict(Tq=2 ** 31 - 1)]:
+               dict(q=P + 4), dict(o=O + 8), dict(Tq=2 ** 31 - 1)]:
         a = {**ok, **kw}
         assert lib.lx_attention_kv4_f32(a["q"], a["ldq"], a["cache"], a["lens"], a["o"], a["ldo"],
                                         a["Tq"], a["heads"], 0.125, 1, 0, None, 0,
@@ -110,9 +111,34 @@ def test_cache_call_refusals():
     need = lib.lx_attention_kv4_ws_floats(big, 1, 4, 0)
     assert need > 0
     for ws, n in [(None, need), (P, need - 1), (P + 8, need)]:
-        assert lib.lx_attention_kv4_f32(P, 256, big, P, P, 256, 1, 4, 0.125, 1, 0, ws, n,
+        assert lib.lx_attention_kv4_f32(P, 256, big, P, O, 256, 1, 4, 0.125, 1, 0, ws, n,
                                         None) == LX_ERR_ARG
         assert b"workspace" in lib.lx_last_error()
+
+
+@pytest.mark.parametrize("y,ldy,shared", [
+    (0, 4096, True), (2044, 4096, True), (2048, 4096, False), (2048, 4000, True),
+    (4064, 4096, False), (4068, 4096, True), (4096, 4096, True), (-32, 4096, False),
+    (-28, 4096, True), (-4096, 4096, True), (15 * 4096 + 2048, 96, False),
+    (15 * 4096 + 2044, 96, True), (-(15 * 4096 + 32), 4096, False), (-15 * 4096, 4096, True)])
+def test_outputs_over_inputs_are_refused(y, ldy, shared):
+    """16 rows of 2048 inputs, 4096 apart; 32 outputs y floats on.  The others are refused for the
+    workspace they need."""
+    x = 1 << 30
+    rc = _linear(x=x, ldx=4096, y=x + 4 * y, ldy=ldy, M=16, N=32, K=2048)
+    assert rc == LX_ERR_ARG
+    assert (b"overlaps" if shared else b"workspace") in lib.lx_last_error()
+
+
+@pytest.mark.parametrize("o,ldo,shared", [
+    (0, 512, True), (256, 512, False), (252, 512, True), (512, 512, True), (1024, 256, False),
+    (764, 512, True), (-256, 512, False), (-252, 512, True), (128, 256, True)])
+def test_attention_outputs_over_queries_are_refused(o, ldo, shared):
+    """2 sequences of a row of 256, 512 apart, over caches that take splits."""
+    q, c = 1 << 30, _cache(batch=2, rows=4096)
+    assert lib.lx_attention_kv4_f32(q, 512, c, P, q + 4 * o, ldo, 1, 4, 0.125, 1, 0, None, 0,
+                                    None) == LX_ERR_ARG
+    assert (b"overlaps" if shared else b"workspace") in lib.lx_last_error()
 
 
 def test_python_refuses_host_tensors():
