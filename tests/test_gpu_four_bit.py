@@ -737,6 +737,35 @@ def test_layer_in_a_graph(gpu):
         lens += 1
 
 
+@pytest.mark.parametrize("M,N,K,G", [(2, 300, 2000, 64), (48, 520, 2052, 32), (64, 9000, 500, 128),
+                                     (7, 33000, 1028, 64)])
+def test_products_in_two_graphs(gpu, M, N, K, G):
+    """Two graphs of the same weight, captured without a call before them, replayed in turn with
+    eager calls between: each replay gives the eager bits, splits and residual included."""
+    from larynx_amd import ops
+    announce(f"q4 linear in two graphs M={M} N={N} K={K} G={G}")
+    g = torch.Generator(device=gpu).manual_seed(M + N)
+    w = ops.q4_pack(torch.randn(N, K, device=gpu, generator=g), G)
+    resid = ops.Epilogue(kind=ops.LX_EPI_RESID)
+    xs = [torch.empty(M, K, device=gpu) for _ in range(2)]
+    ys = [torch.zeros(M, N, device=gpu) for _ in range(2)]
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for graph, x, y in zip(graphs, xs, ys):
+        with torch.cuda.graph(graph):
+            ops.linear_q4(x, w, epilogue=resid, out=y)
+    for step in range(4):
+        want = []
+        for x, y in zip(xs, ys):
+            x.copy_(torch.randn(M, K, device=gpu, generator=g))
+            want.append(ops.linear_q4(x, w, epilogue=resid, out=y.clone()))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for y, b in zip(ys, want):
+            assert torch.equal(y, b), step
+
+
 def test_two_streams_at_once(gpu):
     """Calls of two streams over one cache, both reading, and one weight."""
     from larynx_amd import ops
