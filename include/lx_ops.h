@@ -430,7 +430,7 @@ int lx_kv4_append_f32(const lx_kv4* cache, const float* k, long ldk, const float
 int lx_kv4_read_f32(const lx_kv4* cache, float* k, float* v, int T, const int* pos,
                     hipStream_t stream);
 
-/* Attention over such a cache, flash-style, fp32 arithmetic:
+/* Attention over such a cache, flash-style, fp32 arithmetic on operands in two fp16 parts:
  *   o[b, t, h*hd:(h+1)*hd] = softmax(scale * q_h k~_g^T) v~_g,  g = h / (n_heads / n_kv_heads)
  * over the first lens[b] rows of sequence b (device int32[batch]; a value outside
  * [0, max_rows] is taken as the nearer end).  causal != 0: query t stands at row
@@ -440,7 +440,12 @@ int lx_kv4_read_f32(const lx_kv4* cache, float* k, float* v, int T, const int* p
  * sequences Tq rows apart), 16-byte aligned, head h at column h * hd; o must not
  * overlap q (LX_ERR_ARG).  What unseen rows hold does not matter, NaN included; a NaN or an
  * infinity in a query makes NaN of its row and head, and so may keys above 2^118 in
- * magnitude (their sums are formed with the query scaled to 1 .. 2).
+ * magnitude (their sums are formed with the query scaled to 1 .. 2).  The query enters as
+ * two fp16 parts after a power of two, off by 2^-25 of its row and head's largest element
+ * at most, and so do the products of weights and value scales, off by 2^-31 of the largest
+ * that the sums hold so far: a row counts by its weight times its values, however large
+ * other rows' values are.  Sums are fp32, the largest weight 1: values above 2^127 over the
+ * number of rows that share a weight overflow them, and values below 2^-100 lose digits.
  * max_len: the largest length expected (0: max_rows).  It only sizes the launch:
  * the keys of one sequence are split over more workgroups when there are few, and
  * joined by a second launch; longer sequences are right too.  ws:

@@ -86,12 +86,7 @@ __device__ __forceinline__ unsigned quantise(float x, unsigned* pair) {
     *pair = 0x7fc07fc0u;
     return 0;
   }
-  // no range: every code is 0 whatever s is; 2^-40 of z keeps what the attention makes of the
-  // largest s from dwarfing z
-  unsigned s16 = __float_as_uint(a.s) >> 16;
-  const int ez = (int)(__float_as_uint(a.z) >> 23 & 255u);
-  if (a.s == 0.0f) s16 = (unsigned)max(ez - 40, 0) << 7;
-  *pair = s16 | (__float_as_uint(a.z) & 0xffff0000u);
+  *pair = __float_as_uint(a.s) >> 16 | (__float_as_uint(a.z) & 0xffff0000u);
   return affine_code(x, a);
 }
 
@@ -263,11 +258,16 @@ __device__ __forceinline__ float column_sum(float v) {
   return over_column(v, [](float a, float b) { return a + b; });
 }
 
-// log2 of what the weights carry for values whose largest scale is vtop: 6 - E, within what
-// sums of 2^20 weights leave of fp32's range.
-__device__ __forceinline__ float value_lift(float vtop) {
-  const int e = (int)(__float_as_uint(vtop) >> 23 & 255u) - 127;
-  return (float)(6 - max(e, -90));
+// The weights p s of one group's values as fp16 parts: a column's carry a power of two, `lift`,
+// that brings the largest of them so far to 2^6 .. 2^7, where the second part ends 2^-31 below it.
+// bound: 256 times that largest product; the lift lasts until a product passes it (2^15; fp16 ends
+// at 2^16).  Moves the lift to a new bound; returns what sums that carried the old one, and kept
+// `keep` of themselves, are multiplied by.
+__device__ __forceinline__ float move_lift(float bound, float keep, float& lift) {
+  const int e = (int)(__float_as_uint(bound) >> 23 & 255u);
+  const int now = min(141 - e, 126), was = (int)(__float_as_uint(lift) >> 23) - 127;
+  lift = __uint_as_float((unsigned)(now + 127) << 23);
+  return ldexpf(keep, now - was);
 }
 
 // One workgroup of up to kMaxWaves waves per (sequence, kv head, tile of query rows, split of the
@@ -277,9 +277,10 @@ __device__ __forceinline__ float value_lift(float vtop) {
 // there.  The waves take the steps in turn, each column with a running softmax of its own.
 // Scores are transposed: lane l holds column l % 16.  Codes count from their middle, x~ = (z + 8
 // s) + s (q - 8).  q carries scale * log2 e and the power of two that its two fp16 parts want (S'
-// = S / f, f a constant of the row).  The weights p s of the values want one too: every p carries
-// 2^lg, lg = 6 - E with E the largest exponent of s so far, so that p s stays below 2^7.  It is a
-// running reference like the maximum, and part of the same exponent.
+// = S / f, f a constant of the row).  The weights p s of the values want one too, a running
+// reference like the maximum (move_lift).  It follows the products: taken from the scales alone, a
+// row of large values that weighs nothing pushes the others' parts out of fp16's range (2^20 times
+// as large: outputs off by 5e-4).
 // Half a byte a value and one read of it: the vector instructions beside the products bound long
 // contexts, some 900 a step of four 128-channel records (codes to fragments 576, the softmax and
 // the weights' two parts most of the rest; the matrix pipe is 0.13 busy): 2 sequences of 65536
@@ -402,8 +403,13 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
 #pragma unroll
     for (int ct = 0; ct < 4; ++ct) o[g][ct] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
-  // m: the largest S' so far; vtop: the largest s of a value so far; l, zsum and o carry 2^lg
-  float m = -INFINITY, l = 0.0f, vtop = 0.0f, lg = value_lift(0.0f);
+  // m: the largest S' so far; o[g] carries lift[g]
+  float m = -INFINITY, l = 0.0f, bound[NG], lift[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    bound[g] = 0.0f;
+    lift[g] = 0x1p126f;
+  }
 
   for (int st = s0 + wave; st < s1; st += waves) {
     float s[8];
@@ -449,50 +455,51 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
           for (int g = 0; g < NG; ++g) vp[g][j >> 2][j & 3] = 0;
         }
     }
-    float mx = s[0], vx = vtop;
+    float mx = s[0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s[j]);
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) vx = fmaxf(vx, bf16_lo(vp[g][j >> 2][j & 3]));
-    if (__any(mx > m || vx > vtop)) {
-      // the sums so far move to the new maximum and the new lift of their column
+    if (__any(mx > m)) {
+      // the sums so far move to the new maximum of their column
       const float mn = fmaxf(m, column_max(mx));
-      vx = column_max(vx);
-      const float lgn = value_lift(vx);
-      const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(m - mn, f, lgn - lg));
+      const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * f);
       m = mn;
-      vtop = vx;
-      lg = lgn;
       l *= al;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         zsum[g] *= al;
+        bound[g] *= al;
+        const float alo = move_lift(bound[g], al, lift[g]);
 #pragma unroll
-        for (int ct = 0; ct < 4; ++ct) o[g][ct] *= al;
+        for (int ct = 0; ct < 4; ++ct) o[g][ct] *= alo;
       }
     }
     // a row that has seen no key yet: every weight exp2(-inf) = 0.  The difference comes first,
-    // so that no weight passes 2^lg however large the scores
+    // so that no weight passes 1 however large the scores
     const float ref = m == -INFINITY ? 0.0f : m;
     float p[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      p[j] = __builtin_amdgcn_exp2f(fmaf(s[j] - ref, f, lg));
+      p[j] = __builtin_amdgcn_exp2f((s[j] - ref) * f);
       l += p[j];
     }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      float ps[8];
+      float ps[8], top = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float ss = bf16_lo(vp[g][j >> 2][j & 3]), z = bf16_hi(vp[g][j >> 2][j & 3]);
         ps[j] = p[j] * ss;
+        top = fmaxf(top, ps[j]);
         zsum[g] = fmaf(p[j], fmaf(8.0f, ss, z), zsum[g]);
       }
+      if (__any(top > bound[g])) {
+        bound[g] = fmaxf(bound[g], fminf(256.0f * column_max(top), 0x1p127f));
+        const float up = move_lift(bound[g], 1.0f, lift[g]);
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct) o[g][ct] *= up;
+      }
       half8_t p0, p1;
-      split2(ps, 1.0f, p0, p1);
+      split2(ps, lift[g], p0, p1);
 #pragma unroll
       for (int r = 0; r < KP; ++r) {
         // the weights of this record's columns alone: the others' belong to other values
@@ -508,22 +515,22 @@ __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((
     if (more) load(st + waves, 1, vc, vp);
   }
   // the lane's sums over its keys -> the column's, without the lift
-  const float drop = __builtin_amdgcn_exp2f(-lg);
   l = column_sum(l);
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
+    const float drop = __uint_as_float((254u << 23) - __float_as_uint(lift[g]));
     zsum[g] = column_sum(zsum[g]);
 #pragma unroll
     for (int ct = 0; ct < 4; ++ct) {
-      floatx4 v = o[g][ct] + floatx4{zsum[g], zsum[g], zsum[g], zsum[g]};
+      floatx4 v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] *= drop;
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(o[g][ct][e], drop, zsum[g]);
       *reinterpret_cast<floatx4*>(&om[wave][col][g * kGrp + ct * 16 + 4 * c]) = v;
     }
   }
   if (c == 0) {
     ml[wave][0][col] = m * f;
-    ml[wave][1][col] = l * drop;
+    ml[wave][1][col] = l;
   }
   __syncthreads();
   // the states of the waves and column sets joined, four threads an output taking every fourth,
