@@ -708,11 +708,13 @@ int lx_qwen2_set_decode_graph(lx_qwen2* m, int enable);
  * (32, 64 or 128) inputs (lx_q4_pack_f32, lx_linear_q4_f32): 7.5 MB of them in groups of 64 and
  * o_proj's 3.2 MB of fp32 a layer of Qwen2-0.5B instead of 59.6 MB.  o_proj, whose
  * launch also forms the attention, the embeddings, norms and the K/V cache keep
- * fp32, and so does the whole prefill.  The call waits for the device, packs from
- * the model's fp32 weights, which stay, and drops captured decode graphs; the
- * first one with 4 allocates the copies (held until destroy; LX_ERR_ALLOC changes
- * nothing).  The model's device must be current (else LX_ERR_ARG).  Not to be called
- * during a capture.  No counterpart in the reference. */
+ * fp32, and so does the whole prefill.  The call waits for the device and drops the
+ * library's captured decode graphs; the first one with a group packs the copies for it
+ * from the model's fp32 weights, which stay.  Copies are held until destroy (194, 183 or
+ * 178 MB for groups of 32, 64 or 128), so a decode step that the caller captured keeps
+ * giving what it was captured with.  LX_ERR_ALLOC changes nothing.  The model's device
+ * must be current (else LX_ERR_ARG).  Not to be called during a capture.  No counterpart
+ * in the reference. */
 int lx_qwen2_set_decode_bits(lx_qwen2* m, int bits, int group);
 
 /* Prefill projections' split-operand products, 3 (the default) or 6, as

@@ -32,9 +32,18 @@ struct Layer {
   // the prefill projections' weights in MFMA fragment order (wfrag_pack), for
   // the split-operand GEMM; decode streams the fp32 copies above
   void *qkv_wf = nullptr, *o_wf = nullptr, *gu_wf = nullptr, *down_wf = nullptr;
-  // decode's weights in 4 bits (lx_qwen2_set_decode_bits; o_proj keeps fp32, its launch forms the
-  // attention too)
-  void *qkv_q4 = nullptr, *gu_q4 = nullptr, *down_q4 = nullptr;
+};
+
+// Decode's weights in 4 bits (lx_qwen2_set_decode_bits; o_proj keeps fp32, its launch forms the
+// attention too).  Packed once a group size and kept: a decode step that the caller captured
+// reads them whatever decode runs on since.
+struct Q4Layer {
+  void *qkv = nullptr, *gu = nullptr, *down = nullptr;
+};
+struct Q4Weights {
+  int group = 0;
+  void* head = nullptr;  // llm_decoder
+  std::vector<Q4Layer> layers;
 };
 
 // Six products run on the fragment-operand GEMMs up to this many rows (64 rows 1.05x
@@ -99,8 +108,8 @@ struct lx_qwen2 {
   float* rope_cs = nullptr;   // their cosines and sines at every position (rope_table)
   int device = -1;            // current when the model was made
   bool use_graph = true;      // replay the layer stack as one HIP graph
-  int q4_group = 0;           // decode on 4-bit weights in groups of this many inputs (0: fp32)
-  void* head_q4 = nullptr;    // llm_decoder in 4 bits
+  std::vector<Q4Weights> q4_sets;  // at most one a group size, and room for all from the first
+  const Q4Weights* q4 = nullptr;   // decode's (null: fp32)
   hipStream_t cap_stream = nullptr;
   // [0]: the cache fits one attention split; [1 + c]: split class c
   hipGraphExec_t graph[1 + kDecAttnClasses] = {};
@@ -344,7 +353,7 @@ int prefill_layer(lx_qwen2* m, Layer& L, int rows, const float* next_norm, hipSt
 
 // A decode projection on its fp32 or its 4-bit weight.
 int dec_proj(const lx_qwen2* m, int epi, const DecGemvArgs& a, const void* q4, hipStream_t s) {
-  return m->q4_group ? dec_gemv_q4(epi, a, q4, m->q4_group, s) : dec_gemv(epi, a, s);
+  return m->q4 ? dec_gemv_q4(epi, a, q4, m->q4->group, s) : dec_gemv(epi, a, s);
 }
 
 // One decode layer (src/llm/llm.cpp:254-289): RMSNorm + QKV + rotary + cache
@@ -354,7 +363,9 @@ int dec_proj(const lx_qwen2* m, int epi, const DecGemvArgs& a, const void* q4, h
 // does not cover take a launch each); past it (cls = 1 + split class) the split
 // partials are a launch of their own and merged inside o_proj's.  The position is
 // read from m->d_pos.
-int decode_layer(lx_qwen2* m, Layer& L, int cls, hipStream_t s) {
+int decode_layer(lx_qwen2* m, int l, int cls, hipStream_t s) {
+  Layer& L = m->layers[l];
+  const Q4Layer q4 = m->q4 ? m->q4->layers[l] : Q4Layer{};
   const int H = m->H, KV = m->KV;
   DecGemvArgs q;
   q.x = m->x;
@@ -372,7 +383,7 @@ int decode_layer(lx_qwen2* m, Layer& L, int cls, hipStream_t s) {
   q.k_cache = L.k_cache;
   q.v_cache = L.v_cache;
   q.inv_freq = m->rope_tab;
-  LX_TRY(dec_proj(m, DEC_QKV_ROPE, q, L.qkv_q4, s));
+  LX_TRY(dec_proj(m, DEC_QKV_ROPE, q, q4.qkv, s));
   DecAttnArgs at;
   at.q = m->hn;
   at.k_cache = L.k_cache;
@@ -408,18 +419,18 @@ int decode_layer(lx_qwen2* m, Layer& L, int cls, hipStream_t s) {
   gu.y = m->act;
   gu.N = 2L * m->I;
   gu.K = H;
-  LX_TRY(dec_proj(m, DEC_SWIGLU, gu, L.gu_q4, s));
+  LX_TRY(dec_proj(m, DEC_SWIGLU, gu, q4.gu, s));
   DecGemvArgs d;
   d.x = m->act;
   d.W = L.down_w;
   d.y = m->x;
   d.N = H;
   d.K = m->I;
-  return dec_proj(m, DEC_RESID, d, L.down_q4, s);
+  return dec_proj(m, DEC_RESID, d, q4.down, s);
 }
 
 int decode_stack(lx_qwen2* m, int cls, hipStream_t s) {
-  for (auto& L : m->layers) LX_TRY(decode_layer(m, L, cls, s));
+  for (int l = 0; l < m->NL; ++l) LX_TRY(decode_layer(m, l, cls, s));
   return LX_OK;
 }
 
@@ -460,6 +471,47 @@ int capture_decode(lx_qwen2* m, int cls) {
   }
   if (g) (void)hipGraphDestroy(g);
   return rc;
+}
+
+// A set of decode's weights in 4 bits in groups of `group`, kept in m->q4_sets.
+int pack_q4(lx_qwen2* m, int group, const Q4Weights** out) {
+  const int H = m->H, I = m->I;
+  Q4Weights w;
+  try {
+    m->q4_sets.reserve(3);
+    w.layers.resize(m->NL);
+    m->arena.ptrs.reserve(m->arena.ptrs.size() + 1 + 3 * m->NL);
+  } catch (const std::bad_alloc&) {
+    set_error("qwen2_set_decode_bits: host allocation failed");
+    return LX_ERR_ALLOC;
+  }
+  w.group = group;
+  auto A = [&](void** p, int N, int K) {
+    *p = m->arena.alloc<char>(q4_bytes(N, K, group));
+    return *p != nullptr;
+  };
+  bool ok = A(&w.head, m->speech_vocab, H);
+  for (Q4Layer& q : w.layers)
+    ok = ok && A(&q.qkv, m->QKV, H) && A(&q.gu, 2 * I, H) && A(&q.down, H, I);
+  if (!ok) {
+    set_error("qwen2_set_decode_bits: device allocation failed");
+    return LX_ERR_ALLOC;
+  }
+  LX_TRY(q4_pack(m->llm_decoder, w.head, m->speech_vocab, H, group, 0, nullptr));
+  for (int l = 0; l < m->NL; ++l) {
+    const Layer& L = m->layers[l];
+    const Q4Layer& q = w.layers[l];
+    LX_TRY(q4_pack(L.qkv_w, q.qkv, m->QKV, H, group, 1, nullptr));
+    LX_TRY(q4_pack(L.gu_w, q.gu, 2 * I, H, group, 0, nullptr));
+    LX_TRY(q4_pack(L.down_w, q.down, H, I, group, 0, nullptr));
+  }
+  if (hipStreamSynchronize(nullptr) != hipSuccess) {
+    set_error("qwen2_set_decode_bits: packing failed");
+    return LX_ERR_LAUNCH;
+  }
+  m->q4_sets.push_back(std::move(w));
+  *out = &m->q4_sets.back();
+  return LX_OK;
 }
 
 }  // namespace
@@ -755,7 +807,7 @@ extern "C" int lx_qwen2_decode(lx_qwen2* m, int token, float* logits, float* fin
   h.y2 = final_norm;
   h.N = m->speech_vocab;
   h.K = H;
-  LX_TRY(dec_proj(m, DEC_HEAD, h, m->head_q4, s));
+  LX_TRY(dec_proj(m, DEC_HEAD, h, m->q4 ? m->q4->head : nullptr, s));
   m->cache_len += 1;
   return LX_OK;
 }
@@ -789,53 +841,21 @@ extern "C" int lx_qwen2_set_decode_bits(lx_qwen2* m, int bits, int group) {
   LX_REQUIRE(hipGetDevice(&dev) == hipSuccess && dev == m->device,
              "qwen2_set_decode_bits: device %d is current, the model is on %d", dev, m->device);
   const int want = bits == 4 ? group : 0;
-  if (want == m->q4_group) return LX_OK;
-  // decode steps under way read the weights and the graphs that go
+  if (want == (m->q4 ? m->q4->group : 0)) return LX_OK;
+  const Q4Weights* q4 = nullptr;
+  for (const Q4Weights& w : m->q4_sets)
+    if (w.group == want) q4 = &w;
+  if (want && !q4) LX_TRY(pack_q4(m, want, &q4));
+  // decode steps under way read the graphs that go
   if (hipDeviceSynchronize() != hipSuccess) {
     set_error("qwen2_set_decode_bits: synchronisation failed");
     return LX_ERR_LAUNCH;
   }
-  auto drop_graphs = [&] {  // captured with the other weights
-    for (hipGraphExec_t& g : m->graph) {
-      if (g) (void)hipGraphExecDestroy(g);
-      g = nullptr;
-    }
-  };
-  const int H = m->H, I = m->I;
-  if (!want) drop_graphs();
-  if (want) {
-    // allocated once, for the smallest groups
-    auto A = [&](void** p, int N, int K) {
-      if (!*p) *p = m->arena.alloc<char>(q4_bytes(N, K, 32));
-      return *p != nullptr;
-    };
-    bool ok = true;
-    try {
-      m->arena.ptrs.reserve(m->arena.ptrs.size() + 1 + 3 * m->layers.size());
-      ok = A(&m->head_q4, m->speech_vocab, H);
-      for (auto& L : m->layers)
-        ok = ok && A(&L.qkv_q4, m->QKV, H) && A(&L.gu_q4, 2 * I, H) && A(&L.down_q4, H, I);
-    } catch (const std::bad_alloc&) {
-      ok = false;
-    }
-    if (!ok) {
-      set_error("qwen2_set_decode_bits: device allocation failed");
-      return LX_ERR_ALLOC;
-    }
-    drop_graphs();
-    m->q4_group = 0;  // until every weight is packed
-    LX_TRY(q4_pack(m->llm_decoder, m->head_q4, m->speech_vocab, H, want, 0, nullptr));
-    for (auto& L : m->layers) {
-      LX_TRY(q4_pack(L.qkv_w, L.qkv_q4, m->QKV, H, want, 1, nullptr));
-      LX_TRY(q4_pack(L.gu_w, L.gu_q4, 2 * I, H, want, 0, nullptr));
-      LX_TRY(q4_pack(L.down_w, L.down_q4, H, I, want, 0, nullptr));
-    }
-    if (hipStreamSynchronize(nullptr) != hipSuccess) {
-      set_error("qwen2_set_decode_bits: packing failed");
-      return LX_ERR_LAUNCH;
-    }
+  for (hipGraphExec_t& g : m->graph) {  // captured with the other weights
+    if (g) (void)hipGraphExecDestroy(g);
+    g = nullptr;
   }
-  m->q4_group = want;
+  m->q4 = q4;
   return LX_OK;
 }
 

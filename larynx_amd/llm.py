@@ -199,7 +199,8 @@ class Qwen2LM:
 
     def set_decode_bits(self, bits, group=64):
         """Decode's weights: 32 (fp32, the default) or 4, q|k|v, gate/up, down and the head on 4-bit
-        copies with a scale per `group` (32, 64, 128) inputs.  The prefill keeps fp32."""
+        copies with a scale per `group` (32, 64, 128) inputs.  The prefill keeps fp32.  Copies are
+        packed once a group and kept; decode steps captured by the caller stay on theirs."""
         check(lib.lx_qwen2_set_decode_bits(self._h, int(bits), int(group)))
 
     def set_products(self, products):
