@@ -712,9 +712,9 @@ int lx_qwen2_set_decode_graph(lx_qwen2* m, int enable);
  * library's captured decode graphs; the first one with a group packs the copies for it
  * from the model's fp32 weights, which stay.  Copies are held until destroy (194, 183 or
  * 178 MB for groups of 32, 64 or 128), so a decode step that the caller captured keeps
- * giving what it was captured with.  LX_ERR_ALLOC changes nothing.  The model's device
- * must be current (else LX_ERR_ARG).  Not to be called during a capture.  No counterpart
- * in the reference. */
+ * giving what it was captured with.  LX_ERR_ALLOC and LX_ERR_LAUNCH change nothing.
+ * The model's device must be current (else LX_ERR_ARG).  Not to be called during a
+ * capture.  No counterpart in the reference. */
 int lx_qwen2_set_decode_bits(lx_qwen2* m, int bits, int group);
 
 /* Prefill projections' split-operand products, 3 (the default) or 6, as

@@ -23,14 +23,22 @@ int device_cus();
 // at create time and released together when the object is destroyed.
 struct Arena {
   std::vector<void*> ptrs;
-  ~Arena() {
-    for (void* p : ptrs) (void)hipFree(p);
+  ~Arena() { trim(0); }
+  // Frees all but the first n allocations.
+  void trim(size_t n) {
+    while (ptrs.size() > n) {
+      (void)hipFree(ptrs.back());
+      ptrs.pop_back();
+    }
   }
   template <typename T>
   T* alloc(size_t n) {
     void* p = nullptr;
     if (n == 0) n = 1;
-    if (hipMalloc(&p, n * sizeof(T)) != hipSuccess) return nullptr;
+    if (hipMalloc(&p, n * sizeof(T)) != hipSuccess) {
+      (void)hipGetLastError();  // or the next launch would report it
+      return nullptr;
+    }
     ptrs.push_back(p);
     return static_cast<T*>(p);
   }

@@ -473,19 +473,9 @@ int capture_decode(lx_qwen2* m, int cls) {
   return rc;
 }
 
-// A set of decode's weights in 4 bits in groups of `group`, kept in m->q4_sets.
-int pack_q4(lx_qwen2* m, int group, const Q4Weights** out) {
+// A set of decode's weights in 4 bits in groups of `group`, allocated and packed into w.
+int pack_q4(lx_qwen2* m, int group, Q4Weights& w) {
   const int H = m->H, I = m->I;
-  Q4Weights w;
-  try {
-    m->q4_sets.reserve(3);
-    w.layers.resize(m->NL);
-    m->arena.ptrs.reserve(m->arena.ptrs.size() + 1 + 3 * m->NL);
-  } catch (const std::bad_alloc&) {
-    set_error("qwen2_set_decode_bits: host allocation failed");
-    return LX_ERR_ALLOC;
-  }
-  w.group = group;
   auto A = [&](void** p, int N, int K) {
     *p = m->arena.alloc<char>(q4_bytes(N, K, group));
     return *p != nullptr;
@@ -506,8 +496,29 @@ int pack_q4(lx_qwen2* m, int group, const Q4Weights** out) {
     LX_TRY(q4_pack(L.down_w, q.down, H, I, group, 0, nullptr));
   }
   if (hipStreamSynchronize(nullptr) != hipSuccess) {
+    (void)hipGetLastError();
     set_error("qwen2_set_decode_bits: packing failed");
     return LX_ERR_LAUNCH;
+  }
+  return LX_OK;
+}
+
+// The same, kept in m->q4_sets.  An error leaves the model and its memory as they were.
+int add_q4(lx_qwen2* m, int group, const Q4Weights** out) {
+  const size_t before = m->arena.ptrs.size();
+  Q4Weights w;
+  w.group = group;
+  try {
+    m->q4_sets.reserve(3);
+    w.layers.resize(m->NL);
+    m->arena.ptrs.reserve(before + 1 + 3 * m->NL);
+  } catch (const std::bad_alloc&) {
+    set_error("qwen2_set_decode_bits: host allocation failed");
+    return LX_ERR_ALLOC;
+  }
+  if (const int rc = pack_q4(m, group, w)) {
+    m->arena.trim(before);
+    return rc;
   }
   m->q4_sets.push_back(std::move(w));
   *out = &m->q4_sets.back();
@@ -845,7 +856,7 @@ extern "C" int lx_qwen2_set_decode_bits(lx_qwen2* m, int bits, int group) {
   const Q4Weights* q4 = nullptr;
   for (const Q4Weights& w : m->q4_sets)
     if (w.group == want) q4 = &w;
-  if (want && !q4) LX_TRY(pack_q4(m, want, &q4));
+  if (want && !q4) LX_TRY(add_q4(m, want, &q4));
   // decode steps under way read the graphs that go
   if (hipDeviceSynchronize() != hipSuccess) {
     set_error("qwen2_set_decode_bits: synchronisation failed");
