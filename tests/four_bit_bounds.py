@@ -129,3 +129,24 @@ def value_scale_case(rng, B, Tq, heads, kv, hd, rows, ratio, at, gap, groups=Non
     for g in range(hd // 64) if groups is None else groups:
         v[:, at, :, 64 * g:64 * g + 64] *= np.float32(ratio)
     return q, k, v
+
+
+def linear(x, weight, scales, G, blocks_of=128):
+    """Outputs x @ weight^T in 64 bits and their bounds, (M, N).  weight and scales (N, K) as
+    ref_weight gives them.
+
+    A group's sum runs over both parts of x in G / 2 roundings, of partial sums of signed codes:
+    below B = 8 |s x| (root sum of squares); over the groups, the waves and the splits come K / G +
+    24 of the sum so far.  x's two parts are off by 2^-23 of an element, or 2^-25 of the largest of
+    its block."""
+    K = x.shape[1]
+    x = x.astype(np.float64)
+    want = x @ weight.T
+    B = 8 * np.sqrt(x ** 2 @ (scales ** 2).T)
+    top = np.zeros_like(want)
+    for k in range(0, K, blocks_of):
+        t = np.abs(x[:, k:k + blocks_of]).max(1)
+        top += t[:, None] ** 2 * (weight[:, k:k + blocks_of] ** 2).sum(1)
+    bound = np.sqrt(U * U * (G / 2 * B ** 2 + (K / G + 24) * (np.abs(want) + B) ** 2) +
+                    (2.0 ** -23 * B) ** 2 + 2.0 ** -50 * top)
+    return want, bound

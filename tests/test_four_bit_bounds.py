@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import four_bit_bounds as fb
-from test_gpu_four_bit import ref_cache
+from test_gpu_four_bit import ref_cache, ref_weight
 
 
 def _run(q, k, v, **kw):
@@ -51,3 +51,36 @@ def test_a_query_of_one_part_is_seen(hd, rows):
     fb.check(*_run(q, k, v))
     with pytest.raises(AssertionError):
         fb.check(*_run(q, k, v, parts=1))
+
+
+@pytest.mark.parametrize("rows", [70, 1055, 4000])
+def test_a_lost_key_is_seen(rows):
+    """A key that weighs less than nine tenths of the others."""
+    q, k, v = _plain_case(np.random.default_rng(rows), 64, rows)
+    s = ref_cache(k)[0][0, :, 0] @ q[0, 0, :64]
+    with pytest.raises(AssertionError):
+        fb.check(*_run(q, k, v, skip=int(np.argsort(s)[rows // 10])))
+
+
+LINEAR = [(1, 9728, 896, 64), (3, 6762, 896, 32), (4, 896, 4864, 64), (5, 70, 1000, 128),
+          (16, 384, 2048, 128), (29, 46, 772, 64), (64, 258, 516, 32)]
+
+
+@pytest.mark.parametrize("M,N,K,G", LINEAR)
+def test_projections_of_one_part_are_seen(M, N, K, G):
+    rng = np.random.default_rng(M + N + K)
+    W = (rng.standard_normal((N, K)) * K ** -0.5).astype(np.float32)
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    x[0] *= 1e3
+    want, bound = fb.linear(x, *ref_weight(W, G), G)
+    for parts in (2, 1):
+        xp = np.zeros(x.shape)
+        for k in range(0, K, 128):
+            f = 2.0 ** np.floor(np.log2(np.abs(x[:, k:k + 128]).max(1, keepdims=True)))
+            xp[:, k:k + 128] = fb.two_parts(x[:, k:k + 128] / f, parts) * f
+        err = (xp @ ref_weight(W, G)[0].T).astype(np.float32) - want
+        if parts == 2:
+            fb.check(err, bound)
+        else:
+            with pytest.raises(AssertionError):
+                fb.check(err, bound)
