@@ -382,25 +382,27 @@ int lx_q4_pack_f32(const float* W, void* Wq, int N, int K, int group, hipStream_
 int lx_q4_unpack_f32(const void* Wq, float* W, int N, int K, int group, hipStream_t stream);
 
 /* Projection of few rows on such a weight:  y = epi(x @ W~^T + bias), W~ what the
- * packed codes stand for, fp32 arithmetic (x as two fp16 parts after a power of two
- * per row and 128 inputs, exact products with the codes, fp32 sums; the scale
- * applied to each group's sum).  x: (M, K), 1 <= M <= 64, row stride ldx; y: (M, N), row stride ldy (N / 2 columns for
- * SWIGLU_PAIRED, N even); y must not overlap x (LX_ERR_ARG).  Epilogues: none,
- * GELU_TANH, RESID, SWIGLU_PAIRED (others: LX_ERR_ARG); bias (N) or NULL.  K (at most 2^26 - 1024 with
- * more than 4 rows) and ldx multiples of 4, x and Wq 16-byte aligned.  An infinite or
- * NaN element of x makes NaN of its row.  The result does not depend on timing.  ws: lx_linear_q4_ws_floats() floats
- * of scratch, 16-byte aligned (NULL when that is 0: up to 4 rows, and K up to 1024);
- * calls that share it must not overlap.
+ * packed codes stand for, in fp32 arithmetic: x as two fp16 parts after a power of two
+ * per row and 128 inputs (off by 2^-25 of the largest of these at most), exact products
+ * with the codes, fp32 sums, the scale applied to each group's sum.
+ * x: (M, K), 1 <= M <= 64, row stride ldx; y: (M, N), row stride ldy (N / 2 columns
+ * for SWIGLU_PAIRED, N even).  y must not overlap another operand (x: LX_ERR_ARG; the
+ * rest is not checked).  Epilogues: none, GELU_TANH, RESID, SWIGLU_PAIRED (others:
+ * LX_ERR_ARG); bias (N) or NULL.  K (at most 2^26 - 1024 with more than 4 rows) and ldx
+ * multiples of 4, x and Wq 16-byte aligned.  An infinite or NaN element of x makes NaN
+ * of its row.  The result does not depend on timing.
+ * ws: lx_linear_q4_ws_floats() floats of scratch, 16-byte aligned (NULL when that is 0:
+ * up to 4 rows, and K up to 1024); calls that share it must not overlap.
  * Replaces linear() (src/llm/ops.cpp:13-19) for weights given in 4 bits. */
 size_t lx_linear_q4_ws_floats(int M, int N, int K);
 int lx_linear_q4_f32(const float* x, long ldx, const void* Wq, int group, const float* bias,
                      float* y, long ldy, int M, int N, int K, const lx_epilogue* epi, float* ws,
                      size_t ws_floats, hipStream_t stream);
 
-/* A key/value cache held in 4 bits (4.5 with its scales): `batch` sequences of up
- * to max_rows (at most 2^31 - 129) rows, n_kv_heads heads (at most 65535 and 32767) of head_dim (64 or
- * 128) channels.  Keys and
- * values alike: the 64 channels of a group of a row share z = the largest bf16
+/* A key/value cache held in 4 bits (4.5 with its scales): `batch` sequences (at most
+ * 65535) of up to max_rows rows (at most 2^31 - 129), n_kv_heads heads (at most 32767)
+ * of head_dim (64 or 128) channels.  Keys and values alike:
+ * the 64 channels of a group of a row share z = the largest bf16
  * not above their minimum and s = the smallest bf16 not below (max - z) / 15; a
  * code q = clamp(rint((x - z) / s), 0, 15) stands for z + s * q (no range: z).  A
  * group that holds an infinity or a NaN, or whose |z| + 16 s passes fp32, stands

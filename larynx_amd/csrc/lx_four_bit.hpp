@@ -1,13 +1,14 @@
 // Four-bit codes as MFMA operands (lx_q4.hip, lx_kv4.hip).
 //
-// A dword holds the eight codes of one lane's fp16 fragment (v_mfma_f32_16x16x32_f16: lane l
-// holds row or column l % 16, k = (l / 16) * 8 .. + 7), elements 2r and 2r + 1 at bits 4r and
-// 16 + 4r.  An and-or with the pattern of 1024.0 makes both halves of a fragment register 1024 + q
-// or 1024 + 16 q, a packed fp16 add or fma makes them q - 8, exactly: 9 instructions for eight
-// codes.  Signed codes keep the fp32 sums as small as the values they stand for; an offset left
-// in and taken off later (bf16 has no packed add: 7 instructions) cost a digit where values
-// average out, or twice the matrix instructions.  (The bits alone are subnormal numbers, five
-// instructions, but the sums of their products lose ten bits.)
+// A dword holds the eight codes of one lane's fp16 fragment (v_mfma_f32_16x16x32_f16: lane l holds
+// row or column l % 16, k = (l / 16) * 8 .. + 7), elements 2r and 2r + 1 at bits 4r and 16 + 4r.
+// An and-or with the pattern of 1024.0 makes both halves of a fragment register 1024 + q or 1024 +
+// 16 q, a packed fp16 add or fma makes them q - 8, exactly: 9 instructions for eight codes (a
+// published method: Kim, Henry, Fahim, Awadalla, "Who Says Elephants Can't Run: Bringing Large
+// Scale MoE Models into Cloud Scale Production", 2022).  Signed codes keep the fp32 sums as small
+// as the values they stand for; an offset left in and taken off later (bf16 has no packed add: 7
+// instructions) cost a digit where values average out, or twice the matrix instructions.  (The bits
+// alone are subnormal numbers, five instructions, but the sums of their products lose ten bits.)
 //
 // The other operand is fp32 data as two fp16 parts, after a power of two of its own per row that
 // brings the largest value to 1 .. 2: x = x0 + x1 to within 2^-23 of x, or 2^-25 of the row's

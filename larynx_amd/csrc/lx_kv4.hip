@@ -93,8 +93,8 @@ __device__ __forceinline__ unsigned quantise(float x, unsigned* pair) {
 // One workgroup of eight waves per (32-row record touched, channel group of a kv head, sequence):
 // four for the keys, four for the values, lane = channel.  Wave w of a plane owns the rows whose
 // value codes share dwords, 4 w .. 4 w + 3 of both halves; all eight are requested at once.  A wave
-// is some 145 instructions a group (two wave-wide extremes, two quotients, the code) after one
-// memory round trip, and these bound it: 1531 rows of 2 heads 7.3 us, 1.8 MB; one row 3.3, a launch
+// is some 140 instructions a group (two wave-wide extremes, two quotients, the code) after one
+// memory round trip, and these bound it: 1531 rows of 2 heads 7.2 us, 1.8 MB; one row 3.3, a launch
 // and its chain.
 __global__ __launch_bounds__(512) void kv4_append_kernel(AppendArgs a) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6 & 3, plane = threadIdx.x >> 8;
@@ -282,11 +282,11 @@ __device__ __forceinline__ float move_lift(float bound, float keep, float& lift)
 // row of large values that weighs nothing pushes the others' parts out of fp16's range (2^20 times
 // as large: outputs off by 5e-4).
 // Half a byte a value and one read of it: the vector instructions beside the products bound long
-// contexts, some 900 a step of four 128-channel records (codes to fragments 576, the softmax and
+// contexts, some 920 a step of four 128-channel records (codes to fragments 576, the softmax and
 // the weights' two parts most of the rest; the matrix pipe is 0.13 busy): 2 sequences of 65536
-// rows, 8 kv heads, 114 MB in 33 us, 3.5 TB/s, and 4 to 5 for the join; 64 sequences of up to 4096
-// run at some 5.  Short ones are latency: 1 sequence of 2001 rows 5.4 us and 3.1 for the join, 7.5
-// for both in a graph.
+// rows, 8 kv heads, 114 MB in 33 us, 3.4 TB/s, and 4 to 5 for the join; 64 sequences of all lengths
+// up to 4096, 153 MB, 53 us with the join, 2.9 TB/s.  Short ones are latency: 1 sequence of 2001
+// rows 5.2 us and 3.1 for the join, 7.6 for both in a graph.
 // A spilled register costs more than a wave gains: the registers follow from NG and KP.
 template <int NG, int KP>
 __global__ __launch_bounds__(64 * kMaxWaves) __attribute__((

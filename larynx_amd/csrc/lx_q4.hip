@@ -46,8 +46,10 @@ __host__ __device__ inline long q4_blocks(int K) { return (K + kBlockK - 1) / kB
 
 // ---- quantise and lay out ---------------------------------------------------------------
 
-// One wave per (row tile, block): lane l holds row l % 16, inputs 32 t + 8 (l / 16) + j.  neox:
-// rows 2 i and 2 i + 1 of a head of 64 are its rows i and i + 32, a rotary pair, side by side.
+// One wave per (row tile, block): lane l holds row l % 16, inputs 32 t + 8 (l / 16) + j.  Run once
+// a weight; the fp32 matrix bounds it: 8192 x 8192 in groups of 128 66 us (4.6 TB/s; of 32, whose
+// scales are four times as many, 76), 151936 x 896 171 us (3.6).  A copy asks 57 and 116.
+// neox:// rows 2 i and 2 i + 1 of a head of 64 are its rows i and i + 32, a rotary pair, side by side.
 template <int G>
 __global__ __launch_bounds__(64) void q4_pack_kernel(const float* __restrict__ W,
                                                      uintx4_t* __restrict__ codes,
@@ -122,6 +124,8 @@ __global__ __launch_bounds__(64) void q4_pack_kernel(const float* __restrict__ W
   codes[tile * 64 + lane] = q;
 }
 
+// One thread per eight codes.  A lane writes 32 bytes of a row, 16 rows a wave: 8192 x 8192 315 us
+// (1 TB/s), which a copy moves in 57.  For checks and for going back to fp32; no step runs it.
 __global__ __launch_bounds__(256) void q4_unpack_kernel(const unsigned* __restrict__ codes,
                                                         const unsigned short* __restrict__ scales,
                                                         float* __restrict__ W, int N, int K,
@@ -198,9 +202,10 @@ __device__ __forceinline__ void q4_epi_quad(const Q4Args& a, int m, long n, floa
 // rows at a time), and their sums meet in LDS at the end (in a fixed order).  Column 2 m + part of
 // the fragments is a part of row m.  Everything a wave reads is requested before it computes, and
 // the next block before this one; what remains is a launch, one memory round trip, the split
-// (some 60 instructions a block) and the meeting: in a graph 1 row x 1152 x 896 2.6 us, x 9728 3.5
-// (1.3 TB/s), 4 rows x 896 x 4864 4.4, 8 rows x 9728 x 896 4.9, where a copy asks 0.1 to 1.0.
-// (With a lane per row of x each load touched 64 lines: 3 rows x 6761 5.4 us, now 3.3.)
+// (some 60 instructions a block) and the meeting: in a graph over eight weights in turn 1 row x
+// 1152 x 896 3.2 us, x 9728 4.2 (1.1 TB/s), 4 rows x 896 x 4864 4.8, 8 rows x 9728 x 896 5.6, where
+// a copy asks 0.1 to 0.9.  (With a lane per row of x each load touched 64 lines: 3 rows x 6761 5.4
+// us, now 3.6.)
 constexpr int kFewRow = 272;  // bytes of a staged row (128 fp16, and 16 against bank conflicts)
 
 template <int MB>
@@ -477,13 +482,14 @@ __global__ __launch_bounds__(64 * kRowWaves) void q4_row_kernel(Q4Args a, DecGem
 // of 16 rows at a time, one group of tiles ahead.  The waves' sums meet in one of two LDS buffers
 // (a barrier a group), added in wave order; each thread adds and finishes one quad of outputs.
 // More than one split: partial sums into ws (splits, M, N up to 16), which q4_join_kernel adds in
-// split order.  16 rows x 151936 x 896 stream at 4.4 TB/s (18.7 us in a graph).  Every 16 rows more
-// cost 8192 x 8192 about 5.5 us (16: 14.2, 32: 18.9, 48: 25.1, 64: 31.8, the join's 5 among them):
-// their splitting, 100 instructions a lane, then matrix instructions at the clock the power limit
-// leaves, and 4 MB of partial sums written and read.  (With x in LDS and whole K ranges a wave,
-// every fragment of x is read again for every two tiles: 64 rows 8192 x 8192 33 us, 9728 x 896 17
-// for 11.4 now.  Sums of a group added under the next one's products, with one register buffer
-// of weights for two: 33 us.)
+// split order.  16 rows x 151936 x 896, 82 MB: 24 us in a graph over twelve weights in turn (3.4
+// TB/s), 21 over three, which the last-level cache holds.  Every 16 rows more cost 8192 x 8192
+// about 5 us (eight weights in turn, 16: 16.8, 32: 22.2, 48: 27.9, 64: 31.1, the join's 5 among
+// them): their splitting, 100 instructions a lane, then matrix instructions at the clock the power
+// limit leaves, and 4 MB of partial sums written and read.  (With x in LDS and whole K ranges a
+// wave, every fragment of x is read again for every two tiles: 64 rows 8192 x 8192 33 us, 9728 x
+// 896 17 for 11.3 now.  Sums of a group added under the next one's products, with one register
+// buffer of weights for two: 33 us.)
 constexpr int kManyWaves = 8;
 constexpr int kManyTiles = 2;  // RT
 constexpr size_t many_bytes(int ct) {
@@ -705,10 +711,15 @@ int launch_many(const Q4Args& a, int G, hipStream_t s) {
 #undef LX_Q4_GROUPS
 
 // Calls that run on q4_few_kernel, which has little fixed cost but splits x again for every tile;
-// in units of tile x block, and more where the other kernel needs a second launch (K > 1024; never
-// for up to 4 rows).  Times of both in a graph, us (few / many): K = 896, M = 4, N = 27000 6.9 /
-// 7.5, N = 40000 9.1 / 8.1; M = 8, N = 9728 4.9 / 5.6, N = 20000 7.1 / 6.4; M = 8, N = 896, K =
-// 4864 5.5 / 6.5, 8192 x 4096 9.7 / 10.6, 8192 x 8192 15.7 / 14.0.
+// in units of tile x block, and more where the other kernel needs a second launch (K > 1024).
+// Times of both in a graph over eight weights in turn, us (few / many): K = 896, M = 4, N = 27000
+// (work 11816) 7.3 / 7.8, N = 32000 (14000) 8.1 / 7.8, N = 40000 9.5 / 8.6; M = 8, N = 9728 (4256)
+// 5.6 / 6.3, N = 20000 (8750) 7.6 / 7.0; M = 8, N = 896, K = 4864 5.9 / 6.9, 4096 x 8192 (16384)
+// 9.3 / 10.9, 8192 x 8192 (32768) 17.6 / 15.3.
+// Up to 4 rows with K > 1024 always run here, since such a call takes no workspace.  M = 4: 896 x
+// 4864 (2128) 4.8 / 6.8, 20000 x 1100 (11250) 7.6 / 11.5, 8192 x 8192 (32768) 14.1 / 15.6; past
+// some 35000 the other kernel would win: 3 x 70000 x 1100 (39375) 22.7 / 20.7, 28672 x 8192
+// (114688) 41.5 / 33.6, 151936 x 2048 (151936) 72.7 / 43.6.
 bool q4_takes_few(int M, int N, int K) {
   const long kb = q4_blocks(K), work = q4_tiles(N) * kb;
   if (M <= 4) return kb > kManyWaves || work <= 14000;
