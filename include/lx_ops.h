@@ -459,6 +459,69 @@ int lx_attention_kv4_f32(const float* q, long ldq, const lx_kv4* cache, const in
                          long ldo, int Tq, int n_heads, float scale, int causal, int max_len,
                          float* ws, size_t ws_floats, hipStream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* The LM's prompt in eight bits, and scoring                                */
+/* ------------------------------------------------------------------------ */
+
+/* A matrix (rows, K) held in 8 bits, activations and weights alike: blocks of 128
+ * consecutive elements of a row (the last one short where K ends inside it) share
+ * 2^e, e the smallest integer >= -127 with max|v| <= 448 * 2^e over the block's finite
+ * elements; an element is the e4m3 number nearest to v / 2^e (ties to even) and stands
+ * for that number times 2^e, off by at most 2^-4 of itself or 2^(e - 10).  Infinities
+ * and NaN stand for NaN.  `data`: device memory of lx_q8_bytes() bytes (0 for a bad
+ * shape), 16-byte aligned, which needs no initialisation.
+ * lx_q8_pack_f32 writes x (row stride ldx) into q; lx_q8_unpack_f32 what q stands for
+ * into x.  At most 2^27 blocks of rows, counted one by one.  x and q must not overlap.
+ * No counterpart in the reference (its weights and activations stay fp32). */
+typedef struct lx_q8 {
+  void* data;
+  int rows, K;
+} lx_q8;
+size_t lx_q8_bytes(int rows, int K);
+int lx_q8_pack_f32(const float* x, long ldx, const lx_q8* q, hipStream_t stream);
+int lx_q8_unpack_f32(const lx_q8* q, float* x, long ldx, hipStream_t stream);
+
+/* h = x + add, written to sum (add and sum NULL: h = x); q = h / sqrt(mean(h^2) + eps) * w
+ * in 8 bits.  x, add, sum: q->rows rows of q->K, row strides ldx / lda / lds; sum may be
+ * x or add itself (the same pointer and stride) and must not overlap them otherwise;
+ * w (K).  h is rounded to fp32; the norm is formed in 64 bits and rounded once, to its
+ * code (magnitudes past fp32's count as fp32's largest).  No alignment past 4 bytes.
+ * Replaces the residual add and rms_norm (src/llm/ops.cpp:7-11, src/llm/llm.cpp:141-173)
+ * before a projection whose weight is held in 8 bits. */
+int lx_rmsnorm_q8_f32(const float* x, long ldx, const float* add, long lda, float* sum, long lds,
+                      const float* w, float eps, const lx_q8* q, hipStream_t stream);
+
+/* y = epi(x~ @ w~^T + bias), x~ (M, K) and w~ (N, K) what x and w stand for: exact
+ * products, each block of 128 scaled by its power of two, fp32 sums.  y: (M, N), row
+ * stride ldy (N / 2 columns for SWIGLU_PAIRED, N even).  Epilogues: none, GELU_TANH,
+ * RESID (y = resid + .., resid row stride ldr; NULL: y itself, in place),
+ * SWIGLU_PAIRED; others: LX_ERR_ARG.  bias (N) or NULL.  y must not overlap resid
+ * otherwise, nor another operand.  A NaN in a row of x or w makes NaN of the outputs
+ * it enters.  No alignment past 4 bytes for y, bias, resid.
+ * Replaces linear() (src/llm/ops.cpp:13-19) for operands given in 8 bits. */
+int lx_linear_q8_f32(const lx_q8* x, const lx_q8* w, const float* bias, const lx_epilogue* epi,
+                     const float* resid, long ldr, float* y, long ldy, hipStream_t stream);
+
+/* Scores of rows of logits (rows, V), row stride ld, in one pass over them:
+ *   logp[i] = log softmax(logits[i])[tokens[i]]   (tokens: device int32[rows])
+ *   entropy[i] = -sum_v p_v log p_v
+ *   top_ids[i, :], top_logp[i, :]: the `top` (0 .. 64, at most V) largest logits and their
+ *   log probabilities, largest first, equal ones by the lower id
+ * logp (with tokens), entropy, or the alternatives (top 0) may be left out as NULL.
+ * A token of -1 (a row of padding) has logp 0, any other outside [0, V) NaN.  A logit of
+ * -inf (masked) has probability 0 and adds nothing to the entropy; a row of nothing else
+ * has log probabilities -inf and entropy 0.  A NaN or +inf makes NaN of its row's logp,
+ * entropy and top_logp (NaN counts as the largest logit).  Sums are fp32, formed around the
+ * row's maximum without its own 1.  V <= 2^24.
+ * ws: lx_token_logprobs_ws_floats() floats of scratch, 16-byte aligned (NULL when that is
+ * 0: V up to 8192); calls that share it must not overlap.
+ * Scores what the head of src/llm/llm.cpp:206-216 gives; no counterpart in the reference
+ * (its caller samples on the host). */
+size_t lx_token_logprobs_ws_floats(int rows, int V, int top);
+int lx_token_logprobs_f32(const float* logits, long ld, int rows, int V, const int* tokens,
+                          float* logp, float* entropy, int top, float* top_logp, int* top_ids,
+                          float* ws, size_t ws_floats, hipStream_t stream);
+
 /* Causal grouped conv1d + Mish (one CausalConvPositionEmbedding half):
  *   y[b,t,oc] = mish(bias[oc] + sum_{k<K, ic<C/G} w[oc, ic, k] *
  *                                 x[b, t-(K-1)+k, g*(C/G)+ic]) (+ resid[b,t,oc])

@@ -71,6 +71,10 @@ class Kv4(C.Structure):
                 ("head_dim", C.c_int), ("max_rows", C.c_int)]
 
 
+class Q8(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("rows", C.c_int), ("K", C.c_int)]
+
+
 _DIT_BLOCK_FIELDS = [
     "attn_norm_w", "attn_norm_b", "to_q_w", "to_q_b", "to_k_w", "to_k_b", "to_v_w", "to_v_b",
     "to_out_w", "to_out_b", "ff0_w", "ff0_b", "ff2_w", "ff2_b",
@@ -185,6 +189,17 @@ SIGNATURES = [
     ("lx_attention_kv4_f32", C.c_int,
      [fp, C.c_long, C.POINTER(Kv4), ip, fp, C.c_long, C.c_int, C.c_int, C.c_float, C.c_int,
       C.c_int, fp, C.c_size_t, stream_t]),
+    ("lx_q8_bytes", C.c_size_t, [C.c_int, C.c_int]),
+    ("lx_q8_pack_f32", C.c_int, [fp, C.c_long, C.POINTER(Q8), stream_t]),
+    ("lx_q8_unpack_f32", C.c_int, [C.POINTER(Q8), fp, C.c_long, stream_t]),
+    ("lx_rmsnorm_q8_f32", C.c_int,
+     [fp, C.c_long, fp, C.c_long, fp, C.c_long, fp, C.c_float, C.POINTER(Q8), stream_t]),
+    ("lx_linear_q8_f32", C.c_int,
+     [C.POINTER(Q8), C.POINTER(Q8), fp, C.POINTER(Epilogue), fp, C.c_long, fp, C.c_long,
+      stream_t]),
+    ("lx_token_logprobs_ws_floats", C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    ("lx_token_logprobs_f32", C.c_int,
+     [fp, C.c_long, C.c_int, C.c_int, ip, fp, fp, C.c_int, fp, ip, fp, C.c_size_t, stream_t]),
     ("lx_conv_pos_mish_f32", C.c_int,
      [fp, fp, fp, fp, fp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, stream_t]),
     ("lx_conv_pack_weight_f32", C.c_int, [fp, fp, C.c_int, C.c_int, C.c_int, stream_t]),

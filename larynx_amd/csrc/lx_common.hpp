@@ -54,6 +54,17 @@ inline int raise_lds_limit(const void* kern, size_t bytes, LdsLimit& once, const
   return LX_OK;
 }
 
+// Whether `rows` rows of ca floats every lda from a and of cb every ldb from b share memory; rows of
+// unequal strides that interleave count as sharing.
+inline bool rows_overlap(const float* a, long lda, long ca, const float* b, long ldb, long cb,
+                         long rows) {
+  const intptr_t pa = (intptr_t)a / 4, pb = (intptr_t)b / 4;
+  if (pa + (rows - 1) * lda + ca <= pb || pb + (rows - 1) * ldb + cb <= pa) return false;
+  if (lda != ldb) return true;
+  const long d = ((pb - pa) % lda + lda) % lda;  // the column of a's rows where b's begin
+  return d < ca || d + cb > lda;
+}
+
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 

@@ -1,0 +1,101 @@
+// Matrices in 8 bits (lx_q8.hip, lx_q8_linear.hip): layout, and the forming of codes.
+//
+// Blocks of 128 consecutive elements of a row share 2^e, e the smallest integer >= -127 with
+// max|v| <= 448 * 2^e over the finite ones; a code is the e4m3 number nearest to v / 2^e (exact
+// but for that one rounding: a power of two, and v_cvt_pk_fp8_f32 rounds to nearest even).  The
+// scales are e8m0 bytes e + 127, which the block-scaled matrix instructions of gfx950 take beside
+// the codes, so that a product costs no instruction for its scales.
+//
+// Memory: tiles of 16 rows x 128 elements, 2 KB each, the blocks of K of a row tile side by side.
+// A row's 128 bytes are one line, so that its producer writes whole lines; its eight 16-byte
+// chunks stand at chunk ^ (row / 2 % 8), which spreads the 16 rows that a ds_read_b128 of a
+// fragment touches over all 64 banks: tiles go to LDS as they lie.  (In the lanes' order, the other
+// layout free of conflicts, a row's block is eight pieces in as many lines.)  A fragment of
+// v_mfma_scale_f32_16x16x128_f8f6f4 holds row lane % 16, chunks lane / 16 and lane / 16 + 4: which
+// 32 of the 128 elements a lane multiplies does not matter while both operands agree and a block has
+// one scale.  Behind the codes the scales: per row tile and four blocks 64 bytes, a dword with
+// four blocks' scales per row.
+// Elements past the end of a row are zero; rows past the last may hold anything and only reach
+// outputs that are not stored.
+#pragma once
+
+#include "lx_common.hpp"
+#include "lx_internal.hpp"
+
+namespace lx {
+
+constexpr int kQ8Rows = 16, kQ8Block = 128, kQ8Tile = kQ8Rows * kQ8Block;
+
+inline long q8_tiles(long rows) { return (rows + kQ8Rows - 1) / kQ8Rows; }
+inline long q8_blocks(long K) { return (K + kQ8Block - 1) / kQ8Block; }
+inline size_t q8_code_bytes(long rows, long K) {
+  return (size_t)q8_tiles(rows) * q8_blocks(K) * kQ8Tile;
+}
+
+// A matrix in 8 bits as the kernels see it.
+struct Q8Mat {
+  unsigned char* codes;
+  unsigned char* scales;
+  int rows, K, kb, kb4;  // kb blocks of K, kb4 dwords of scales per row
+};
+
+inline bool q8_shape_ok(int rows, int K) {
+  return rows > 0 && K > 0 && K <= INT_MAX - 127 && rows <= INT_MAX - 15;
+}
+inline bool q8_ok(const lx_q8* q) {
+  return q && q->data && (uintptr_t)q->data % 16 == 0 && q8_shape_ok(q->rows, q->K);
+}
+inline Q8Mat q8_mat(const lx_q8* q) {
+  unsigned char* p = static_cast<unsigned char*>(q->data);
+  const int kb = (int)q8_blocks(q->K);
+  return Q8Mat{p, p + q8_code_bytes(q->rows, q->K), q->rows, q->K, kb, (kb + 3) / 4};
+}
+
+// Byte offset of element k (of its chunk, for k a multiple of 16) of a row.
+__device__ __forceinline__ long q8_at(const Q8Mat& q, int row, int k) {
+  const int r = row & 15;
+  return ((long)(row >> 4) * q.kb + (k >> 7)) * kQ8Tile + r * kQ8Block +
+         ((((k >> 4) & 7) ^ (r >> 1)) << 4) + (k & 15);
+}
+__device__ __forceinline__ long q8_scale_at(const Q8Mat& q, int row, int kb) {
+  return ((long)(row >> 4) * q.kb4 + (kb >> 2)) * 64 + (row & 15) * 4 + (kb & 3);
+}
+
+// The e8m0 byte of a block whose largest finite magnitude is `top`: 448 = 1.75 * 2^8.
+__device__ __forceinline__ int q8_scale(float top) {
+  const unsigned u = __float_as_uint(top);
+  return max((int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0), 0);
+}
+__device__ __forceinline__ float q8_power(int byte) {  // 2^(byte - 127)
+  return __uint_as_float(byte ? (unsigned)byte << 23 : 0x400000u);
+}
+
+// Sixteen lanes hold a block of a row, elements 8 (lane % 16) .. + 7 each: forms its codes and
+// scale and stores them at chunk k / 16 of the row.
+__device__ __forceinline__ void q8_store_block(const Q8Mat& q, int row, int k, const float (&v)[8]) {
+  float top = 0.0f;
+  float w[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool fin = fabsf(v[j]) < __builtin_huge_valf();
+    w[j] = fin ? v[j] : __builtin_nanf("");
+    top = fmaxf(top, fin ? fabsf(v[j]) : 0.0f);
+  }
+  top = fmaxf(top, dpp_mov<kDppXor1>(top));
+  top = fmaxf(top, dpp_mov<kDppXor2>(top));
+  top = fmaxf(top, dpp_mov<kDppHalfMirror>(top));
+  top = fmaxf(top, dpp_mov<kDppMirror>(top));
+  const int byte = q8_scale(top);
+  const float inv = __uint_as_float((unsigned)(254 - byte) << 23);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] *= inv;
+  int lo = 0, hi = 0;
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(w[0], w[1], lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(w[2], w[3], lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(w[4], w[5], hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(w[6], w[7], hi, true);
+  *reinterpret_cast<int2*>(q.codes + q8_at(q, row, k)) = make_int2(lo, hi);
+  if ((k & 127) == 0) q.scales[q8_scale_at(q, row, k >> 7)] = (unsigned char)byte;
+}
+
+}  // namespace lx

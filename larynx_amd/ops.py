@@ -7,12 +7,13 @@ layout; work is enqueued on torch's current stream.  Every call goes through
 liblxops.so; a failing call raises LxError (no fallback path exists).
 """
 import ctypes as C
+from typing import NamedTuple, Optional
 
 import torch
 
 from ._lib import (LX_BX_OUT_F32, LX_BX_OUT_PACKED, LX_BX_OUT_PARTIAL, LX_EPI_GATED_RESID,
                    LX_EPI_GELU_TANH, LX_EPI_NONE, LX_EPI_RESID, LX_EPI_ROPE_PARTIAL,
-                   LX_EPI_SWIGLU_PAIRED, Epilogue, Kv4, LinearBx, check, lib)
+                   LX_EPI_SWIGLU_PAIRED, Q8, Epilogue, Kv4, LinearBx, check, lib)
 
 __all__ = [
     "stream", "ada_ln", "adaln_resid", "adaln_emb", "rope_partial", "gelu_tanh", "gated_residual",
@@ -22,7 +23,8 @@ __all__ = [
     "LX_EPI_NONE", "LX_EPI_GELU_TANH", "LX_EPI_GATED_RESID", "LX_EPI_ROPE_PARTIAL",
     "LX_EPI_RESID", "LX_EPI_SWIGLU_PAIRED", "LX_BX_OUT_F32", "LX_BX_OUT_PARTIAL",
     "LX_BX_OUT_PACKED", "Q4Weight", "q4_pack", "q4_unpack", "linear_q4", "Kv4Cache", "kv4_cache",
-    "kv4_append", "kv4_read", "attention_kv4",
+    "kv4_append", "kv4_read", "attention_kv4", "Q8Matrix", "q8_pack", "q8_unpack", "rms_norm_q8",
+    "linear_q8", "TokenLogprobs", "token_logprobs",
 ]
 
 
@@ -523,3 +525,168 @@ def attention_kv4(q, cache, lens, n_heads, scale=None, causal=True, out=None, ma
                                    int(causal), max_len, ws.data_ptr() if n else None, n,
                                    _raw_stream(dev)))
     return out
+
+
+# ---- the LM's prompt in eight bits, and scoring ------------------------------------------
+
+
+class Q8Matrix:
+    """A matrix (rows, K) in 8 bits: e4m3 codes with a power of two per 128 elements of a row, as
+    q8_pack and rms_norm_q8 lay them out in `data`."""
+    __slots__ = ("data", "rows", "K", "_dev", "_c", "_ref")
+
+    def __init__(self, data, rows, K):
+        self.data, self.rows, self.K = data, rows, K
+        self._dev = data.get_device()
+        self._c = Q8(data.data_ptr(), rows, K)
+        self._ref = C.byref(self._c)
+        n = lib.lx_q8_bytes(rows, K)
+        if not n or data.dtype is not torch.uint8 or not data.is_contiguous() or data.numel() != n:
+            raise ValueError(f"not the 8-bit form of a ({rows}, {K}) matrix")
+
+
+def _q8_out(like, rows, K, out):
+    if out is None:
+        n = lib.lx_q8_bytes(rows, K)
+        if not n:
+            raise ValueError(f"no 8-bit form of a ({rows}, {K}) matrix")
+        return Q8Matrix(like.new_empty(n, dtype=torch.uint8), rows, K)
+    if out.rows != rows or out.K != K:
+        raise ValueError(f"out must hold a ({rows}, {K}) matrix")
+    if out._dev != like.get_device():
+        _elsewhere("out")
+    return out
+
+
+def _matrix(t, name):
+    """Row stride of the fp32 matrix t on the current device, its rows contiguous."""
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be 2-dimensional")
+    ld = _rows(t, name, t.shape)
+    dev = t.get_device()
+    if dev < 0 or dev != _current():
+        _elsewhere(name)
+    return ld
+
+
+def q8_pack(x, out=None):
+    """x (rows, K) fp32 (row stride may exceed K) -> Q8Matrix, a weight or activations: blocks of
+    128 elements of a row share 2^e, e the smallest integer >= -127 with max|v| <= 448 * 2^e; codes
+    are the nearest e4m3 numbers to v / 2^e.  Infinities and NaN stand for NaN."""
+    ld = _matrix(x, "x")
+    q = _q8_out(x, *x.shape, out)
+    check(lib.lx_q8_pack_f32(x.data_ptr(), ld, q._ref, _raw_stream(q._dev)))
+    return q
+
+
+def q8_unpack(q):
+    """The fp32 (rows, K) matrix that a Q8Matrix stands for."""
+    if q._dev < 0 or q._dev != _current():
+        _elsewhere("q")
+    x = q.data.new_empty((q.rows, q.K), dtype=_F32)
+    check(lib.lx_q8_unpack_f32(q._ref, x.data_ptr(), q.K, _raw_stream(q._dev)))
+    return x
+
+
+def rms_norm_q8(x, w, eps=1e-6, add=None, sum_out=None, out=None):
+    """RMSNorm of x (rows, K), after add (rows, K) if given, as a Q8Matrix (`out` or a new one): h =
+    x + add goes to sum_out (default: x, in place), h / sqrt(mean(h^2) + eps) * w to the codes,
+    formed in 64 bits.  src/llm/ops.cpp:7-11, src/llm/llm.cpp:141-173."""
+    ldx = _matrix(x, "x")
+    rows, K = x.shape
+    dev = x.get_device()
+    if w.dtype is not _F32 or w.numel() != K or not w.is_contiguous():
+        raise ValueError(f"w must be {K} contiguous float32 values")
+    if w.get_device() != dev:
+        _elsewhere("w")
+    pa = ps = None
+    lda = lds = 0
+    if add is not None:
+        if sum_out is None:
+            sum_out = x
+        lda, lds = _rows(add, "add", x.shape), _rows(sum_out, "sum_out", x.shape)
+        if add.get_device() != dev or sum_out.get_device() != dev:
+            _elsewhere("add, as sum_out,")
+        pa, ps = add.data_ptr(), sum_out.data_ptr()
+    elif sum_out is not None:
+        raise ValueError("sum_out without add")
+    q = _q8_out(x, rows, K, out)
+    check(lib.lx_rmsnorm_q8_f32(x.data_ptr(), ldx, pa, lda, ps, lds, w.data_ptr(), eps, q._ref,
+                                _raw_stream(dev)))
+    return q
+
+
+def linear_q8(x, w, b=None, epilogue=None, resid=None, out=None):
+    """epi(x~ @ w~^T + b) of two Q8Matrix, x (M, K) and w (N, K); epilogue: none, GELU, residual
+    (resid + .., or into out= the residual stream) or SwiGLU over interleaved rows of w.
+    src/llm/ops.cpp:13-19."""
+    dev = x._dev
+    if dev < 0 or dev != w._dev or dev != _current():
+        _elsewhere("x, as w,")
+    M, N = x.rows, w.rows
+    kind = LX_EPI_NONE if epilogue is None else epilogue.kind
+    cols = N // 2 if kind == LX_EPI_SWIGLU_PAIRED else N
+    bias = pr = None
+    ldr = 0
+    if b is not None:
+        if b.dtype is not _F32 or b.numel() != N or not b.is_contiguous():
+            raise ValueError(f"b must be {N} contiguous float32 values")
+        if b.get_device() != dev:
+            _elsewhere("b")
+        bias = b.data_ptr()
+    if resid is not None:
+        ldr = _rows(resid, "resid", (M, cols))
+        if resid.get_device() != dev:
+            _elsewhere("resid")
+        pr = resid.data_ptr()
+    if out is None:
+        if kind == LX_EPI_RESID and resid is None:
+            raise ValueError("residual epilogues need resid=, or out= (the residual stream)")
+        out = x.data.new_empty((M, cols), dtype=_F32)
+        ldy = cols
+    else:
+        ldy = _rows(out, "out", (M, cols))
+        if out.get_device() != dev:
+            _elsewhere("out")
+    check(lib.lx_linear_q8_f32(x._ref, w._ref, bias,
+                               None if epilogue is None else C.byref(epilogue), pr, ldr,
+                               out.data_ptr(), ldy, _raw_stream(dev)))
+    return out
+
+
+class TokenLogprobs(NamedTuple):
+    """Of token_logprobs: logp and entropy (rows), top_logp and top_ids (rows, top), or None."""
+    logp: Optional[torch.Tensor]
+    entropy: Optional[torch.Tensor]
+    top_logp: Optional[torch.Tensor]
+    top_ids: Optional[torch.Tensor]
+
+
+def token_logprobs(logits, tokens=None, top=0, entropy=True):
+    """Scores rows of logits (rows, V) (row stride may exceed V): log probabilities of tokens (device
+    int32 (rows); -1: padding, 0), the distribution's entropy, and the `top` (at most 64) most
+    likely ids with their log probabilities, equal logits by the lower id.  Logits of -inf are
+    masked.  Scores the head's output, src/llm/llm.cpp:206-216."""
+    ld = _matrix(logits, "logits")
+    rows, V = logits.shape
+    dev = logits.get_device()
+    logp = pt = pl = pe = ptl = pti = ent = tl = ti = None
+    if tokens is not None:
+        if tokens.dtype is not _I32 or tokens.numel() != rows or not tokens.is_contiguous():
+            raise ValueError(f"tokens must be {rows} contiguous int32 values")
+        if tokens.get_device() != dev:
+            _elsewhere("tokens")
+        logp = logits.new_empty(rows)
+        pt, pl = tokens.data_ptr(), logp.data_ptr()
+    if entropy:
+        ent = logits.new_empty(rows)
+        pe = ent.data_ptr()
+    if top > 0:
+        tl = logits.new_empty((rows, top))
+        ti = logits.new_empty((rows, top), dtype=_I32)
+        ptl, pti = tl.data_ptr(), ti.data_ptr()
+    n = lib.lx_token_logprobs_ws_floats(rows, V, top)
+    ws = logits.new_empty(n) if n else None
+    check(lib.lx_token_logprobs_f32(logits.data_ptr(), ld, rows, V, pt, pl, pe, top, ptl, pti,
+                                    ws.data_ptr() if n else None, n, _raw_stream(dev)))
+    return TokenLogprobs(logp, ent, tl, ti)

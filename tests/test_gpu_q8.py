@@ -1,0 +1,418 @@
+"""Matrices in 8 bits on the GPU: codes against the format in 64 bits (bit for bit), the norm that
+feeds them, products against 64-bit sums over what the codes stand for."""
+import math
+
+import pytest
+import torch
+
+from conftest import announce
+from larynx_amd import ops
+from larynx_amd._lib import LxError
+from q8_reference import E4M3, held
+
+pytestmark = pytest.mark.gpu
+EPS = 1e-6
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _same(a, b):
+    """Equal, NaN where the other is."""
+    a, b = a.double().cpu(), b.double().cpu()
+    assert a.shape == b.shape
+    bad = ~((a == b) | (a.isnan() & b.isnan()))
+    assert not bad.any(), (bad.sum().item(), bad.nonzero()[:4].tolist(), a[bad][:4], b[bad][:4])
+
+
+def _fp32(v):
+    """The fp32 that stands for a held value: exact, but for numbers past its range."""
+    return v.float()
+
+
+# ---- codes ----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("scale", [-127, -126, -60, -1, 0, 3, 119])
+def test_every_code_and_border(gpu, scale):
+    """All e4m3 numbers, the borders between them and the fp32 numbers beside these, at one scale."""
+    announce(f"q8 codes at 2^{scale}")
+    t = E4M3.float()
+    mid = (t[1:] + t[:-1]) / 2
+    inf = torch.tensor(float("inf"))
+    v = torch.cat([t, mid, torch.nextafter(mid, inf), torch.nextafter(mid, -inf)])
+    v = torch.cat([v, -v])
+    v = torch.nn.functional.pad(v, (0, -v.numel() % 127)).view(-1, 127)
+    v = torch.cat([v, torch.full((v.shape[0], 1), 448.0)], 1)  # each block at this scale
+    x = (v.double() * 2.0 ** scale).float()
+    want, powers = held(x)
+    assert (powers == 2.0 ** scale).all()
+    _same(ops.q8_unpack(ops.q8_pack(x.to(gpu))), _fp32(want))
+
+
+@pytest.mark.parametrize("rows,K", [(1, 1), (1, 127), (2, 128), (3, 129), (15, 500), (16, 896),
+                                    (17, 1001), (37, 4864), (300, 13)])
+@pytest.mark.parametrize("pad", [0, 1, 4])
+def test_pack_sizes_and_strides(gpu, rows, K, pad):
+    announce(f"q8 pack {rows} x {K} stride +{pad}")
+    x = torch.randn(rows, K, generator=_gen(rows * K)) * torch.exp(
+        3 * torch.randn(rows, 1, generator=_gen(7)))
+    wide = torch.full((rows, K + pad), float("nan"))  # what lies between rows counts for nothing
+    wide[:, :K] = x
+    q = ops.q8_pack(wide.to(gpu)[:, :K])
+    assert (q.rows, q.K) == (rows, K)
+    _same(ops.q8_unpack(q), _fp32(held(x)[0]))
+
+
+def test_pack_extremes(gpu):
+    inf, nan = float("inf"), float("nan")
+    x = torch.randn(8, 300, generator=_gen(3))
+    x[0] = 0.0
+    x[1] = 1e-42          # subnormal numbers of fp32
+    x[2, :128] = 3.4e38   # the largest: stands for 2^128, infinity in fp32
+    x[3, 5] = nan
+    x[4, 130] = inf
+    x[4, 131] = -inf
+    x[5] = nan
+    x[6] = -0.0
+    x[7, 128:256] = torch.tensor([2.0 ** -149, 448 * 2.0 ** -127] * 64)
+    _same(ops.q8_unpack(ops.q8_pack(x.to(gpu))), _fp32(held(x)[0]))
+
+
+def test_pack_into_a_given_matrix(gpu):
+    """The rows of the matrix are written whole, whatever it held: nothing of a row's tail stays."""
+    q = ops.q8_pack(torch.full((20, 300), float("nan"), device=gpu))
+    data = q.data
+    x, w = torch.randn(20, 300, generator=_gen(4)), torch.randn(24, 300, generator=_gen(5))
+    assert ops.q8_pack(x.to(gpu), out=q) is q and q.data is data
+    y = ops.linear_q8(q, ops.q8_pack(w.to(gpu)))
+    assert not y.isnan().any()
+    with pytest.raises(ValueError, match="out must hold"):
+        ops.q8_pack(x[:19].to(gpu), out=q)
+
+
+# ---- norm -----------------------------------------------------------------------------
+
+
+def _norm64(h, w, eps=EPS):
+    h = h.double()
+    eps = float(torch.tensor(eps, dtype=torch.float32))
+    return h / torch.sqrt(h.square().mean(1, keepdim=True) + eps) * w.double()
+
+
+NORMS = [(1, 896), (5, 1), (3, 128), (33, 1001), (64, 1024), (7, 1025), (130, 2047), (9, 2049),
+         (4, 4096), (5, 4100), (6, 8192), (3, 8193), (2, 20000)]
+
+
+@pytest.mark.parametrize("rows,D", NORMS)
+def test_norm_codes(gpu, rows, D):
+    announce(f"rms_norm_q8 {rows} x {D}")
+    g = _gen(D)
+    x = torch.randn(rows, D, generator=g)
+    x[:, ::97] *= 20
+    w = 1 + 0.2 * torch.randn(D, generator=g)
+    q = ops.rms_norm_q8(x.to(gpu), w.to(gpu))
+    _same(ops.q8_unpack(q), _fp32(held(_norm64(x, w))[0]))
+
+
+@pytest.mark.parametrize("rows,D", NORMS)
+@pytest.mark.parametrize("where", ["x", "add", "apart"])
+def test_norm_with_residual(gpu, rows, D, where):
+    announce(f"rms_norm_q8 {rows} x {D} sum in {where}")
+    g = _gen(D + 1)
+    x, add = torch.randn(rows, D, generator=g), torch.randn(rows, D, generator=g)
+    w = 1 + 0.2 * torch.randn(D, generator=g)
+    h = x + add
+    xd, ad = x.to(gpu), add.to(gpu)
+    out = {"x": None, "add": ad, "apart": torch.full((rows, D), 7.0, device=gpu)}[where]
+    q = ops.rms_norm_q8(xd, w.to(gpu), add=ad, sum_out=out)
+    _same(xd if out is None else out, h)
+    if where != "x":
+        _same(xd, x)
+    if where != "add":
+        _same(ad, add)
+    _same(ops.q8_unpack(q), _fp32(held(_norm64(h, w))[0]))
+
+
+def test_norm_strides(gpu):
+    """Rows of unequal strides at odd offsets; what lies between them stays."""
+    g = _gen(9)
+    rows, D = 21, 515
+    buf = [torch.randn(rows, D + p, generator=g) for p in (1, 2, 6)]
+    w = torch.randn(D + 1, generator=g)
+    dev = [b.to(gpu) for b in buf]
+    q = ops.rms_norm_q8(dev[0][:, 1:], w.to(gpu)[1:], add=dev[1][:, 2:], sum_out=dev[2][:, 3:-3])
+    h = buf[0][:, 1:] + buf[1][:, 2:]
+    want = buf[2].clone()
+    want[:, 3:-3] = h
+    _same(dev[2], want)
+    _same(ops.q8_unpack(q), _fp32(held(_norm64(h, w[1:]))[0]))
+
+
+def test_norm_extremes(gpu):
+    """Rows of zeros, of very large and very small numbers, with infinities and NaN."""
+    g = _gen(11)
+    x = torch.randn(7, 896, generator=g)
+    x[0] = 0.0
+    x[1] *= 1e30
+    x[2] *= 1e-30
+    x[3, 17] = float("inf")
+    x[4, 600] = float("nan")
+    x[5, 895] = 3e38
+    x[6] = 2.0 ** -149
+    w = torch.randn(896, generator=g)
+    _same(ops.q8_unpack(ops.rms_norm_q8(x.to(gpu), w.to(gpu))), _fp32(held(_norm64(x, w))[0]))
+
+
+def test_norm_refusals(gpu):
+    x, w = torch.zeros(4, 256, device=gpu), torch.ones(256, device=gpu)
+    for kw in [dict(w=w[:255]), dict(w=w.double()), dict(w=w.cpu()), dict(sum_out=x),
+               dict(add=x[:3]), dict(add=x.cpu()), dict(add=x.double()),
+               dict(add=torch.zeros_like(x), sum_out=x[:, :255]),
+               dict(out=ops.q8_pack(x[:3]))]:
+        with pytest.raises(ValueError):
+            ops.rms_norm_q8(**{"x": x, "w": w, **kw})
+    both = torch.zeros(4, 260, device=gpu)
+    with pytest.raises(LxError):
+        ops.rms_norm_q8(both[:, :256], w, add=x, sum_out=both[:, 4:])
+
+
+# ---- products -------------------------------------------------------------------------
+
+
+def _pair(M, N, K, seed, gpu):
+    g = _gen(seed)
+    x, w = torch.randn(M, K, generator=g), torch.randn(N, K, generator=g) * K ** -0.5
+    x[:, ::31] *= 6
+    xq, wq = ops.q8_pack(x.to(gpu)), ops.q8_pack(w.to(gpu))
+    return xq, wq, ops.q8_unpack(xq).double().cpu(), ops.q8_unpack(wq).double().cpu()
+
+
+def _bound(X, W):
+    """Exact products, at most K + 16 fp32 additions of partial sums below S = sum |x w|, each off
+    by less than its last place (2^-23), in the instruction as between them."""
+    K = X.shape[1]
+    return (K + 16) * 2.0 ** -23 * (X.abs() @ W.abs().t())
+
+
+LINEARS = [(1, 1, 1), (1, 16, 128), (1, 1152, 896), (2, 17, 129), (4, 6761, 896), (15, 33, 1000),
+           (16, 100, 4864), (17, 64, 300), (31, 9, 256), (33, 130, 896), (64, 64, 640),
+           (65, 257, 500), (100, 1152, 896), (128, 256, 128), (129, 895, 1280), (177, 6761, 896),
+           (256, 9728, 896), (300, 896, 4864), (513, 300, 2000), (1531, 896, 896),
+           (1025, 1030, 130), (3, 900, 8192), (2000, 1500, 1100), (2049, 2305, 257),
+           (2100, 4100, 384)]
+
+
+@pytest.mark.parametrize("M,N,K", LINEARS)
+def test_products(gpu, M, N, K):
+    announce(f"linear_q8 {M} x {N} x {K}")
+    xq, wq, X, W = _pair(M, N, K, M + N + K, gpu)
+    y = ops.linear_q8(xq, wq).double().cpu()
+    want = X @ W.t()
+    err = (y - want).abs()
+    assert (err <= _bound(X, W)).all(), (err / _bound(X, W)).max()
+    # the sums of a whole call: rounding errors average out, a lost product would not
+    rel = (err.square().sum() / want.square().sum()).sqrt()
+    assert rel <= 2.0 ** -24 * (2 + math.sqrt(K)), rel
+
+
+@pytest.mark.parametrize("M,N,K", LINEARS)
+def test_every_product_counts(gpu, M, N, K):
+    """Whole numbers with exact fp32 sums (below 2^24): no product is lost, doubled or moved."""
+    announce(f"linear_q8 whole numbers {M} x {N} x {K}")
+    g = _gen(M * 7 + N * 3 + K)
+    x = torch.randint(-15, 16, (M, K), generator=g).float()
+    w = torch.randint(-15, 16, (N, K), generator=g).float()
+    x[:, 0] = 15  # |x| <= 15 and steps of 1: held as they are at any scale up to 2^0
+    w[:, 0] = 15
+    xq, wq = ops.q8_pack(x.to(gpu)), ops.q8_pack(w.to(gpu))
+    X, W = ops.q8_unpack(xq).double().cpu(), ops.q8_unpack(wq).double().cpu()
+    assert torch.equal(X, x.double()) and torch.equal(W, w.double())
+    _same(ops.linear_q8(xq, wq), X @ W.t())
+
+
+@pytest.mark.parametrize("M,N", [(3, 40), (40, 33), (300, 200), (1100, 1300)])
+def test_scales_of_every_row_and_block(gpu, M, N):
+    """Blocks at powers of two of their own, one element each: every product has its scales."""
+    K = 128 * 9 + 5
+    g = _gen(M)
+    kb = (K + 127) // 128
+    ex = torch.randint(-40, 40, (M, kb), generator=g)
+    ew = torch.randint(-40, 40, (N, kb), generator=g)
+    at = torch.randint(0, 5, (kb,), generator=g) + 128 * torch.arange(kb)
+    x, w = torch.zeros(M, K), torch.zeros(N, K)
+    x[:, at] = torch.ldexp(torch.ones(()), ex)
+    # one block a row of w: its product stands alone
+    one = torch.arange(N) % kb
+    w[torch.arange(N), at[one]] = torch.ldexp(torch.ones(()), ew[torch.arange(N), one])
+    y = ops.linear_q8(ops.q8_pack(x.to(gpu)), ops.q8_pack(w.to(gpu)))
+    _same(y, x.double() @ w.double().t())
+
+
+def _epi(kind, acc, b=None, r=None):
+    if b is not None:
+        acc = acc + b.double()
+    if kind == "gelu":
+        return 0.5 * acc * (1 + torch.tanh(0.7978845608028654 * (acc + 0.044715 * acc ** 3)))
+    if kind == "resid":
+        return r.double() + acc
+    if kind == "swiglu":
+        return acc[:, 0::2] / (1 + torch.exp(-acc[:, 0::2])) * acc[:, 1::2]
+    return acc
+
+
+KINDS = {"none": None, "gelu": ops.LX_EPI_GELU_TANH, "resid": ops.LX_EPI_RESID,
+         "swiglu": ops.LX_EPI_SWIGLU_PAIRED}
+EPI_SHAPES = [(1, 66, 896), (9, 68, 200), (40, 130, 300), (70, 1152, 896), (257, 514, 896),
+              (1030, 1026, 150)]
+
+
+@pytest.mark.parametrize("M,N,K", EPI_SHAPES)
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("bias", [False, True])
+def test_epilogues(gpu, M, N, K, kind, bias):
+    announce(f"linear_q8 {kind} bias {bias} {M} x {N} x {K}")
+    xq, wq, X, W = _pair(M, N, K, M + K, gpu)
+    g = _gen(5)
+    b = torch.randn(N, generator=g) if bias else None
+    r = torch.randn(M, N, generator=g) if kind == "resid" else None
+    epi = None if KINDS[kind] is None else ops.Epilogue(kind=KINDS[kind])
+    y = ops.linear_q8(xq, wq, None if b is None else b.to(gpu), epilogue=epi,
+                      resid=None if r is None else r.to(gpu)).double().cpu()
+    acc = X @ W.t()
+    want = _epi(kind, acc, b, r)
+    # the sums' bound, carried through the epilogue (slopes: GELU and SiLU at most 1.13; a SwiGLU
+    # output's other factor), and its own fp32 steps: bias and residual additions 2^-24 of what
+    # they give, the activations a few 2^-23 of their result (hardware exponentials and
+    # reciprocals, arguments off by 2^-22 of themselves: |u| e^-|u| <= 1/2 of it, times |acc|)
+    e = _bound(X, W) + 2.0 ** -24 * (acc.abs() + (b.abs().double() if bias else 0.0))
+    if kind == "resid":
+        tol = e + 2.0 ** -24 * want.abs() + 1e-45
+    elif kind == "gelu":
+        tol = 1.13 * e + 2.0 ** -20 * (acc + (b.double() if bias else 0.0)).abs()
+    elif kind == "swiglu":
+        full = acc + (b.double() if bias else 0.0)
+        gate, up = full[:, 0::2], full[:, 1::2]
+        tol = 1.13 * e[:, 0::2] * (up.abs() + e[:, 1::2]) + gate.abs() * e[:, 1::2] + \
+            2.0 ** -20 * (gate * up).abs()
+    else:
+        tol = e + 2.0 ** -24 * want.abs()
+    assert ((y - want).abs() <= tol + 1e-37).all(), ((y - want).abs() / tol).max()
+
+
+@pytest.mark.parametrize("M,N,K", EPI_SHAPES)
+@pytest.mark.parametrize("pad", [0, 1, 3, 4])
+def test_outputs_in_place_and_strided(gpu, M, N, K, pad):
+    """Residual in place, rows of y apart: what lies behind and between them stays."""
+    announce(f"linear_q8 in place {M} x {N} x {K} pad {pad}")
+    xq, wq, X, W = _pair(M, N, K, K, gpu)
+    g = _gen(6)
+    buf = torch.randn(M + 3, N + pad, generator=g)
+    y = buf.to(gpu)
+    out = y[:M, pad:]
+    ops.linear_q8(xq, wq, epilogue=ops.Epilogue(kind=ops.LX_EPI_RESID), out=out)
+    plain = ops.linear_q8(xq, wq)
+    want = buf.clone()
+    want[:M, pad:] += plain.cpu()
+    _same(y, want)
+    z = torch.full_like(y, 3.0)
+    ops.linear_q8(xq, wq, out=z[:M, pad:])
+    want = torch.full((M + 3, N + pad), 3.0)
+    want[:M, pad:] = plain.cpu()
+    _same(z, want)
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 40, 300), (70, 200, 300), (300, 300, 300), (1100, 1300, 300)])
+def test_nan_stays_in_its_rows(gpu, M, N, K):
+    g = _gen(8)
+    x, w = torch.randn(M, K, generator=g), torch.randn(N, K, generator=g)
+    clean = ops.linear_q8(ops.q8_pack(x.to(gpu)), ops.q8_pack(w.to(gpu))).cpu()
+    x[M // 2, 7] = float("nan")
+    x[0, 299] = float("inf")
+    w[N - 1, 130] = -float("inf")
+    y = ops.linear_q8(ops.q8_pack(x.to(gpu)), ops.q8_pack(w.to(gpu))).cpu()
+    bad = torch.zeros(M, N, dtype=torch.bool)
+    bad[[0, M // 2]] = True
+    bad[:, N - 1] = True
+    assert y[bad].isnan().all()
+    # the non-finite elements do not change their block's scale here: the rest is as before
+    same = ~bad
+    assert torch.equal(y[same], clean[same])
+
+
+def test_rows_past_the_last(gpu):
+    """The last tile's memory behind the last row of x and w holds NaN codes: nothing shows."""
+    for M, N in [(3, 21), (37, 70), (261, 300), (1029, 1100)]:
+        xq, wq, X, W = _pair(M, N, 300, 12, gpu)
+        y = ops.linear_q8(xq, wq)
+        held_x = ops.q8_pack(torch.full((-(-M // 16) * 16, 300), float("nan"), device=gpu))
+        held_w = ops.q8_pack(torch.full((-(-N // 16) * 16, 300), float("nan"), device=gpu))
+        x2 = ops.q8_pack(ops.q8_unpack(xq), out=ops.Q8Matrix(held_x.data, M, 300))
+        w2 = ops.q8_pack(ops.q8_unpack(wq), out=ops.Q8Matrix(held_w.data, N, 300))
+        assert torch.equal(ops.linear_q8(x2, w2), y)
+
+
+def test_linear_refusals(gpu):
+    xq, wq = ops.q8_pack(torch.zeros(4, 256, device=gpu)), ops.q8_pack(torch.zeros(6, 256, device=gpu))
+    other = ops.q8_pack(torch.zeros(6, 255, device=gpu))
+    with pytest.raises(LxError):
+        ops.linear_q8(xq, other)
+    resid = ops.Epilogue(kind=ops.LX_EPI_RESID)
+    y = torch.zeros(4, 6, device=gpu)
+    for kw in [dict(b=torch.zeros(5, device=gpu)), dict(b=torch.zeros(6)), dict(epilogue=resid),
+               dict(epilogue=resid, resid=y[:3]), dict(epilogue=resid, resid=y.cpu()),
+               dict(out=y[:, :5]), dict(out=y.cpu()), dict(out=y.double())]:
+        with pytest.raises(ValueError):
+            ops.linear_q8(xq, wq, **kw)
+    for kw in [dict(epilogue=ops.Epilogue(kind=ops.LX_EPI_GATED_RESID)), dict(resid=y),
+               dict(epilogue=ops.Epilogue(kind=17))]:
+        with pytest.raises(LxError):
+            ops.linear_q8(xq, wq, **kw)
+
+
+# ---- streams and graphs ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_captured_with_an_eager_call_between(gpu, M):
+    """A norm and its projection captured and replayed over changing inputs, eager calls of the
+    same sizes between the replays."""
+    announce(f"q8 graph {M}")
+    D, N = 896, 300
+    g = _gen(M)
+    xs = [torch.randn(M, D, generator=g).to(gpu) for _ in range(4)]
+    w = torch.rand(D, generator=g).to(gpu) + 0.5
+    wq = ops.q8_pack(torch.randn(N, D, generator=g).to(gpu))
+    want = [ops.linear_q8(ops.rms_norm_q8(x, w), wq) for x in xs]
+    x = xs[0].clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        ops.linear_q8(ops.rms_norm_q8(x, w), wq)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.linear_q8(ops.rms_norm_q8(x, w), wq)
+    for i in [1, 2, 3, 0]:
+        x.copy_(xs[i])
+        graph.replay()
+        eager = ops.linear_q8(ops.rms_norm_q8(xs[(i + 1) % 4], w), wq)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[i]) and torch.equal(eager, want[(i + 1) % 4])
+
+
+def test_two_streams(gpu):
+    g = _gen(2)
+    x = [torch.randn(200, 896, generator=g).to(gpu) for _ in range(2)]
+    wq = ops.q8_pack(torch.randn(500, 896, generator=g).to(gpu))
+    want = [ops.linear_q8(ops.q8_pack(v), wq) for v in x]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.linear_q8(ops.q8_pack(x[i]), wq))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
