@@ -31,6 +31,7 @@ LX_BX_OUT_PARTIAL = 1
 LX_BX_OUT_PACKED = 2
 
 fp = C.c_void_p  # device pointer
+q8p = C.c_void_p  # an lx_q8, as a Q8 by reference or as its bytes
 ip = C.c_void_p
 stream_t = C.c_void_p
 
@@ -190,12 +191,12 @@ SIGNATURES = [
      [fp, C.c_long, C.POINTER(Kv4), ip, fp, C.c_long, C.c_int, C.c_int, C.c_float, C.c_int,
       C.c_int, fp, C.c_size_t, stream_t]),
     ("lx_q8_bytes", C.c_size_t, [C.c_int, C.c_int]),
-    ("lx_q8_pack_f32", C.c_int, [fp, C.c_long, C.POINTER(Q8), stream_t]),
-    ("lx_q8_unpack_f32", C.c_int, [C.POINTER(Q8), fp, C.c_long, stream_t]),
+    ("lx_q8_pack_f32", C.c_int, [fp, C.c_long, q8p, stream_t]),
+    ("lx_q8_unpack_f32", C.c_int, [q8p, fp, C.c_long, stream_t]),
     ("lx_rmsnorm_q8_f32", C.c_int,
-     [fp, C.c_long, fp, C.c_long, fp, C.c_long, fp, C.c_float, C.POINTER(Q8), stream_t]),
+     [fp, C.c_long, fp, C.c_long, fp, C.c_long, fp, C.c_float, q8p, stream_t]),
     ("lx_linear_q8_f32", C.c_int,
-     [C.POINTER(Q8), C.POINTER(Q8), fp, C.POINTER(Epilogue), fp, C.c_long, fp, C.c_long,
+     [q8p, q8p, fp, C.POINTER(Epilogue), fp, C.c_long, fp, C.c_long,
       stream_t]),
     ("lx_token_logprobs_ws_floats", C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     ("lx_token_logprobs_f32", C.c_int,

@@ -9,9 +9,11 @@
 // a second launch joins.
 //
 // Alternatives are ordered by 64-bit keys, unlike for any two logits: the value's bits in an order
-// that whole numbers share, then the complement of the index.  In each wave the k-th largest of the
-// lanes' own largest keys bounds the k-th largest key from below; the largest of these bounds
-// leaves a few more than k candidates, and a candidate's rank among them is its place.
+// that whole numbers share, then the complement of the index.  The k-th largest of the 256 threads'
+// maxima (its leading 16 bits, found bit by bit with ballots, each wave for itself) bounds the k-th
+// largest logit from below and leaves little more than k candidates (21 of 8192 normal logits for
+// k = 20, 74 for 64), whose ranks among each other are their places.  Where ties or an order crowd
+// more of them into few threads, the exact bound is found the same way over all logits.
 #include <algorithm>
 #include <climits>
 
@@ -27,6 +29,7 @@ typedef unsigned long long key_t64;
 constexpr int kPiece = 8192;   // logits of a workgroup
 constexpr int kMaxTop = 64;    // a lane each
 constexpr int kCand = 1024;    // candidates ranked at once
+constexpr int kSeg = kCand / 4;  // of a wave
 
 struct LpArgs {
   const float* x;
@@ -55,71 +58,60 @@ __device__ __forceinline__ key_t64 key_of(unsigned order, int index) {
 __device__ __forceinline__ float exp_of(float d) {
   return __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
 }
+__device__ __forceinline__ int lanes(bool c) { return __popcll(__ballot(c)); }
+// How many of the lanes below this one have their bit in m.
+__device__ __forceinline__ int lanes_below(unsigned long long m) {
+  return __builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32),
+                                   __builtin_amdgcn_mbcnt_lo((unsigned)m, 0));
+}
 
-// The k-th largest of the 64 lanes' keys.
-__device__ __forceinline__ key_t64 wave_kth(key_t64 key, int k) {
-  key_t64 at = 0;
+// The largest number of `high` + 1 bits, its bits below `low` zero, that count() says at least k of.
+template <class Count>
+__device__ __forceinline__ unsigned largest_with(int k, int high, int low, Count count) {
+  unsigned at = 0;
 #pragma unroll 1
-  for (int b = 63; b >= 0; --b) {
-    const key_t64 mid = at | 1ull << b;
-    if (__popcll(__ballot(key >= mid)) >= k) at = mid;
+  for (int b = high; b >= low; --b) {
+    const unsigned mid = at | 1u << b;
+    if (count(mid) >= k) at = mid;
   }
   return at;
 }
 
-struct LpShared {
-  float f[4][4];
-  key_t64 bound[4];
-  int count;
-  key_t64 cand[kCand];
-};
-
-// The `top` largest of the keys that `each` calls its argument with (each thread's own), largest
-// first, handed to out(place, key).  `mine`: the largest of this thread's keys (0: none).
-template <class Each, class Out>
-__device__ void block_top(LpShared& sh, int top, key_t64 mine, Each each, Out out) {
-  const int tid = threadIdx.x;
-  const key_t64 b = wave_kth(mine, top);
-  if ((tid & 63) == 0) sh.bound[tid >> 6] = b;
-  if (tid == 0) sh.count = 0;
-  __syncthreads();
-  key_t64 bound = max(max(sh.bound[0], sh.bound[1]), max(sh.bound[2], sh.bound[3]));
-  for (;;) {
-    each([&](key_t64 key) {
-      if (key >= bound && key) {
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < kCand) sh.cand[at] = key;
+// Candidates in SEGS segments of n[..] keys, ranked by how many of them are larger, four threads
+// each: the `top` largest go to out(place, key).  All threads of the workgroup take part.
+template <int THREADS, int SEGS, int STRIDE, class Out>
+__device__ __forceinline__ void rank_keys(const key_t64* cand, const int (&n)[SEGS], int top,
+                                          Out out) {
+  const int part = threadIdx.x & 3;
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < SEGS; ++w) total += n[w];
+  for (int i = threadIdx.x >> 2; i < (total + 15) / 16 * 16; i += THREADS / 4) {
+    int at = i, seg = 0;
+#pragma unroll
+    for (int w = 0; w + 1 < SEGS; ++w)
+      if (seg == w && at >= n[w]) {
+        at -= n[w];
+        seg = w + 1;
       }
-    });
-    __syncthreads();
-    if (sh.count <= kCand) break;
-    // many large keys in few lanes: the exact bound, bit by bit
-    key_t64 at = 0;
-#pragma unroll 1
-    for (int bit = 63; bit >= 0; --bit) {
-      const key_t64 mid = at | 1ull << bit;
-      __syncthreads();
-      if (tid == 0) sh.count = 0;
-      __syncthreads();
-      int n = 0;
-      each([&](key_t64 key) { n += key >= mid; });
-      if (n) atomicAdd(&sh.count, n);
-      __syncthreads();
-      if (sh.count >= top) at = mid;
-    }
-    bound = at;
-    __syncthreads();
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-  }
-  const int n = sh.count;
-  for (int i = tid; i < n; i += 256) {
-    const key_t64 key = sh.cand[i];
+    const key_t64 key = i < total ? cand[seg * STRIDE + at] : 0;
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += sh.cand[j] > key;
-    if (rank < top) out(rank, key);
+#pragma unroll
+    for (int w = 0; w < SEGS; ++w)
+#pragma unroll 4
+      for (int j = part; j < n[w]; j += 4) rank += cand[w * STRIDE + j] > key;
+    rank += __builtin_amdgcn_mov_dpp(rank, kDppXor1, 0xF, 0xF, false);
+    rank += __builtin_amdgcn_mov_dpp(rank, kDppXor2, 0xF, 0xF, false);
+    if (part == 0 && i < total && rank < top) out(rank, key);
   }
 }
+
+struct LpShared {
+  float f[4][4];
+  uint4 order[64];  // of the threads' maxima
+  int n[2][4];
+  key_t64 cand[kCand];
+};
 
 struct RowSums {
   float m, s, t;
@@ -132,12 +124,25 @@ __device__ __forceinline__ float logp_of(const RowSums& r, float ls, float x) {
   if (row_empty(r)) return -__builtin_huge_valf();
   return (float)(((double)x - (double)r.m) - (double)ls);
 }
-__device__ __forceinline__ void write_row(const LpArgs& a, int row, const RowSums& r, float ls) {
+// A row's token and its logit, asked for first and used last.
+struct Given {
+  int t;
+  float x;
+};
+__device__ __forceinline__ Given given(const LpArgs& a, int row) {
+  Given g{-1, 0.0f};
   if (a.logp) {
-    const int t = a.tokens[row];
+    g.t = a.tokens[row];
+    if (g.t >= 0 && g.t < a.V) g.x = a.x[row * a.ld + g.t];
+  }
+  return g;
+}
+__device__ __forceinline__ void write_row(const LpArgs& a, int row, const Given& g,
+                                          const RowSums& r, float ls) {
+  if (a.logp) {
     float v = 0.0f;
-    if (t >= a.V || t < -1) v = __builtin_nanf("");
-    else if (t >= 0) v = logp_of(r, ls, a.x[row * a.ld + t]);
+    if (g.t >= a.V || g.t < -1) v = __builtin_nanf("");
+    else if (g.t >= 0) v = logp_of(r, ls, g.x);
     a.logp[row] = v;
   }
   if (a.entropy) a.entropy[row] = row_empty(r) ? 0.0f : ls - r.t / (1.0f + r.s);
@@ -151,6 +156,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(LpArgs a) {
   const int begin = piece * a.len, n = min(a.len, a.V - begin);
   const float* x = a.x + row * a.ld + begin;
   const float inf = __builtin_huge_valf();
+  const Given tok = a.pieces > 1 ? Given{} : given(a, row);
   float v[NV][4];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -169,24 +175,36 @@ __global__ __launch_bounds__(256) void logprob_kernel(LpArgs a) {
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) m = fmaxf(m, v[i][e]);
+  if constexpr (TOP) {
+    // a NaN is no maximum, but the largest logit
+    unsigned o = order_of(m);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o = v[i][e] != v[i][e] ? 0xffffffffu : o;
+    reinterpret_cast<unsigned*>(sh.order)[tid] = o;
+  }
   m = wave_max(m);
   if ((tid & 63) == 0) sh.f[wave][0] = m;
   __syncthreads();
   m = fmaxf(fmaxf(sh.f[0][0], sh.f[1][0]), fmaxf(sh.f[2][0], sh.f[3][0]));
   const float ref = m == -inf ? 0.0f : m;
-  float s = 0.0f, t = 0.0f, tops = 0.0f;
+  float s = 0.0f, t = 0.0f;
+  int maxima = 0;  // of the wave
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float d = v[i][e] - ref;
       const float p = exp_of(d);
-      if (d == 0.0f) tops += 1.0f; else s += p;
+      const bool is_max = d == 0.0f;
+      maxima += lanes(is_max);
+      s += is_max ? 0.0f : p;
       t = fmaf(p, fmaxf(d, -200.0f), t);  // far below, p is 0
     }
   s = wave_sum(s);
   t = wave_sum(t);
-  tops = wave_sum(tops);
+  float tops = (float)maxima;
   if ((tid & 63) == 0) {
     sh.f[wave][1] = s;
     sh.f[wave][2] = t;
@@ -203,48 +221,123 @@ __global__ __launch_bounds__(256) void logprob_kernel(LpArgs a) {
   if (a.pieces > 1) {
     if (tid == 0) a.part[blockIdx.x] = make_float4(r.m, r.s, r.t, 0.0f);
   } else if (tid == 0) {
-    write_row(a, row, r, ls);
+    write_row(a, row, tok, r, ls);
   }
   if constexpr (TOP) {
-    key_t64 mine = 0;
+    const int top = a.top;
+    const uint4 g = sh.order[tid & 63];
+    const unsigned bound = largest_with(top, 31, 16, [&](unsigned mid) {
+      return lanes(g.x >= mid) + lanes(g.y >= mid) + lanes(g.z >= mid) + lanes(g.w >= mid);
+    });
+    // not below the bound as a number: a NaN is never below, and nothing is below a bound that
+    // is no number (an order of NaNs, or below that of -inf)
+    float from = value_of(bound);
+    int last = kPiece;  // of the logits equal to `from`, the ones up to here
+    bool nans = false;
+    int n[4];
+    // Every pass over the logits takes them and their indices anew: what the compiler would keep
+    // of one pass for the next (masks, orders, indices: 32 of each) costs the occupancy.
+    auto anew = [&](int& t4) {
+      asm volatile("" : "+v"(t4));
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        mine = max(mine, key_of(order_of(v[i][e]), begin + (tid + 256 * i) * 4 + e));
-    block_top(sh, a.top, mine,
-              [&](auto f) {
+        for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(v[i][e]));
+    };
+    auto gather = [&]() {  // into this wave's segment; false if one is too small
+      int at = 0, t4 = 4 * tid;
+      anew(t4);
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i)
 #pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    f(key_of(order_of(v[i][e]), begin + (tid + 256 * i) * 4 + e));
-              },
-              [&](int at, key_t64 key) {
-                if (a.pieces > 1) {
-                  a.keys[(long)blockIdx.x * a.top + at] = key;
-                } else {
-                  a.top_ids[(long)row * a.top + at] = (int)~(unsigned)key;
-                  a.top_logp[(long)row * a.top + at] =
-                      logp_of(r, ls, value_of((unsigned)(key >> 32)));
-                }
-              });
+        for (int e = 0; e < 4; ++e) {
+          const int k = t4 + 1024 * i + e;
+          const bool c = !(v[i][e] < from) && (!(v[i][e] == from) || k <= last);
+          const unsigned long long mask = __ballot(c);
+          if (mask) {
+            const int to = at + lanes_below(mask);
+            if (c && to < kSeg)
+              sh.cand[wave * kSeg + to] =
+                  key_of(nans ? 0xffffffffu : order_of(v[i][e]), begin + k);
+            at += __popcll(mask);
+          }
+        }
+      if ((tid & 63) == 0) sh.n[0][wave] = at;
+      __syncthreads();
+      bool fit = true;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        n[w] = sh.n[0][w];
+        fit &= n[w] <= kSeg;
+      }
+      return fit;
+    };
+    if (!gather()) {
+      // counts of all four waves, a barrier each
+      int turn = 1;
+      auto count = [&](auto f) {
+        int c = 0, t4 = 4 * tid;
+        anew(t4);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c += lanes(f(v[i][e], t4 + 1024 * i + e));
+        if ((tid & 63) == 0) sh.n[turn][wave] = c;
+        __syncthreads();
+        c = (sh.n[turn][0] + sh.n[turn][1]) + (sh.n[turn][2] + sh.n[turn][3]);
+        turn ^= 1;
+        return c;
+      };
+      nans = count([](float x, int) { return x != x; }) >= top;
+      if (nans) {
+        // NaNs alone, the lowest indices: as infinities, the rest as nothing
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[i][e] = v[i][e] != v[i][e] ? inf : -inf;
+      }
+      // orders up to that of +inf
+      const unsigned exact = largest_with(top, 31, 0, [&](unsigned mid) {
+        const float at = value_of(mid);
+        return mid > 0xff800000u ? 0 : count([&](float x, int) { return !(x < at); });
+      });
+      from = value_of(exact);
+      const int above = count([&](float x, int) { return !(x <= from); });
+      last = kPiece - 1 - (int)largest_with(top - above, 12, 0, [&](unsigned mid) {
+        return count([&](float x, int k) { return x == from && kPiece - 1 - k >= (int)mid; });
+      });
+      __syncthreads();  // the last counts are read
+      gather();
+    }
+    rank_keys<256, 4, kSeg>(sh.cand, n, top, [&](int at, key_t64 key) {
+      if (a.pieces > 1) {
+        a.keys[(long)blockIdx.x * top + at] = key;
+      } else {
+        a.top_ids[(long)row * top + at] = (int)~(unsigned)key;
+        a.top_logp[(long)row * top + at] = logp_of(r, ls, value_of((unsigned)(key >> 32)));
+      }
+    });
   }
 }
 
-__global__ __launch_bounds__(256) void logprob_join_kernel(LpArgs a) {
-  __shared__ LpShared sh;
-  const int tid = threadIdx.x, wave = tid >> 6, row = blockIdx.x;
+// The pieces of a row, one wave.  NR: keys a lane holds (0: any number, read again for each bit).
+template <int NR>
+__global__ __launch_bounds__(64) void logprob_join_kernel(LpArgs a) {
+  __shared__ key_t64 cand[kCand];
+  const int lane = threadIdx.x, row = blockIdx.x;
   const float4* part = a.part + (long)row * a.pieces;
   const float inf = __builtin_huge_valf();
+  const key_t64* keys = a.keys + (long)row * a.pieces * a.top;
+  const int n = a.pieces * a.top, each = (n + 63) / 64;
+  const Given tok = given(a, row);
+  key_t64 own[NR ? NR : 1];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) own[i] = lane + 64 * i < n ? keys[lane + 64 * i] : 0;
   float m = -inf;
-  for (int i = tid; i < a.pieces; i += 256) m = fmaxf(m, part[i].x);
+  for (int i = lane; i < a.pieces; i += 64) m = fmaxf(m, part[i].x);
   m = wave_max(m);
-  if ((tid & 63) == 0) sh.f[wave][0] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(sh.f[0][0], sh.f[1][0]), fmaxf(sh.f[2][0], sh.f[3][0]));
   float s = 0.0f, t = 0.0f, tops = 0.0f;
-  for (int i = tid; i < a.pieces; i += 256) {
+  for (int i = lane; i < a.pieces; i += 64) {
     const float4 p = part[i];
     if (p.x == m) {
       s += p.y;
@@ -258,38 +351,58 @@ __global__ __launch_bounds__(256) void logprob_join_kernel(LpArgs a) {
       t = fmaf(w, fmaf(1.0f + p.y, fmaxf(d, -200.0f), p.z), t);
     }
   }
-  s = wave_sum(s);
-  t = wave_sum(t);
-  tops = wave_sum(tops);
-  if ((tid & 63) == 0) {
-    sh.f[wave][1] = s;
-    sh.f[wave][2] = t;
-    sh.f[wave][3] = tops;
-  }
-  __syncthreads();
   RowSums r;
   r.m = m;
-  r.t = (sh.f[0][2] + sh.f[1][2]) + (sh.f[2][2] + sh.f[3][2]);
-  tops = (sh.f[0][3] + sh.f[1][3]) + (sh.f[2][3] + sh.f[3][3]);
-  r.s = (sh.f[0][1] + sh.f[1][1]) + (sh.f[2][1] + sh.f[3][1]);
+  r.t = wave_sum(t);
+  r.s = wave_sum(s);
+  tops = wave_sum(tops);
   if (m != -inf) r.s += tops - 1.0f;
   const float ls = log1pf(r.s);
-  if (tid == 0) write_row(a, row, r, ls);
-  if (a.top) {
-    const key_t64* keys = a.keys + (long)row * a.pieces * a.top;
-    const int n = a.pieces * a.top;
-    key_t64 mine = 0;
-    for (int i = tid; i < n; i += 256) mine = max(mine, keys[i]);
-    block_top(sh, a.top, mine,
-              [&](auto f) {
-                for (int i = tid; i < n; i += 256) f(keys[i]);
-              },
-              [&](int at, key_t64 key) {
-                a.top_ids[(long)row * a.top + at] = (int)~(unsigned)key;
-                a.top_logp[(long)row * a.top + at] =
-                    logp_of(r, ls, value_of((unsigned)(key >> 32)));
-              });
+  if (lane == 0) write_row(a, row, tok, r, ls);
+  if (!a.top) return;
+  // every lane calls f with `each` keys, 0 for none
+  auto all = [&](auto f) {
+    if constexpr (NR) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i) f(own[i]);
+    } else {
+      for (int i = 0; i < each; ++i) f(lane + 64 * i < n ? keys[lane + 64 * i] : 0);
+    }
+  };
+  auto count = [&](auto f) {
+    int c = 0;
+    all([&](key_t64 key) { c += lanes(f(key)); });
+    return c;
+  };
+  auto with = [&](unsigned mid) {
+    return count([&](key_t64 key) { return (unsigned)(key >> 32) >= mid; });
+  };
+  unsigned order = largest_with(a.top, 31, 16, with);
+  key_t64 bound = (key_t64)order << 32;
+  int c = with(order);
+  if (c > kCand) {  // crowded: the exact order, and of its ties the lowest indices, 24 bits of them
+    order = largest_with(a.top, 31, 0, with);
+    const int above = count([&](key_t64 key) { return (unsigned)(key >> 32) > order; });
+    bound = (key_t64)order << 32 | 0xff000000u;
+    bound |= largest_with(a.top - above, 23, 0, [&](unsigned mid) {
+      const key_t64 from = bound | mid;
+      return count([&](key_t64 key) { return key >= from && (unsigned)(key >> 32) == order; });
+    });
+    c = a.top;
   }
+  int at = 0;
+  all([&](key_t64 key) {
+    const bool in = key >= bound;
+    const unsigned long long mask = __ballot(in);
+    if (in) cand[at + lanes_below(mask)] = key;
+    at += __popcll(mask);
+  });
+  __syncthreads();
+  const int in_all[1] = {c};
+  rank_keys<64, 1, kCand>(cand, in_all, a.top, [&](int place, key_t64 key) {
+    a.top_ids[(long)row * a.top + place] = (int)~(unsigned)key;
+    a.top_logp[(long)row * a.top + place] = logp_of(r, ls, value_of((unsigned)(key >> 32)));
+  });
 }
 
 int lp_pieces(int V) { return (V + kPiece - 1) / kPiece; }
@@ -359,6 +472,12 @@ extern "C" int lx_token_logprobs_f32(const float* logits, long ld, int rows, int
     launch_logprob<false>(a, rows, stream);
   LX_TRY(check_launch("logprob_kernel"));
   if (a.pieces == 1) return LX_OK;
-  hipLaunchKernelGGL(logprob_join_kernel, dim3((unsigned)rows), dim3(256), 0, stream, a);
+  const dim3 grid((unsigned)rows), block(64);
+  if (a.pieces * a.top <= 8 * 64)
+    hipLaunchKernelGGL(logprob_join_kernel<8>, grid, block, 0, stream, a);
+  else if (a.pieces * a.top <= 20 * 64)
+    hipLaunchKernelGGL(logprob_join_kernel<20>, grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL(logprob_join_kernel<0>, grid, block, 0, stream, a);
   return check_launch("logprob_join_kernel");
 }

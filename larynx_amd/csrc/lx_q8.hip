@@ -196,7 +196,7 @@ using namespace lx;
 
 extern "C" size_t lx_q8_bytes(int rows, int K) {
   if (!q8_shape_ok(rows, K)) return 0;
-  return q8_code_bytes(rows, K) + (size_t)q8_tiles(rows) * ((q8_blocks(K) + 3) / 4) * 64;
+  return q8_code_bytes(rows, K) + (size_t)q8_tiles(rows) * q8_blocks(K) * kQ8Rows;
 }
 
 namespace {

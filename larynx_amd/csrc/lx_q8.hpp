@@ -3,18 +3,16 @@
 // Blocks of 128 consecutive elements of a row share 2^e, e the smallest integer >= -127 with
 // max|v| <= 448 * 2^e over the finite ones; a code is the e4m3 number nearest to v / 2^e (exact
 // but for that one rounding: a power of two, and v_cvt_pk_fp8_f32 rounds to nearest even).  The
-// scales are e8m0 bytes e + 127, which the block-scaled matrix instructions of gfx950 take beside
-// the codes, so that a product costs no instruction for its scales.
+// scales are held as bytes e + 127, the exponent field of 2^e.
 //
 // Memory: tiles of 16 rows x 128 elements, 2 KB each, the blocks of K of a row tile side by side.
 // A row's 128 bytes are one line, so that its producer writes whole lines; its eight 16-byte
 // chunks stand at chunk ^ (row / 2 % 8), which spreads the 16 rows that a ds_read_b128 of a
 // fragment touches over all 64 banks: tiles go to LDS as they lie.  (In the lanes' order, the other
-// layout free of conflicts, a row's block is eight pieces in as many lines.)  A fragment of
-// v_mfma_scale_f32_16x16x128_f8f6f4 holds row lane % 16, chunks lane / 16 and lane / 16 + 4: which
-// 32 of the 128 elements a lane multiplies does not matter while both operands agree and a block has
-// one scale.  Behind the codes the scales: per row tile and four blocks 64 bytes, a dword with
-// four blocks' scales per row.
+// layout free of conflicts, a row's block is eight pieces in as many lines.)  Which
+// elements of a block a lane multiplies in one instruction does not matter while both operands
+// agree and a block has one scale: a lane takes 16-byte chunks.  Behind the codes the scales, a byte a row: 16 bytes per tile, tiles in the
+// same order.
 // Elements past the end of a row are zero; rows past the last may hold anything and only reach
 // outputs that are not stored.
 #pragma once
@@ -36,7 +34,7 @@ inline size_t q8_code_bytes(long rows, long K) {
 struct Q8Mat {
   unsigned char* codes;
   unsigned char* scales;
-  int rows, K, kb, kb4;  // kb blocks of K, kb4 dwords of scales per row
+  int rows, K, kb;  // kb blocks of K
 };
 
 inline bool q8_shape_ok(int rows, int K) {
@@ -48,7 +46,7 @@ inline bool q8_ok(const lx_q8* q) {
 inline Q8Mat q8_mat(const lx_q8* q) {
   unsigned char* p = static_cast<unsigned char*>(q->data);
   const int kb = (int)q8_blocks(q->K);
-  return Q8Mat{p, p + q8_code_bytes(q->rows, q->K), q->rows, q->K, kb, (kb + 3) / 4};
+  return Q8Mat{p, p + q8_code_bytes(q->rows, q->K), q->rows, q->K, kb};
 }
 
 // Byte offset of element k (of its chunk, for k a multiple of 16) of a row.
@@ -58,7 +56,7 @@ __device__ __forceinline__ long q8_at(const Q8Mat& q, int row, int k) {
          ((((k >> 4) & 7) ^ (r >> 1)) << 4) + (k & 15);
 }
 __device__ __forceinline__ long q8_scale_at(const Q8Mat& q, int row, int kb) {
-  return ((long)(row >> 4) * q.kb4 + (kb >> 2)) * 64 + (row & 15) * 4 + (kb & 3);
+  return ((long)(row >> 4) * q.kb + kb) * kQ8Rows + (row & 15);
 }
 
 // The e8m0 byte of a block whose largest finite magnitude is `top`: 448 = 1.75 * 2^8.

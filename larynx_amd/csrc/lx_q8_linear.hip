@@ -1,6 +1,7 @@
 // y = epi(x~ W~^T + bias), both operands in 8 bits with a power of two per block of 128 (lx_q8.hpp).
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "lx_q8.hpp"
 
@@ -8,6 +9,10 @@ namespace lx {
 namespace {
 
 typedef int intx4 __attribute__((ext_vector_type(4)));
+// floats at a 4-byte boundary: y, bias and resid need no other (their vectors reach memory in one
+// instruction on gfx950 all the same; rows of an odd N by single floats cost 30%)
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float float2u __attribute__((ext_vector_type(2), aligned(4)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
@@ -17,7 +22,7 @@ struct Q8Lin {
   const float* resid;
   float* y;
   long ldr, ldy;
-  int epi, vec;
+  int epi;
   int tiles_m, tiles_n;  // of the launch
 };
 
@@ -36,18 +41,18 @@ __device__ __forceinline__ void epi_one(const Q8Lin& a, int m, long n, float v, 
 // Columns n .. n + 3 (n a multiple of 4) of row m.
 __device__ __forceinline__ void epi_quad(const Q8Lin& a, int m, long n, floatx4 v) {
   if (m >= a.x.rows) return;
-  if (a.vec && n + 3 < a.w.rows) {
-    if (a.bias) v += *reinterpret_cast<const floatx4*>(a.bias + n);
+  if (n + 3 < a.w.rows) {
+    if (a.bias) v += *reinterpret_cast<const float4u*>(a.bias + n);
     if (a.epi == LX_EPI_SWIGLU_PAIRED) {
-      *reinterpret_cast<float2*>(a.y + m * a.ldy + (n >> 1)) =
-          make_float2((v[0] / (1.0f + expf(-v[0]))) * v[1], (v[2] / (1.0f + expf(-v[2]))) * v[3]);
+      *reinterpret_cast<float2u*>(a.y + m * a.ldy + (n >> 1)) = float2u{
+          (v[0] / (1.0f + expf(-v[0]))) * v[1], (v[2] / (1.0f + expf(-v[2]))) * v[3]};
       return;
     }
     if (a.epi == LX_EPI_GELU_TANH)
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = gelu_tanh(v[e]);
-    if (a.epi == LX_EPI_RESID) v = *reinterpret_cast<const floatx4*>(a.resid + m * a.ldr + n) + v;
-    *reinterpret_cast<floatx4*>(a.y + m * a.ldy + n) = v;
+    if (a.epi == LX_EPI_RESID) v = *reinterpret_cast<const float4u*>(a.resid + m * a.ldr + n) + v;
+    *reinterpret_cast<float4u*>(a.y + m * a.ldy + n) = v;
     return;
   }
   const int step = a.epi == LX_EPI_SWIGLU_PAIRED ? 2 : 1;
@@ -93,20 +98,20 @@ __global__ __launch_bounds__(64 * WAVES) void q8_stream_kernel(Q8Lin a) {
   for (int kb = wave; kb < a.x.kb; kb += WAVES) {
     intx4 xf[MT][2], wf[NT][2];
     float xs[MT], ws[NT];
-    const int so = (kb >> 2) * 64 + r * 4 + (kb & 3);
+    const int so = kb * 16 + r;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const unsigned char* p = a.w.codes + (wt[i] * a.w.kb + kb) * kQ8Tile;
       wf[i][0] = *reinterpret_cast<const intx4*>(p + at);
       wf[i][1] = *reinterpret_cast<const intx4*>(p + (at ^ 64));
-      ws[i] = __uint_as_float((unsigned)a.w.scales[wt[i] * a.w.kb4 * 64 + so] << 23);
+      ws[i] = __uint_as_float((unsigned)a.w.scales[wt[i] * a.w.kb * 16 + so] << 23);
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const unsigned char* p = a.x.codes + (xt[i] * a.x.kb + kb) * kQ8Tile;
       xf[i][0] = *reinterpret_cast<const intx4*>(p + at);
       xf[i][1] = *reinterpret_cast<const intx4*>(p + (at ^ 64));
-      xs[i] = __uint_as_float((unsigned)a.x.scales[xt[i] * a.x.kb4 * 64 + so] << 23);
+      xs[i] = __uint_as_float((unsigned)a.x.scales[xt[i] * a.x.kb * 16 + so] << 23);
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -136,6 +141,236 @@ __global__ __launch_bounds__(64 * WAVES) void q8_stream_kernel(Q8Lin a) {
     const int m = (u >> 6) % MT, n = (u >> 6) / MT, l = u & 63;
     epi_quad(a, (mt * MT + m) * 16 + (l & 15), (long)(nt * NT + n) * 16 + 4 * (l >> 4), s);
   }
+}
+
+// Many rows.  A workgroup owns (32 RB WM) x (32 CB WN) outputs; both operands go through LDS as they
+// lie in memory (no registers, no ds_write), a block of K a stage, NS stages deep.  WK waves share
+// each (32 RB) x (32 CB) of the outputs, taking 128 / WK of a stage's 128 each: a wave's tile is as
+// large as its registers hold, since what a tile costs beside its products is the conversion of
+// its operands (8 cycles for 128 codes; an instruction of 32 x 32 x 16 takes 32).
+// A step is 16 of K; while its products run, the next step's codes are converted, and those of
+// the step after are on their way from LDS.  The one barrier of a stage stands before its last two
+// steps, whose operands every wave has by then: the buffer is free for the stage NS further on, and
+// the next stage's first reads return behind those steps' products.
+template <int N>
+__device__ __forceinline__ void wait_vm() {  // vmcnt(N) lgkmcnt(0)
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4 & 3) << 14 | 7 << 4);
+}
+
+template <int RB, int CB, int WM, int WN, int WK, int NS>
+struct TileShape {
+  static constexpr int WAVES = WM * WN * WK;
+  static constexpr int XT = 2 * RB * WM, WT = 2 * CB * WN;  // 16-row tiles of a stage
+  static constexpr int PIECES = (XT + WT) * 2;              // 1 KB each, of a stage
+  static constexpr int CHUNKS = (PIECES + WAVES - 1) / WAVES;  // a wave's; the last repeat
+  static_assert(XT + WT <= 16 * WAVES, "a wave loads the scales of 16 tiles");
+  static constexpr int SCALES = WAVES * CHUNKS * 1024;  // of a stage, then 256 bytes a wave
+  static constexpr int STAGE = SCALES + 256 * WAVES;
+  static constexpr int ROW = 32 * CB + 4;  // floats of a row of outputs in LDS
+  static constexpr int OUT = 32 * ROW * 4;  // a wave's 32 rows
+  static constexpr int LDS = NS * STAGE > WAVES * OUT ? NS * STAGE : WAVES * OUT;
+  static_assert(LDS <= 160 * 1024, "LDS of a CU");
+  static_assert((NS - 2) * (CHUNKS + 1) < 64, "vmcnt");
+};
+
+template <int RB, int CB, int WM, int WN, int WK, int NS, int OCC>
+__global__ __launch_bounds__(64 * WM * WN * WK, OCC) void q8_tile_kernel(Q8Lin a) {
+  using S = TileShape<RB, CB, WM, WN, WK, NS>;
+  constexpr int XT = S::XT, WT = S::WT, CHUNKS = S::CHUNKS, SPW = 4 / WK;
+  extern __shared__ __attribute__((aligned(16))) unsigned char sm[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wk = wave % WK, wm = wave / WK % WM, wn = wave / (WK * WM);
+  // each XCD (workgroups are dealt to them round-robin) takes a contiguous run of tiles
+  int id = blockIdx.x;
+  {
+    const int full = gridDim.x / 8 * 8;
+    if (id < full) id = (id % 8) * (full / 8) + id / 8;
+  }
+  const int mt = id % a.tiles_m, nt = id / a.tiles_m;
+  const int mtiles = (a.x.rows + 15) / 16, ntiles = (a.w.rows + 15) / 16;
+  const int kb = a.x.kb;
+  // tile t of a stage: rows of x, then of W; past the last it repeats that
+  auto tile_of = [&](int t) {
+    return t < XT ? min(mt * XT + t, mtiles - 1) : min(nt * WT + min(t - XT, WT - 1), ntiles - 1);
+  };
+  const unsigned char* src[CHUNKS];
+#pragma unroll
+  for (int j = 0; j < CHUNKS; ++j) {
+    const int c = wave * CHUNKS + j, t = c >> 1;
+    src[j] = (t < XT ? a.x.codes : a.w.codes) + (long)tile_of(t) * kb * kQ8Tile + (c & 1) * 1024 +
+             lane * 16;
+  }
+  const unsigned char* ssrc;
+  {
+    const int t = wave * 16 + (lane >> 2);
+    ssrc = (t < XT ? a.x.scales : a.w.scales) + (long)tile_of(t) * kb * 16 + (lane & 3) * 4;
+  }
+  typedef const __attribute__((address_space(1))) void* global_ptr;
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  auto load = [&](int k, int buf) {
+    unsigned char* d = sm + buf * S::STAGE;
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j)
+      __builtin_amdgcn_global_load_lds((global_ptr)(src[j] + (long)k * kQ8Tile),
+                                       (lds_ptr)(d + (wave * CHUNKS + j) * 1024), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((global_ptr)(ssrc + (long)k * 16),
+                                     (lds_ptr)(d + S::SCALES + wave * 256), 4, 0, 0);
+  };
+  const int r = lane & 15, h = lane >> 5, half = (lane >> 4) & 1;
+  int at[SPW];
+#pragma unroll
+  for (int s = 0; s < SPW; ++s)
+    at[s] = half * kQ8Tile + r * kQ8Block + (((2 * (wk * SPW + s) + h) ^ (r >> 1)) << 4);
+  floatx16 acc[CB][RB];
+#pragma unroll
+  for (int n = 0; n < CB; ++n)
+#pragma unroll
+    for (int m = 0; m < RB; ++m)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[n][m][e] = 0.0f;
+
+  intx4 raw[2][RB + CB];
+  bf16x8_t frag[2][RB + CB];
+  float scale[RB + CB];
+  auto read = [&](intx4 (&f)[RB + CB], int buf, int s) {
+    const unsigned char* b = sm + buf * S::STAGE + at[s];
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+      f[i] = *reinterpret_cast<const intx4*>(b + (wm * RB + i) * 2 * kQ8Tile);
+#pragma unroll
+    for (int i = 0; i < CB; ++i)
+      f[RB + i] = *reinterpret_cast<const intx4*>(b + (XT + (wn * CB + i) * 2) * kQ8Tile);
+  };
+  auto read_scales = [&](unsigned (&u)[RB + CB], int buf) {
+    const unsigned char* b = sm + buf * S::STAGE + S::SCALES + half * 16 + r;
+#pragma unroll
+    for (int i = 0; i < RB; ++i) u[i] = b[(wm * RB + i) * 32];
+#pragma unroll
+    for (int i = 0; i < CB; ++i) u[RB + i] = b[(XT + (wn * CB + i) * 2) * 16];
+  };
+  auto convert = [&](bf16x8_t (&f)[RB + CB], const intx4 (&u)[RB + CB], int t) {
+#pragma unroll
+    for (int i = 0; i < RB + CB; ++i) f[i] = q8_frag(u[i][2 * t], u[i][2 * t + 1], scale[i]);
+  };
+  // stage k is in LDS (NS - 2 later ones may be on their way), and this wave's reads are done
+  auto wait = [&](int k) {
+    if (k + NS - 2 < kb)
+      wait_vm<(NS - 2) * (CHUNKS + 1)>();
+    else
+      wait_vm<0>();
+  };
+#pragma unroll
+  for (int k = 0; k < NS; ++k)
+    if (k < kb) load(k, k);
+  wait(0);
+  __syncthreads();
+  unsigned us[RB + CB];
+  read_scales(us, 0);
+  read(raw[0], 0, 0);
+#pragma unroll
+  for (int i = 0; i < RB + CB; ++i) scale[i] = __uint_as_float(us[i] << 23);
+  convert(frag[0], raw[0], 0);
+  int buf = 0;
+  // one stage; raw[P] holds its first operands
+  auto stage = [&](int k, auto parity) {
+    constexpr int P = decltype(parity)::value;
+    const int next = buf + 1 == NS ? 0 : buf + 1;
+#pragma unroll
+    for (int u = 0; u < 2 * SPW; ++u) {
+      const int s = u >> 1, t = u & 1;
+      if (u == 2 * SPW - 2) {
+        // the conversions so far stay in front of the branches, beside their step's products
+#pragma unroll
+        for (int i = 0; i < RB + CB; ++i) asm volatile("" : "+v"(frag[0][i]));
+        if (k + 1 < kb) wait(k + 1);
+        __builtin_amdgcn_s_barrier();
+        if (k + NS < kb) load(k + NS, buf);
+        read_scales(us, next);
+        read(raw[(P + s + 1) & 1], next, 0);  // past the last stage: bytes of a buffer, not used
+      } else if (t == 0) {
+        read(raw[(P + s + 1) & 1], buf, s + 1);
+      }
+      if (u == 2 * SPW - 1)
+#pragma unroll
+        for (int i = 0; i < RB + CB; ++i) scale[i] = __uint_as_float(us[i] << 23);
+      convert(frag[(u + 1) & 1], raw[(P + s + t) & 1], t ^ 1);
+#pragma unroll
+      for (int n = 0; n < CB; ++n)
+#pragma unroll
+        for (int m = 0; m < RB; ++m)
+          acc[n][m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag[u & 1][RB + n], frag[u & 1][m],
+                                                              acc[n][m], 0, 0, 0);
+      constexpr int CV = (4 * (RB + CB) + RB * CB - 1) / (RB * CB);
+      if (t == 0) __builtin_amdgcn_sched_group_barrier(0x100, RB + CB, 0);
+      if (u == 2 * SPW - 2) __builtin_amdgcn_sched_group_barrier(0x100, RB + CB, 0);
+#pragma unroll
+      for (int i = 0; i < RB * CB; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, CV, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    buf = next;
+  };
+#pragma unroll 1
+  for (int k = 0; k < kb; k += SPW & 1 ? 2 : 1) {
+    stage(k, std::integral_constant<int, 0>{});
+    if ((SPW & 1) && k + 1 < kb) stage(k + 1, std::integral_constant<int, SPW & 1>{});
+  }
+  // outputs through LDS, 32 rows a wave at a time: the WK waves' sums meet there, and stores are
+  // whole lines of y
+  float* out = reinterpret_cast<float*>(sm + (wave - wk) * S::OUT);
+#pragma unroll
+  for (int m = 0; m < RB; ++m) {
+    if (m == 0 || WK > 1) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+#pragma unroll
+    for (int n = 0; n < CB; ++n)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<floatx4*>(out + wk * S::OUT / 4 + (lane & 31) * S::ROW + 32 * n + 8 * q +
+                                    4 * h) =
+            floatx4{acc[n][m][4 * q], acc[n][m][4 * q + 1], acc[n][m][4 * q + 2],
+                    acc[n][m][4 * q + 3]};
+    if (WK > 1) {
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    constexpr int QUADS = 32 * 8 * CB / WK;  // of this wave
+#pragma unroll 2
+    for (int i = lane; i < QUADS; i += 64) {
+      const int e = wk * QUADS + i, row = e / (8 * CB), col = e % (8 * CB) * 4;
+      const float* p = out + row * S::ROW + col;
+      floatx4 v = *reinterpret_cast<const floatx4*>(p);
+#pragma unroll
+      for (int w = 1; w < WK; ++w) v += *reinterpret_cast<const floatx4*>(p + w * S::OUT / 4);
+      epi_quad(a, mt * XT * 16 + (wm * RB + m) * 32 + row, (long)nt * WT * 16 + wn * CB * 32 + col,
+               v);
+    }
+  }
+}
+
+template <int RB, int CB, int WM, int WN, int WK, int NS, int OCC>
+int launch_tile(Q8Lin& a, hipStream_t s) {
+  using S = TileShape<RB, CB, WM, WN, WK, NS>;
+  const auto kern = q8_tile_kernel<RB, CB, WM, WN, WK, NS, OCC>;
+  static LdsLimit once;
+  LX_TRY(raise_lds_limit(reinterpret_cast<const void*>(kern), S::LDS, once, "q8_tile_kernel"));
+  a.tiles_m = (a.x.rows + 32 * RB * WM - 1) / (32 * RB * WM);
+  a.tiles_n = (a.w.rows + 32 * CB * WN - 1) / (32 * CB * WN);
+  const long grid = (long)a.tiles_m * a.tiles_n;
+  LX_REQUIRE(grid <= INT_MAX / (64 * S::WAVES), "linear_q8: %d x %d outputs are too many",
+             a.x.rows, a.w.rows);
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * S::WAVES), S::LDS, s, a);
+  return check_launch("q8_tile_kernel");
 }
 
 template <int MT, int NT, int WAVES>
@@ -190,8 +425,24 @@ extern "C" int lx_linear_q8_f32(const lx_q8* x, const lx_q8* w, const float* bia
   a.ldr = ldr;
   a.ldy = ldy;
   a.epi = kind;
-  a.vec = ldy % 4 == 0 && ldr % 4 == 0 &&
-          ((uintptr_t)y | (uintptr_t)bias | (uintptr_t)resid) % 16 == 0;
-  if (M <= 16) return launch_stream<1, 1, 8>(a, stream);
-  return launch_stream<4, 4, 4>(a, stream);
+  if (M <= 16) {
+    // 16 columns of y a workgroup, 32 where there are thousands of them (8192 x 8192 14.8 -> 12.7
+    // us; 9728 x 896 3.8 and 3.9)
+    if ((long)N * a.w.kb >= 1 << 18) return launch_stream<1, 2, 8>(a, stream);
+    return launch_stream<1, 1, 8>(a, stream);
+  }
+  // The largest tiles that still give (nearly) every CU one; us, in the order of the tiles below:
+  //   4096 x 6761 x 896      73.7  81.4  95.6 112.5       4096 x 896 x 896  28.0  14.4  16.9  16.8
+  //   1000 x 6761 x 896      32.1  21.5  23.3  28.4        400 x 6761       30.7  15.5  12.5  14.7
+  //   1531 x 1152 x 896      27.5  12.3   9.5  10.6  10.8
+  //    177 x 6761 x 896      30.0  14.1   9.2   8.4  10.0
+  //    200 x 1500 x 3000     67.8  25.6  11.7   9.2  10.3
+  //    150 x  896 x 4864     99.6  35.5  15.9  12.1   8.9
+  const long cus = device_cus();
+  auto tiles = [&](long m, long n) { return ((M + m - 1) / m) * ((N + n - 1) / n); };
+  if (8 * tiles(256, 256) >= 7 * cus) return launch_tile<4, 2, 2, 4, 1, 2, 1>(a, stream);
+  if (8 * tiles(128, 128) >= 7 * cus) return launch_tile<2, 2, 2, 2, 1, 2, 2>(a, stream);
+  if (2 * tiles(64, 64) >= 3 * cus) return launch_tile<2, 2, 1, 1, 4, 3, 3>(a, stream);
+  if (8 * tiles(32, 64) >= 5 * cus) return launch_tile<1, 2, 1, 1, 4, 4, 3>(a, stream);
+  return launch_stream<2, 2, 8>(a, stream);
 }

@@ -7,13 +7,14 @@ layout; work is enqueued on torch's current stream.  Every call goes through
 liblxops.so; a failing call raises LxError (no fallback path exists).
 """
 import ctypes as C
+import struct
 from typing import NamedTuple, Optional
 
 import torch
 
 from ._lib import (LX_BX_OUT_F32, LX_BX_OUT_PACKED, LX_BX_OUT_PARTIAL, LX_EPI_GATED_RESID,
                    LX_EPI_GELU_TANH, LX_EPI_NONE, LX_EPI_RESID, LX_EPI_ROPE_PARTIAL,
-                   LX_EPI_SWIGLU_PAIRED, Q8, Epilogue, Kv4, LinearBx, check, lib)
+                   LX_EPI_SWIGLU_PAIRED, Epilogue, Kv4, LinearBx, check, lib)
 
 __all__ = [
     "stream", "ada_ln", "adaln_resid", "adaln_emb", "rope_partial", "gelu_tanh", "gated_residual",
@@ -533,16 +534,21 @@ def attention_kv4(q, cache, lens, n_heads, scale=None, causal=True, out=None, ma
 class Q8Matrix:
     """A matrix (rows, K) in 8 bits: e4m3 codes with a power of two per 128 elements of a row, as
     q8_pack and rms_norm_q8 lay them out in `data`."""
-    __slots__ = ("data", "rows", "K", "_dev", "_c", "_ref")
+    __slots__ = ("data", "rows", "K", "_dev", "_ref")
 
     def __init__(self, data, rows, K):
-        self.data, self.rows, self.K = data, rows, K
-        self._dev = data.get_device()
-        self._c = Q8(data.data_ptr(), rows, K)
-        self._ref = C.byref(self._c)
         n = lib.lx_q8_bytes(rows, K)
         if not n or data.dtype is not torch.uint8 or not data.is_contiguous() or data.numel() != n:
             raise ValueError(f"not the 8-bit form of a ({rows}, {K}) matrix")
+        self._set(data, rows, K)
+
+    def _set(self, data, rows, K):
+        self.data, self.rows, self.K, self._dev = data, rows, K, data.get_device()
+        self._ref = _pack_q8(data.data_ptr(), rows, K)  # an lx_q8: a ctypes one takes 0.5 us
+        return self
+
+
+_pack_q8 = struct.Struct("@Pii").pack
 
 
 def _q8_out(like, rows, K, out):
@@ -550,7 +556,7 @@ def _q8_out(like, rows, K, out):
         n = lib.lx_q8_bytes(rows, K)
         if not n:
             raise ValueError(f"no 8-bit form of a ({rows}, {K}) matrix")
-        return Q8Matrix(like.new_empty(n, dtype=torch.uint8), rows, K)
+        return Q8Matrix.__new__(Q8Matrix)._set(like.new_empty(n, dtype=torch.uint8), rows, K)
     if out.rows != rows or out.K != K:
         raise ValueError(f"out must hold a ({rows}, {K}) matrix")
     if out._dev != like.get_device():
@@ -559,32 +565,46 @@ def _q8_out(like, rows, K, out):
 
 
 def _matrix(t, name):
-    """Row stride of the fp32 matrix t on the current device, its rows contiguous."""
-    if t.dim() != 2:
+    """Rows, columns, row stride and device of the fp32 matrix t on the current device, its rows
+    contiguous."""
+    shape = t.shape
+    if len(shape) != 2:
         raise ValueError(f"{name} must be 2-dimensional")
-    ld = _rows(t, name, t.shape)
+    rows, cols = shape
+    ld = cols if t.dtype is _F32 and t.is_contiguous() else _rows(t, name, shape)
     dev = t.get_device()
     if dev < 0 or dev != _current():
         _elsewhere(name)
-    return ld
+    return rows, cols, ld, dev
+
+
+def _like(t, name, shape, dev):
+    """Row stride of the fp32 matrix t of `shape` on device dev."""
+    if t.get_device() != dev:
+        _elsewhere(name)
+    if t.dtype is _F32 and t.is_contiguous() and t.shape == shape:
+        return shape[-1]
+    return _rows(t, name, shape)
 
 
 def q8_pack(x, out=None):
     """x (rows, K) fp32 (row stride may exceed K) -> Q8Matrix, a weight or activations: blocks of
     128 elements of a row share 2^e, e the smallest integer >= -127 with max|v| <= 448 * 2^e; codes
     are the nearest e4m3 numbers to v / 2^e.  Infinities and NaN stand for NaN."""
-    ld = _matrix(x, "x")
-    q = _q8_out(x, *x.shape, out)
-    check(lib.lx_q8_pack_f32(x.data_ptr(), ld, q._ref, _raw_stream(q._dev)))
+    rows, K, ld, dev = _matrix(x, "x")
+    q = _q8_out(x, rows, K, out)
+    check(lib.lx_q8_pack_f32(x.data_ptr(), ld, q._ref, _raw_stream(dev)))
     return q
 
 
 def q8_unpack(q):
     """The fp32 (rows, K) matrix that a Q8Matrix stands for."""
-    if q._dev < 0 or q._dev != _current():
+    dev = q._dev
+    if dev < 0 or dev != _current():
         _elsewhere("q")
-    x = q.data.new_empty((q.rows, q.K), dtype=_F32)
-    check(lib.lx_q8_unpack_f32(q._ref, x.data_ptr(), q.K, _raw_stream(q._dev)))
+    K = q.K
+    x = q.data.new_empty((q.rows, K), dtype=_F32)
+    check(lib.lx_q8_unpack_f32(q._ref, x.data_ptr(), K, _raw_stream(dev)))
     return x
 
 
@@ -592,9 +612,7 @@ def rms_norm_q8(x, w, eps=1e-6, add=None, sum_out=None, out=None):
     """RMSNorm of x (rows, K), after add (rows, K) if given, as a Q8Matrix (`out` or a new one): h =
     x + add goes to sum_out (default: x, in place), h / sqrt(mean(h^2) + eps) * w to the codes,
     formed in 64 bits.  src/llm/ops.cpp:7-11, src/llm/llm.cpp:141-173."""
-    ldx = _matrix(x, "x")
-    rows, K = x.shape
-    dev = x.get_device()
+    rows, K, ldx, dev = _matrix(x, "x")
     if w.dtype is not _F32 or w.numel() != K or not w.is_contiguous():
         raise ValueError(f"w must be {K} contiguous float32 values")
     if w.get_device() != dev:
@@ -604,9 +622,8 @@ def rms_norm_q8(x, w, eps=1e-6, add=None, sum_out=None, out=None):
     if add is not None:
         if sum_out is None:
             sum_out = x
-        lda, lds = _rows(add, "add", x.shape), _rows(sum_out, "sum_out", x.shape)
-        if add.get_device() != dev or sum_out.get_device() != dev:
-            _elsewhere("add, as sum_out,")
+        lda = _like(add, "add", x.shape, dev)
+        lds = ldx if sum_out is x else _like(sum_out, "sum_out", x.shape, dev)
         pa, ps = add.data_ptr(), sum_out.data_ptr()
     elif sum_out is not None:
         raise ValueError("sum_out without add")
@@ -635,9 +652,7 @@ def linear_q8(x, w, b=None, epilogue=None, resid=None, out=None):
             _elsewhere("b")
         bias = b.data_ptr()
     if resid is not None:
-        ldr = _rows(resid, "resid", (M, cols))
-        if resid.get_device() != dev:
-            _elsewhere("resid")
+        ldr = _like(resid, "resid", (M, cols), dev)
         pr = resid.data_ptr()
     if out is None:
         if kind == LX_EPI_RESID and resid is None:
@@ -645,9 +660,7 @@ def linear_q8(x, w, b=None, epilogue=None, resid=None, out=None):
         out = x.data.new_empty((M, cols), dtype=_F32)
         ldy = cols
     else:
-        ldy = _rows(out, "out", (M, cols))
-        if out.get_device() != dev:
-            _elsewhere("out")
+        ldy = _like(out, "out", (M, cols), dev)
     check(lib.lx_linear_q8_f32(x._ref, w._ref, bias,
                                None if epilogue is None else C.byref(epilogue), pr, ldr,
                                out.data_ptr(), ldy, _raw_stream(dev)))
@@ -667,9 +680,7 @@ def token_logprobs(logits, tokens=None, top=0, entropy=True):
     int32 (rows); -1: padding, 0), the distribution's entropy, and the `top` (at most 64) most
     likely ids with their log probabilities, equal logits by the lower id.  Logits of -inf are
     masked.  Scores the head's output, src/llm/llm.cpp:206-216."""
-    ld = _matrix(logits, "logits")
-    rows, V = logits.shape
-    dev = logits.get_device()
+    rows, V, ld, dev = _matrix(logits, "logits")
     logp = pt = pl = pe = ptl = pti = ent = tl = ti = None
     if tokens is not None:
         if tokens.dtype is not _I32 or tokens.numel() != rows or not tokens.is_contiguous():
@@ -685,8 +696,12 @@ def token_logprobs(logits, tokens=None, top=0, entropy=True):
         tl = logits.new_empty((rows, top))
         ti = logits.new_empty((rows, top), dtype=_I32)
         ptl, pti = tl.data_ptr(), ti.data_ptr()
-    n = lib.lx_token_logprobs_ws_floats(rows, V, top)
-    ws = logits.new_empty(n) if n else None
-    check(lib.lx_token_logprobs_f32(logits.data_ptr(), ld, rows, V, pt, pl, pe, top, ptl, pti,
-                                    ws.data_ptr() if n else None, n, _raw_stream(dev)))
+    n, ws, pw = 0, None, None
+    if V > 8192:
+        n = lib.lx_token_logprobs_ws_floats(rows, V, top)
+        if n:
+            ws = logits.new_empty(n)
+            pw = ws.data_ptr()
+    check(lib.lx_token_logprobs_f32(logits.data_ptr(), ld, rows, V, pt, pl, pe, top, ptl, pti, pw,
+                                    n, _raw_stream(dev)))
     return TokenLogprobs(logp, ent, tl, ti)

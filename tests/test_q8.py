@@ -29,12 +29,12 @@ def test_reference_is_the_format():
 
 
 def test_sizes():
-    # codes: tiles of 16 rows x 128 elements at 2 KB; 64 bytes of scales per tile row and 4 blocks
-    assert lib.lx_q8_bytes(1152, 896) == 72 * (7 * 2048 + 2 * 64)
-    assert lib.lx_q8_bytes(1, 1) == 2048 + 64
-    assert lib.lx_q8_bytes(17, 129) == 2 * (2 * 2048 + 64)
-    assert lib.lx_q8_bytes(151936, 8192) == 9496 * (64 * 2048 + 16 * 64)
-    assert lib.lx_q8_bytes(1 << 22, 8192) == (1 << 18) * (64 * 2048 + 16 * 64)  # past 32 bits
+    # tiles of 16 rows x 128 elements at 2 KB, and 16 bytes of scales each
+    assert lib.lx_q8_bytes(1152, 896) == 72 * 7 * 2064
+    assert lib.lx_q8_bytes(1, 1) == 2064
+    assert lib.lx_q8_bytes(17, 129) == 2 * 2 * 2064
+    assert lib.lx_q8_bytes(151936, 8192) == 9496 * 64 * 2064
+    assert lib.lx_q8_bytes(1 << 22, 8192) == (1 << 18) * 64 * 2064  # past 32 bits
     for bad in [(0, 1), (1, 0), (-1, 5), (5, -1), (2 ** 31 - 1, 1), (1, 2 ** 31 - 1)]:
         assert lib.lx_q8_bytes(*bad) == 0, bad
 
