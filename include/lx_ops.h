@@ -782,6 +782,19 @@ int lx_qwen2_set_decode_graph(lx_qwen2* m, int enable);
  * capture.  No counterpart in the reference. */
 int lx_qwen2_set_decode_bits(lx_qwen2* m, int bits, int group);
 
+/* The prefill's weights: bits = 32 (the default) or 8, every projection and the head on
+ * copies in 8 bits with a power of two per 128 inputs (lx_q8_pack_f32, lx_linear_q8_f32).
+ * The rows they read are held in 8 bits too: the norms write them (lx_rmsnorm_q8_f32),
+ * attention's and SwiGLU's output is quantised on its way.  Attention, the residual stream,
+ * the K/V cache, hidden and final_norm stay fp32, and so does decode (lx_qwen2_set_decode_bits
+ * is a setting of its own).  The first call packs the copies from the model's fp32 weights,
+ * which stay, and allocates the rows for max_ctx (364 and 24 MB for Qwen2-0.5B at 4096); both are
+ * held until destroy, so a prefill that the caller captured keeps giving what it was captured
+ * with.  The call waits for that packing, and for nothing else.  LX_ERR_ALLOC and LX_ERR_LAUNCH
+ * change nothing.  The model's device must be current (else LX_ERR_ARG).  Not to be called
+ * during a capture.  No counterpart in the reference. */
+int lx_qwen2_set_prefill_bits(lx_qwen2* m, int bits);
+
 /* Prefill projections' split-operand products, 3 (the default) or 6, as
  * lx_dit_set_products (decode's GEMVs are fp32 either way).  No counterpart
  * in the reference (src/llm/llm.cpp:141-173 runs fp32 ggml_mul_mat). */

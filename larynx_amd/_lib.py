@@ -251,6 +251,7 @@ SIGNATURES = [
     ("lx_qwen2_set_decode_graph", C.c_int, [C.c_void_p, C.c_int]),
     ("lx_qwen2_set_products", C.c_int, [C.c_void_p, C.c_int]),
     ("lx_qwen2_set_decode_bits", C.c_int, [C.c_void_p, C.c_int, C.c_int]),
+    ("lx_qwen2_set_prefill_bits", C.c_int, [C.c_void_p, C.c_int]),
 ]
 
 

@@ -46,6 +46,17 @@ struct Q4Weights {
   std::vector<Q4Layer> layers;
 };
 
+// The prefill's weights in 8 bits (lx_qwen2_set_prefill_bits), packed once and kept, and the rows
+// its products read, of up to max_ctx each.
+struct Q8Layer {
+  void *qkv = nullptr, *o = nullptr, *gu = nullptr, *down = nullptr;
+};
+struct Q8Weights {
+  void* head = nullptr;  // llm_decoder
+  std::vector<Q8Layer> layers;
+  void *rows = nullptr, *act = nullptr;  // (max_ctx, H) and (max_ctx, I)
+};
+
 // Six products run on the fragment-operand GEMMs up to this many rows (64 rows 1.05x
 // the split-operand GEMM's prefill; 100 rows 0.93x: three parts per operand make
 // their tiles wait on the L2s).
@@ -110,6 +121,8 @@ struct lx_qwen2 {
   bool use_graph = true;      // replay the layer stack as one HIP graph
   std::vector<Q4Weights> q4_sets;  // at most one a group size, and room for all from the first
   const Q4Weights* q4 = nullptr;   // decode's (null: fp32)
+  Q8Weights q8;                    // layers empty: never packed
+  bool prefill8 = false;           // the prefill runs on them
   hipStream_t cap_stream = nullptr;
   // [0]: the cache fits one attention split; [1 + c]: split class c
   hipGraphExec_t graph[1 + kDecAttnClasses] = {};
@@ -351,6 +364,34 @@ int prefill_layer(lx_qwen2* m, Layer& L, int rows, const float* next_norm, hipSt
   return prefill_mlp(m, L, rows, next_norm, s, LX_ACT_F32, LX_ACT_F32);
 }
 
+// The same layer on 8-bit weights, over the 8-bit rows in m->q8.rows (its input's norm on entry,
+// next_norm of its output on exit): what each projection reads is quantised by its producer (the
+// norms) or on its way (attention's and SwiGLU's output); attention, the residual stream and the
+// cache stay fp32.
+int prefill_layer_q8(lx_qwen2* m, const Layer& L, const Q8Layer& w, int rows,
+                     const float* next_norm, hipStream_t s) {
+  const int H = m->H, KV = m->KV, QKV = m->QKV, I = m->I;
+  const lx_q8 hn{m->q8.rows, rows, H}, act{m->q8.act, rows, I};
+  const lx_q8 qkv{w.qkv, QKV, H}, o{w.o, H, H}, gu{w.gu, 2 * I, H}, down{w.down, H, I};
+  lx_epilogue resid{}, swiglu{};
+  resid.kind = LX_EPI_RESID;
+  swiglu.kind = LX_EPI_SWIGLU_PAIRED;
+  LX_TRY(lx_linear_q8_f32(&hn, &qkv, nullptr, nullptr, nullptr, 0, m->ws, QKV, s));
+  LX_TRY(splitk_qkv_rope_cache(m->ws, 1, rows, L.qkv_b, m->NH, m->NKV, m->pos, m->rope_tab, m->qkv,
+                               QKV, L.k_cache, L.v_cache, 0, s));
+  const float scale = 1.0f / std::sqrt((float)m->HD);
+  LX_TRY(attention(m->qkv, QKV, L.k_cache, KV, L.v_cache, KV, m->att, H, 1, rows, rows, m->NH,
+                   m->NKV, m->HD, scale, /*causal*/ 1, /*q_offset*/ 0, /*products*/ 6,
+                   LX_ACT_F32, s));
+  LX_TRY(lx_q8_pack_f32(m->att, H, &hn, s));
+  LX_TRY(lx_linear_q8_f32(&hn, &o, nullptr, &resid, nullptr, 0, m->x, H, s));
+  LX_TRY(lx_rmsnorm_q8_f32(m->x, H, nullptr, 0, nullptr, 0, L.post_norm, m->eps, &hn, s));
+  LX_TRY(lx_linear_q8_f32(&hn, &gu, nullptr, &swiglu, nullptr, 0, m->act, I, s));
+  LX_TRY(lx_q8_pack_f32(m->act, I, &act, s));
+  LX_TRY(lx_linear_q8_f32(&act, &down, nullptr, &resid, nullptr, 0, m->x, H, s));
+  return lx_rmsnorm_q8_f32(m->x, H, nullptr, 0, nullptr, 0, next_norm, m->eps, &hn, s);
+}
+
 // A decode projection on its fp32 or its 4-bit weight.
 int dec_proj(const lx_qwen2* m, int epi, const DecGemvArgs& a, const void* q4, hipStream_t s) {
   return m->q4 ? dec_gemv_q4(epi, a, q4, m->q4->group, s) : dec_gemv(epi, a, s);
@@ -522,6 +563,60 @@ int add_q4(lx_qwen2* m, int group, const Q4Weights** out) {
   }
   m->q4_sets.push_back(std::move(w));
   *out = &m->q4_sets.back();
+  return LX_OK;
+}
+
+// The prefill's weights in 8 bits and its rows, allocated and packed into w.
+int pack_q8(lx_qwen2* m, Q8Weights& w) {
+  const int H = m->H, I = m->I;
+  auto A = [&](void** p, int N, int K) {
+    *p = m->arena.alloc<char>(lx_q8_bytes(N, K));
+    return *p != nullptr;
+  };
+  bool ok = A(&w.head, m->speech_vocab, H) && A(&w.rows, m->max_ctx, H) && A(&w.act, m->max_ctx, I);
+  for (Q8Layer& q : w.layers)
+    ok = ok && A(&q.qkv, m->QKV, H) && A(&q.o, H, H) && A(&q.gu, 2 * I, H) && A(&q.down, H, I);
+  if (!ok) {
+    set_error("qwen2_set_prefill_bits: device allocation failed");
+    return LX_ERR_ALLOC;
+  }
+  auto P = [&](const float* W, void* q, int N, int K) {
+    const lx_q8 out{q, N, K};
+    return lx_q8_pack_f32(W, K, &out, nullptr);
+  };
+  LX_TRY(P(m->llm_decoder, w.head, m->speech_vocab, H));
+  for (int l = 0; l < m->NL; ++l) {
+    const Layer& L = m->layers[l];
+    const Q8Layer& q = w.layers[l];
+    LX_TRY(P(L.qkv_w, q.qkv, m->QKV, H));
+    LX_TRY(P(L.o_w, q.o, H, H));
+    LX_TRY(P(L.gu_w, q.gu, 2 * I, H));
+    LX_TRY(P(L.down_w, q.down, H, I));
+  }
+  if (hipStreamSynchronize(nullptr) != hipSuccess) {
+    (void)hipGetLastError();
+    set_error("qwen2_set_prefill_bits: packing failed");
+    return LX_ERR_LAUNCH;
+  }
+  return LX_OK;
+}
+
+// The same, kept in m->q8.  An error leaves the model and its memory as they were.
+int add_q8(lx_qwen2* m) {
+  const size_t before = m->arena.ptrs.size();
+  Q8Weights w;
+  try {
+    w.layers.resize(m->NL);
+    m->arena.ptrs.reserve(before + 3 + 4 * m->NL);
+  } catch (const std::bad_alloc&) {
+    set_error("qwen2_set_prefill_bits: host allocation failed");
+    return LX_ERR_ALLOC;
+  }
+  if (const int rc = pack_q8(m, w)) {
+    m->arena.trim(before);
+    return rc;
+  }
+  m->q8 = std::move(w);
   return LX_OK;
 }
 
@@ -754,26 +849,39 @@ extern "C" int lx_qwen2_prefill(lx_qwen2* m, const float* lm_input, int L, float
     return LX_ERR_LAUNCH;
   }
   m->cache_len = 0;
-  const bool frag = m->frag && (m->products == 3 || L <= kFragRows6);
-  if (frag)
+  const bool q8 = m->prefill8;
+  const bool frag = !q8 && m->frag && (m->products == 3 || L <= kFragRows6);
+  const lx_q8 rows{m->q8.rows, L, H};
+  if (q8)
+    LX_TRY(lx_rmsnorm_q8_f32(m->x, H, nullptr, 0, nullptr, 0, m->layers[0].in_norm, m->eps, &rows,
+                             s));
+  else if (frag)
     LX_TRY(splitk_resid_rmsnorm(nullptr, 0, L, H, nullptr, m->x, m->layers[0].in_norm, m->eps,
                                 m->hn, s, m->products == 3 ? LX_ACT_FRAG2 : LX_ACT_FRAG3));
   else
     LX_TRY(lx_rmsnorm_f32(m->x, m->layers[0].in_norm, m->hn, L, H, m->eps, s));
   for (int l = 0; l < m->NL; ++l) {
     const float* next_norm = l + 1 < m->NL ? m->layers[l + 1].in_norm : m->final_norm;
-    LX_TRY(frag ? prefill_layer_frag(m, m->layers[l], L, next_norm, s, l + 1 == m->NL)
-                : prefill_layer(m, m->layers[l], L, next_norm, s));
+    LX_TRY(q8     ? prefill_layer_q8(m, m->layers[l], m->q8.layers[l], L, next_norm, s)
+           : frag ? prefill_layer_frag(m, m->layers[l], L, next_norm, s, l + 1 == m->NL)
+                  : prefill_layer(m, m->layers[l], L, next_norm, s));
     if (hidden)
       (void)hipMemcpyAsync(hidden + (size_t)l * L * H, m->x, sizeof(float) * (size_t)L * H,
                            hipMemcpyDeviceToDevice, s);
   }
-  if (final_norm)
+  if (final_norm && q8)
+    LX_TRY(lx_rmsnorm_f32(m->x, m->final_norm, final_norm, L, H, m->eps, s));
+  else if (final_norm)
     (void)hipMemcpyAsync(final_norm, m->hn, sizeof(float) * (size_t)L * H, hipMemcpyDeviceToDevice,
                          s);
-  if (logits)
+  if (logits && q8) {
+    const lx_q8 head{m->q8.head, m->speech_vocab, H};
+    LX_TRY(lx_linear_q8_f32(&rows, &head, nullptr, nullptr, nullptr, 0, logits, m->speech_vocab,
+                            s));
+  } else if (logits) {
     LX_TRY(lx_linear_f32(m->hn, H, m->llm_decoder, nullptr, logits, m->speech_vocab, L,
                          m->speech_vocab, H, nullptr, s));
+  }
   m->cache_len = L;
   return check_launch("qwen2_prefill");
 }
@@ -867,6 +975,17 @@ extern "C" int lx_qwen2_set_decode_bits(lx_qwen2* m, int bits, int group) {
     g = nullptr;
   }
   m->q4 = q4;
+  return LX_OK;
+}
+
+extern "C" int lx_qwen2_set_prefill_bits(lx_qwen2* m, int bits) {
+  LX_REQUIRE(m, "qwen2_set_prefill_bits: null model");
+  LX_REQUIRE(bits == 32 || bits == 8, "qwen2_set_prefill_bits: %d bits (32 or 8)", bits);
+  int dev = -1;
+  LX_REQUIRE(hipGetDevice(&dev) == hipSuccess && dev == m->device,
+             "qwen2_set_prefill_bits: device %d is current, the model is on %d", dev, m->device);
+  if (bits == 8 && m->q8.layers.empty()) LX_TRY(add_q8(m));
+  m->prefill8 = bits == 8;
   return LX_OK;
 }
 

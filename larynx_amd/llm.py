@@ -12,7 +12,7 @@ from dataclasses import dataclass
 import torch
 
 from ._lib import Qwen2LayerWeights, Qwen2Weights, check, lib
-from .ops import stream
+from .ops import stream, token_logprobs
 
 
 @dataclass(frozen=True)
@@ -185,6 +185,20 @@ class Qwen2LM:
                                   fn.data_ptr() if fn is not None else None, stream()))
         return (logits, fn) if final_norm else logits
 
+    def score(self, text_tokens, prompt_speech_tokens, tokens, top=0, device="cuda"):
+        """How likely the model finds speech `tokens` (host ids) after a text and a prompt: the
+        TokenLogprobs (ops.token_logprobs) of one row per token.  One prefill over [sos; text;
+        task_id; prompt; tokens but the last], which the cache holds afterwards."""
+        t = [int(v) for v in tokens]
+        if not t:
+            raise ValueError("score: no tokens")
+        if not 0 <= t[-1] < self.cfg.speech_vocab:  # the others are checked as inputs
+            raise ValueError(f"score: token {t[-1]} outside [0, {self.cfg.speech_vocab})")
+        lm_input = self.build_lm_input(text_tokens, list(prompt_speech_tokens) + t[:-1], device)
+        logits = self.prefill(lm_input)
+        ids = torch.tensor(t, dtype=torch.int32, device=logits.device)
+        return token_logprobs(logits[-len(t):], ids, top=top)
+
     @property
     def cache_len(self):
         return lib.lx_qwen2_cache_len(self._h)
@@ -202,6 +216,12 @@ class Qwen2LM:
         copies with a scale per `group` (32, 64, 128) inputs.  The prefill keeps fp32.  Copies are
         packed once a group and kept; decode steps captured by the caller stay on theirs."""
         check(lib.lx_qwen2_set_decode_bits(self._h, int(bits), int(group)))
+
+    def set_prefill_bits(self, bits):
+        """The prefill's weights: 32 (fp32, the default) or 8, every projection and the head on 8-bit
+        copies over 8-bit rows (ops.linear_q8, ops.rms_norm_q8).  Decode keeps its own setting.
+        Copies are packed at the first call and kept."""
+        check(lib.lx_qwen2_set_prefill_bits(self._h, int(bits)))
 
     def set_products(self, products):
         """Split-operand products of the prefill projections: 3 (the default) or 6."""
