@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(LpArgs a) {
   for (int i = 0; i < NV; ++i) {
     const int k = (tid + 256 * i) * 4;
     if (k + 4 <= n) {
-      const float4u u = *reinterpret_cast<const float4u*>(x + k);
+      const float4u u = __builtin_nontemporal_load(reinterpret_cast<const float4u*>(x + k));
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[i][e] = u[e];
     } else {

@@ -23,7 +23,7 @@ struct Q8Lin {
   float* y;
   long ldr, ldy;
   int epi;
-  int tiles_m, tiles_n;  // of the launch
+  int tiles_m, tiles_n, band;  // of the launch
 };
 
 __device__ __forceinline__ void epi_one(const Q8Lin& a, int m, long n, float v, float up) {
@@ -152,6 +152,29 @@ __global__ __launch_bounds__(64 * WAVES) void q8_stream_kernel(Q8Lin a) {
 // the step after are on their way from LDS.  The one barrier of a stage stands before its last two
 // steps, whose operands every wave has by then: the buffer is free for the stage NS further on, and
 // the next stage's first reads return behind those steps' products.
+// This workgroup's tile of y.  Each XCD (workgroups are dealt to them round-robin) takes a
+// contiguous run of tiles, which go down and then along bands of a.band rows of tiles: about a
+// square, the fewest bytes for its L2 (4096 x 8192 x 8192 442 -> 423 us against runs of columns).
+__device__ __forceinline__ void tile_at(const Q8Lin& a, int& mt, int& nt) {
+  int id = blockIdx.x;
+  const int full = gridDim.x / 8 * 8;
+  if (id < full) id = (id % 8) * (full / 8) + id / 8;
+  const int band = id / (a.band * a.tiles_n), in_band = id % (a.band * a.tiles_n);
+  const int high = min(a.band, a.tiles_m - band * a.band);
+  mt = band * a.band + in_band % high;
+  nt = in_band / high;
+}
+int tile_grid(Q8Lin& a, int rows, int cols, int threads, long* grid) {
+  a.tiles_m = (a.x.rows + rows - 1) / rows;
+  a.tiles_n = (a.w.rows + cols - 1) / cols;
+  *grid = (long)a.tiles_m * a.tiles_n;
+  LX_REQUIRE(*grid <= INT_MAX / threads, "linear_q8: %d x %d outputs are too many", a.x.rows,
+             a.w.rows);
+  a.band = 1;
+  while (a.band < a.tiles_m && (long)(a.band + 1) * (a.band + 1) * 8 <= *grid) ++a.band;
+  return LX_OK;
+}
+
 template <int N>
 __device__ __forceinline__ void wait_vm() {  // vmcnt(N) lgkmcnt(0)
   __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4 & 3) << 14 | 7 << 4);
@@ -181,13 +204,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, OCC) void q8_tile_kernel(Q8Lin a
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wk = wave % WK, wm = wave / WK % WM, wn = wave / (WK * WM);
-  // each XCD (workgroups are dealt to them round-robin) takes a contiguous run of tiles
-  int id = blockIdx.x;
-  {
-    const int full = gridDim.x / 8 * 8;
-    if (id < full) id = (id % 8) * (full / 8) + id / 8;
-  }
-  const int mt = id % a.tiles_m, nt = id / a.tiles_m;
+  int mt, nt;
+  tile_at(a, mt, nt);
   const int mtiles = (a.x.rows + 15) / 16, ntiles = (a.w.rows + 15) / 16;
   const int kb = a.x.kb;
   // tile t of a stage: rows of x, then of W; past the last it repeats that
@@ -364,11 +382,8 @@ int launch_tile(Q8Lin& a, hipStream_t s) {
   const auto kern = q8_tile_kernel<RB, CB, WM, WN, WK, NS, OCC>;
   static LdsLimit once;
   LX_TRY(raise_lds_limit(reinterpret_cast<const void*>(kern), S::LDS, once, "q8_tile_kernel"));
-  a.tiles_m = (a.x.rows + 32 * RB * WM - 1) / (32 * RB * WM);
-  a.tiles_n = (a.w.rows + 32 * CB * WN - 1) / (32 * CB * WN);
-  const long grid = (long)a.tiles_m * a.tiles_n;
-  LX_REQUIRE(grid <= INT_MAX / (64 * S::WAVES), "linear_q8: %d x %d outputs are too many",
-             a.x.rows, a.w.rows);
+  long grid;
+  LX_TRY(tile_grid(a, 32 * RB * WM, 32 * CB * WN, 64 * S::WAVES, &grid));
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * S::WAVES), S::LDS, s, a);
   return check_launch("q8_tile_kernel");
 }
