@@ -239,8 +239,10 @@ extern "C" int lx_rmsnorm_q8_f32(const float* x, long ldx, const float* add, lon
     LX_REQUIRE((sum == add && lds == lda) || !rows_overlap(add, lda, D, sum, lds, D, rows),
                "rmsnorm_q8: sum overlaps add");
   }
+  LX_REQUIRE((D <= 2048 ? ((long)rows + 3) / 4 : (long)rows) <= INT_MAX / 256,
+             "rmsnorm_q8: %d rows of %d are too many", rows, D);
   NormArgs a{x, add, w, sum, ldx, lda, lds, eps, q8_mat(q)};
-  const dim3 wide((unsigned)rows), four((unsigned)((rows + 3) / 4)), block(256);
+  const dim3 wide((unsigned)rows), four((unsigned)(((long)rows + 3) / 4)), block(256);
   if (D <= 1024)
     hipLaunchKernelGGL((norm_q8_kernel<64, 2>), four, block, 0, stream, a);
   else if (D <= 2048)

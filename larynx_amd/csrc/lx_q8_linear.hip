@@ -165,8 +165,8 @@ __device__ __forceinline__ void tile_at(const Q8Lin& a, int& mt, int& nt) {
   nt = in_band / high;
 }
 int tile_grid(Q8Lin& a, int rows, int cols, int threads, long* grid) {
-  a.tiles_m = (a.x.rows + rows - 1) / rows;
-  a.tiles_n = (a.w.rows + cols - 1) / cols;
+  a.tiles_m = (int)(((long)a.x.rows + rows - 1) / rows);
+  a.tiles_n = (int)(((long)a.w.rows + cols - 1) / cols);
   *grid = (long)a.tiles_m * a.tiles_n;
   LX_REQUIRE(*grid <= INT_MAX / threads, "linear_q8: %d x %d outputs are too many", a.x.rows,
              a.w.rows);
@@ -395,11 +395,8 @@ int launch_stream(Q8Lin& a, hipStream_t s) {
   if (lds > 65536)
     LX_TRY(raise_lds_limit(reinterpret_cast<const void*>(q8_stream_kernel<MT, NT, WAVES>), lds,
                            once, "q8_stream_kernel"));
-  a.tiles_m = (a.x.rows + 16 * MT - 1) / (16 * MT);
-  a.tiles_n = (a.w.rows + 16 * NT - 1) / (16 * NT);
-  const long grid = (long)a.tiles_m * a.tiles_n;
-  LX_REQUIRE(grid <= INT_MAX / (64 * WAVES), "linear_q8: %d x %d outputs are too many", a.x.rows,
-             a.w.rows);
+  long grid;
+  LX_TRY(tile_grid(a, 16 * MT, 16 * NT, 64 * WAVES, &grid));
   hipLaunchKernelGGL((q8_stream_kernel<MT, NT, WAVES>), dim3((unsigned)grid), dim3(64 * WAVES), lds,
                      s, a);
   return check_launch("q8_stream_kernel");

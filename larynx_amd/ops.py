@@ -337,7 +337,7 @@ def conv_pos_mish_bx(x, wf, bias, resid=None, groups=16, kernel=31, products=3):
 
 # ---- the LM in four bits ----------------------------------------------------------------
 
-_F32, _I32 = torch.float32, torch.int32
+_F32, _I32, _U8 = torch.float32, torch.int32, torch.uint8
 
 
 def _rows(t, name, shape):
@@ -549,6 +549,7 @@ class Q8Matrix:
 
 
 _pack_q8 = struct.Struct("@Pii").pack
+_new = object.__new__
 
 
 def _q8_out(like, rows, K, out):
@@ -556,7 +557,7 @@ def _q8_out(like, rows, K, out):
         n = lib.lx_q8_bytes(rows, K)
         if not n:
             raise ValueError(f"no 8-bit form of a ({rows}, {K}) matrix")
-        return Q8Matrix.__new__(Q8Matrix)._set(like.new_empty(n, dtype=torch.uint8), rows, K)
+        return _new(Q8Matrix)._set(like.new_empty(n, dtype=_U8), rows, K)
     if out.rows != rows or out.K != K:
         raise ValueError(f"out must hold a ({rows}, {K}) matrix")
     if out._dev != like.get_device():
@@ -578,13 +579,13 @@ def _matrix(t, name):
     return rows, cols, ld, dev
 
 
-def _like(t, name, shape, dev):
-    """Row stride of the fp32 matrix t of `shape` on device dev."""
+def _like(t, name, rows, cols, dev):
+    """Row stride of the fp32 matrix t (rows, cols) on device dev."""
     if t.get_device() != dev:
         _elsewhere(name)
-    if t.dtype is _F32 and t.is_contiguous() and t.shape == shape:
-        return shape[-1]
-    return _rows(t, name, shape)
+    if t.dtype is _F32 and t.is_contiguous() and t.shape == (rows, cols):
+        return cols
+    return _rows(t, name, (rows, cols))
 
 
 def q8_pack(x, out=None):
@@ -603,7 +604,7 @@ def q8_unpack(q):
     if dev < 0 or dev != _current():
         _elsewhere("q")
     K = q.K
-    x = q.data.new_empty((q.rows, K), dtype=_F32)
+    x = q.data.new_empty(q.rows, K, dtype=_F32)
     check(lib.lx_q8_unpack_f32(q._ref, x.data_ptr(), K, _raw_stream(dev)))
     return x
 
@@ -622,8 +623,8 @@ def rms_norm_q8(x, w, eps=1e-6, add=None, sum_out=None, out=None):
     if add is not None:
         if sum_out is None:
             sum_out = x
-        lda = _like(add, "add", x.shape, dev)
-        lds = ldx if sum_out is x else _like(sum_out, "sum_out", x.shape, dev)
+        lda = _like(add, "add", rows, K, dev)
+        lds = ldx if sum_out is x else _like(sum_out, "sum_out", rows, K, dev)
         pa, ps = add.data_ptr(), sum_out.data_ptr()
     elif sum_out is not None:
         raise ValueError("sum_out without add")
@@ -652,15 +653,15 @@ def linear_q8(x, w, b=None, epilogue=None, resid=None, out=None):
             _elsewhere("b")
         bias = b.data_ptr()
     if resid is not None:
-        ldr = _like(resid, "resid", (M, cols), dev)
+        ldr = _like(resid, "resid", M, cols, dev)
         pr = resid.data_ptr()
     if out is None:
         if kind == LX_EPI_RESID and resid is None:
             raise ValueError("residual epilogues need resid=, or out= (the residual stream)")
-        out = x.data.new_empty((M, cols), dtype=_F32)
+        out = x.data.new_empty(M, cols, dtype=_F32)
         ldy = cols
     else:
-        ldy = _like(out, "out", (M, cols), dev)
+        ldy = _like(out, "out", M, cols, dev)
     check(lib.lx_linear_q8_f32(x._ref, w._ref, bias,
                                None if epilogue is None else C.byref(epilogue), pr, ldr,
                                out.data_ptr(), ldy, _raw_stream(dev)))
@@ -693,8 +694,8 @@ def token_logprobs(logits, tokens=None, top=0, entropy=True):
         ent = logits.new_empty(rows)
         pe = ent.data_ptr()
     if top > 0:
-        tl = logits.new_empty((rows, top))
-        ti = logits.new_empty((rows, top), dtype=_I32)
+        tl = logits.new_empty(rows, top)
+        ti = logits.new_empty(rows, top, dtype=_I32)
         ptl, pti = tl.data_ptr(), ti.data_ptr()
     n, ws, pw = 0, None, None
     if V > 8192:

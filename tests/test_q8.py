@@ -98,6 +98,13 @@ def test_norm_refusals(kw):
     assert b"rmsnorm_q8" in lib.lx_last_error()
 
 
+@pytest.mark.parametrize("rows,K", [(2 ** 23, 2049), (2 ** 23, 10 ** 5), (2 ** 25, 896)])
+def test_norm_too_many_rows(rows, K):
+    assert lib.lx_rmsnorm_q8_f32(O, K, None, 0, None, 0, P, 1e-6, _q(rows=rows, K=K),
+                                 None) == LX_ERR_ARG
+    assert b"too many" in lib.lx_last_error()
+
+
 def _linear(x=None, w=None, bias=None, kind=None, resid=None, ldr=0, y=O, ldy=32):
     epi = None if kind is None else C.byref(Epilogue(kind=kind))
     return lib.lx_linear_q8_f32(x or _q(), w or _q(rows=32), bias, epi, resid, ldr, y, ldy, None)
