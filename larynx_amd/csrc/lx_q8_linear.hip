@@ -380,10 +380,10 @@ template <int RB, int CB, int WM, int WN, int WK, int NS, int OCC>
 int launch_tile(Q8Lin& a, hipStream_t s) {
   using S = TileShape<RB, CB, WM, WN, WK, NS>;
   const auto kern = q8_tile_kernel<RB, CB, WM, WN, WK, NS, OCC>;
-  static LdsLimit once;
-  LX_TRY(raise_lds_limit(reinterpret_cast<const void*>(kern), S::LDS, once, "q8_tile_kernel"));
   long grid;
   LX_TRY(tile_grid(a, 32 * RB * WM, 32 * CB * WN, 64 * S::WAVES, &grid));
+  static LdsLimit once;
+  LX_TRY(raise_lds_limit(reinterpret_cast<const void*>(kern), S::LDS, once, "q8_tile_kernel"));
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * S::WAVES), S::LDS, s, a);
   return check_launch("q8_tile_kernel");
 }
@@ -391,10 +391,7 @@ int launch_tile(Q8Lin& a, hipStream_t s) {
 template <int MT, int NT, int WAVES>
 int launch_stream(Q8Lin& a, hipStream_t s) {
   constexpr size_t lds = (size_t)MT * NT * WAVES * 1024;
-  static LdsLimit once;
-  if (lds > 65536)
-    LX_TRY(raise_lds_limit(reinterpret_cast<const void*>(q8_stream_kernel<MT, NT, WAVES>), lds,
-                           once, "q8_stream_kernel"));
+  static_assert(lds <= 65536, "raise the limit");
   long grid;
   LX_TRY(tile_grid(a, 16 * MT, 16 * NT, 64 * WAVES, &grid));
   hipLaunchKernelGGL((q8_stream_kernel<MT, NT, WAVES>), dim3((unsigned)grid), dim3(64 * WAVES), lds,
