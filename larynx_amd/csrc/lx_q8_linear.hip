@@ -26,11 +26,23 @@ struct Q8Lin {
   int tiles_m, tiles_n, band;  // of the launch
 };
 
+// x / (1 + e^-x) on the hardware's exponential and reciprocal, each within an ulp or so; the
+// argument's product with log2(e) in two parts, so that the exponential keeps its relative error
+// far from zero.  (Against expf and a division a third of the instructions; 256 x 9728 x 896 12.5 ->
+// 11.9 us.)  Below -87 the factor stays e^-87.
+__device__ __forceinline__ float silu_hw(float x) {
+  const float c = fmaxf(x, -87.0f), hi = c * -1.4426950408889634f;
+  const float lo = fmaf(c, -1.4426950408889634f, -hi) + c * -1.9259629911266175e-8f;
+  float e = __builtin_amdgcn_exp2f(hi);
+  e = fmaf(e, lo * 0.6931471805599453f, e);
+  return x * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
 __device__ __forceinline__ void epi_one(const Q8Lin& a, int m, long n, float v, float up) {
   if (a.bias) v += a.bias[n];
   if (a.epi == LX_EPI_SWIGLU_PAIRED) {
     if (a.bias) up += a.bias[n + 1];
-    a.y[m * a.ldy + (n >> 1)] = (v / (1.0f + expf(-v))) * up;
+    a.y[m * a.ldy + (n >> 1)] = silu_hw(v) * up;
     return;
   }
   if (a.epi == LX_EPI_GELU_TANH) v = gelu_tanh(v);
@@ -45,7 +57,7 @@ __device__ __forceinline__ void epi_quad(const Q8Lin& a, int m, long n, floatx4 
     if (a.bias) v += *reinterpret_cast<const float4u*>(a.bias + n);
     if (a.epi == LX_EPI_SWIGLU_PAIRED) {
       *reinterpret_cast<float2u*>(a.y + m * a.ldy + (n >> 1)) = float2u{
-          (v[0] / (1.0f + expf(-v[0]))) * v[1], (v[2] / (1.0f + expf(-v[2]))) * v[3]};
+          silu_hw(v[0]) * v[1], silu_hw(v[2]) * v[3]};
       return;
     }
     if (a.epi == LX_EPI_GELU_TANH)
@@ -178,6 +190,7 @@ int tile_grid(Q8Lin& a, int rows, int cols, int threads, long* grid) {
 template <int N>
 __device__ __forceinline__ void wait_vm() {  // vmcnt(N) lgkmcnt(0)
   __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4 & 3) << 14 | 7 << 4);
+  asm volatile("" ::: "memory");  // no read of LDS moves in front of it
 }
 
 template <int RB, int CB, int WM, int WN, int WK, int NS>
@@ -303,6 +316,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, OCC) void q8_tile_kernel(Q8Lin a
         for (int i = 0; i < RB + CB; ++i) asm volatile("" : "+v"(frag[0][i]));
         if (k + 1 < kb) wait(k + 1);
         __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
         if (k + NS < kb) load(k + NS, buf);
         read_scales(us, next);
         read(raw[(P + s + 1) & 1], next, 0);  // past the last stage: bytes of a buffer, not used
@@ -388,6 +402,191 @@ int launch_tile(Q8Lin& a, hipStream_t s) {
   return check_launch("q8_tile_kernel");
 }
 
+// Fewer rows.  A workgroup owns (32 RB) x (32 CB) outputs and each of its W waves takes every W-th 64
+// of K, through a ring of R slots of LDS of its own: no barrier until the waves' sums meet, and
+// (R - 1) slots of every wave on their way.  A slot's tile is 16 rows x 64 bytes, 1 KB, which one
+// instruction brings: lane 4 row + q loads chunk q ^ (row / 4 % 4) of its row's half block, so that
+// the 16 rows of a read are spread over all banks.
+template <int RB, int CB, int W, int R>
+struct RingShape {
+  static constexpr int T = 2 * (RB + CB);  // 16-row tiles of a slot: rows of x, then of W
+  static_assert(T <= 16, "one instruction loads a slot's scales");
+  static constexpr int SLOT = T * 1024 + 256;  // the scales behind the codes
+  static constexpr int ROW = 32 * CB + 4;  // floats of a row of outputs in LDS
+  static constexpr int OUT = 32 * ROW * 4;  // a wave's 32 rows
+  static constexpr int LDS = W * (R * SLOT > OUT ? R * SLOT : OUT);
+  static_assert(LDS <= 160 * 1024, "LDS of a CU");
+  static_assert((R - 2) * (T + 1) < 64, "vmcnt");
+};
+
+template <int RB, int CB, int W, int R, int OCC>
+__global__ __launch_bounds__(64 * W, OCC) void q8_ring_kernel(Q8Lin a) {
+  using S = RingShape<RB, CB, W, R>;
+  constexpr int T = S::T;
+  extern __shared__ __attribute__((aligned(16))) unsigned char sm[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int mt, nt;
+  tile_at(a, mt, nt);
+  const int mtiles = (a.x.rows + 15) / 16, ntiles = (a.w.rows + 15) / 16;
+  const int kb = a.x.kb, slots = (2 * kb - wave + W - 1) / W;  // this wave's
+  auto tile_of = [&](int t) {
+    return t < 2 * RB ? min(mt * 2 * RB + t, mtiles - 1)
+                      : min(nt * 2 * CB + min(t - 2 * RB, 2 * CB - 1), ntiles - 1);
+  };
+  const unsigned char* base[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+    base[t] = (t < 2 * RB ? a.x.codes : a.w.codes) + (long)tile_of(t) * kb * kQ8Tile;
+  const unsigned char* sbase;
+  {
+    const int t = lane >> 2;
+    sbase = (t < 2 * RB ? a.x.scales : a.w.scales) + (long)tile_of(t) * kb * 16 + (lane & 3) * 4;
+  }
+  // the chunk of half block 0 that this lane loads; of half block 1 it is this ^ 64
+  const int lr = lane >> 2;
+  const int lat = lr * kQ8Block + ((((lane & 3) ^ (lr >> 2)) ^ (lr >> 1)) << 4);
+  typedef const __attribute__((address_space(1))) void* global_ptr;
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  unsigned char* ring = sm + wave * R * S::SLOT;
+  auto load = [&](int i, int slot) {
+    const int hb = i * W + wave;
+    const long off = (long)(hb >> 1) * kQ8Tile;
+    const int at = lat ^ ((hb & 1) << 6);
+    unsigned char* d = ring + slot * S::SLOT;
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+      __builtin_amdgcn_global_load_lds((global_ptr)(base[t] + off + at), (lds_ptr)(d + t * 1024),
+                                       16, 0, 0);
+    __builtin_amdgcn_global_load_lds((global_ptr)(sbase + (long)(hb >> 1) * 16),
+                                     (lds_ptr)(d + T * 1024), 4, 0, 0);
+  };
+  const int r = lane & 15, h = lane >> 5, half = (lane >> 4) & 1;
+  int at[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) at[s] = half * 1024 + r * 64 + (((2 * s + h) ^ (r >> 2)) << 4);
+  floatx16 acc[CB][RB];
+#pragma unroll
+  for (int n = 0; n < CB; ++n)
+#pragma unroll
+    for (int m = 0; m < RB; ++m)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[n][m][e] = 0.0f;
+  intx4 raw[2][RB + CB];
+  bf16x8_t frag[2][RB + CB];
+  float scale[RB + CB];
+  unsigned us[RB + CB];
+  auto read = [&](intx4 (&f)[RB + CB], int slot, int s) {
+    const unsigned char* b = ring + slot * S::SLOT + at[s];
+#pragma unroll
+    for (int i = 0; i < RB + CB; ++i) f[i] = *reinterpret_cast<const intx4*>(b + i * 2048);
+  };
+  auto read_scales = [&](int slot) {
+    const unsigned char* b = ring + slot * S::SLOT + T * 1024 + half * 16 + r;
+#pragma unroll
+    for (int i = 0; i < RB + CB; ++i) us[i] = b[i * 32];
+  };
+  auto set_scales = [&]() {
+#pragma unroll
+    for (int i = 0; i < RB + CB; ++i) scale[i] = __uint_as_float(us[i] << 23);
+  };
+  auto convert = [&](bf16x8_t (&f)[RB + CB], const intx4 (&u)[RB + CB], int t) {
+#pragma unroll
+    for (int i = 0; i < RB + CB; ++i) f[i] = q8_frag(u[i][2 * t], u[i][2 * t + 1], scale[i]);
+  };
+  // slot i is in LDS (R - 2 later ones may be on their way), and this wave's reads are done
+  auto wait = [&](int i) {
+    if (i + R - 2 < slots)
+      wait_vm<(R - 2) * (T + 1)>();
+    else
+      wait_vm<0>();
+  };
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (i < slots) load(i, i);
+  if (slots > 0) {
+    wait(0);
+    read_scales(0);
+    read(raw[0], 0, 0);
+    set_scales();
+    convert(frag[0], raw[0], 0);
+  }
+  int slot = 0;
+#pragma unroll 1
+  for (int i = 0; i < slots; ++i) {
+    const int next = slot + 1 == R ? 0 : slot + 1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int s = u >> 1, t = u & 1;
+      if (u == 2) {
+        // the conversions so far stay in front of the branches, beside their step's products
+#pragma unroll
+        for (int e = 0; e < RB + CB; ++e) asm volatile("" : "+v"(frag[0][e]));
+        if (i + 1 < slots) wait(i + 1);
+        if (i + R < slots) load(i + R, slot);
+        read_scales(next);
+        read(raw[0], next, 0);  // past the last slot: bytes of the ring, not used
+      } else if (u == 0) {
+        read(raw[1], slot, 1);
+      }
+      if (u == 3) set_scales();
+      convert(frag[(u + 1) & 1], raw[(s + t) & 1], t ^ 1);
+#pragma unroll
+      for (int n = 0; n < CB; ++n)
+#pragma unroll
+        for (int m = 0; m < RB; ++m)
+          acc[n][m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag[u & 1][RB + n], frag[u & 1][m],
+                                                              acc[n][m], 0, 0, 0);
+      constexpr int CV = (4 * (RB + CB) + RB * CB - 1) / (RB * CB);
+      if (t == 0) __builtin_amdgcn_sched_group_barrier(0x100, RB + CB, 0);
+      if (u == 2) __builtin_amdgcn_sched_group_barrier(0x100, RB + CB, 0);
+#pragma unroll
+      for (int e = 0; e < RB * CB; ++e) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, CV, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    slot = next;
+  }
+  // the waves' sums meet in LDS, 32 rows at a time, in the order of the waves
+  float* out = reinterpret_cast<float*>(sm);
+#pragma unroll
+  for (int m = 0; m < RB; ++m) {
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < CB; ++n)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<floatx4*>(out + wave * S::OUT / 4 + (lane & 31) * S::ROW + 32 * n + 8 * q +
+                                    4 * h) =
+            floatx4{acc[n][m][4 * q], acc[n][m][4 * q + 1], acc[n][m][4 * q + 2],
+                    acc[n][m][4 * q + 3]};
+    __syncthreads();
+#pragma unroll 1
+    for (int e = tid; e < 32 * 8 * CB; e += 64 * W) {
+      const int row = e / (8 * CB), col = e % (8 * CB) * 4;
+      const float* p = out + row * S::ROW + col;
+      floatx4 v = *reinterpret_cast<const floatx4*>(p);
+#pragma unroll
+      for (int w = 1; w < W; ++w) v += *reinterpret_cast<const floatx4*>(p + w * S::OUT / 4);
+      epi_quad(a, mt * RB * 32 + m * 32 + row, (long)nt * CB * 32 + col, v);
+    }
+  }
+}
+
+template <int RB, int CB, int W, int R, int OCC>
+int launch_ring(Q8Lin& a, hipStream_t s) {
+  using S = RingShape<RB, CB, W, R>;
+  const auto kern = q8_ring_kernel<RB, CB, W, R, OCC>;
+  long grid;
+  LX_TRY(tile_grid(a, 32 * RB, 32 * CB, 64 * W, &grid));
+  static LdsLimit once;
+  LX_TRY(raise_lds_limit(reinterpret_cast<const void*>(kern), S::LDS, once, "q8_ring_kernel"));
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * W), S::LDS, s, a);
+  return check_launch("q8_ring_kernel");
+}
+
 template <int MT, int NT, int WAVES>
 int launch_stream(Q8Lin& a, hipStream_t s) {
   constexpr size_t lds = (size_t)MT * NT * WAVES * 1024;
@@ -440,18 +639,32 @@ extern "C" int lx_linear_q8_f32(const lx_q8* x, const lx_q8* w, const float* bia
     if ((long)N * a.w.kb >= 1 << 18) return launch_stream<1, 2, 8>(a, stream);
     return launch_stream<1, 1, 8>(a, stream);
   }
-  // The largest tiles that still give (nearly) every CU one; us, in the order of the tiles below:
-  //   4096 x 6761 x 896      73.7  81.4  95.6 112.5       4096 x 896 x 896  28.0  14.4  16.9  16.8
-  //   1000 x 6761 x 896      32.1  21.5  23.3  28.4        400 x 6761       30.7  15.5  12.5  14.7
-  //   1531 x 1152 x 896      27.5  12.3   9.5  10.6  10.8
-  //    177 x 6761 x 896      30.0  14.1   9.2   8.4  10.0
-  //    200 x 1500 x 3000     67.8  25.6  11.7   9.2  10.3
-  //    150 x  896 x 4864     99.6  35.5  15.9  12.1   8.9
   const long cus = device_cus();
   auto tiles = [&](long m, long n) { return ((M + m - 1) / m) * ((N + n - 1) / n); };
+  // The largest tiles that still give (nearly) every CU one: shared by a workgroup's waves
+  // while there are many (256 x 256, 128 x 128, 64 x 64, 32 x 64 on the tile kernel; us)
+  //   4096 x 6761 x 896   73.7  81.4  95.6 112.5      4096 x 896 x 896  28.0  14.4  16.9  16.8
+  //   1000 x 6761 x 896   32.1  21.5  23.3  28.4       400 x 6761       30.7  15.5  12.5  14.7
+  //   1531 x 1152 x 896   27.5  12.3   9.5  10.6       177 x 6761       30.0  14.1   9.2   8.4
   if (8 * tiles(256, 256) >= 7 * cus) return launch_tile<4, 2, 2, 4, 1, 2, 1>(a, stream);
   if (8 * tiles(128, 128) >= 7 * cus) return launch_tile<2, 2, 2, 2, 1, 2, 2>(a, stream);
-  if (2 * tiles(64, 64) >= 3 * cus) return launch_tile<2, 2, 1, 1, 4, 3, 3>(a, stream);
-  if (8 * tiles(32, 64) >= 5 * cus) return launch_tile<1, 2, 1, 1, 4, 4, 3>(a, stream);
-  return launch_stream<2, 2, 8>(a, stream);
+  // while the smallest give each CU one at most, and at 12 blocks of K or more while larger ones
+  // do, every wave on K of its own (32 x 32, 32 x 64, 64 x 64, 96 x 64 on the ring kernel, then 64 x
+  // 64 and 32 x 64 on the tile kernel)
+  //    256 x  896 x  896   3.7   4.3   5.9   7.4   6.0   4.8
+  //    256 x 1152 x  896   4.7   4.3   5.9   7.4   6.0   4.9
+  //    500 x 1500 x  896   6.6   7.6   6.5   8.3   6.7   6.5
+  //    500 x 1500 x 1500   8.2   9.9   7.8   9.9   8.4   8.4
+  //   1024 x 1024 x 4864  20.8  18.6  15.2  18.7  17.4  18.9
+  //   1531 x  896 x 1500  13.3  14.4  11.7  10.8  10.7  10.8
+  //   1531 x  896 x 4864  27.7  26.8  24.2  20.0  22.9  25.2
+  if (tiles(32, 32) <= cus) return launch_ring<1, 1, 8, 2, 2>(a, stream);
+  if (tiles(32, 64) <= cus) return launch_ring<1, 2, 8, 2, 2>(a, stream);
+  if (a.x.kb >= 12) {
+    if (tiles(64, 64) <= cus) return launch_ring<2, 2, 4, 2, 2>(a, stream);
+    if (tiles(96, 64) <= cus) return launch_ring<3, 2, 4, 2, 1>(a, stream);
+  } else if (2 * tiles(64, 64) < 3 * cus) {
+    return launch_tile<1, 2, 1, 1, 4, 4, 3>(a, stream);
+  }
+  return launch_tile<2, 2, 1, 1, 4, 3, 3>(a, stream);
 }

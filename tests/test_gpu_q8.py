@@ -201,7 +201,11 @@ LINEARS = [(1, 1, 1), (1, 16, 128), (1, 1152, 896), (2, 17, 129), (4, 6761, 896)
            (65, 257, 500), (100, 1152, 896), (128, 256, 128), (129, 895, 1280), (177, 6761, 896),
            (256, 9728, 896), (300, 896, 4864), (513, 300, 2000), (1531, 896, 896),
            (1025, 1030, 130), (3, 900, 8192), (2000, 1500, 1100), (2049, 2305, 257),
-           (2100, 4100, 384)]
+           (2100, 4100, 384),
+           # each tile size with one block of K, a short one, or a long and ragged one
+           (9, 4100, 8192), (300, 896, 100), (300, 898, 2100), (1531, 896, 64), (500, 1500, 1600),
+           (300, 1600, 4864), (1531, 900, 1600), (1400, 1000, 2177), (256, 9728, 100),
+           (2049, 2305, 100), (3600, 3800, 100), (3500, 3590, 700)]
 
 
 @pytest.mark.parametrize("M,N,K", LINEARS)
@@ -232,10 +236,11 @@ def test_every_product_counts(gpu, M, N, K):
     _same(ops.linear_q8(xq, wq), X @ W.t())
 
 
-@pytest.mark.parametrize("M,N", [(3, 40), (40, 33), (300, 200), (1100, 1300)])
-def test_scales_of_every_row_and_block(gpu, M, N):
+@pytest.mark.parametrize("M,N,K", [(3, 40, 1157), (40, 33, 1157), (300, 900, 1157),
+                                   (500, 1500, 1700), (1400, 900, 1700), (1100, 1300, 1157),
+                                   (1531, 1152, 300), (2100, 2100, 1157), (3590, 3598, 700)])
+def test_scales_of_every_row_and_block(gpu, M, N, K):
     """Blocks at powers of two of their own, one element each: every product has its scales."""
-    K = 128 * 9 + 5
     g = _gen(M)
     kb = (K + 127) // 128
     ex = torch.randint(-40, 40, (M, kb), generator=g)
@@ -265,7 +270,8 @@ def _epi(kind, acc, b=None, r=None):
 KINDS = {"none": None, "gelu": ops.LX_EPI_GELU_TANH, "resid": ops.LX_EPI_RESID,
          "swiglu": ops.LX_EPI_SWIGLU_PAIRED}
 EPI_SHAPES = [(1, 66, 896), (9, 68, 200), (40, 130, 300), (70, 1152, 896), (257, 514, 896),
-              (1030, 1026, 150)]
+              (1030, 1026, 150), (300, 898, 260), (500, 1502, 1600), (1531, 898, 1600),
+              (1531, 1152, 300), (2100, 2050, 130), (3590, 3598, 130)]
 
 
 @pytest.mark.parametrize("M,N,K", EPI_SHAPES)
@@ -323,7 +329,9 @@ def test_outputs_in_place_and_strided(gpu, M, N, K, pad):
     _same(z, want)
 
 
-@pytest.mark.parametrize("M,N,K", [(5, 40, 300), (70, 200, 300), (300, 300, 300), (1100, 1300, 300)])
+@pytest.mark.parametrize("M,N,K", [(5, 40, 300), (70, 200, 300), (300, 900, 300), (500, 1500, 1600),
+                                   (1400, 900, 1600), (1100, 1300, 300), (2100, 2100, 300),
+                                   (3590, 3598, 300)])
 def test_nan_stays_in_its_rows(gpu, M, N, K):
     g = _gen(8)
     x, w = torch.randn(M, K, generator=g), torch.randn(N, K, generator=g)
@@ -343,13 +351,14 @@ def test_nan_stays_in_its_rows(gpu, M, N, K):
 
 def test_rows_past_the_last(gpu):
     """The last tile's memory behind the last row of x and w holds NaN codes: nothing shows."""
-    for M, N in [(3, 21), (37, 70), (261, 300), (1029, 1100)]:
-        xq, wq, X, W = _pair(M, N, 300, 12, gpu)
+    for M, N, K in [(3, 21, 300), (37, 70, 300), (261, 900, 300), (499, 1501, 1600),
+                    (1401, 901, 1600), (1029, 1100, 300), (2101, 2101, 300), (3587, 3587, 200)]:
+        xq, wq, X, W = _pair(M, N, K, 12, gpu)
         y = ops.linear_q8(xq, wq)
-        held_x = ops.q8_pack(torch.full((-(-M // 16) * 16, 300), float("nan"), device=gpu))
-        held_w = ops.q8_pack(torch.full((-(-N // 16) * 16, 300), float("nan"), device=gpu))
-        x2 = ops.q8_pack(ops.q8_unpack(xq), out=ops.Q8Matrix(held_x.data, M, 300))
-        w2 = ops.q8_pack(ops.q8_unpack(wq), out=ops.Q8Matrix(held_w.data, N, 300))
+        held_x = ops.q8_pack(torch.full((-(-M // 16) * 16, K), float("nan"), device=gpu))
+        held_w = ops.q8_pack(torch.full((-(-N // 16) * 16, K), float("nan"), device=gpu))
+        x2 = ops.q8_pack(ops.q8_unpack(xq), out=ops.Q8Matrix(held_x.data, M, K))
+        w2 = ops.q8_pack(ops.q8_unpack(wq), out=ops.Q8Matrix(held_w.data, N, K))
         assert torch.equal(ops.linear_q8(x2, w2), y)
 
 
