@@ -244,7 +244,8 @@ __global__ __launch_bounds__(256) void logprob_kernel(LpArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(v[i][e]));
     };
-    auto gather = [&]() {  // into this wave's segment; false if one is too small
+    // into this wave's segment; false if one is too small
+    auto gather = [&](auto chosen) {
       int at = 0, t4 = 4 * tid;
       anew(t4);
 #pragma unroll
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(LpArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int k = t4 + 1024 * i + e;
-          const bool c = !(v[i][e] < from) && (!(v[i][e] == from) || k <= last);
+          const bool c = chosen(v[i][e], k);
           const unsigned long long mask = __ballot(c);
           if (mask) {
             const int to = at + lanes_below(mask);
@@ -272,7 +273,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(LpArgs a) {
       }
       return fit;
     };
-    if (!gather()) {
+    if (!gather([&](float x, int) { return !(x < from); })) {
       // counts of all four waves, a barrier each
       int turn = 1;
       auto count = [&](auto f) {
@@ -307,7 +308,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(LpArgs a) {
         return count([&](float x, int k) { return x == from && kPiece - 1 - k >= (int)mid; });
       });
       __syncthreads();  // the last counts are read
-      gather();
+      gather([&](float x, int k) { return !(x < from) && (!(x == from) || k <= last); });
     }
     rank_keys<256, 4, kSeg>(sh.cand, n, top, [&](int at, key_t64 key) {
       if (a.pieces > 1) {
