@@ -30,6 +30,7 @@ constexpr int kPiece = 8192;   // logits of a workgroup
 constexpr int kMaxTop = 64;    // a lane each
 constexpr int kCand = 1024;    // candidates ranked at once
 constexpr int kSeg = kCand / 4;  // of a wave
+constexpr int kJoin = 192;     // candidates ranked by the joining wave
 
 struct LpArgs {
   const float* x;
@@ -273,22 +274,33 @@ __global__ __launch_bounds__(256) void logprob_kernel(LpArgs a) {
       }
       return fit;
     };
-    if (!gather([&](float x, int) { return !(x < from); })) {
-      // counts of all four waves, a barrier each
-      int turn = 1;
-      auto count = [&](auto f) {
-        int c = 0, t4 = 4 * tid;
-        anew(t4);
+    // counts of all four waves, a barrier each
+    int turn = 1;
+    auto count = [&](auto f) {
+      int c = 0, t4 = 4 * tid;
+      anew(t4);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) c += lanes(f(v[i][e], t4 + 1024 * i + e));
-        if ((tid & 63) == 0) sh.n[turn][wave] = c;
-        __syncthreads();
-        c = (sh.n[turn][0] + sh.n[turn][1]) + (sh.n[turn][2] + sh.n[turn][3]);
-        turn ^= 1;
-        return c;
-      };
+        for (int e = 0; e < 4; ++e) c += lanes(f(v[i][e], t4 + 1024 * i + e));
+      if ((tid & 63) == 0) sh.n[turn][wave] = c;
+      __syncthreads();
+      c = (sh.n[turn][0] + sh.n[turn][1]) + (sh.n[turn][2] + sh.n[turn][3]);
+      turn ^= 1;
+      return c;
+    };
+    bool fit;
+    if (bound <= order_of(-inf)) {
+      // Fewer threads than `top` have a logit that is not masked (the others of a constrained
+      // choice, a whole piece of a masked vocabulary): these logits, and of the masked ones the
+      // lowest indices, `top` of which stand among as many indices as both together.
+      const int open = count([&](float x, int) { return !(x <= -inf); });
+      fit = gather([&](float x, int k) { return !(x <= -inf) || k < open + top; });
+    } else {
+      fit = gather([&](float x, int) { return !(x < from); });
+    }
+    if (!fit) {
+      turn = 1;  // sh.n[0] may still be read
       nans = count([](float x, int) { return x != x; }) >= top;
       if (nans) {
         // NaNs alone, the lowest indices: as infinities, the rest as nothing
@@ -324,7 +336,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(LpArgs a) {
 // The pieces of a row, one wave.  NR: keys a lane holds (0: any number, read again for each bit).
 template <int NR>
 __global__ __launch_bounds__(64) void logprob_join_kernel(LpArgs a) {
-  __shared__ key_t64 cand[kCand];
+  __shared__ key_t64 cand[kJoin];
   const int lane = threadIdx.x, row = blockIdx.x;
   const float4* part = a.part + (long)row * a.pieces;
   const float inf = __builtin_huge_valf();
@@ -381,7 +393,7 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LpArgs a) {
   unsigned order = largest_with(a.top, 31, 16, with);
   key_t64 bound = (key_t64)order << 32;
   int c = with(order);
-  if (c > kCand) {  // crowded: the exact order, and of its ties the lowest indices, 24 bits of them
+  if (c > kJoin) {  // crowded: the exact order, and of its ties the lowest indices, 24 bits of them
     order = largest_with(a.top, 31, 0, with);
     const int above = count([&](key_t64 key) { return (unsigned)(key >> 32) > order; });
     bound = (key_t64)order << 32 | 0xff000000u;
@@ -400,7 +412,7 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LpArgs a) {
   });
   __syncthreads();
   const int in_all[1] = {c};
-  rank_keys<64, 1, kCand>(cand, in_all, a.top, [&](int place, key_t64 key) {
+  rank_keys<64, 1, kJoin>(cand, in_all, a.top, [&](int place, key_t64 key) {
     a.top_ids[(long)row * a.top + place] = (int)~(unsigned)key;
     a.top_logp[(long)row * a.top + place] = logp_of(r, ls, value_of((unsigned)(key >> 32)));
   });

@@ -86,6 +86,36 @@ def test_masks(gpu, V):
     _check(x, t, 64, gpu)
 
 
+@pytest.mark.parametrize("V", [64, 130, 2048, 2500, 6761, 20000, 151936])
+@pytest.mark.parametrize("open_", [0, 1, 5, 63, 64, 200, 1500])
+def test_few_open_among_masked(gpu, V, open_):
+    """Logits open at the end, the start or anywhere of a masked row; the rest by lowest index."""
+    if open_ > V:
+        open_ = V // 2
+    announce(f"token_logprobs {open_} open of {V}")
+    g = _gen(V + open_)
+    x = torch.full((4, V), -INF)
+    for r, at in enumerate([torch.arange(open_), V - 1 - torch.arange(open_),
+                            torch.randperm(V, generator=g)[:open_],
+                            torch.randperm(V, generator=g)[:open_]]):
+        x[r, at] = torch.randn(open_, generator=g)
+    x[3, torch.randperm(V, generator=g)[:min(3, V)]] = float("nan")  # the largest logits
+    for top in (3, min(64, V)):
+        got = ops.token_logprobs(x.to(gpu), top=top)
+        key = torch.where(x.isnan(), torch.full_like(x, INF), x)
+        ids = torch.sort(key, dim=1, descending=True, stable=True).indices[:, :top]
+        assert torch.equal(got.top_ids.cpu().long(), ids)
+        assert got.top_logp[3].isnan().all()
+        if open_:
+            lp = torch.log_softmax(x[:3].double(), 1).gather(1, ids[:3])
+            fin = torch.isfinite(lp)
+            tl = got.top_logp[:3].cpu().double()
+            assert torch.equal(tl[~fin], lp[~fin])
+            assert ((tl - lp).abs()[fin] <= 2.0 ** -16 + 2.0 ** -24 * lp.abs()[fin]).all()
+        else:
+            assert (got.top_logp[:3] == -INF).all()
+
+
 @pytest.mark.parametrize("V", [70, 6761, 9000])
 def test_rows_of_nothing(gpu, V):
     x = torch.full((3, V), -INF)
