@@ -467,8 +467,8 @@ int lx_attention_kv4_f32(const float* q, long ldq, const lx_kv4* cache, const in
  * consecutive elements of a row (the last one short where K ends inside it) share
  * 2^e, e the smallest integer >= -127 with max|v| <= 448 * 2^e over the block's finite
  * elements; an element is the e4m3 number nearest to v / 2^e (ties to even) and stands
- * for that number times 2^e, off by at most 2^-4 of itself or 2^(e - 10).  Infinities
- * and NaN stand for NaN.  `data`: device memory of lx_q8_bytes() bytes (0 for a bad
+ * for that number times 2^e, off by at most 2^-4 of itself or 2^(e - 10) (past fp32's
+ * range, from 2^128 on: infinity).  Infinities and NaN stand for NaN.  `data`: device memory of lx_q8_bytes() bytes (0 for a bad
  * shape), 16-byte aligned, which needs no initialisation.
  * lx_q8_pack_f32 writes x (row stride ldx) into q; lx_q8_unpack_f32 what q stands for
  * into x.  At most 2^27 blocks of rows, counted one by one.  x and q must not overlap.
@@ -493,8 +493,8 @@ int lx_rmsnorm_q8_f32(const float* x, long ldx, const float* add, long lda, floa
                       const float* w, float eps, const lx_q8* q, hipStream_t stream);
 
 /* y = epi(x~ @ w~^T + bias), x~ (M, K) and w~ (N, K) what x and w stand for: exact
- * products, each block of 128 scaled by its power of two, fp32 sums.  y: (M, N), row
- * stride ldy (N / 2 columns for SWIGLU_PAIRED, N even).  Epilogues: none, GELU_TANH,
+ * products, fp32 sums (elements below 2^-126 in magnitude lose digits, below 2^-133 they
+ * count as zero).  y: (M, N), row stride ldy (N / 2 columns for SWIGLU_PAIRED, N even).  Epilogues: none, GELU_TANH,
  * RESID (y = resid + .., resid row stride ldr; NULL: y itself, in place),
  * SWIGLU_PAIRED; others: LX_ERR_ARG.  bias (N) or NULL.  y must not overlap resid
  * otherwise, nor another operand.  A NaN in a row of x or w makes NaN of the outputs

@@ -5,16 +5,15 @@
 // but for that one rounding: a power of two, and v_cvt_pk_fp8_f32 rounds to nearest even).  The
 // scales are held as bytes e + 127, the exponent field of 2^e.
 //
-// Memory: tiles of 16 rows x 128 elements, 2 KB each, the blocks of K of a row tile side by side.
-// A row's 128 bytes are one line, so that its producer writes whole lines; its eight 16-byte
-// chunks stand at chunk ^ (row / 2 % 8), which spreads the 16 rows that a ds_read_b128 of a
-// fragment touches over all 64 banks: tiles go to LDS as they lie.  (In the lanes' order, the other
-// layout free of conflicts, a row's block is eight pieces in as many lines.)  Which
-// elements of a block a lane multiplies in one instruction does not matter while both operands
-// agree and a block has one scale: a lane takes 16-byte chunks.  Behind the codes the scales, a byte a row: 16 bytes per tile, tiles in the
-// same order.
-// Elements past the end of a row are zero; rows past the last may hold anything and only reach
-// outputs that are not stored.
+// Memory: tiles of 16 rows x 128 elements, 2 KB each, the blocks of K of a row tile side by side. A
+// row's 128 bytes are one line, so that its producer writes whole lines; its eight 16-byte chunks
+// stand at chunk ^ (row / 2 % 8), which spreads the 16 rows that a ds_read_b128 of a fragment
+// touches over all 64 banks: tiles go to LDS as they lie.  (In the lanes' order, the other layout
+// free of conflicts, a row's block is eight pieces in as many lines.)  Which elements of a block a
+// lane multiplies in one instruction does not matter while both operands agree and a block has one
+// scale: a lane takes 16-byte chunks.  Behind the codes the scales, a byte a row: 16 bytes per
+// tile, tiles in the same order. Elements past the end of a row are zero; rows past the last may
+// hold anything and only reach outputs that are not stored.
 #pragma once
 
 #include "lx_common.hpp"

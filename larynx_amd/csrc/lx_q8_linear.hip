@@ -1,4 +1,5 @@
-// y = epi(x~ W~^T + bias), both operands in 8 bits with a power of two per block of 128 (lx_q8.hpp).
+// y = epi(x~ W~^T + bias), both operands in 8 bits with a power of two per block of 128
+// (lx_q8.hpp).
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -28,8 +29,8 @@ struct Q8Lin {
 
 // x / (1 + e^-x) on the hardware's exponential and reciprocal, each within an ulp or so; the
 // argument's product with log2(e) in two parts, so that the exponential keeps its relative error
-// far from zero.  (Against expf and a division a third of the instructions; 256 x 9728 x 896 12.5 ->
-// 11.9 us.)  Below -87 the factor stays e^-87.
+// far from zero.  (Against expf and a division a third of the instructions; 256 x 9728 x 896 12.5
+// -> 11.9 us.)  Below -87 the factor stays e^-87.
 __device__ __forceinline__ float silu_hw(float x) {
   const float c = fmaxf(x, -87.0f), hi = c * -1.4426950408889634f;
   const float lo = fmaf(c, -1.4426950408889634f, -hi) + c * -1.9259629911266175e-8f;
@@ -86,9 +87,11 @@ __device__ __forceinline__ bf16x8_t q8_frag(int lo, int hi, float scale) {
   return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// A workgroup owns 16 MT rows of x and 16 NT rows of W; its waves take the blocks of K in turn and
-// their sums meet in LDS.  W is the instruction's A operand: a lane's four sums are four
-// consecutive columns of one row of y.
+// Up to 16 rows.  A workgroup owns 16 MT rows of x and 16 NT rows of W; its waves take the blocks
+// of K in turn, straight from memory to registers, and their sums meet in LDS.  W is the
+// instruction's A operand: a lane's four sums are four consecutive columns of one row of y.  Bound
+// by the weights' bytes (16 x 8192 x 8192 12.7 us, 5.3 TB/s; 16 x 151936 x 896 31, 4.7) or a launch
+// and one round trip (1 x 1152 x 896 2.6 us in a graph).
 template <int MT, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void q8_stream_kernel(Q8Lin a) {
   extern __shared__ __attribute__((aligned(16))) floatx4 red[];
@@ -155,15 +158,6 @@ __global__ __launch_bounds__(64 * WAVES) void q8_stream_kernel(Q8Lin a) {
   }
 }
 
-// Many rows.  A workgroup owns (32 RB WM) x (32 CB WN) outputs; both operands go through LDS as they
-// lie in memory (no registers, no ds_write), a block of K a stage, NS stages deep.  WK waves share
-// each (32 RB) x (32 CB) of the outputs, taking 128 / WK of a stage's 128 each: a wave's tile is as
-// large as its registers hold, since what a tile costs beside its products is the conversion of
-// its operands (8 cycles for 128 codes; an instruction of 32 x 32 x 16 takes 32).
-// A step is 16 of K; while its products run, the next step's codes are converted, and those of
-// the step after are on their way from LDS.  The one barrier of a stage stands before its last two
-// steps, whose operands every wave has by then: the buffer is free for the stage NS further on, and
-// the next stage's first reads return behind those steps' products.
 // This workgroup's tile of y.  Each XCD (workgroups are dealt to them round-robin) takes a
 // contiguous run of tiles, which go down and then along bands of a.band rows of tiles: about a
 // square, the fewest bytes for its L2 (4096 x 8192 x 8192 442 -> 423 us against runs of columns).
@@ -193,6 +187,20 @@ __device__ __forceinline__ void wait_vm() {  // vmcnt(N) lgkmcnt(0)
   asm volatile("" ::: "memory");  // no read of LDS moves in front of it
 }
 
+// Many rows.  A workgroup owns (32 RB WM) x (32 CB WN) outputs; both operands go through LDS as
+// they lie in memory (no registers, no ds_write), a block of K a stage, NS stages deep.  WK waves
+// share each (32 RB) x (32 CB) of the outputs, taking 128 / WK of a stage's 128 each: a wave's tile
+// is as large as its registers hold, since what a tile costs beside its products is the conversion
+// of its operands (8 cycles for 128 codes; an instruction of 32 x 32 x 16 takes 32). A step is 16
+// of K; while its products run, the next step's codes are converted, and those of the step after
+// are on their way from LDS.  The one barrier of a stage stands before its last two steps, whose
+// operands every wave has by then: the buffer is free for the stage NS further on, and the next
+// stage's first reads return behind those steps' products. 4096 x 8192 x 8192 on 256 x 256 tiles:
+// 400-455 us by box and heat, 1.2-1.38 PFLOP/s, as a bf16 product of the library (1.37): the power
+// limit leaves 1.8 GHz, at which the matrix pipe is 0.65 to 0.68 busy; four waves of 128 x 128 and
+// eight of 64 x 128 give the same.  256 x 9728 x 896 on 64 x 64: 11 us, of which 3 move its bytes:
+// 608 tiles of seven stages, each bounded by its loads' and its reads' latency (without the
+// products 9.3, without conversions 10.5).
 template <int RB, int CB, int WM, int WN, int WK, int NS>
 struct TileShape {
   static constexpr int WAVES = WM * WN * WK;
@@ -402,11 +410,14 @@ int launch_tile(Q8Lin& a, hipStream_t s) {
   return check_launch("q8_tile_kernel");
 }
 
-// Fewer rows.  A workgroup owns (32 RB) x (32 CB) outputs and each of its W waves takes every W-th 64
-// of K, through a ring of R slots of LDS of its own: no barrier until the waves' sums meet, and
-// (R - 1) slots of every wave on their way.  A slot's tile is 16 rows x 64 bytes, 1 KB, which one
-// instruction brings: lane 4 row + q loads chunk q ^ (row / 4 % 4) of its row's half block, so that
-// the 16 rows of a read are spread over all banks.
+// Fewer tiles than CUs.  A workgroup owns (32 RB) x (32 CB) outputs and each of its W waves takes
+// every W-th 64 of K, through a ring of R slots of LDS of its own: no barrier until the waves' sums
+// meet, and R - 1 slots of every wave on their way.  A slot's tile is 16 rows x 64 bytes, 1 KB,
+// which one instruction brings: lane 4 row + q loads chunk q ^ (row / 4 % 4) of its row's half
+// block, so that the 16 rows of a read are spread over all banks. 1531 x 896 x 4864 on 96 x 64:
+// 20-22 us (0.65 PFLOP/s) where 64 x 64 on the tile kernel takes 22.5: 224 workgroups, a wave a
+// SIMD, whose 456 matrix instructions and 1520 conversions hardly overlap in one wave.  256 x 896 x
+// 4864 on 32 x 32: 7.9.
 template <int RB, int CB, int W, int R>
 struct RingShape {
   static constexpr int T = 2 * (RB + CB);  // 16-row tiles of a slot: rows of x, then of W
@@ -649,8 +660,8 @@ extern "C" int lx_linear_q8_f32(const lx_q8* x, const lx_q8* w, const float* bia
   if (8 * tiles(256, 256) >= 7 * cus) return launch_tile<4, 2, 2, 4, 1, 2, 1>(a, stream);
   if (8 * tiles(128, 128) >= 7 * cus) return launch_tile<2, 2, 2, 2, 1, 2, 2>(a, stream);
   // while the smallest give each CU one at most, and at 12 blocks of K or more while larger ones
-  // do, every wave on K of its own (32 x 32, 32 x 64, 64 x 64, 96 x 64 on the ring kernel, then 64 x
-  // 64 and 32 x 64 on the tile kernel)
+  // do, every wave on K of its own (32 x 32, 32 x 64, 64 x 64, 96 x 64 on the ring kernel, then 64
+  // x 64 and 32 x 64 on the tile kernel)
   //    256 x  896 x  896   3.7   4.3   5.9   7.4   6.0   4.8
   //    256 x 1152 x  896   4.7   4.3   5.9   7.4   6.0   4.9
   //    500 x 1500 x  896   6.6   7.6   6.5   8.3   6.7   6.5
