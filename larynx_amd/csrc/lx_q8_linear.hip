@@ -411,28 +411,33 @@ int launch_tile(Q8Lin& a, hipStream_t s) {
 }
 
 // Fewer tiles than CUs.  A workgroup owns (32 RB) x (32 CB) outputs and each of its W waves takes
-// every W-th 64 of K, through a ring of R slots of LDS of its own: no barrier until the waves' sums
-// meet, and R - 1 slots of every wave on their way.  A slot's tile is 16 rows x 64 bytes, 1 KB,
-// which one instruction brings: lane 4 row + q loads chunk q ^ (row / 4 % 4) of its row's half
-// block, so that the 16 rows of a read are spread over all banks. 1531 x 896 x 4864 on 96 x 64:
-// 20-22 us (0.65 PFLOP/s) where 64 x 64 on the tile kernel takes 22.5: 224 workgroups, a wave a
-// SIMD, whose 456 matrix instructions and 1520 conversions hardly overlap in one wave.  256 x 896 x
-// 4864 on 32 x 32: 7.9.
-template <int RB, int CB, int W, int R>
+// every W-th block of K (H = 2) or half of one (H = 1), through a ring of R slots of LDS of its own:
+// no barrier until the waves' sums meet, and R - 1 slots of every wave on their way.  A block's
+// tile is 2 KB as it lies, two instructions.  Of a half block it is 16 rows x 64 bytes, one
+// instruction: lane 4 row + q loads chunk q ^ (row / 4 % 4) of its row's half, so that the 16 rows
+// of a read are spread over all banks.  Halves of lines arrive at 17-23 TB/s of the card, whole
+// ones at 27-31; but whole blocks of 96 x 64 leave LDS for three waves.  1531 x 896 x 4864 on 96 x
+// 64: 20-22 us (0.65 PFLOP/s) with four waves on halves, 21.9 with three on blocks, where 64 x 64
+// on the tile kernel takes 22.5; the loads alone take 18, the products and conversions alone 16.
+// 256 x 896 x 4864 on 32 x 32: 6.9 on blocks, 7.9 on halves.
+template <int RB, int CB, int W, int H, int R>
 struct RingShape {
   static constexpr int T = 2 * (RB + CB);  // 16-row tiles of a slot: rows of x, then of W
   static_assert(T <= 16, "one instruction loads a slot's scales");
-  static constexpr int SLOT = T * 1024 + 256;  // the scales behind the codes
+  static constexpr int CODES = T * H * 1024;
+  static constexpr int SLOT = CODES + 256;  // the scales behind the codes
   static constexpr int ROW = 32 * CB + 4;  // floats of a row of outputs in LDS
   static constexpr int OUT = 32 * ROW * 4;  // a wave's 32 rows
   static constexpr int LDS = W * (R * SLOT > OUT ? R * SLOT : OUT);
   static_assert(LDS <= 160 * 1024, "LDS of a CU");
-  static_assert((R - 2) * (T + 1) < 64, "vmcnt");
+  static constexpr int LOADS = T * H + 1;  // instructions that load a slot
+  static_assert(H == 1 || H == 2, "half a block or a block");
+  static_assert((R - 2) * LOADS < 64, "vmcnt");
 };
 
-template <int RB, int CB, int W, int R, int OCC>
+template <int RB, int CB, int W, int H, int R, int OCC>
 __global__ __launch_bounds__(64 * W, OCC) void q8_ring_kernel(Q8Lin a) {
-  using S = RingShape<RB, CB, W, R>;
+  using S = RingShape<RB, CB, W, H, R>;
   constexpr int T = S::T;
   extern __shared__ __attribute__((aligned(16))) unsigned char sm[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -440,7 +445,7 @@ __global__ __launch_bounds__(64 * W, OCC) void q8_ring_kernel(Q8Lin a) {
   int mt, nt;
   tile_at(a, mt, nt);
   const int mtiles = (a.x.rows + 15) / 16, ntiles = (a.w.rows + 15) / 16;
-  const int kb = a.x.kb, slots = (2 * kb - wave + W - 1) / W;  // this wave's
+  const int kb = a.x.kb, slots = (2 * kb / H - wave + W - 1) / W;  // this wave's
   auto tile_of = [&](int t) {
     return t < 2 * RB ? min(mt * 2 * RB + t, mtiles - 1)
                       : min(nt * 2 * CB + min(t - 2 * RB, 2 * CB - 1), ntiles - 1);
@@ -454,28 +459,34 @@ __global__ __launch_bounds__(64 * W, OCC) void q8_ring_kernel(Q8Lin a) {
     const int t = lane >> 2;
     sbase = (t < 2 * RB ? a.x.scales : a.w.scales) + (long)tile_of(t) * kb * 16 + (lane & 3) * 4;
   }
-  // the chunk of half block 0 that this lane loads; of half block 1 it is this ^ 64
+  // where this lane loads of a tile; of a block's second half it is this ^ 64
   const int lr = lane >> 2;
-  const int lat = lr * kQ8Block + ((((lane & 3) ^ (lr >> 2)) ^ (lr >> 1)) << 4);
+  const int lat =
+      H == 2 ? lane * 16 : lr * kQ8Block + ((((lane & 3) ^ (lr >> 2)) ^ (lr >> 1)) << 4);
   typedef const __attribute__((address_space(1))) void* global_ptr;
   typedef __attribute__((address_space(3))) void* lds_ptr;
   unsigned char* ring = sm + wave * R * S::SLOT;
   auto load = [&](int i, int slot) {
-    const int hb = i * W + wave;
-    const long off = (long)(hb >> 1) * kQ8Tile;
-    const int at = lat ^ ((hb & 1) << 6);
+    const int j = i * W + wave, block = H == 2 ? j : j >> 1;
+    const long off = (long)block * kQ8Tile;
+    const int at = H == 2 ? lat : lat ^ ((j & 1) << 6);
     unsigned char* d = ring + slot * S::SLOT;
 #pragma unroll
-    for (int t = 0; t < T; ++t)
-      __builtin_amdgcn_global_load_lds((global_ptr)(base[t] + off + at), (lds_ptr)(d + t * 1024),
-                                       16, 0, 0);
-    __builtin_amdgcn_global_load_lds((global_ptr)(sbase + (long)(hb >> 1) * 16),
-                                     (lds_ptr)(d + T * 1024), 4, 0, 0);
+    for (int t = 0; t < T; ++t) {
+      __builtin_amdgcn_global_load_lds((global_ptr)(base[t] + off + at),
+                                       (lds_ptr)(d + t * H * 1024), 16, 0, 0);
+      if constexpr (H == 2)  // the offset counts on both sides
+        __builtin_amdgcn_global_load_lds((global_ptr)(base[t] + off + at),
+                                         (lds_ptr)(d + t * H * 1024), 16, 1024, 0);
+    }
+    __builtin_amdgcn_global_load_lds((global_ptr)(sbase + (long)block * 16),
+                                     (lds_ptr)(d + S::CODES), 4, 0, 0);
   };
   const int r = lane & 15, h = lane >> 5, half = (lane >> 4) & 1;
-  int at[2];
+  int at[2 * H];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) at[s] = half * 1024 + r * 64 + (((2 * s + h) ^ (r >> 2)) << 4);
+  for (int s = 0; s < 2 * H; ++s)
+    at[s] = (half * 16 + r) * H * 64 + (((2 * s + h) ^ (H == 2 ? r >> 1 : r >> 2)) << 4);
   floatx16 acc[CB][RB];
 #pragma unroll
   for (int n = 0; n < CB; ++n)
@@ -490,10 +501,10 @@ __global__ __launch_bounds__(64 * W, OCC) void q8_ring_kernel(Q8Lin a) {
   auto read = [&](intx4 (&f)[RB + CB], int slot, int s) {
     const unsigned char* b = ring + slot * S::SLOT + at[s];
 #pragma unroll
-    for (int i = 0; i < RB + CB; ++i) f[i] = *reinterpret_cast<const intx4*>(b + i * 2048);
+    for (int i = 0; i < RB + CB; ++i) f[i] = *reinterpret_cast<const intx4*>(b + i * H * 2048);
   };
   auto read_scales = [&](int slot) {
-    const unsigned char* b = ring + slot * S::SLOT + T * 1024 + half * 16 + r;
+    const unsigned char* b = ring + slot * S::SLOT + S::CODES + half * 16 + r;
 #pragma unroll
     for (int i = 0; i < RB + CB; ++i) us[i] = b[i * 32];
   };
@@ -508,7 +519,7 @@ __global__ __launch_bounds__(64 * W, OCC) void q8_ring_kernel(Q8Lin a) {
   // slot i is in LDS (R - 2 later ones may be on their way), and this wave's reads are done
   auto wait = [&](int i) {
     if (i + R - 2 < slots)
-      wait_vm<(R - 2) * (T + 1)>();
+      wait_vm<(R - 2) * S::LOADS>();
     else
       wait_vm<0>();
   };
@@ -527,9 +538,9 @@ __global__ __launch_bounds__(64 * W, OCC) void q8_ring_kernel(Q8Lin a) {
   for (int i = 0; i < slots; ++i) {
     const int next = slot + 1 == R ? 0 : slot + 1;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < 4 * H; ++u) {
       const int s = u >> 1, t = u & 1;
-      if (u == 2) {
+      if (u == 4 * H - 2) {
         // the conversions so far stay in front of the branches, beside their step's products
 #pragma unroll
         for (int e = 0; e < RB + CB; ++e) asm volatile("" : "+v"(frag[0][e]));
@@ -537,10 +548,10 @@ __global__ __launch_bounds__(64 * W, OCC) void q8_ring_kernel(Q8Lin a) {
         if (i + R < slots) load(i + R, slot);
         read_scales(next);
         read(raw[0], next, 0);  // past the last slot: bytes of the ring, not used
-      } else if (u == 0) {
-        read(raw[1], slot, 1);
+      } else if (t == 0) {
+        read(raw[(s + 1) & 1], slot, s + 1);
       }
-      if (u == 3) set_scales();
+      if (u == 4 * H - 1) set_scales();
       convert(frag[(u + 1) & 1], raw[(s + t) & 1], t ^ 1);
 #pragma unroll
       for (int n = 0; n < CB; ++n)
@@ -550,7 +561,7 @@ __global__ __launch_bounds__(64 * W, OCC) void q8_ring_kernel(Q8Lin a) {
                                                               acc[n][m], 0, 0, 0);
       constexpr int CV = (4 * (RB + CB) + RB * CB - 1) / (RB * CB);
       if (t == 0) __builtin_amdgcn_sched_group_barrier(0x100, RB + CB, 0);
-      if (u == 2) __builtin_amdgcn_sched_group_barrier(0x100, RB + CB, 0);
+      if (u == 4 * H - 2) __builtin_amdgcn_sched_group_barrier(0x100, RB + CB, 0);
 #pragma unroll
       for (int e = 0; e < RB * CB; ++e) {
         __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
@@ -586,10 +597,10 @@ __global__ __launch_bounds__(64 * W, OCC) void q8_ring_kernel(Q8Lin a) {
   }
 }
 
-template <int RB, int CB, int W, int R, int OCC>
+template <int RB, int CB, int W, int H, int R, int OCC>
 int launch_ring(Q8Lin& a, hipStream_t s) {
-  using S = RingShape<RB, CB, W, R>;
-  const auto kern = q8_ring_kernel<RB, CB, W, R, OCC>;
+  using S = RingShape<RB, CB, W, H, R>;
+  const auto kern = q8_ring_kernel<RB, CB, W, H, R, OCC>;
   long grid;
   LX_TRY(tile_grid(a, 32 * RB, 32 * CB, 64 * W, &grid));
   static LdsLimit once;
@@ -662,18 +673,20 @@ extern "C" int lx_linear_q8_f32(const lx_q8* x, const lx_q8* w, const float* bia
   // while the smallest give each CU one at most, and at 12 blocks of K or more while larger ones
   // do, every wave on K of its own (32 x 32, 32 x 64, 64 x 64, 96 x 64 on the ring kernel, then 64
   // x 64 and 32 x 64 on the tile kernel)
-  //    256 x  896 x  896   3.7   4.3   5.9   7.4   6.0   4.8
-  //    256 x 1152 x  896   4.7   4.3   5.9   7.4   6.0   4.9
-  //    500 x 1500 x  896   6.6   7.6   6.5   8.3   6.7   6.5
-  //    500 x 1500 x 1500   8.2   9.9   7.8   9.9   8.4   8.4
-  //   1024 x 1024 x 4864  20.8  18.6  15.2  18.7  17.4  18.9
-  //   1531 x  896 x 1500  13.3  14.4  11.7  10.8  10.7  10.8
-  //   1531 x  896 x 4864  27.7  26.8  24.2  20.0  22.9  25.2
-  if (tiles(32, 32) <= cus) return launch_ring<1, 1, 8, 2, 2>(a, stream);
-  if (tiles(32, 64) <= cus) return launch_ring<1, 2, 8, 2, 2>(a, stream);
+  //    256 x  896 x  896   3.5   4.3   5.8   7.3   6.0   4.8
+  //    256 x  896 x 4864   6.9   9.3  13.1  17.5  16.1  12.3
+  //    256 x 1152 x  896   5.6   4.3   5.8   7.4   6.1   4.9
+  //    128 x 4096 x 4864  12.7  10.2  13.5  16.8  16.4  12.8
+  //    500 x 1500 x  896   8.6   7.8   6.5   8.5   6.7   6.4
+  //    500 x 1500 x 1500  10.4   9.8   7.8  10.0   8.5   8.4
+  //   1024 x 1024 x 4864  22.3  18.0  16.2  18.7  17.0  17.6
+  //   1531 x  896 x 1500  18.1  14.1  11.5  10.4  10.7  10.7
+  //   1531 x  896 x 4864  31.3  24.8  24.1  19.6  21.8  23.0
+  if (tiles(32, 32) <= cus) return launch_ring<1, 1, 8, 2, 2, 1>(a, stream);
+  if (tiles(32, 64) <= cus) return launch_ring<1, 2, 4, 2, 2, 1>(a, stream);
   if (a.x.kb >= 12) {
-    if (tiles(64, 64) <= cus) return launch_ring<2, 2, 4, 2, 2>(a, stream);
-    if (tiles(96, 64) <= cus) return launch_ring<3, 2, 4, 2, 1>(a, stream);
+    if (tiles(64, 64) <= cus) return launch_ring<2, 2, 4, 1, 2, 2>(a, stream);
+    if (tiles(96, 64) <= cus) return launch_ring<3, 2, 4, 1, 2, 1>(a, stream);
   } else if (2 * tiles(64, 64) < 3 * cus) {
     return launch_tile<1, 2, 1, 1, 4, 4, 3>(a, stream);
   }
