@@ -8,6 +8,7 @@ liblxops.so; a failing call raises LxError (no fallback path exists).
 """
 import ctypes as C
 import struct
+from operator import attrgetter
 from typing import NamedTuple, Optional
 
 import torch
@@ -534,7 +535,11 @@ def attention_kv4(q, cache, lens, n_heads, scale=None, causal=True, out=None, ma
 class Q8Matrix:
     """A matrix (rows, K) in 8 bits: e4m3 codes with a power of two per 128 elements of a row, as
     q8_pack and rms_norm_q8 lay them out in `data`."""
-    __slots__ = ("data", "rows", "K", "_dev", "_ref")
+    __slots__ = ("_data", "_rows", "_K", "_dev", "_ref")
+    # read only: _ref holds what they say
+    data = property(attrgetter("_data"))
+    rows = property(attrgetter("_rows"))
+    K = property(attrgetter("_K"))
 
     def __init__(self, data, rows, K):
         n = lib.lx_q8_bytes(rows, K)
@@ -543,9 +548,12 @@ class Q8Matrix:
         self._set(data, rows, K)
 
     def _set(self, data, rows, K):
-        self.data, self.rows, self.K, self._dev = data, rows, K, data.get_device()
+        self._data, self._rows, self._K, self._dev = data, rows, K, data.get_device()
         self._ref = _pack_q8(data.data_ptr(), rows, K)  # an lx_q8: a ctypes one takes 0.5 us
         return self
+
+    def __reduce__(self):  # a copy has bytes, and an address, of its own
+        return Q8Matrix, (self._data, self._rows, self._K)
 
 
 _pack_q8 = struct.Struct("@Pii").pack
@@ -558,7 +566,7 @@ def _q8_out(like, rows, K, out):
         if not n:
             raise ValueError(f"no 8-bit form of a ({rows}, {K}) matrix")
         return _new(Q8Matrix)._set(like.new_empty(n, dtype=_U8), rows, K)
-    if out.rows != rows or out.K != K:
+    if out._rows != rows or out._K != K:
         raise ValueError(f"out must hold a ({rows}, {K}) matrix")
     if out._dev != like.get_device():
         _elsewhere("out")
@@ -603,8 +611,8 @@ def q8_unpack(q):
     dev = q._dev
     if dev < 0 or dev != _current():
         _elsewhere("q")
-    K = q.K
-    x = q.data.new_empty(q.rows, K, dtype=_F32)
+    K = q._K
+    x = q._data.new_empty(q._rows, K, dtype=_F32)
     check(lib.lx_q8_unpack_f32(q._ref, x.data_ptr(), K, _raw_stream(dev)))
     return x
 
@@ -641,7 +649,7 @@ def linear_q8(x, w, b=None, epilogue=None, resid=None, out=None):
     dev = x._dev
     if dev < 0 or dev != w._dev or dev != _current():
         _elsewhere("x, as w,")
-    M, N = x.rows, w.rows
+    M, N = x._rows, w._rows
     kind = LX_EPI_NONE if epilogue is None else epilogue.kind
     cols = N // 2 if kind == LX_EPI_SWIGLU_PAIRED else N
     bias = pr = None
@@ -658,7 +666,7 @@ def linear_q8(x, w, b=None, epilogue=None, resid=None, out=None):
     if out is None:
         if kind == LX_EPI_RESID and resid is None:
             raise ValueError("residual epilogues need resid=, or out= (the residual stream)")
-        out = x.data.new_empty(M, cols, dtype=_F32)
+        out = x._data.new_empty(M, cols, dtype=_F32)
         ldy = cols
     else:
         ldy = _like(out, "out", M, cols, dev)

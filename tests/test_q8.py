@@ -1,5 +1,7 @@
 """The 8-bit and scoring entry points without a GPU: sizes, and what they refuse before any work."""
+import copy
 import ctypes as C
+import pickle
 
 import pytest
 import torch
@@ -184,6 +186,20 @@ def test_matrix_of_other_bytes():
             ops.Q8Matrix(data, 4, 256)
     with pytest.raises(ValueError, match="8-bit"):
         ops.Q8Matrix(torch.zeros(n, dtype=torch.uint8), 0, 256)
+
+
+def test_matrix_copies():
+    """A copy names its own bytes, not those of the matrix that it was made from; what a matrix says
+    of itself does not change under it."""
+    n = lib.lx_q8_bytes(4, 256)
+    q = ops.Q8Matrix(torch.arange(n).to(torch.uint8), 4, 256)
+    for c in [copy.deepcopy(q), pickle.loads(pickle.dumps(q)), copy.copy(q)]:
+        assert (c.rows, c.K) == (4, 256) and torch.equal(c.data, q.data)
+        assert Q8.from_buffer_copy(c._ref).data == c.data.data_ptr()
+    assert copy.deepcopy(q).data.data_ptr() != q.data.data_ptr()
+    for name, value in [("data", torch.zeros(n, dtype=torch.uint8)), ("rows", 3), ("K", 128)]:
+        with pytest.raises(AttributeError):
+            setattr(q, name, value)
 
 
 @pytest.mark.parametrize("x", [torch.zeros(4, 8, dtype=torch.float64), torch.zeros(4),
