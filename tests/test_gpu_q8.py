@@ -205,7 +205,9 @@ LINEARS = [(1, 1, 1), (1, 16, 128), (1, 1152, 896), (2, 17, 129), (4, 6761, 896)
            # each tile size with one block of K, a short one, or a long and ragged one
            (9, 4100, 8192), (300, 896, 100), (300, 898, 2100), (1531, 896, 64), (500, 1500, 1600),
            (300, 1600, 4864), (1531, 900, 1600), (1400, 1000, 2177), (256, 9728, 100),
-           (2049, 2305, 100), (3600, 3800, 100), (3500, 3590, 700)]
+           (2049, 2305, 100), (3600, 3800, 100), (3500, 3590, 700),
+           # several blocks a wave on the smallest tiles
+           (200, 700, 4864), (40, 900, 2200), (130, 800, 1200)]
 
 
 @pytest.mark.parametrize("M,N,K", LINEARS)
@@ -238,7 +240,8 @@ def test_every_product_counts(gpu, M, N, K):
 
 @pytest.mark.parametrize("M,N,K", [(3, 40, 1157), (40, 33, 1157), (300, 900, 1157),
                                    (500, 1500, 1700), (1400, 900, 1700), (1100, 1300, 1157),
-                                   (1531, 1152, 300), (2100, 2100, 1157), (3590, 3598, 700)])
+                                   (1531, 1152, 300), (2100, 2100, 1157), (3590, 3598, 700),
+                                   (60, 200, 2300), (60, 6100, 2300)])
 def test_scales_of_every_row_and_block(gpu, M, N, K):
     """Blocks at powers of two of their own, one element each: every product has its scales."""
     g = _gen(M)
