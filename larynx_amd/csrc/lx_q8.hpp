@@ -6,14 +6,16 @@
 // scales are held as bytes e + 127, the exponent field of 2^e.
 //
 // Memory: tiles of 16 rows x 128 elements, 2 KB each, the blocks of K of a row tile side by side. A
-// row's 128 bytes are one line, so that its producer writes whole lines; its eight 16-byte chunks
-// stand at chunk ^ (row / 2 % 8), which spreads the 16 rows that a ds_read_b128 of a fragment
-// touches over all 64 banks: tiles go to LDS as they lie.  (In the lanes' order, the other layout
-// free of conflicts, a row's block is eight pieces in as many lines.)  Which elements of a block a
-// lane multiplies in one instruction does not matter while both operands agree and a block has one
-// scale: a lane takes 16-byte chunks.  Behind the codes the scales, a byte a row: 16 bytes per
-// tile, tiles in the same order. Elements past the end of a row are zero; rows past the last may
-// hold anything and only reach outputs that are not stored.
+// tile is its first 64 columns, then its last, 1 KB each: 16 rows of four 16-byte chunks, which
+// stand at chunk ^ (row / 4 % 4).  That spreads the 16 rows that a ds_read_b128 of a fragment
+// touches over all 64 banks, so tiles and halves of them go to LDS as they lie, whole lines at a
+// time.  (With a row's 128 bytes as one line its producer writes whole lines, 8192 x 8192 with
+// residual 166 us in place of 174, but a kernel that takes halves of blocks moves half lines, 1531 x
+// 896 x 4864 19.9 in place of 18.5, and 16 rows on 151936 x 896 take 30.9 in place of 28.7.)  Which
+// elements of a block a lane multiplies in one instruction does not matter while both operands
+// agree and a block has one scale: a lane takes 16-byte chunks.  Behind the codes the scales, a
+// byte a row: 16 bytes per tile, tiles in the same order. Elements past the end of a row are zero;
+// rows past the last may hold anything and only reach outputs that are not stored.
 #pragma once
 
 #include "lx_common.hpp"
@@ -48,11 +50,15 @@ inline Q8Mat q8_mat(const lx_q8* q) {
   return Q8Mat{p, p + q8_code_bytes(q->rows, q->K), q->rows, q->K, kb};
 }
 
+// Where chunk c (0 .. 7) of row r (0 .. 15) stands in a tile.
+__device__ __forceinline__ int q8_chunk(int r, int c) {
+  return (c >> 2) * (kQ8Tile / 2) + r * (kQ8Block / 2) + (((c & 3) ^ (r >> 2)) << 4);
+}
+
 // Byte offset of element k (of its chunk, for k a multiple of 16) of a row.
 __device__ __forceinline__ long q8_at(const Q8Mat& q, int row, int k) {
-  const int r = row & 15;
-  return ((long)(row >> 4) * q.kb + (k >> 7)) * kQ8Tile + r * kQ8Block +
-         ((((k >> 4) & 7) ^ (r >> 1)) << 4) + (k & 15);
+  return ((long)(row >> 4) * q.kb + (k >> 7)) * kQ8Tile + q8_chunk(row & 15, (k >> 4) & 7) +
+         (k & 15);
 }
 __device__ __forceinline__ long q8_scale_at(const Q8Mat& q, int row, int kb) {
   return ((long)(row >> 4) * q.kb + kb) * kQ8Rows + (row & 15);

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(64 * WAVES) void q8_stream_kernel(Q8Lin a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int mt = blockIdx.x % a.tiles_m, nt = blockIdx.x / a.tiles_m;
   const int r = lane & 15, c = lane >> 4;
-  const int at = r * kQ8Block + ((c ^ (r >> 1)) << 4);
+  const int at = q8_chunk(r, c);
   const int mtiles = (a.x.rows + 15) / 16, ntiles = (a.w.rows + 15) / 16;
   long xt[MT], wt[NT];
 #pragma unroll
@@ -118,14 +118,14 @@ __global__ __launch_bounds__(64 * WAVES) void q8_stream_kernel(Q8Lin a) {
     for (int i = 0; i < NT; ++i) {
       const unsigned char* p = a.w.codes + (wt[i] * a.w.kb + kb) * kQ8Tile;
       wf[i][0] = *reinterpret_cast<const intx4*>(p + at);
-      wf[i][1] = *reinterpret_cast<const intx4*>(p + (at ^ 64));
+      wf[i][1] = *reinterpret_cast<const intx4*>(p + at + kQ8Tile / 2);
       ws[i] = __uint_as_float((unsigned)a.w.scales[wt[i] * a.w.kb * 16 + so] << 23);
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const unsigned char* p = a.x.codes + (xt[i] * a.x.kb + kb) * kQ8Tile;
       xf[i][0] = *reinterpret_cast<const intx4*>(p + at);
-      xf[i][1] = *reinterpret_cast<const intx4*>(p + (at ^ 64));
+      xf[i][1] = *reinterpret_cast<const intx4*>(p + at + kQ8Tile / 2);
       xs[i] = __uint_as_float((unsigned)a.x.scales[xt[i] * a.x.kb * 16 + so] << 23);
     }
 #pragma unroll
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, OCC) void q8_tile_kernel(Q8Lin a
   int at[SPW];
 #pragma unroll
   for (int s = 0; s < SPW; ++s)
-    at[s] = half * kQ8Tile + r * kQ8Block + (((2 * (wk * SPW + s) + h) ^ (r >> 1)) << 4);
+    at[s] = half * kQ8Tile + q8_chunk(r, 2 * (wk * SPW + s) + h);
   floatx16 acc[CB][RB];
 #pragma unroll
   for (int n = 0; n < CB; ++n)
@@ -459,24 +459,19 @@ __global__ __launch_bounds__(64 * W, OCC) void q8_ring_kernel(Q8Lin a) {
     const int t = lane >> 2;
     sbase = (t < 2 * RB ? a.x.scales : a.w.scales) + (long)tile_of(t) * kb * 16 + (lane & 3) * 4;
   }
-  // where this lane loads of a tile; of a block's second half it is this ^ 64
-  const int lr = lane >> 2;
-  const int lat =
-      H == 2 ? lane * 16 : lr * kQ8Block + ((((lane & 3) ^ (lr >> 2)) ^ (lr >> 1)) << 4);
   typedef const __attribute__((address_space(1))) void* global_ptr;
   typedef __attribute__((address_space(3))) void* lds_ptr;
   unsigned char* ring = sm + wave * R * S::SLOT;
   auto load = [&](int i, int slot) {
     const int j = i * W + wave, block = H == 2 ? j : j >> 1;
-    const long off = (long)block * kQ8Tile;
-    const int at = H == 2 ? lat : lat ^ ((j & 1) << 6);
+    const long off = (long)j * (H * 1024) + lane * 16;
     unsigned char* d = ring + slot * S::SLOT;
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      __builtin_amdgcn_global_load_lds((global_ptr)(base[t] + off + at),
+      __builtin_amdgcn_global_load_lds((global_ptr)(base[t] + off),
                                        (lds_ptr)(d + t * H * 1024), 16, 0, 0);
       if constexpr (H == 2)  // the offset counts on both sides
-        __builtin_amdgcn_global_load_lds((global_ptr)(base[t] + off + at),
+        __builtin_amdgcn_global_load_lds((global_ptr)(base[t] + off),
                                          (lds_ptr)(d + t * H * 1024), 16, 1024, 0);
     }
     __builtin_amdgcn_global_load_lds((global_ptr)(sbase + (long)block * 16),
@@ -486,7 +481,7 @@ __global__ __launch_bounds__(64 * W, OCC) void q8_ring_kernel(Q8Lin a) {
   int at[2 * H];
 #pragma unroll
   for (int s = 0; s < 2 * H; ++s)
-    at[s] = (half * 16 + r) * H * 64 + (((2 * s + h) ^ (H == 2 ? r >> 1 : r >> 2)) << 4);
+    at[s] = half * H * 1024 + q8_chunk(r, 2 * s + h);
   floatx16 acc[CB][RB];
 #pragma unroll
   for (int n = 0; n < CB; ++n)
