@@ -471,7 +471,7 @@ int lx_attention_kv4_f32(const float* q, long ldq, const lx_kv4* cache, const in
  * range, from 2^128 on: infinity).  Infinities and NaN stand for NaN.  `data`: device memory of lx_q8_bytes() bytes (0 for a bad
  * shape), 16-byte aligned, which needs no initialisation.
  * lx_q8_pack_f32 writes x (row stride ldx) into q; lx_q8_unpack_f32 what q stands for
- * into x.  At most 2^27 blocks of rows, counted one by one.  x and q must not overlap.
+ * into x.  At most 2^27 - 16 blocks, of an even number of rows.  x and q must not overlap.
  * No counterpart in the reference (its weights and activations stay fp32). */
 typedef struct lx_q8 {
   void* data;

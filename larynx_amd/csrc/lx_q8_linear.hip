@@ -39,7 +39,20 @@ __device__ __forceinline__ float silu_hw(float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + e);
 }
 
-__device__ __forceinline__ void epi_one(const Q8Lin& a, int m, long n, float v, float up) {
+// What the residual holds at columns n .. n + 3 of row m.  Asked for ahead of the sums, since it comes
+// from memory: 1531 x 896 x 4864 20.5 -> 18.7 us, 4096 x 896 x 896 18.2 -> 16.1.
+__device__ __forceinline__ floatx4 resid_quad(const Q8Lin& a, int m, long n) {
+  floatx4 r{0.f, 0.f, 0.f, 0.f};
+  if (m >= a.x.rows) return r;
+  const float* p = a.resid + m * a.ldr + n;
+  if (n + 3 < a.w.rows) return *reinterpret_cast<const float4u*>(p);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < a.w.rows) r[e] = p[e];
+  return r;
+}
+
+__device__ __forceinline__ void epi_one(const Q8Lin& a, int m, long n, float v, float up, float r) {
   if (a.bias) v += a.bias[n];
   if (a.epi == LX_EPI_SWIGLU_PAIRED) {
     if (a.bias) up += a.bias[n + 1];
@@ -47,12 +60,12 @@ __device__ __forceinline__ void epi_one(const Q8Lin& a, int m, long n, float v, 
     return;
   }
   if (a.epi == LX_EPI_GELU_TANH) v = gelu_tanh(v);
-  if (a.epi == LX_EPI_RESID) v = a.resid[m * a.ldr + n] + v;
+  if (a.epi == LX_EPI_RESID) v = r + v;
   a.y[m * a.ldy + n] = v;
 }
 
-// Columns n .. n + 3 (n a multiple of 4) of row m.
-__device__ __forceinline__ void epi_quad(const Q8Lin& a, int m, long n, floatx4 v) {
+// Columns n .. n + 3 (n a multiple of 4) of row m; r: their residual.
+__device__ __forceinline__ void epi_quad(const Q8Lin& a, int m, long n, floatx4 v, floatx4 r) {
   if (m >= a.x.rows) return;
   if (n + 3 < a.w.rows) {
     if (a.bias) v += *reinterpret_cast<const float4u*>(a.bias + n);
@@ -64,14 +77,14 @@ __device__ __forceinline__ void epi_quad(const Q8Lin& a, int m, long n, floatx4 
     if (a.epi == LX_EPI_GELU_TANH)
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = gelu_tanh(v[e]);
-    if (a.epi == LX_EPI_RESID) v = *reinterpret_cast<const float4u*>(a.resid + m * a.ldr + n) + v;
+    if (a.epi == LX_EPI_RESID) v = r + v;
     *reinterpret_cast<float4u*>(a.y + m * a.ldy + n) = v;
     return;
   }
   const int step = a.epi == LX_EPI_SWIGLU_PAIRED ? 2 : 1;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (e % step == 0 && n + e < a.w.rows) epi_one(a, m, n + e, v[e], v[e | 1]);
+    if (e % step == 0 && n + e < a.w.rows) epi_one(a, m, n + e, v[e], v[e | 1], r[e]);
 }
 
 // Codes as operands of the bf16 matrix instructions: exact, eight bits hold e4m3's four, and the
@@ -154,7 +167,11 @@ __global__ __launch_bounds__(64 * WAVES) void q8_stream_kernel(Q8Lin a) {
 #pragma unroll
     for (int i = 1; i < WAVES; ++i) s += red[i * NT * MT * 64 + u];
     const int m = (u >> 6) % MT, n = (u >> 6) / MT, l = u & 63;
-    epi_quad(a, (mt * MT + m) * 16 + (l & 15), (long)(nt * NT + n) * 16 + 4 * (l >> 4), s);
+    const int row = (mt * MT + m) * 16 + (l & 15);
+    const long col = (long)(nt * NT + n) * 16 + 4 * (l >> 4);
+    floatx4 res{};
+    if (a.epi == LX_EPI_RESID) res = resid_quad(a, row, col);
+    epi_quad(a, row, col, s, res);
   }
 }
 
@@ -363,6 +380,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK, OCC) void q8_tile_kernel(Q8Lin a
   float* out = reinterpret_cast<float*>(sm + (wave - wk) * S::OUT);
 #pragma unroll
   for (int m = 0; m < RB; ++m) {
+    constexpr int QUADS = 32 * 8 * CB / WK;  // of this wave
+    floatx4 res[QUADS / 64];
+    if (a.epi == LX_EPI_RESID)
+#pragma unroll
+      for (int i = 0; i < QUADS / 64; ++i) {
+        const int e = wk * QUADS + lane + 64 * i;
+        res[i] = resid_quad(a, mt * XT * 16 + (wm * RB + m) * 32 + e / (8 * CB),
+                            (long)nt * WT * 16 + wn * CB * 32 + e % (8 * CB) * 4);
+      }
     if (m == 0 || WK > 1) {
       __syncthreads();
     } else {
@@ -384,16 +410,15 @@ __global__ __launch_bounds__(64 * WM * WN * WK, OCC) void q8_tile_kernel(Q8Lin a
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
-    constexpr int QUADS = 32 * 8 * CB / WK;  // of this wave
-#pragma unroll 2
-    for (int i = lane; i < QUADS; i += 64) {
-      const int e = wk * QUADS + i, row = e / (8 * CB), col = e % (8 * CB) * 4;
+#pragma unroll
+    for (int i = 0; i < QUADS / 64; ++i) {
+      const int e = wk * QUADS + lane + 64 * i, row = e / (8 * CB), col = e % (8 * CB) * 4;
       const float* p = out + row * S::ROW + col;
       floatx4 v = *reinterpret_cast<const floatx4*>(p);
 #pragma unroll
       for (int w = 1; w < WK; ++w) v += *reinterpret_cast<const floatx4*>(p + w * S::OUT / 4);
       epi_quad(a, mt * XT * 16 + (wm * RB + m) * 32 + row, (long)nt * WT * 16 + wn * CB * 32 + col,
-               v);
+               v, res[i]);
     }
   }
 }
@@ -412,14 +437,11 @@ int launch_tile(Q8Lin& a, hipStream_t s) {
 
 // Fewer tiles than CUs.  A workgroup owns (32 RB) x (32 CB) outputs and each of its W waves takes
 // every W-th block of K (H = 2) or half of one (H = 1), through a ring of R slots of LDS of its own:
-// no barrier until the waves' sums meet, and R - 1 slots of every wave on their way.  A block's
-// tile is 2 KB as it lies, two instructions.  Of a half block it is 16 rows x 64 bytes, one
-// instruction: lane 4 row + q loads chunk q ^ (row / 4 % 4) of its row's half, so that the 16 rows
-// of a read are spread over all banks.  Halves of lines arrive at 17-23 TB/s of the card, whole
-// ones at 27-31; but whole blocks of 96 x 64 leave LDS for three waves.  1531 x 896 x 4864 on 96 x
-// 64: 20-22 us (0.65 PFLOP/s) with four waves on halves, 21.9 with three on blocks, where 64 x 64
-// on the tile kernel takes 22.5; the loads alone take 18, the products and conversions alone 16.
-// 256 x 896 x 4864 on 32 x 32: 6.9 on blocks, 7.9 on halves.
+// no barrier until the waves' sums meet, and R - 1 slots of every wave on their way.  A half
+// block's tile is 1 KB, one instruction.  1531 x 896 x 4864 on 96 x 64: 18.4 us (0.73 PFLOP/s; with
+// residual 18.7) where 64 x 64 on the tile kernel takes 22.4; a launch, the first slots and the sums
+// alone take 8.2, with the loads 15, with conversions and products but no loads 14.3; three slots
+// deep it is the same.  256 x 896 x 4864 on 32 x 32: 7.0, 256 x 896 x 896 3.6 (3.8 on half blocks).
 template <int RB, int CB, int W, int H, int R>
 struct RingShape {
   static constexpr int T = 2 * (RB + CB);  // 16-row tiles of a slot: rows of x, then of W
@@ -427,12 +449,13 @@ struct RingShape {
   static constexpr int CODES = T * H * 1024;
   static constexpr int SLOT = CODES + 256;  // the scales behind the codes
   static constexpr int ROW = 32 * CB + 4;  // floats of a row of outputs in LDS
-  static constexpr int OUT = 32 * ROW * 4;  // a wave's 32 rows
+  static constexpr int OUT = 32 * RB * ROW * 4;  // a wave's sums
   static constexpr int LDS = W * (R * SLOT > OUT ? R * SLOT : OUT);
   static_assert(LDS <= 160 * 1024, "LDS of a CU");
+  static constexpr int QUADS = 32 * RB * 8 * CB;  // of four outputs
   static constexpr int LOADS = T * H + 1;  // instructions that load a slot
   static_assert(H == 1 || H == 2, "half a block or a block");
-  static_assert((R - 2) * LOADS < 64, "vmcnt");
+  static_assert((R - 1) * LOADS < 64, "vmcnt");
 };
 
 template <int RB, int CB, int W, int H, int R, int OCC>
@@ -518,11 +541,30 @@ __global__ __launch_bounds__(64 * W, OCC) void q8_ring_kernel(Q8Lin a) {
     else
       wait_vm<0>();
   };
+  // the residual, whose latency would stand alone behind the sums
+  constexpr int EACH = (S::QUADS + 64 * W - 1) / (64 * W);
+  floatx4 res[EACH];
+  auto at_quad = [&](int i, int& row, int& col) {
+    const int e = tid + 64 * W * i;
+    row = e / (8 * CB);
+    col = e % (8 * CB) * 4;
+    return e < S::QUADS;
+  };
+  if (a.epi == LX_EPI_RESID)
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      int row, col;
+      if (at_quad(i, row, col))
+        res[i] = resid_quad(a, mt * RB * 32 + row, (long)nt * CB * 32 + col);
+    }
 #pragma unroll
   for (int i = 0; i < R; ++i)
     if (i < slots) load(i, i);
   if (slots > 0) {
-    wait(0);
+    if (slots >= R)
+      wait_vm<(R - 1) * S::LOADS>();
+    else
+      wait_vm<0>();
     read_scales(0);
     read(raw[0], 0, 0);
     set_scales();
@@ -566,29 +608,29 @@ __global__ __launch_bounds__(64 * W, OCC) void q8_ring_kernel(Q8Lin a) {
     }
     slot = next;
   }
-  // the waves' sums meet in LDS, 32 rows at a time, in the order of the waves
+  // the waves' sums meet in LDS, in the order of the waves
   float* out = reinterpret_cast<float*>(sm);
+  __syncthreads();
 #pragma unroll
-  for (int m = 0; m < RB; ++m) {
-    __syncthreads();
+  for (int m = 0; m < RB; ++m)
 #pragma unroll
     for (int n = 0; n < CB; ++n)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<floatx4*>(out + wave * S::OUT / 4 + (lane & 31) * S::ROW + 32 * n + 8 * q +
-                                    4 * h) =
+        *reinterpret_cast<floatx4*>(out + wave * S::OUT / 4 + (32 * m + (lane & 31)) * S::ROW +
+                                    32 * n + 8 * q + 4 * h) =
             floatx4{acc[n][m][4 * q], acc[n][m][4 * q + 1], acc[n][m][4 * q + 2],
                     acc[n][m][4 * q + 3]};
-    __syncthreads();
-#pragma unroll 1
-    for (int e = tid; e < 32 * 8 * CB; e += 64 * W) {
-      const int row = e / (8 * CB), col = e % (8 * CB) * 4;
-      const float* p = out + row * S::ROW + col;
-      floatx4 v = *reinterpret_cast<const floatx4*>(p);
+  __syncthreads();
 #pragma unroll
-      for (int w = 1; w < W; ++w) v += *reinterpret_cast<const floatx4*>(p + w * S::OUT / 4);
-      epi_quad(a, mt * RB * 32 + m * 32 + row, (long)nt * CB * 32 + col, v);
-    }
+  for (int i = 0; i < EACH; ++i) {
+    int row, col;
+    if (!at_quad(i, row, col)) break;
+    const float* p = out + row * S::ROW + col;
+    floatx4 v = *reinterpret_cast<const floatx4*>(p);
+#pragma unroll
+    for (int w = 1; w < W; ++w) v += *reinterpret_cast<const floatx4*>(p + w * S::OUT / 4);
+    epi_quad(a, mt * RB * 32 + row, (long)nt * CB * 32 + col, v, res[i]);
   }
 }
 
@@ -665,23 +707,26 @@ extern "C" int lx_linear_q8_f32(const lx_q8* x, const lx_q8* w, const float* bia
   //   1531 x 1152 x 896   27.5  12.3   9.5  10.6       177 x 6761       30.0  14.1   9.2   8.4
   if (8 * tiles(256, 256) >= 7 * cus) return launch_tile<4, 2, 2, 4, 1, 2, 1>(a, stream);
   if (8 * tiles(128, 128) >= 7 * cus) return launch_tile<2, 2, 2, 2, 1, 2, 2>(a, stream);
-  // while the smallest give each CU one at most, and at 12 blocks of K or more while larger ones
-  // do, every wave on K of its own (32 x 32, 32 x 64, 64 x 64, 96 x 64 on the ring kernel, then 64
-  // x 64 and 32 x 64 on the tile kernel)
-  //    256 x  896 x  896   3.5   4.3   5.8   7.3   6.0   4.8
-  //    256 x  896 x 4864   6.9   9.3  13.1  17.5  16.1  12.3
-  //    256 x 1152 x  896   5.6   4.3   5.8   7.4   6.1   4.9
-  //    128 x 4096 x 4864  12.7  10.2  13.5  16.8  16.4  12.8
-  //    500 x 1500 x  896   8.6   7.8   6.5   8.5   6.7   6.4
-  //    500 x 1500 x 1500  10.4   9.8   7.8  10.0   8.5   8.4
-  //   1024 x 1024 x 4864  22.3  18.0  16.2  18.7  17.0  17.6
-  //   1531 x  896 x 1500  18.1  14.1  11.5  10.4  10.7  10.7
-  //   1531 x  896 x 4864  31.3  24.8  24.1  19.6  21.8  23.0
+  // while the smallest give each CU one at most, and at 12 blocks of K or more (24 for the largest)
+  // while larger ones do, every wave on K of its own (32 x 32, 32 x 64, 64 x 64, 96 x 64, 128 x 64
+  // on the ring kernel, then 64 x 64 and 32 x 64 on the tile kernel)
+  //    256 x  896 x  896   3.6   4.3   5.7   7.0   8.7   6.0   4.9
+  //    256 x  896 x 4864   7.2   8.8  13.2  15.8  20.0  16.0  12.4
+  //    256 x 1152 x  896   5.8   4.4   5.8   7.2   8.8   6.1   5.0
+  //    128 x 4096 x 4864  12.3   9.5  13.4  16.5  20.2  16.5  12.6
+  //    500 x 1500 x  896   8.9   7.8   6.3   7.9   9.4   6.7   6.4
+  //    500 x 1500 x 1500  10.4   9.5   7.8   9.5  11.4   8.5   8.3
+  //   1024 x 1024 x 4864  22.4  16.9  15.0  16.8  20.6  18.3  18.0
+  //   1531 x  896 x 1500  18.6  13.8  11.1   9.7  11.7  11.0  10.7
+  //   1531 x  896 x 4864  32.3  24.1  23.2  18.3  20.9  22.4  22.9
+  //   2000 x 1000 x 1600                    17.9  13.4  12.5  15.2
+  //   2000 x 1000 x 4864  42.2  32.3  25.6  31.7  23.7  25.9  31.1
   if (tiles(32, 32) <= cus) return launch_ring<1, 1, 8, 2, 2, 1>(a, stream);
-  if (tiles(32, 64) <= cus) return launch_ring<1, 2, 4, 2, 2, 1>(a, stream);
+  if (tiles(32, 64) <= cus) return launch_ring<1, 2, 8, 1, 2, 2>(a, stream);
   if (a.x.kb >= 12) {
     if (tiles(64, 64) <= cus) return launch_ring<2, 2, 4, 1, 2, 2>(a, stream);
     if (tiles(96, 64) <= cus) return launch_ring<3, 2, 4, 1, 2, 1>(a, stream);
+    if (tiles(128, 64) <= cus && a.x.kb >= 24) return launch_ring<4, 2, 4, 1, 3, 1>(a, stream);
   } else if (2 * tiles(64, 64) < 3 * cus) {
     return launch_tile<1, 2, 1, 1, 4, 4, 3>(a, stream);
   }

@@ -207,7 +207,9 @@ LINEARS = [(1, 1, 1), (1, 16, 128), (1, 1152, 896), (2, 17, 129), (4, 6761, 896)
            (300, 1600, 4864), (1531, 900, 1600), (1400, 1000, 2177), (256, 9728, 100),
            (2049, 2305, 100), (3600, 3800, 100), (3500, 3590, 700),
            # several blocks a wave on the smallest tiles
-           (200, 700, 4864), (40, 900, 2200), (130, 800, 1200)]
+           (200, 700, 4864), (40, 900, 2200), (130, 800, 1200),
+           # and on the largest that have K to themselves
+           (1900, 1000, 3000), (2290, 890, 4864)]
 
 
 @pytest.mark.parametrize("M,N,K", LINEARS)
@@ -241,7 +243,7 @@ def test_every_product_counts(gpu, M, N, K):
 @pytest.mark.parametrize("M,N,K", [(3, 40, 1157), (40, 33, 1157), (300, 900, 1157),
                                    (500, 1500, 1700), (1400, 900, 1700), (1100, 1300, 1157),
                                    (1531, 1152, 300), (2100, 2100, 1157), (3590, 3598, 700),
-                                   (60, 200, 2300), (60, 6100, 2300)])
+                                   (60, 200, 2300), (60, 6100, 2300), (1900, 990, 3000)])
 def test_scales_of_every_row_and_block(gpu, M, N, K):
     """Blocks at powers of two of their own, one element each: every product has its scales."""
     g = _gen(M)
@@ -274,7 +276,7 @@ KINDS = {"none": None, "gelu": ops.LX_EPI_GELU_TANH, "resid": ops.LX_EPI_RESID,
          "swiglu": ops.LX_EPI_SWIGLU_PAIRED}
 EPI_SHAPES = [(1, 66, 896), (9, 68, 200), (40, 130, 300), (70, 1152, 896), (257, 514, 896),
               (1030, 1026, 150), (300, 898, 260), (500, 1502, 1600), (1531, 898, 1600),
-              (1531, 1152, 300), (2100, 2050, 130), (3590, 3598, 130)]
+              (1531, 1152, 300), (2100, 2050, 130), (3590, 3598, 130), (1900, 990, 3000)]
 
 
 @pytest.mark.parametrize("M,N,K", EPI_SHAPES)
