@@ -2,7 +2,6 @@
 // (lx_q8.hpp).
 #include <algorithm>
 #include <climits>
-#include <type_traits>
 
 #include "lx_q8.hpp"
 
@@ -205,20 +204,20 @@ __device__ __forceinline__ void wait_vm() {  // vmcnt(N) lgkmcnt(0)
 }
 
 // Many rows.  A workgroup owns (32 RB WM) x (32 CB WN) outputs; both operands go through LDS as
-// they lie in memory (no registers, no ds_write), a block of K a stage, NS stages deep.  WK waves
-// share each (32 RB) x (32 CB) of the outputs, taking 128 / WK of a stage's 128 each: a wave's tile
-// is as large as its registers hold, since what a tile costs beside its products is the conversion
-// of its operands (8 cycles for 128 codes; an instruction of 32 x 32 x 16 takes 32). A step is 16
-// of K; while its products run, the next step's codes are converted, and those of the step after
-// are on their way from LDS.  The one barrier of a stage stands before its last two steps, whose
-// operands every wave has by then: the buffer is free for the stage NS further on, and the next
-// stage's first reads return behind those steps' products. 4096 x 8192 x 8192 on 256 x 256 tiles:
-// 400-455 us by box and heat, 1.2-1.38 PFLOP/s, as a bf16 product of the library (1.37): the power
-// limit leaves 1.8 GHz, at which the matrix pipe is 0.65 to 0.68 busy; four waves of 128 x 128 and
-// eight of 64 x 128 give the same.  256 x 9728 x 896 on 64 x 64: 11 us, of which 3 move its bytes:
-// 608 tiles of seven stages, each bounded by its loads' and its reads' latency (without the
-// products 9.3, without conversions 10.5).
-template <int RB, int CB, int WM, int WN, int WK, int NS>
+// they lie in memory (no registers, no ds_write), a block of K a stage, two stages.  WK waves share
+// each (32 RB) x (32 CB) of the outputs, taking 128 / WK of a stage's 128 each: what a tile costs
+// beside its products is the conversion of its operands (8 cycles for 128 codes; an instruction of
+// 32 x 32 x 16 takes 32), less of it the larger a wave's tile is, and the way of its WK partial
+// sums through LDS (256 x 9728 x 896 on 64 x 64: 2 us of 11.5 with WK = 4, three workgroups a CU;
+// 10.7 with WK = 2 and four; 10.6 to 10.9 with 1).  A step is 16 of K; while its products run, the
+// next step's codes are converted, and those of the step after are on their way from LDS.  The one
+// barrier of a stage stands before its last two steps, whose operands every wave has by then: the
+// buffer is free for the stage after the next, and the next stage's first reads return behind those
+// steps' products.  4096 x 8192 x 8192 on 256 x 256 tiles: 400-455 us by box and heat, 1.2-1.38
+// PFLOP/s, as a bf16 product of the library (1.37): the power limit leaves 1.8 GHz, at which the
+// matrix pipe is 0.65 to 0.68 busy; four waves of 128 x 128 and eight of 64 x 128 give the same.
+// 1000 x 6761 x 896 on 128 x 128: 18.7 us with eight waves of 64 x 32, 20.0 with four of 64 x 64.
+template <int RB, int CB, int WM, int WN, int WK>
 struct TileShape {
   static constexpr int WAVES = WM * WN * WK;
   static constexpr int XT = 2 * RB * WM, WT = 2 * CB * WN;  // 16-row tiles of a stage
@@ -229,14 +228,14 @@ struct TileShape {
   static constexpr int STAGE = SCALES + 256 * WAVES;
   static constexpr int ROW = 32 * CB + 4;  // floats of a row of outputs in LDS
   static constexpr int OUT = 32 * ROW * 4;  // a wave's 32 rows
-  static constexpr int LDS = NS * STAGE > WAVES * OUT ? NS * STAGE : WAVES * OUT;
+  static constexpr int LDS = 2 * STAGE > WAVES * OUT ? 2 * STAGE : WAVES * OUT;
   static_assert(LDS <= 160 * 1024, "LDS of a CU");
-  static_assert((NS - 2) * (CHUNKS + 1) < 64, "vmcnt");
+  static_assert(WK <= 2 && CHUNKS + 1 < 64, "four steps or more; vmcnt");
 };
 
-template <int RB, int CB, int WM, int WN, int WK, int NS, int OCC>
+template <int RB, int CB, int WM, int WN, int WK, int OCC>
 __global__ __launch_bounds__(64 * WM * WN * WK, OCC) void q8_tile_kernel(Q8Lin a) {
-  using S = TileShape<RB, CB, WM, WN, WK, NS>;
+  using S = TileShape<RB, CB, WM, WN, WK>;
   constexpr int XT = S::XT, WT = S::WT, CHUNKS = S::CHUNKS, SPW = 4 / WK;
   extern __shared__ __attribute__((aligned(16))) unsigned char sm[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -309,17 +308,13 @@ __global__ __launch_bounds__(64 * WM * WN * WK, OCC) void q8_tile_kernel(Q8Lin a
 #pragma unroll
     for (int i = 0; i < RB + CB; ++i) f[i] = q8_frag(u[i][2 * t], u[i][2 * t + 1], scale[i]);
   };
-  // stage k is in LDS (NS - 2 later ones may be on their way), and this wave's reads are done
-  auto wait = [&](int k) {
-    if (k + NS - 2 < kb)
-      wait_vm<(NS - 2) * (CHUNKS + 1)>();
-    else
-      wait_vm<0>();
-  };
-#pragma unroll
-  for (int k = 0; k < NS; ++k)
-    if (k < kb) load(k, k);
-  wait(0);
+  load(0, 0);
+  if (kb > 1) {
+    load(1, 1);
+    wait_vm<CHUNKS + 1>();  // the second stage's may be on their way
+  } else {
+    wait_vm<0>();
+  }
   __syncthreads();
   unsigned us[RB + CB];
   read_scales(us, 0);
@@ -327,11 +322,9 @@ __global__ __launch_bounds__(64 * WM * WN * WK, OCC) void q8_tile_kernel(Q8Lin a
 #pragma unroll
   for (int i = 0; i < RB + CB; ++i) scale[i] = __uint_as_float(us[i] << 23);
   convert(frag[0], raw[0], 0);
-  int buf = 0;
-  // one stage; raw[P] holds its first operands
-  auto stage = [&](int k, auto parity) {
-    constexpr int P = decltype(parity)::value;
-    const int next = buf + 1 == NS ? 0 : buf + 1;
+#pragma unroll 1
+  for (int k = 0; k < kb; ++k) {
+    const int buf = k & 1;
 #pragma unroll
     for (int u = 0; u < 2 * SPW; ++u) {
       const int s = u >> 1, t = u & 1;
@@ -339,19 +332,20 @@ __global__ __launch_bounds__(64 * WM * WN * WK, OCC) void q8_tile_kernel(Q8Lin a
         // the conversions so far stay in front of the branches, beside their step's products
 #pragma unroll
         for (int i = 0; i < RB + CB; ++i) asm volatile("" : "+v"(frag[0][i]));
-        if (k + 1 < kb) wait(k + 1);
+        // this wave's part of the next stage is in LDS, and its reads of this one are done
+        if (k + 1 < kb) wait_vm<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (k + NS < kb) load(k + NS, buf);
-        read_scales(us, next);
-        read(raw[(P + s + 1) & 1], next, 0);  // past the last stage: bytes of a buffer, not used
+        if (k + 2 < kb) load(k + 2, buf);
+        read_scales(us, buf ^ 1);
+        read(raw[0], buf ^ 1, 0);  // past the last stage: bytes of a buffer, not used
       } else if (t == 0) {
-        read(raw[(P + s + 1) & 1], buf, s + 1);
+        read(raw[(s + 1) & 1], buf, s + 1);
       }
       if (u == 2 * SPW - 1)
 #pragma unroll
         for (int i = 0; i < RB + CB; ++i) scale[i] = __uint_as_float(us[i] << 23);
-      convert(frag[(u + 1) & 1], raw[(P + s + t) & 1], t ^ 1);
+      convert(frag[(u + 1) & 1], raw[(s + t) & 1], t ^ 1);
 #pragma unroll
       for (int n = 0; n < CB; ++n)
 #pragma unroll
@@ -368,12 +362,6 @@ __global__ __launch_bounds__(64 * WM * WN * WK, OCC) void q8_tile_kernel(Q8Lin a
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    buf = next;
-  };
-#pragma unroll 1
-  for (int k = 0; k < kb; k += SPW & 1 ? 2 : 1) {
-    stage(k, std::integral_constant<int, 0>{});
-    if ((SPW & 1) && k + 1 < kb) stage(k + 1, std::integral_constant<int, SPW & 1>{});
   }
   // outputs through LDS, 32 rows a wave at a time: the WK waves' sums meet there, and stores are
   // whole lines of y
@@ -423,10 +411,10 @@ __global__ __launch_bounds__(64 * WM * WN * WK, OCC) void q8_tile_kernel(Q8Lin a
   }
 }
 
-template <int RB, int CB, int WM, int WN, int WK, int NS, int OCC>
+template <int RB, int CB, int WM, int WN, int WK, int OCC>
 int launch_tile(Q8Lin& a, hipStream_t s) {
-  using S = TileShape<RB, CB, WM, WN, WK, NS>;
-  const auto kern = q8_tile_kernel<RB, CB, WM, WN, WK, NS, OCC>;
+  using S = TileShape<RB, CB, WM, WN, WK>;
+  const auto kern = q8_tile_kernel<RB, CB, WM, WN, WK, OCC>;
   long grid;
   LX_TRY(tile_grid(a, 32 * RB * WM, 32 * CB * WN, 64 * S::WAVES, &grid));
   static LdsLimit once;
@@ -701,27 +689,34 @@ extern "C" int lx_linear_q8_f32(const lx_q8* x, const lx_q8* w, const float* bia
   }
   const long cus = device_cus();
   auto tiles = [&](long m, long n) { return ((M + m - 1) / m) * ((N + n - 1) / n); };
-  // The largest tiles that still give (nearly) every CU one: shared by a workgroup's waves
-  // while there are many (256 x 256, 128 x 128, 64 x 64, 32 x 64 on the tile kernel; us)
-  //   4096 x 6761 x 896   73.7  81.4  95.6 112.5      4096 x 896 x 896  28.0  14.4  16.9  16.8
-  //   1000 x 6761 x 896   32.1  21.5  23.3  28.4       400 x 6761       30.7  15.5  12.5  14.7
-  //   1531 x 1152 x 896   27.5  12.3   9.5  10.6       177 x 6761       30.0  14.1   9.2   8.4
-  if (8 * tiles(256, 256) >= 7 * cus) return launch_tile<4, 2, 2, 4, 1, 2, 1>(a, stream);
-  if (8 * tiles(128, 128) >= 7 * cus) return launch_tile<2, 2, 2, 2, 1, 2, 2>(a, stream);
+  // Large tiles while they fill the rounds that they take: a tile of 256 x 256 costs a CU as much as
+  // 3.5 of 128 x 128, the first of those as much as 3.3 of 64 x 64 (four of which share a CU, so that
+  // their rounds need not be full) and another one 2.5 (256 x 256, 128 x 128, 64 x 64, 32 x 64; us)
+  //   4096 x 8192 x 4096   227   260   321         1000 x 6761 x 896  30.7  19.0  22.3  23.7
+  //   1531 x 9728 x  896  33.4  35.5  41.9         4096 x 1152 x 896  27.6  17.8  15.8  16.9
+  //   1600 x 9728 x  896  57.1  36.9  44.8         1024 x 4096 x 896  27.6  12.7  13.6  15.5
+  //   2304 x 8192 x 4096   190   155   173         1531 x 2000 x 896  27.3  12.4  11.4  12.5
+  auto rounds = [&](long m, long n) { return (tiles(m, n) + cus - 1) / cus; };
+  if (7 * rounds(256, 256) <= 2 * rounds(128, 128))
+    return launch_tile<4, 2, 2, 4, 1, 1>(a, stream);
+  if (10 * tiles(64, 64) >= (25 * rounds(128, 128) + 8) * cus)
+    return launch_tile<2, 1, 2, 4, 1, 2>(a, stream);
   // while the smallest give each CU one at most, and at 12 blocks of K or more (24 for the largest)
   // while larger ones do, every wave on K of its own (32 x 32, 32 x 64, 64 x 64, 96 x 64, 128 x 64
   // on the ring kernel, then 64 x 64 and 32 x 64 on the tile kernel)
-  //    256 x  896 x  896   3.6   4.3   5.7   7.0   8.7   6.0   4.9
-  //    256 x  896 x 4864   7.2   8.8  13.2  15.8  20.0  16.0  12.4
-  //    256 x 1152 x  896   5.8   4.4   5.8   7.2   8.8   6.1   5.0
-  //    128 x 4096 x 4864  12.3   9.5  13.4  16.5  20.2  16.5  12.6
-  //    500 x 1500 x  896   8.9   7.8   6.3   7.9   9.4   6.7   6.4
-  //    500 x 1500 x 1500  10.4   9.5   7.8   9.5  11.4   8.5   8.3
-  //   1024 x 1024 x 4864  22.4  16.9  15.0  16.8  20.6  18.3  18.0
-  //   1531 x  896 x 1500  18.6  13.8  11.1   9.7  11.7  11.0  10.7
-  //   1531 x  896 x 4864  32.3  24.1  23.2  18.3  20.9  22.4  22.9
-  //   2000 x 1000 x 1600                    17.9  13.4  12.5  15.2
-  //   2000 x 1000 x 4864  42.2  32.3  25.6  31.7  23.7  25.9  31.1
+  //    256 x  896 x  896   3.6   4.4   5.8   7.1   8.8   5.7   4.6
+  //    256 x  896 x 4864   7.0   8.8  13.5  16.0  20.1  19.9  18.2
+  //    256 x 1152 x  896   5.6   4.3   5.8   7.2   8.8   5.8   4.7
+  //    128 x 4096 x 4864  12.6   9.3  13.7  16.6  20.3  19.9  18.2
+  //    500 x 1500 x  896   8.2   7.7   6.2   7.8   9.2   6.2   6.1
+  //    500 x 1500 x 1500  10.4   9.4   7.7   9.4  11.3   9.1   8.5
+  //   1024 x 1024 x 4864  22.9  16.6  15.2  16.5  20.3  20.5  19.2
+  //   1531 x  896 x 1500  18.0  13.4  11.0   9.8  11.6  10.7   9.8
+  //   1531 x  896 x 4864  30.6  23.7  22.7  17.5  21.2  22.9  21.4
+  //   2000 x 1000 x 1600  25.8  17.9  12.6  18.1  13.3  11.9  13.1
+  //   2000 x 1000 x 4864  41.4  31.3  24.8  31.3  23.3  25.8  30.1
+  //    256 x 9728 x  896  25.3  18.6  12.7  14.8  18.1  10.6  11.0
+  //    177 x 6761 x  896  13.4  11.6   9.0   8.8  10.4   8.5   7.7
   if (tiles(32, 32) <= cus) return launch_ring<1, 1, 8, 2, 2, 1>(a, stream);
   if (tiles(32, 64) <= cus) return launch_ring<1, 2, 8, 1, 2, 2>(a, stream);
   if (a.x.kb >= 12) {
@@ -729,7 +724,7 @@ extern "C" int lx_linear_q8_f32(const lx_q8* x, const lx_q8* w, const float* bia
     if (tiles(96, 64) <= cus) return launch_ring<3, 2, 4, 1, 2, 1>(a, stream);
     if (tiles(128, 64) <= cus && a.x.kb >= 24) return launch_ring<4, 2, 4, 1, 3, 1>(a, stream);
   } else if (2 * tiles(64, 64) < 3 * cus) {
-    return launch_tile<1, 2, 1, 1, 4, 4, 3>(a, stream);
+    return launch_tile<1, 1, 1, 2, 2, 5>(a, stream);
   }
-  return launch_tile<2, 2, 1, 1, 4, 3, 3>(a, stream);
+  return launch_tile<2, 1, 1, 2, 2, 4>(a, stream);
 }
