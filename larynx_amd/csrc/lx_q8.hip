@@ -95,6 +95,15 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return v;
 }
 
+__device__ __forceinline__ double half_sum64(double v) {
+  v += dpp_mov64<kDppXor1>(v);
+  v += dpp_mov64<kDppXor2>(v);
+  v += dpp_mov64<kDppHalfMirror>(v);
+  v += dpp_mov64<kDppMirror>(v);
+  v += __shfl_xor(v, 32);
+  return v;
+}
+
 // d rounded to fp32 towards the odd neighbour: a further rounding to fewer bits than fp32's less
 // two, and comparisons with numbers of fewer bits, come out as d's own would.
 __device__ __forceinline__ float to_odd(double d) {
@@ -113,7 +122,7 @@ struct NormArgs {
 };
 
 // The row of a workgroup that has one: of sixteen, two that share lines go to one XCD (workgroups
-// are dealt to them round-robin).  8192 x 8192 79.5 -> 77.7 us, with add 175.2 -> 174.3.
+// are dealt to them round-robin).  30000 x 2500 102 -> 97.5 us, with add 202 -> 198.
 __device__ __forceinline__ int row_of(const Q8Mat& q) {
   const int b = blockIdx.x;
   return b < q.rows / 16 * 16 ? b / 16 * 16 + b % 8 * 2 + (b >> 3 & 1) : b;
@@ -121,16 +130,23 @@ __device__ __forceinline__ int row_of(const Q8Mat& q) {
 
 // G threads a row, each NC chunks of eight elements in registers (one pass over x and add); the
 // row's power and the normalised values in 64 bits, where a code next to a border is decided: some
-// 40 instructions an element, which a row's bytes hide.  8192 x 8192 with add 172-180 us, 4.9-5.1
-// TB/s (a copy: 4.7); 1531 x 896 6.5, a launch and one round trip; without add, whose bytes are
-// half, 77 (4.3 TB/s, the instructions).  Four elements a lane, whole lines an instruction, need a
-// fifth step of each block's maximum for half the elements: 178 and 93 us.
-template <int G, int NC>
-__global__ __launch_bounds__(256) void norm_q8_kernel(NormArgs a) {
-  constexpr int RPB = 256 / G;
-  const int t = threadIdx.x % G, row = G == 64 ? blockIdx.x * RPB + threadIdx.x / G : row_of(a.q);
-  const int D = a.q.K, chunks = a.q.kb * 16;
-  __shared__ double part[4];
+// 40 instructions an element, which a row's bytes hide.  PAIR: a workgroup has the two rows whose
+// codes share lines, sixteen lanes of one beside sixteen of the other, so that a wave stores whole
+// lines.  8192 x 8192 with add 175 -> 159 us, 5.5 TB/s (a copy: 4.7), 3000 x 8192 67 -> 62; where
+// the bytes come from the last cache or there is no add it is as fast or slower (1000 x 8192 23.8
+// and 24.3, 1 x 8192 7.0 and 8.2; 6000 x 8192 without add 52 and 53).  1531 x 896 6.5, a launch and
+// one round trip; 8192 x 8192 without add, whose bytes are half, 80 (4.2 TB/s, the instructions).
+// Four elements a lane need a fifth step of each block's maximum for half the elements: 6 to 20%
+// slower.
+template <int G, int NC, bool PAIR>
+__global__ __launch_bounds__(PAIR ? 2 * G : 256) void norm_q8_kernel(NormArgs a) {
+  const int side = threadIdx.x >> 4 & 1;  // of a pair
+  const int t = PAIR ? (threadIdx.x >> 5) * 16 + (threadIdx.x & 15) : threadIdx.x % G;
+  const int row = PAIR      ? blockIdx.x * 2 + side
+                  : G == 64 ? blockIdx.x * 4 + threadIdx.x / 64
+                            : row_of(a.q);
+  const int D = a.q.K, chunks = row < a.q.rows ? a.q.kb * 16 : 0;
+  __shared__ double part[PAIR ? 2 : 1][PAIR ? 8 : 4];
   if (G == 64 && row >= a.q.rows) return;
   float h[NC][8];
   double s = 0.0;
@@ -150,11 +166,13 @@ __global__ __launch_bounds__(256) void norm_q8_kernel(NormArgs a) {
       for (int j = 0; j < 8; ++j) s = fma((double)h[c][j], (double)h[c][j], s);
     }
   }
-  s = wave_sum64(s);
-  if (G > 64) {
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  s = PAIR ? half_sum64(s) : wave_sum64(s);
+  if constexpr (G > 64) {
+    if ((threadIdx.x & (PAIR ? 47 : 63)) == 0) part[PAIR ? side : 0][threadIdx.x >> 6] = s;
     __syncthreads();
-    s = (part[0] + part[1]) + (part[2] + part[3]);
+    const double* p = part[PAIR ? side : 0];
+    s = (p[0] + p[1]) + (p[2] + p[3]);
+    if constexpr (PAIR) s += (p[4] + p[5]) + (p[6] + p[7]);
   }
   const double r = 1.0 / sqrt(s / D + (double)a.eps);
 #pragma unroll
@@ -260,13 +278,16 @@ extern "C" int lx_rmsnorm_q8_f32(const float* x, long ldx, const float* add, lon
   NormArgs a{x, add, w, sum, ldx, lda, lds, eps, q8_mat(q)};
   const dim3 wide((unsigned)rows), four((unsigned)(((long)rows + 3) / 4)), block(256);
   if (D <= 1024)
-    hipLaunchKernelGGL((norm_q8_kernel<64, 2>), four, block, 0, stream, a);
+    hipLaunchKernelGGL((norm_q8_kernel<64, 2, false>), four, block, 0, stream, a);
   else if (D <= 2048)
-    hipLaunchKernelGGL((norm_q8_kernel<64, 4>), four, block, 0, stream, a);
+    hipLaunchKernelGGL((norm_q8_kernel<64, 4, false>), four, block, 0, stream, a);
   else if (D <= 4096)
-    hipLaunchKernelGGL((norm_q8_kernel<256, 2>), wide, block, 0, stream, a);
+    hipLaunchKernelGGL((norm_q8_kernel<256, 2, false>), wide, block, 0, stream, a);
+  else if (D <= 8192 && add && rows >= 2048)
+    hipLaunchKernelGGL((norm_q8_kernel<256, 4, true>), dim3((unsigned)(((long)rows + 1) / 2)),
+                       dim3(512), 0, stream, a);
   else if (D <= 8192)
-    hipLaunchKernelGGL((norm_q8_kernel<256, 4>), wide, block, 0, stream, a);
+    hipLaunchKernelGGL((norm_q8_kernel<256, 4, false>), wide, block, 0, stream, a);
   else
     hipLaunchKernelGGL(norm_q8_long_kernel, wide, block, 0, stream, a);
   return check_launch("norm_q8_kernel");

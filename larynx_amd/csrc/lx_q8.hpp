@@ -9,13 +9,13 @@
 // tile is its first 64 columns, then its last, 1 KB each: 16 rows of four 16-byte chunks, which
 // stand at chunk ^ (row / 4 % 4).  That spreads the 16 rows that a ds_read_b128 of a fragment
 // touches over all 64 banks, so tiles and halves of them go to LDS as they lie, whole lines at a
-// time.  (With a row's 128 bytes as one line its producer writes whole lines, 8192 x 8192 with
-// residual 166 us in place of 174, but a kernel that takes halves of blocks moves half lines, 1531 x
-// 896 x 4864 19.9 in place of 18.5, and 16 rows on 151936 x 896 take 30.9 in place of 28.7.)  Which
-// elements of a block a lane multiplies in one instruction does not matter while both operands
-// agree and a block has one scale: a lane takes 16-byte chunks.  Behind the codes the scales, a
-// byte a row: 16 bytes per tile, tiles in the same order. Elements past the end of a row are zero;
-// rows past the last may hold anything and only reach outputs that are not stored.
+// time.  (With a row's 128 bytes as one line a producer of one row writes whole lines, but a kernel
+// that takes halves of blocks moves half lines: 1531 x 896 x 4864 19.9 us in place of 18.5, 16 rows
+// on 151936 x 896 30.9 in place of 28.7.)  Which elements of a block a lane multiplies in one
+// instruction does not matter while both operands agree and a block has one scale: a lane takes
+// 16-byte chunks.  Behind the codes the scales, a byte a row: 16 bytes per tile, tiles in the same
+// order. Elements past the end of a row are zero; rows past the last may hold anything and only
+// reach outputs that are not stored.
 #pragma once
 
 #include "lx_common.hpp"

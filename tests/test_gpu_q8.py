@@ -102,7 +102,7 @@ def _norm64(h, w, eps=EPS):
 
 
 NORMS = [(1, 896), (5, 1), (3, 128), (33, 1001), (64, 1024), (7, 1025), (130, 2047), (9, 2049),
-         (4, 4096), (5, 4100), (6, 8192), (3, 8193), (2, 20000)]
+         (4, 4096), (5, 4100), (6, 8192), (3, 8193), (2, 20000), (37, 2100), (50, 5000), (33, 8300)]
 
 
 @pytest.mark.parametrize("rows,D", NORMS)
@@ -133,6 +133,12 @@ def test_norm_with_residual(gpu, rows, D, where):
     if where != "add":
         _same(ad, add)
     _same(ops.q8_unpack(q), _fp32(held(_norm64(h, w))[0]))
+
+
+@pytest.mark.parametrize("rows,D", [(2048, 4100), (2049, 8192), (2063, 5001)])
+@pytest.mark.parametrize("where", ["x", "add", "apart"])
+def test_norm_of_many_long_rows(gpu, rows, D, where):
+    test_norm_with_residual(gpu, rows, D, where)
 
 
 def test_norm_strides(gpu):
