@@ -723,8 +723,10 @@ extern "C" int lx_linear_q8_f32(const lx_q8* x, const lx_q8* w, const float* bia
     if (tiles(64, 64) <= cus) return launch_ring<2, 2, 4, 1, 2, 2>(a, stream);
     if (tiles(96, 64) <= cus) return launch_ring<3, 2, 4, 1, 2, 1>(a, stream);
     if (tiles(128, 64) <= cus && a.x.kb >= 24) return launch_ring<4, 2, 4, 1, 3, 1>(a, stream);
-  } else if (2 * tiles(64, 64) < 3 * cus) {
-    return launch_tile<1, 1, 1, 2, 2, 5>(a, stream);
   }
+  // and where tiles of 64 rows hold few of them (24 x 30000 x 896 8.4 and 7.6, 80 x 20000 x 896 11.6
+  // and 10.2)
+  if ((a.x.kb < 12 && 2 * tiles(64, 64) < 3 * cus) || 10 * tiles(32, 64) < 17 * tiles(64, 64))
+    return launch_tile<1, 1, 1, 2, 2, 5>(a, stream);
   return launch_tile<2, 1, 1, 2, 2, 4>(a, stream);
 }

@@ -215,7 +215,7 @@ LINEARS = [(1, 1, 1), (1, 16, 128), (1, 1152, 896), (2, 17, 129), (4, 6761, 896)
            # several blocks a wave on the smallest tiles
            (200, 700, 4864), (40, 900, 2200), (130, 800, 1200),
            # and on the largest that have K to themselves
-           (1900, 1000, 3000), (2290, 890, 4864)]
+           (1900, 1000, 3000), (2290, 890, 4864), (20, 17000, 300), (80, 18000, 1600)]
 
 
 @pytest.mark.parametrize("M,N,K", LINEARS)
