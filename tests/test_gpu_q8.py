@@ -373,6 +373,26 @@ def test_rows_past_the_last(gpu):
         assert torch.equal(ops.linear_q8(x2, w2), y)
 
 
+def test_past_32_bits(gpu):
+    """Matrices of more than 2^31 bytes, as rows and as a weight: whole numbers, exact sums."""
+    announce("8-bit matrices past 2^31 bytes")
+    g = _gen(21)
+    n, K = 270000, 8192  # 2.2 GB of codes
+    base = torch.randint(-15, 16, (1000, K), generator=g).float()
+    few = torch.randint(-15, 16, (48, K), generator=g).float()
+    want = base.double() @ few.double().t()
+    big = ops.q8_pack(base.to(gpu).repeat(n // 1000, 1))
+    for M in (3, 48):
+        q = ops.q8_pack(few[:M].to(gpu))
+        _same(ops.linear_q8(big, q)[-1000:], want[:, :M])
+        _same(ops.linear_q8(q, big)[:, -1000:], want[:, :M].t())
+    x = ops.q8_unpack(big)
+    assert torch.equal(x[-1000:].cpu(), base) and torch.equal(x[:1000].cpu(), base)
+    h = ops.rms_norm_q8(x, torch.ones(K, device=gpu), add=torch.zeros_like(x), out=big)
+    small = ops.q8_unpack(ops.rms_norm_q8(base.to(gpu), torch.ones(K, device=gpu)))
+    assert torch.equal(ops.q8_unpack(h)[-1000:], small)
+
+
 def test_linear_refusals(gpu):
     xq, wq = ops.q8_pack(torch.zeros(4, 256, device=gpu)), ops.q8_pack(torch.zeros(6, 256, device=gpu))
     other = ops.q8_pack(torch.zeros(6, 255, device=gpu))
