@@ -26,16 +26,20 @@ struct Q8Lin {
   int tiles_m, tiles_n, band;  // of the launch
 };
 
-// x / (1 + e^-x) on the hardware's exponential and reciprocal, each within an ulp or so; the
-// argument's product with log2(e) in two parts, so that the exponential keeps its relative error
-// far from zero.  (Against expf and a division a third of the instructions; 256 x 9728 x 896 12.5
-// -> 11.9 us.)  Below -87 the factor stays e^-87.
+// x / (1 + e^-x) on the hardware's exponential and reciprocal, each within an ulp or so.  v^2 (1 + r)
+// is e^-x: v = 2^y with y the rounded -x log2(e) / 2, r what -x - 2 y ln(2) leaves, so that the
+// exponential keeps its relative error far from zero.  (Against expf and a division a third of the
+// instructions; 256 x 9728 x 896 12.5 -> 11.9 us.)  1 + v^2 is formed in units of 2^32: nothing
+// overflows or leaves the normal numbers before the last products, so that x down to the type's
+// lowest value gives -0 (the factor is 0 from -105 on: e^-105 < 2^-150) and x up to the largest, and
+// infinity, gives x.
 __device__ __forceinline__ float silu_hw(float x) {
-  const float c = fmaxf(x, -87.0f), hi = c * -1.4426950408889634f;
-  const float lo = fmaf(c, -1.4426950408889634f, -hi) + c * -1.9259629911266175e-8f;
-  float e = __builtin_amdgcn_exp2f(hi);
-  e = fmaf(e, lo * 0.6931471805599453f, e);
-  return x * __builtin_amdgcn_rcpf(1.0f + e);
+  constexpr float kUnit = 0x1p-32f;
+  const float c = fminf(fmaxf(x, -105.0f), 105.0f), y = c * -0.7213475204444817f;
+  const float r = fmaf(y, 3.80930853e-9f, fmaf(y, -1.3862943611198906f, -c));
+  const float v = __builtin_amdgcn_exp2f(y);
+  const float d = fmaf(v * kUnit, fmaf(v, r, v), kUnit);
+  return x * (__builtin_amdgcn_rcpf(d) * kUnit);
 }
 
 // What the residual holds at columns n .. n + 3 of row m.  Asked for ahead of the sums, since it comes

@@ -12,6 +12,7 @@ from q8_reference import E4M3, held
 
 pytestmark = pytest.mark.gpu
 EPS = 1e-6
+INF, MAX = float("inf"), torch.finfo(torch.float32).max
 
 
 def _gen(seed):
@@ -316,6 +317,35 @@ def test_epilogues(gpu, M, N, K, kind, bias):
     else:
         tol = e + 2.0 ** -24 * want.abs()
     assert ((y - want).abs() <= tol + 1e-37).all(), ((y - want).abs() / tol).max()
+
+
+GATES = [0.0, 1e-30, 0.5, 7.0, 20.0, 60.0, 86.9, 87.2, 88.5, 88.8, 90.0, 100.0, 104.0, 105.5, 130.0,
+         1e4, 1e30, 2.3e38, 2.4e38, MAX]
+
+
+@pytest.mark.parametrize("M,N,K", EPI_SHAPES)
+def test_swiglu_of_any_gate(gpu, M, N, K):
+    """Gates from the type's lowest value to its largest, and past it, through the bias."""
+    announce(f"linear_q8 SwiGLU of any gate {M} x {N} x {K}")
+    gates = torch.tensor(GATES + [-v for v in GATES] + [INF, -INF, float("nan")])
+    up = torch.tensor([1.0, -3.5, 1e-3, 700.0])[torch.arange(N // 2) // 3 % 4]
+    xq = ops.q8_pack(torch.zeros(M, K, device=gpu))
+    wq = ops.q8_pack(torch.zeros(N, K, device=gpu))
+    for roll in (0, 33):  # few columns take two calls
+        gate = gates[(torch.arange(N // 2) + roll) % len(gates)]
+        y = ops.linear_q8(xq, wq, torch.stack([gate, up], 1).reshape(-1).to(gpu),
+                          epilogue=ops.Epilogue(kind=ops.LX_EPI_SWIGLU_PAIRED)).double().cpu()
+        g, u = gate.double(), up.double()
+        want = g * torch.sigmoid(g) * u
+        fin = torch.isfinite(want) & (want.abs() <= MAX)
+        # the exponential's square off by two last places (2^-22), the reciprocal by one or two, four
+        # roundings of 2^-24: below 2^-20 of the result; a subnormal sigmoid is off by 2^-149, a
+        # subnormal result once more
+        tol = 2.0 ** -20 * want.abs() + 2.0 ** -149 * (1 + (g * u).abs())
+        assert ((y - want).abs() <= tol)[:, fin].all(), (gate[fin], (y - want)[0, fin])
+        over = want.isinf() | (want.abs() > MAX)
+        assert torch.equal(y[:, over], (torch.sign(want[over]) * INF).expand(M, -1))
+        assert y[:, want.isnan()].isnan().all()
 
 
 @pytest.mark.parametrize("M,N,K", EPI_SHAPES)
