@@ -513,7 +513,8 @@ int lx_linear_q8_f32(const lx_q8* x, const lx_q8* w, const float* bias, const lx
  * -inf (masked) has probability 0 and adds nothing to the entropy; a row of nothing else
  * has log probabilities -inf and entropy 0.  A NaN or +inf makes NaN of its row's logp,
  * entropy and top_logp (NaN counts as the largest logit).  Sums are fp32, formed around the
- * row's maximum without its own 1.  V <= 2^24.
+ * row's maximum without its own 1, of terms down to e^-131 of it: what lies beside a
+ * probability near one keeps its digits.  V <= 2^24.
  * ws: lx_token_logprobs_ws_floats() floats of scratch, 16-byte aligned (NULL when that is
  * 0: V up to 8192); calls that share it must not overlap.
  * Scores what the head of src/llm/llm.cpp:206-216 gives; no counterpart in the reference

@@ -5,7 +5,8 @@
 // m) over all but one of the maxima, t = the sum of e^(x - m) (x - m), then
 //   log sum e^x = m + log1p(s),   entropy = log1p(s) - t / (1 + s)
 // (the 1 of the maximum left out of the sum, so that a row with one likely token keeps the digits
-// of the rest).  Longer rows are cut into pieces of equal length, whose (m, s, t) and leading keys
+// of the rest; where these are below 2^-70 they are summed again in units of 2^-64, in which a
+// logit counts down to e^-131 of the maximum).  Longer rows are cut into pieces of equal length, whose (m, s, t) and leading keys
 // a second launch joins.
 //
 // Alternatives are ordered by 64-bit keys, unlike for any two logits: the value's bits in an order
@@ -64,6 +65,21 @@ __device__ __forceinline__ key_t64 key_of(unsigned order, int index) {
 __device__ __forceinline__ float exp_of(float d) {
   return __builtin_amdgcn_exp2f(d * 1.4426950408889634f);
 }
+// Sums are handed on in units of 2^-64.  Where too_small does not say so, the terms that the plain
+// exponential flushes, below 2^-126 each, are less than 2^-32 of their sum (2^24 of them at most).
+constexpr float kUnits = 0x1p64f, kUnit = 0x1p-64f;
+__device__ __forceinline__ bool too_small(float m, float s) {  // s in units
+  return m > -__builtin_huge_valf() && s < 0x1p-6f;
+}
+// e^d in units, for d < -48 as all terms of such a sum are: y + 64 is exact then, and the argument's
+// product with log2(e) is in two parts, at these distances some 2^-18 of the result.
+__device__ __forceinline__ float exp_units(float d) {
+#pragma clang fp contract(off)
+  const float c = fmaxf(d, -200.0f), y = c * 1.4426950408889634f;
+  const float lo = fmaf(c, 1.9259629911266175e-8f, fmaf(c, 1.4426950408889634f, -y));
+  const float e = __builtin_amdgcn_exp2f(y + 64.0f);
+  return fmaf(e, lo * 0.6931471805599453f, e);
+}
 __device__ __forceinline__ int lanes(bool c) { return __popcll(__ballot(c)); }
 // How many of the lanes below this one have their bit in m.
 __device__ __forceinline__ int lanes_below(unsigned long long m) {
@@ -120,10 +136,10 @@ struct LpShared {
   key_t64 cand[kCand];
 };
 
+// m; s and t in units.
 struct RowSums {
   float m, s, t;
 };
-// What a row gives: log1p(s), 0 where no logit is above -inf.
 __device__ __forceinline__ bool row_empty(const RowSums& r) {
   return r.m == -__builtin_huge_valf() && r.s == 0.0f;
 }
@@ -152,7 +168,7 @@ __device__ __forceinline__ void write_row(const LpArgs& a, int row, const Given&
     else if (g.t >= 0) v = logp_of(r, ls, g.x);
     a.logp[row] = v;
   }
-  if (a.entropy) a.entropy[row] = row_empty(r) ? 0.0f : ls - r.t / (1.0f + r.s);
+  if (a.entropy) a.entropy[row] = row_empty(r) ? 0.0f : ls - r.t * kUnit / (1.0f + r.s * kUnit);
 }
 
 template <int NV, bool TOP>
@@ -199,7 +215,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(LpArgs a) {
   float s = 0.0f, t = 0.0f;
   int maxima = 0;  // of the wave
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float d = v[i][e] - ref;
@@ -209,6 +225,8 @@ __global__ __launch_bounds__(256) void logprob_kernel(LpArgs a) {
       s += is_max ? 0.0f : p;
       t = fmaf(p, fmaxf(d, -200.0f), t);  // far below, p is 0
     }
+    asm volatile("" : "+s"(maxima));  // counted here, not kept as 4 NV masks
+  }
   s = wave_sum(s);
   t = wave_sum(t);
   float tops = (float)maxima;
@@ -220,11 +238,44 @@ __global__ __launch_bounds__(256) void logprob_kernel(LpArgs a) {
   __syncthreads();
   RowSums r;
   r.m = m;
-  r.t = (sh.f[0][2] + sh.f[1][2]) + (sh.f[2][2] + sh.f[3][2]);
+  r.t = kUnits * ((sh.f[0][2] + sh.f[1][2]) + (sh.f[2][2] + sh.f[3][2]));
   tops = (sh.f[0][3] + sh.f[1][3]) + (sh.f[2][3] + sh.f[3][3]);
   r.s = (sh.f[0][1] + sh.f[1][1]) + (sh.f[2][1] + sh.f[3][1]);
   if (tops > 0.0f) r.s += tops - 1.0f;
-  const float ls = log1pf(r.s);
+  r.s *= kUnits;
+  if (too_small(m, r.s)) {  // of the whole workgroup
+    s = t = 0.0f;
+    // read again: kept for this they would cost the usual row its occupancy (1000 x 151936 with 20
+    // alternatives 135 -> 156 us)
+#pragma unroll 2
+    for (int k = 4 * tid; k < n; k += 1024) {
+      float4u u{-inf, -inf, -inf, -inf};
+      if (k + 4 <= n) {
+        u = *reinterpret_cast<const float4u*>(x + k);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (k + e < n) u[e] = x[k + e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float d = u[e] - m, p = d == 0.0f ? 0.0f : exp_units(d);
+        s += p;
+        t = fmaf(p, fmaxf(d, -200.0f), t);
+      }
+    }
+    s = wave_sum(s);
+    t = wave_sum(t);
+    __syncthreads();  // the first sums are read
+    if ((tid & 63) == 0) {
+      sh.f[wave][1] = s;
+      sh.f[wave][2] = t;
+    }
+    __syncthreads();
+    r.s = (sh.f[0][1] + sh.f[1][1]) + (sh.f[2][1] + sh.f[3][1]);
+    r.t = (sh.f[0][2] + sh.f[1][2]) + (sh.f[2][2] + sh.f[3][2]);
+  }
+  const float ls = log1pf(r.s * kUnit);
   if (a.pieces > 1) {
     if (tid == 0) a.part[blockIdx.x] = make_float4(r.m, r.s, r.t, 0.0f);
   } else if (tid == 0) {
@@ -355,28 +406,34 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(LpArgs a) {
   float m = -inf;
   for (int i = lane; i < a.pieces; i += 64) m = fmaxf(m, part[i].x);
   m = wave_max(m);
-  float s = 0.0f, t = 0.0f, tops = 0.0f;
-  for (int i = lane; i < a.pieces; i += 64) {
-    const float4 p = part[i];
-    if (p.x == m) {
-      s += p.y;
-      t += p.z;
-      tops += 1.0f;
-    } else if (p.x == -inf) {
-      s += p.y;  // 0, or the NaN of such a piece
-    } else {
-      const float d = p.x - m, w = exp_of(d);
-      s = fmaf(w, 1.0f + p.y, s);
-      t = fmaf(w, fmaf(1.0f + p.y, fmaxf(d, -200.0f), p.z), t);
-    }
-  }
   RowSums r;
   r.m = m;
-  r.t = wave_sum(t);
-  r.s = wave_sum(s);
-  tops = wave_sum(tops);
-  if (m != -inf) r.s += tops - 1.0f;
-  const float ls = log1pf(r.s);
+  auto sums = [&](bool small) {
+    float s = 0.0f, t = 0.0f, tops = 0.0f;
+    for (int i = lane; i < a.pieces; i += 64) {
+      const float4 p = part[i];
+      if (p.x == m) {
+        s += p.y;
+        t += p.z;
+        tops += 1.0f;
+      } else if (p.x == -inf) {
+        s += p.y;  // 0, or the NaN of such a piece
+      } else {
+        const float d = p.x - m, far = fmaxf(d, -200.0f);
+        const float w = small ? exp_units(d) : exp_of(d) * kUnits;
+        const float one = 1.0f + p.y * kUnit;  // of the piece's own maximum
+        s = fmaf(w, one, s);
+        t = fmaf(w, fmaf(one, far, p.z * kUnit), t);
+      }
+    }
+    r.t = wave_sum(t);
+    r.s = wave_sum(s);
+    tops = wave_sum(tops);
+    if (m != -inf) r.s += (tops - 1.0f) * kUnits;
+  };
+  sums(false);
+  if (too_small(m, r.s)) sums(true);
+  const float ls = log1pf(r.s * kUnit);
   if (lane == 0) write_row(a, row, tok, r, ls);
   if (!a.top) return;
   // every lane calls f with `each` keys, 0 for none

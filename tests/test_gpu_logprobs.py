@@ -190,6 +190,38 @@ def test_one_likely_token(gpu, V, gap):
     assert (e <= 4 * rel * H + 1e-38).all(), (e / H)
 
 
+@pytest.mark.parametrize("V", [2, 700, 6761, 20000, 151936])
+@pytest.mark.parametrize("gap", [45.0, 50.0, 70.0, 85.0, 87.0, 88.0, 95.0, 100.0, 103.0, 110.0,
+                                 1e30])
+def test_one_token_far_ahead(gpu, V, gap):
+    """All others below 2^-126 of the maximum each: their sum keeps its digits."""
+    announce(f"token_logprobs one of {V} ahead by {gap}")
+    x = torch.randn(6, V, generator=_gen(V))
+    x[1] = x[1].round()
+    x[2] = 0.25
+    x[3, V // 2:] = -INF
+    at = torch.tensor([0, V - 1, V // 2, 0, V // 3, V - 1])
+    one = torch.nn.functional.one_hot(at, V).bool()
+    x[one] = x.amax(1) + gap
+    if V > 2:
+        x[4, (V // 3 + 1) % V] = x[4].amax() - gap / 2  # another one between
+    got = ops.token_logprobs(x.to(gpu), at.int().to(gpu), top=2)
+    d = (x - x[one][:, None]).double()  # as fp32 has them: off by 2^-24 of the gap
+    d = torch.where(one, torch.full_like(d, -INF), d)
+    p = d.exp()
+    s = p.sum(1)
+    logp = -torch.log1p(s)
+    H = torch.log1p(s) - torch.where(p > 0, p * d, torch.zeros_like(p)).sum(1) / (1 + s)
+    # a term below 2^-61 is scaled, its argument carried to 2^-40: 2^-22 of it by the exponential;
+    # the others' arguments (up to 62 log2(e)) are off by 2^-24 of themselves.  Sums: as everywhere
+    rel = 230 * 2.0 ** -24 + 110 * 2.0 ** -23
+    e = (got.logp.cpu().double() - logp).abs()
+    assert (e <= rel * logp.abs() + 2.0 ** -149).all(), (e, logp)
+    assert torch.equal(got.top_logp[:, 0], got.logp)
+    e = (got.entropy.cpu().double() - H).abs()
+    assert (e <= 4 * rel * H + 2.0 ** -147).all(), (e, H)
+
+
 def test_parts_left_out(gpu):
     x = torch.randn(6, 9000, generator=_gen(5)).to(gpu)
     t = torch.arange(6).int().to(gpu)
