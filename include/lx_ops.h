@@ -493,9 +493,9 @@ int lx_rmsnorm_q8_f32(const float* x, long ldx, const float* add, long lda, floa
                       const float* w, float eps, const lx_q8* q, hipStream_t stream);
 
 /* y = epi(x~ @ w~^T + bias), x~ (M, K) and w~ (N, K) what x and w stand for: exact
- * products, fp32 sums (elements below 2^-126 in magnitude lose digits, below 2^-133 they
- * count as zero).  y: (M, N), row stride ldy (N / 2 columns for SWIGLU_PAIRED, N even).  Epilogues: none, GELU_TANH,
- * RESID (y = resid + .., resid row stride ldr; NULL: y itself, in place),
+ * products, fp32 sums (elements below 2^-126 in magnitude count as the nearest multiple of
+ * 2^-133).  y: (M, N), row stride ldy (N / 2 columns for SWIGLU_PAIRED, N even).  Epilogues:
+ * none, GELU_TANH, RESID (y = resid + .., resid row stride ldr; NULL: y itself, in place),
  * SWIGLU_PAIRED; others: LX_ERR_ARG.  bias (N) or NULL.  y must not overlap resid
  * otherwise, nor another operand.  A NaN in a row of x or w makes NaN of the outputs
  * it enters.  No alignment past 4 bytes for y, bias, resid.

@@ -91,7 +91,9 @@ __device__ __forceinline__ void epi_quad(const Q8Lin& a, int m, long n, floatx4 
 }
 
 // Codes as operands of the bf16 matrix instructions: exact, eight bits hold e4m3's four, and the
-// power of two comes with the conversion (v_cvt_scalef32_pk_bf16_fp8, two codes an instruction).
+// power of two comes with the conversion (v_cvt_scalef32_pk_bf16_fp8, two codes an instruction; it
+// reads the scale's exponent field alone, so the bits of 0.0f are 2^-127, and what lies between
+// bf16's subnormal numbers, multiples of 2^-133, goes to the nearest).
 // The 8-bit matrix instructions would take the codes as they are at twice the rate, but they add
 // the products of eight neighbours with some 13 bits below the largest of them, 1.5e-5 of a sum
 // where these keep fp32's 1e-7.

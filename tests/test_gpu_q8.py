@@ -267,6 +267,63 @@ def test_scales_of_every_row_and_block(gpu, M, N, K):
     _same(y, x.double() @ w.double().t())
 
 
+@pytest.mark.parametrize("M,N,K", [(3, 40, 1157), (40, 33, 1157), (300, 900, 1157),
+                                   (500, 1500, 1700), (1400, 900, 1700), (1100, 1300, 1157),
+                                   (1531, 1152, 900), (2100, 2100, 1157), (3590, 3598, 900),
+                                   (60, 200, 2300), (60, 6100, 2300), (1900, 990, 3000)])
+def test_ends_of_the_scales(gpu, M, N, K):
+    """Blocks at the smallest and the largest powers of two, the other operand's at the opposite:
+    whole numbers, exact sums."""
+    announce(f"linear_q8 ends of the scales {M} x {N} x {K}")
+    g = _gen(M + K)
+    ends = torch.tensor([-127, -126, -125, 120, 119, 118, 0])
+    e = ends[torch.arange((K + 127) // 128) % len(ends)]
+    ex = e.repeat_interleave(128)[:K].double()
+    a = torch.randint(-15, 16, (M, K), generator=g).double()
+    b = torch.randint(-15, 16, (N, K), generator=g).double()
+    # 240 sets its block's power; the other operand is zero there
+    a[:, 0::128], b[:, 0::128] = 240, 0
+    a[:, 1::128], b[:, 1::128] = 0, 240
+    x, w = a * 2.0 ** ex, b * 2.0 ** (-7 - ex)
+    assert torch.equal(x.float().double(), x) and torch.equal(w.float().double(), w)
+    if M == 3:
+        assert torch.equal(held(x)[1], (2.0 ** e.double()).expand(M, -1))
+    y = ops.linear_q8(ops.q8_pack(x.float().to(gpu)), ops.q8_pack(w.float().to(gpu)))
+    _same(y, a @ b.t() * 2.0 ** -7)
+
+
+@pytest.mark.parametrize("M", [3, 40, 300, 1531])
+def test_smallest_elements(gpu, M):
+    """One element a row from 2^-119 down to the smallest, 2^-136: whole from 2^-126 on, the nearest
+    multiple of 2^-133 (bf16's subnormal numbers) below."""
+    codes = E4M3[1:].float().double()
+    K, N = 130, 1152
+    x = torch.zeros(M, K, dtype=torch.float64)
+    x[:, 1] = codes[torch.arange(M) % len(codes)] * 2.0 ** -127
+    w = torch.zeros(N, K)
+    w[:, 1] = 2.0 ** 100
+    for flip in (False, True):
+        p, q = (w, x.float()) if flip else (x.float(), w)
+        y = ops.linear_q8(ops.q8_pack(p.to(gpu)), ops.q8_pack(q.to(gpu))).double().cpu()
+        y = (y.t() if flip else y) * 2.0 ** -100
+        v = x[:, 1:2]
+        assert torch.equal(y[v[:, 0] >= 2.0 ** -126], v.expand(-1, N)[v[:, 0] >= 2.0 ** -126])
+        assert ((y - v).abs() <= 2.0 ** -134).all()
+        assert ((y * 2.0 ** 133).frac() == 0).all()
+
+
+@pytest.mark.parametrize("M,N", [(3, 40), (40, 33), (300, 900), (1531, 1152)])
+def test_past_the_largest_number(gpu, M, N):
+    """An element that stands for 2^128 is infinity in a product as in the read-back."""
+    x, w = torch.ones(M, 300), torch.ones(N, 300)
+    x[M // 2, 200] = 3.4e38
+    w[N - 1, 5] = -3.4e38
+    y = ops.linear_q8(ops.q8_pack(x.to(gpu)), ops.q8_pack(w.to(gpu))).cpu()
+    assert (y[M // 2, :N - 1] == INF).all() and y[M // 2, N - 1].isnan()
+    rest = torch.arange(M) != M // 2
+    assert (y[rest, N - 1] == -INF).all() and torch.isfinite(y[rest, :N - 1]).all()
+
+
 def _epi(kind, acc, b=None, r=None):
     if b is not None:
         acc = acc + b.double()
