@@ -468,8 +468,9 @@ int lx_attention_kv4_f32(const float* q, long ldq, const lx_kv4* cache, const in
  * 2^e, e the smallest integer >= -127 with max|v| <= 448 * 2^e over the block's finite
  * elements; an element is the e4m3 number nearest to v / 2^e (ties to even) and stands
  * for that number times 2^e, off by at most 2^-4 of itself or 2^(e - 10) (past fp32's
- * range, from 2^128 on: infinity).  Infinities and NaN stand for NaN.  `data`: device memory of lx_q8_bytes() bytes (0 for a bad
- * shape), 16-byte aligned, which needs no initialisation.
+ * range, from 2^128 on: infinity).  Infinities and NaN stand for NaN.  `data`: device
+ * memory of lx_q8_bytes() bytes (0 for a bad shape), 16-byte aligned, which needs no
+ * initialisation.
  * lx_q8_pack_f32 writes x (row stride ldx) into q; lx_q8_unpack_f32 what q stands for
  * into x.  At most 2^27 - 16 blocks, of an even number of rows.  x and q must not overlap.
  * No counterpart in the reference (its weights and activations stay fp32). */
@@ -483,8 +484,8 @@ int lx_q8_unpack_f32(const lx_q8* q, float* x, long ldx, hipStream_t stream);
 
 /* h = x + add, written to sum (add and sum NULL: h = x); q = h / sqrt(mean(h^2) + eps) * w
  * in 8 bits.  x, add, sum: q->rows rows of q->K, row strides ldx / lda / lds; sum may be
- * x or add itself (the same pointer and stride) and must not overlap them otherwise;
- * w (K).  h is rounded to fp32; the norm is formed in 64 bits and rounded once, to its
+ * x or add itself (the same pointer and stride) and must not overlap them otherwise, nor
+ * w (K); q must not overlap any of them.  h is rounded to fp32; the norm is formed in 64 bits and rounded once, to its
  * code (magnitudes past fp32's count as fp32's largest).  No alignment past 4 bytes.  At
  * most 2^23 - 1 rows (2^25 - 4 of up to 2048 columns).
  * Replaces the residual add and rms_norm (src/llm/ops.cpp:7-11, src/llm/llm.cpp:141-173)

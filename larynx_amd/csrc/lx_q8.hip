@@ -243,6 +243,7 @@ extern "C" int lx_q8_pack_f32(const float* x, long ldx, const lx_q8* q, hipStrea
   LX_REQUIRE(ldx >= q->K && (uintptr_t)x % 4 == 0, "q8_pack: bad row stride %ld", ldx);
   const Q8Mat m = q8_mat(q);
   LX_REQUIRE(q8_grid(m) <= INT_MAX / 256, "q8_pack: %d rows of %d are too many", m.rows, m.K);
+  LX_REQUIRE(!q8_overlaps(q, x, ldx, m.K, m.rows), "q8_pack: the matrix overlaps x");
   hipLaunchKernelGGL(q8_quant_kernel, dim3((unsigned)q8_grid(m)), dim3(256), 0, stream, x, ldx, m);
   return check_launch("q8_quant_kernel");
 }
@@ -252,6 +253,7 @@ extern "C" int lx_q8_unpack_f32(const lx_q8* q, float* x, long ldx, hipStream_t 
   LX_REQUIRE(ldx >= q->K && (uintptr_t)x % 4 == 0, "q8_unpack: bad row stride %ld", ldx);
   const Q8Mat m = q8_mat(q);
   LX_REQUIRE(q8_grid(m) <= INT_MAX / 256, "q8_unpack: %d rows of %d are too many", m.rows, m.K);
+  LX_REQUIRE(!q8_overlaps(q, x, ldx, m.K, m.rows), "q8_unpack: x overlaps the matrix");
   hipLaunchKernelGGL(q8_dequant_kernel, dim3((unsigned)q8_grid(m)), dim3(256), 0, stream, m, x,
                      ldx);
   return check_launch("q8_dequant_kernel");
@@ -275,6 +277,11 @@ extern "C" int lx_rmsnorm_q8_f32(const float* x, long ldx, const float* add, lon
   }
   LX_REQUIRE((D <= 2048 ? ((long)rows + 3) / 4 : (long)rows) <= INT_MAX / 256,
              "rmsnorm_q8: %d rows of %d are too many", rows, D);
+  LX_REQUIRE(!q8_overlaps(q, x, ldx, D, rows) && !q8_overlaps(q, w, D, D, 1) &&
+                 (!add || (!q8_overlaps(q, add, lda, D, rows) &&
+                           !q8_overlaps(q, sum, lds, D, rows))),
+             "rmsnorm_q8: the matrix overlaps x, add, sum or w");
+  LX_REQUIRE(!sum || !rows_overlap(sum, lds, D, w, 0, D, rows), "rmsnorm_q8: sum overlaps w");
   NormArgs a{x, add, w, sum, ldx, lda, lds, eps, q8_mat(q)};
   const dim3 wide((unsigned)rows), four((unsigned)(((long)rows + 3) / 4)), block(256);
   if (D <= 1024)

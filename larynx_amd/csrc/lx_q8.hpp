@@ -50,6 +50,12 @@ inline Q8Mat q8_mat(const lx_q8* q) {
   return Q8Mat{p, p + q8_code_bytes(q->rows, q->K), q->rows, q->K, kb};
 }
 
+// Whether `rows` rows of n floats every ld from p share memory with the matrix.
+inline bool q8_overlaps(const lx_q8* q, const float* p, long ld, long n, long rows) {
+  return rows_overlap(p, ld, n, static_cast<const float*>(q->data), 0,
+                      (long)(lx_q8_bytes(q->rows, q->K) / 4), rows);
+}
+
 // Where chunk c (0 .. 7) of row r (0 .. 15) stands in a tile.
 __device__ __forceinline__ int q8_chunk(int r, int c) {
   return (c >> 2) * (kQ8Tile / 2) + r * (kQ8Block / 2) + (((c & 3) ^ (r >> 2)) << 4);

@@ -678,6 +678,9 @@ extern "C" int lx_linear_q8_f32(const lx_q8* x, const lx_q8* w, const float* bia
   LX_REQUIRE(((uintptr_t)y | (uintptr_t)bias | (uintptr_t)resid) % 4 == 0, "linear_q8: unaligned");
   LX_REQUIRE((resid == y && ldr == ldy) || !rows_overlap(resid, ldr, cols, y, ldy, cols, M),
              "linear_q8: y overlaps resid");
+  LX_REQUIRE(!q8_overlaps(x, y, ldy, cols, M) && !q8_overlaps(w, y, ldy, cols, M) &&
+                 (!bias || !rows_overlap(y, ldy, cols, bias, 0, N, M)),
+             "linear_q8: y overlaps x, w or bias");
   Q8Lin a{};
   a.x = q8_mat(x);
   a.w = q8_mat(w);

@@ -163,6 +163,53 @@ def test_score_workspace():
         assert b"workspace" in lib.lx_last_error()
 
 
+A, Q8_BYTES = 1 << 41, 4128  # an 8-bit matrix (8, 256)
+
+
+@pytest.mark.parametrize("where", ["first", "last", "before"])
+def test_outputs_over_inputs(where):
+    """fp32 rows (8, 256) of stride 300 with elements in an 8-bit matrix's memory, one of the two
+    written."""
+    def rows(cols):
+        return {"first": A, "last": A + Q8_BYTES - 4, "before": A - 4 * (7 * 300 + cols) + 4}[where]
+
+    at = rows(256)
+    q, other = _q(data=A), _q(data=1 << 50)
+    far = 1 << 51
+    calls = {
+        "pack": lambda: lib.lx_q8_pack_f32(at, 300, q, None),
+        "unpack": lambda: lib.lx_q8_unpack_f32(q, at, 300, None),
+        "x": lambda: lib.lx_rmsnorm_q8_f32(at, 300, None, 0, None, 0, P, 1e-6, q, None),
+        "x of a sum": lambda: lib.lx_rmsnorm_q8_f32(at, 300, far, 256, 2 * far, 256, P, 1e-6, q,
+                                                    None),
+        "add": lambda: lib.lx_rmsnorm_q8_f32(far, 256, at, 300, 2 * far, 256, P, 1e-6, q, None),
+        "sum": lambda: lib.lx_rmsnorm_q8_f32(far, 256, 2 * far, 256, at, 300, P, 1e-6, q, None),
+        "sum in place": lambda: lib.lx_rmsnorm_q8_f32(at, 300, far, 256, at, 300, P, 1e-6, q, None),
+        "y over x": lambda: lib.lx_linear_q8_f32(q, _q(data=1 << 50, rows=256), None, None, None, 0,
+                                                 at, 300, None),
+        "y over w": lambda: lib.lx_linear_q8_f32(other, q, None, None, None, 0, rows(8), 300, None),
+    }
+    for name, call in calls.items():
+        assert call() == LX_ERR_ARG, name
+        assert b"overlap" in lib.lx_last_error(), (name, lib.lx_last_error())
+
+
+def test_outputs_over_vectors():
+    """The norm's weight under its sum or its codes, a bias under y."""
+    far = 1 << 51
+    for w, s in [(far + 4 * 255, far), (far - 4 * 255, far), (far + 4 * (7 * 256 + 255), far)]:
+        assert lib.lx_rmsnorm_q8_f32(2 * far, 256, 3 * far, 256, s, 256, w, 1e-6, _q(data=A),
+                                     None) == LX_ERR_ARG
+        assert b"overlap" in lib.lx_last_error()
+    for w in (A, A + Q8_BYTES - 4, A - 4 * 255):
+        assert lib.lx_rmsnorm_q8_f32(2 * far, 256, None, 0, None, 0, w, 1e-6, _q(data=A),
+                                     None) == LX_ERR_ARG
+        assert b"overlap" in lib.lx_last_error()
+    for b in (O, O - 4 * 31, O + 4 * (7 * 32 + 31)):
+        assert _linear(bias=b) == LX_ERR_ARG
+        assert b"overlap" in lib.lx_last_error()
+
+
 def test_ops_refuse_host_tensors():
     x, w = torch.zeros(4, 256), torch.ones(256)
     with pytest.raises(ValueError, match="current device"):
