@@ -517,7 +517,8 @@ int lx_linear_q8_f32(const lx_q8* x, const lx_q8* w, const float* bias, const lx
  * row's maximum without its own 1, of terms down to e^-131 of it: what lies beside a
  * probability near one keeps its digits.  V <= 2^24.
  * ws: lx_token_logprobs_ws_floats() floats of scratch, 16-byte aligned (NULL when that is
- * 0: V up to 8192); calls that share it must not overlap.
+ * 0: V up to 8192); calls that share it must not overlap.  Neither it nor an output may
+ * overlap the logits.
  * Scores what the head of src/llm/llm.cpp:206-216 gives; no counterpart in the reference
  * (its caller samples on the host). */
 size_t lx_token_logprobs_ws_floats(int rows, int V, int top);

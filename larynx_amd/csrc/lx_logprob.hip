@@ -542,6 +542,15 @@ extern "C" int lx_token_logprobs_f32(const float* logits, long ld, int rows, int
     a.part = reinterpret_cast<float4*>(ws);
     a.keys = reinterpret_cast<key_t64*>(ws + (size_t)rows * a.pieces * 4);
   }
+  // rows of logits may be read behind another row's outputs
+  auto over = [&](const void* p, size_t floats) {
+    return p && rows_overlap(logits, ld, V, static_cast<const float*>(p), 0, (long)floats, rows);
+  };
+  const size_t alts = (size_t)rows * top;
+  LX_REQUIRE(!over(logp, rows) && !over(entropy, rows) &&
+                 !(top && (over(top_logp, alts) || over(top_ids, alts))) &&
+                 !(a.pieces > 1 && over(ws, lx_token_logprobs_ws_floats(rows, V, top))),
+             "token_logprobs: an output or the workspace overlaps the logits");
   if (top)
     launch_logprob<true>(a, rows, stream);
   else

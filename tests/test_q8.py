@@ -210,6 +210,19 @@ def test_outputs_over_vectors():
         assert b"overlap" in lib.lx_last_error()
 
 
+@pytest.mark.parametrize("at", [O, O + 4 * (3 * 1100 + 999), O - 4])
+def test_scores_over_logits(at):
+    """Outputs with an element in the first or last of the rows of logits, workspaces too."""
+    for kw in [dict(logp=at), dict(ent=at), dict(tl=at), dict(ti=at),
+               dict(tokens=None, logp=None, ent=at, top=0)]:
+        assert _score(ld=1100, **kw) == LX_ERR_ARG, kw
+        assert b"overlaps the logits" in lib.lx_last_error(), kw
+    need = lib.lx_token_logprobs_ws_floats(4, 20000, 3)
+    for ws in (O, O - 4 * need + 16, O + 4 * (3 * 20100 + 19996)):
+        assert _score(V=20000, ld=20100, ws=ws, n=need) == LX_ERR_ARG, ws
+        assert b"overlaps the logits" in lib.lx_last_error()
+
+
 def test_ops_refuse_host_tensors():
     x, w = torch.zeros(4, 256), torch.ones(256)
     with pytest.raises(ValueError, match="current device"):
