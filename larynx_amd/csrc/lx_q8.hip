@@ -132,12 +132,9 @@ __device__ __forceinline__ int row_of(const Q8Mat& q) {
 // row's power and the normalised values in 64 bits, where a code next to a border is decided: some
 // 40 instructions an element, which a row's bytes hide.  PAIR: a workgroup has the two rows whose
 // codes share lines, sixteen lanes of one beside sixteen of the other, so that a wave stores whole
-// lines.  8192 x 8192 with add 175 -> 159 us, 5.5 TB/s (a copy: 4.7), 3000 x 8192 67 -> 62; where
-// the bytes come from the last cache or there is no add it is as fast or slower (1000 x 8192 23.8
-// and 24.3, 1 x 8192 7.0 and 8.2; 6000 x 8192 without add 52 and 53).  1531 x 896 6.5, a launch and
-// one round trip; 8192 x 8192 without add, whose bytes are half, 80 (4.2 TB/s, the instructions).
-// Four elements a lane need a fifth step of each block's maximum for half the elements: 6 to 20%
-// slower.
+// lines (pairs_pay).  1531 x 896 6.5 us, a launch and one round trip; 8192 x 8192 with add 156 (5.6
+// TB/s; a copy: 4.7), without add, whose bytes are half, 80 (4.2 TB/s, the instructions).  Four
+// elements a lane need a fifth step of each block's maximum for half the elements: 6 to 20% slower.
 template <int G, int NC, bool PAIR>
 __global__ __launch_bounds__(PAIR ? 2 * G : 256) void norm_q8_kernel(NormArgs a) {
   const int side = threadIdx.x >> 4 & 1;  // of a pair
@@ -283,6 +280,17 @@ extern "C" int lx_rmsnorm_q8_f32(const float* x, long ldx, const float* add, lon
              "rmsnorm_q8: the matrix overlaps x, add, sum or w");
   LX_REQUIRE(!sum || !rows_overlap(sum, lds, D, w, 0, D, rows), "rmsnorm_q8: sum overlaps w");
   NormArgs a{x, add, w, sum, ldx, lda, lds, eps, q8_mat(q)};
+  // Rows of 4097 to 8192 two a workgroup?  Where the call's bytes come from memory and, of the four
+  // chunks that a thread may hold, more than two are taken (us, one row and two; the same buffers
+  // every call, then several in turn, more than the 256 MB of the last cache)
+  //    1531 x 8192 163 MB   29.4 30.4   38.7 36.8       8192 x 4100  437 MB   93.6  97.4
+  //    2048 x 7000 186      35.0 34.6   46.2 47.8       8192 x 4300  458     101.3 104.7
+  //    2048 x 8192 218      37.8 38.4   47.6 44.9       8192 x 4480  477      97.8  94.8
+  //    3000 x 6400 250      46.6 46.0   56.3 54.3       8192 x 4864  518     108.1 101.5
+  //    4000 x 5000 260      48.7 48.3   58.6 57.3       8192 x 8192  872     176.8 156.1
+  //    3000 x 8192 319      63.2 58.8   68.1 62.3      30000 x 4608 1797     372   340
+  // Without add the bytes are fewer than the instructions (6000 x 8192 52 and 53).
+  const bool pairs_pay = add && D >= 4480 && D <= 8192 && 13.0 * rows * D >= 2e8;
   const dim3 wide((unsigned)rows), four((unsigned)(((long)rows + 3) / 4)), block(256);
   if (D <= 1024)
     hipLaunchKernelGGL((norm_q8_kernel<64, 2, false>), four, block, 0, stream, a);
@@ -290,7 +298,7 @@ extern "C" int lx_rmsnorm_q8_f32(const float* x, long ldx, const float* add, lon
     hipLaunchKernelGGL((norm_q8_kernel<64, 4, false>), four, block, 0, stream, a);
   else if (D <= 4096)
     hipLaunchKernelGGL((norm_q8_kernel<256, 2, false>), wide, block, 0, stream, a);
-  else if (D <= 8192 && add && rows >= 2048)
+  else if (pairs_pay)
     hipLaunchKernelGGL((norm_q8_kernel<256, 4, true>), dim3((unsigned)(((long)rows + 1) / 2)),
                        dim3(512), 0, stream, a);
   else if (D <= 8192)

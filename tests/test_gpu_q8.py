@@ -142,6 +142,13 @@ def test_norm_of_many_long_rows(gpu, rows, D, where):
     test_norm_with_residual(gpu, rows, D, where)
 
 
+@pytest.mark.parametrize("rows,D,where", [(3500, 4480, "x"), (3101, 5001, "add"),
+                                          (1901, 8192, "apart"), (3434, 4479, "apart")])
+def test_norm_of_rows_from_memory(gpu, rows, D, where):
+    """Two rows a workgroup and, just below, one."""
+    test_norm_with_residual(gpu, rows, D, where)
+
+
 def test_norm_strides(gpu):
     """Rows of unequal strides at odd offsets; what lies between them stays."""
     g = _gen(9)
