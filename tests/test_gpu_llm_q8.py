@@ -114,6 +114,36 @@ def test_other_geometries(gpu, kw):
     lm.close()
 
 
+@pytest.mark.parametrize("L", [600, 1531])
+def test_long_prompts(gpu, L):
+    """Gate/up on 128 x 128 and 256 x 256 tiles, down on the tiles of long K."""
+    announce(f"8-bit prefill of {L} rows")
+    from larynx_amd.llm import Qwen2Config, Qwen2LM, qwen2_param_shapes
+    cfg = Qwen2Config(n_layers=1, text_vocab=2000, hidden=320, intermediate=4864, n_heads=5,
+                      n_kv_heads=1)
+    params = orc.make_params(qwen2_param_shapes(cfg), 97)
+    for k in params:
+        if k.endswith("layernorm.weight") or k == "norm.weight":
+            params[k] = (params[k] + 1.0).astype(np.float32)
+    lm = Qwen2LM({k: torch.from_numpy(v).to(gpu) for k, v in params.items()}, cfg, max_ctx=1600)
+    lm.set_prefill_bits(8)
+    x = torch.randn(L, cfg.hidden, generator=torch.Generator().manual_seed(L)) * 0.5
+    logits, hidden, final = lm.prefill(x.to(gpu), capture=True)
+    want, k, v = _layer(x.double(), "layers.0.", cfg, params)
+    _near(hidden[0], want, "layer 0")
+    kd, vd = lm.cache_views(0)
+    # the rotary angles are fp32: a frequency below 1 is off by two roundings of itself, its product
+    # with the position by one more, so the angle by 3 L 2^-24 (2.7e-4 at 1531), and a rotated pair
+    # by that of its length, at most sqrt(2) of the largest element
+    assert orc.rel_err(kd[:L].cpu().numpy(), k.numpy()) < 1e-5 + 1.5 * 3 * L * 2.0 ** -24
+    assert orc.rel_err(vd[:L].cpu().numpy(), v.numpy()) < 1e-5
+    fn = _norm(hidden[0].double().cpu(), _t(params["norm.weight"]), cfg.rms_eps)
+    assert orc.rel_err(final.cpu().numpy(), fn.numpy()) < 1e-6
+    head = held(fn)[0] @ held(torch.from_numpy(params["llm_decoder.weight"]))[0].t()
+    assert orc.rel_err(logits.cpu().numpy(), head.numpy()) < 1e-5
+    lm.close()
+
+
 def test_switching_back_gives_the_fp32_bits(gpu, lm8):
     cfg, params, lm = lm8
     x = lm.build_lm_input([1, 2, 3], list(range(60)))
