@@ -794,9 +794,10 @@ int lx_qwen2_set_decode_bits(lx_qwen2* m, int bits, int group);
  * is a setting of its own).  The first call packs the copies from the model's fp32 weights,
  * which stay, and allocates the rows for max_ctx (364 and 24 MB for Qwen2-0.5B at 4096); both are
  * held until destroy, so a prefill that the caller captured keeps giving what it was captured
- * with.  The call waits for that packing, and for nothing else.  LX_ERR_ALLOC and LX_ERR_LAUNCH
- * change nothing.  The model's device must be current (else LX_ERR_ARG).  Not to be called
- * during a capture.  No counterpart in the reference. */
+ * with.  That call waits for the packing, which is queued on the null stream and so behind the
+ * work that it and blocking streams hold; later calls wait for nothing.  LX_ERR_ALLOC and
+ * LX_ERR_LAUNCH change nothing.  The model's device must be current (else LX_ERR_ARG).  Not to
+ * be called during a capture.  No counterpart in the reference. */
 int lx_qwen2_set_prefill_bits(lx_qwen2* m, int bits);
 
 /* Prefill projections' split-operand products, 3 (the default) or 6, as
