@@ -17,9 +17,10 @@
 // more of them into few threads, the exact bound is found the same way over all logits.
 //
 // Bound by the logits' bytes where rows are many: 1000 x 151936 98-110 us without alternatives (5.5
-// to 6.2 TB/s, above a copy's 4.7), 125 with 20 (4.9 TB/s: 876 vector instructions a wave for 32
-// logits a lane, 487 without); 1531 x 6761 11-12 us (3.6 TB/s: one generation of workgroups, a
-// round trip and a tail).  One row of 6761: 4 us in a graph, 7 with alternatives.
+// to 6.2 TB/s, above a copy's 4.7), 123 with 20 (4.9 TB/s: 883 vector instructions a wave for 32
+// logits a lane, 493 without); 1531 x 6761 11-12 us (3.7 TB/s: one generation of workgroups, a
+// round trip and a tail), 15 where each row is summed a second time.  One row of 6761: 3.8 us in a
+// graph, 6.4 with alternatives.
 #include <algorithm>
 #include <climits>
 

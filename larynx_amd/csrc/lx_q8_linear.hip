@@ -43,7 +43,7 @@ __device__ __forceinline__ float silu_hw(float x) {
 }
 
 // What the residual holds at columns n .. n + 3 of row m.  Asked for ahead of the sums, since it comes
-// from memory: 1531 x 896 x 4864 20.5 -> 18.7 us, 4096 x 896 x 896 18.2 -> 16.1.
+// from memory: 4096 x 896 x 896 18.2 -> 16.1 us.
 __device__ __forceinline__ floatx4 resid_quad(const Q8Lin& a, int m, long n) {
   floatx4 r{0.f, 0.f, 0.f, 0.f};
   if (m >= a.x.rows) return r;
@@ -108,7 +108,7 @@ __device__ __forceinline__ bf16x8_t q8_frag(int lo, int hi, float scale) {
 // Up to 16 rows.  A workgroup owns 16 MT rows of x and 16 NT rows of W; its waves take the blocks
 // of K in turn, straight from memory to registers, and their sums meet in LDS.  W is the
 // instruction's A operand: a lane's four sums are four consecutive columns of one row of y.  Bound
-// by the weights' bytes (16 x 8192 x 8192 12.7 us, 5.3 TB/s; 16 x 151936 x 896 31, 4.7) or a launch
+// by the weights' bytes (16 x 8192 x 8192 12.7 us, 5.3 TB/s; 16 x 151936 x 896 28.7, 4.8) or a launch
 // and one round trip (1 x 1152 x 896 2.6 us in a graph).
 template <int MT, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void q8_stream_kernel(Q8Lin a) {
@@ -432,8 +432,8 @@ int launch_tile(Q8Lin& a, hipStream_t s) {
 // Fewer tiles than CUs.  A workgroup owns (32 RB) x (32 CB) outputs and each of its W waves takes
 // every W-th block of K (H = 2) or half of one (H = 1), through a ring of R slots of LDS of its own:
 // no barrier until the waves' sums meet, and R - 1 slots of every wave on their way.  A half
-// block's tile is 1 KB, one instruction.  1531 x 896 x 4864 on 96 x 64: 18.4 us (0.73 PFLOP/s; with
-// residual 18.7) where 64 x 64 on the tile kernel takes 22.4; a launch, the first slots and the sums
+// block's tile is 1 KB, one instruction.  1531 x 896 x 4864 on 96 x 64: 17.5 us (0.76 PFLOP/s; with
+// residual as much) where 64 x 64 on the tile kernel takes 22.9; a launch, the first slots and the sums
 // alone take 8.2, with the loads 15, with conversions and products but no loads 14.3; three slots
 // deep it is the same.  256 x 896 x 4864 on 32 x 32: 7.0, 256 x 896 x 896 3.6 (3.8 on half blocks).
 template <int RB, int CB, int W, int H, int R>
