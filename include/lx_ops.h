@@ -485,9 +485,9 @@ int lx_q8_unpack_f32(const lx_q8* q, float* x, long ldx, hipStream_t stream);
 /* h = x + add, written to sum (add and sum NULL: h = x); q = h / sqrt(mean(h^2) + eps) * w
  * in 8 bits.  x, add, sum: q->rows rows of q->K, row strides ldx / lda / lds; sum may be
  * x or add itself (the same pointer and stride) and must not overlap them otherwise, nor
- * w (K); q must not overlap any of them.  h is rounded to fp32; the norm is formed in 64 bits and rounded once, to its
- * code (magnitudes past fp32's count as fp32's largest).  No alignment past 4 bytes.  At
- * most 2^23 - 1 rows (2^25 - 4 of up to 2048 columns).
+ * w (K); q must not overlap any of them.  h is rounded to fp32; the norm is formed in 64
+ * bits and rounded once, to its code (magnitudes past fp32's count as fp32's largest).  No
+ * alignment past 4 bytes.  At most 2^23 - 1 rows (2^25 - 4 of up to 2048 columns).
  * Replaces the residual add and rms_norm (src/llm/ops.cpp:7-11, src/llm/llm.cpp:141-173)
  * before a projection whose weight is held in 8 bits. */
 int lx_rmsnorm_q8_f32(const float* x, long ldx, const float* add, long lda, float* sum, long lds,

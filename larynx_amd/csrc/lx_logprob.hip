@@ -6,8 +6,8 @@
 //   log sum e^x = m + log1p(s),   entropy = log1p(s) - t / (1 + s)
 // (the 1 of the maximum left out of the sum, so that a row with one likely token keeps the digits
 // of the rest; where these are below 2^-70 they are summed again in units of 2^-64, in which a
-// logit counts down to e^-131 of the maximum).  Longer rows are cut into pieces of equal length, whose (m, s, t) and leading keys
-// a second launch joins.
+// logit counts down to e^-131 of the maximum).  Longer rows are cut into pieces of equal length,
+// whose (m, s, t) and leading keys a second launch joins.
 //
 // Alternatives are ordered by 64-bit keys, unlike for any two logits: the value's bits in an order
 // that whole numbers share, then the complement of the index.  The k-th largest of the 256 threads'
