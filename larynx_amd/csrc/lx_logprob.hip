@@ -244,7 +244,16 @@ __global__ __launch_bounds__(256) void logprob_kernel(LpArgs a) {
   r.s = (sh.f[0][1] + sh.f[1][1]) + (sh.f[2][1] + sh.f[3][1]);
   if (tops > 0.0f) r.s += tops - 1.0f;
   r.s *= kUnits;
-  if (too_small(m, r.s)) {  // of the whole workgroup
+  // rows of one open logit have nothing to sum (1531 x 6761 of these 10.8 us in place of 14.7)
+  auto others = [&]() {
+    bool c = false;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c |= v[i][e] > -inf && v[i][e] < m;
+    return __syncthreads_or(c);
+  };
+  if (too_small(m, r.s) && others()) {  // of the whole workgroup
     s = t = 0.0f;
     // read again: kept for this they would cost the usual row its occupancy (1000 x 151936 with 20
     // alternatives 135 -> 156 us)
